@@ -293,6 +293,69 @@ int vtl_hip_linear_backward_host_f32(const float *grad, const float *x, const fl
 int vtl_hip_linear_backward_host_f64(const double *grad, const double *x, const double *W, double *dx, double *dw,
                                      double *db, int M, int N, int K);
 
+/* ---- int8 key/value cache and attention ------------------------------------ */
+
+/* Keys and values of sequences, kept as int8 codes with a scale for each token and head, in pages of
+ * page_size tokens.  A page holds, for each of kv_heads heads in turn (P = page_size, D = head_dim rounded up to a
+ * multiple of 16; so many bytes: vtl_hip_kv_cache_bytes with num_pages = 1, over kv_heads):
+ *   codes of the keys    int8 [D / 16, P, 16]    16 dimensions of a token lie together,
+ *   codes of the values  int8 [P / 16, D, 16]    16 tokens of a dimension lie together,
+ *   scales of the keys   f32 [P],
+ *   scales of the values f32 [P]:
+ * the order in which the matrix units take both.  page_size is a multiple of 16 up to 4096, head_dim 1 to
+ * 256; `pages` (device memory, 16-byte aligned) need not be initialised.  The library keeps nothing about a cache. */
+typedef struct {
+    void *pages;
+    int num_pages, page_size;
+    int kv_heads, head_dim;
+} vtl_hip_kv_cache;
+
+/* Which sequences a call works on.  page_table, lengths and starts are device pointers.  Sequence b has lengths[b] tokens
+ * in the cache, the call's among them; token i is in slot i % page_size of page page_table[b, i / page_size].  Rows starts[b] ..
+ * starts[b + 1] - 1 of the call's tensors are the LAST tokens of sequence b, in order; starts == NULL: row b is the last token of
+ * sequence b (rows == batch).  Rows of no sequence are left as they are.
+ * What the device finds there is taken as follows, and nothing is read or written outside the cache and the call's tensors:
+ * lengths below 0 and above max_pages * page_size (at most 2^28) count as these; starts outside 0 .. rows as the nearest of
+ * these; a page number outside 0 .. num_pages - 1 is no page: tokens there are not written, are read as zeros and
+ * are not attended to.  The same holds for rows in front of a sequence's first token (more rows than tokens): not
+ * written, read as zeros, and attending to nothing where causal.
+ * most_rows and most_length are the largest number of rows and the largest length of any sequence, for the host's choice of
+ * launches: larger ones on the device are computed all the same, only slower.  0: not known. */
+typedef struct {
+    int batch, max_pages;
+    const int32_t *page_table;   /* [batch, max_pages] */
+    const int32_t *lengths;      /* [batch] */
+    const int32_t *starts;       /* [batch + 1] or NULL */
+    int rows, most_rows, most_length;
+} vtl_hip_kv_batch;
+
+/* Bytes of num_pages pages; 0 for sizes that no cache may have. */
+size_t vtl_hip_kv_cache_bytes(int num_pages, int page_size, int kv_heads, int head_dim);
+
+/* Rows of keys and values [rows, kv_heads, head_dim] into the cache, k_stride and v_stride elements from one row
+ * to the next (a fused projection's output goes in as it is): every token and head quantized as vtl_hip_quantize_f32_i8 with
+ * per_row = 1 quantizes a row.  Codes of dimensions from head_dim on are written as zeros.  Two rows that share a place leave it
+ * undefined. */
+int vtl_hip_kv_write_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, const float *k, int64_t k_stride,
+                         const float *v, int64_t v_stride);
+
+/* The same rows back: f32(code) * scale, as vtl_hip_dequantize_i8_f32.  k or v may be NULL.  Rows that are whole
+ * sequences (starts[b + 1] - starts[b] = lengths[b]) read all of them. */
+int vtl_hip_kv_read_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, float *k, int64_t k_stride, float *v,
+                        int64_t v_stride);
+
+/* Attention of the rows q [rows, heads, head_dim] over their sequences' keys and values (which hold the rows' own tokens
+ * already): out[r, h] = sum_j w_j v_j, w = softmax over j of scale * q[r, h] . k_j, with head h reading key/value head
+ * h / (heads / kv_heads).  causal: a row sees the tokens up to its own; otherwise all of its sequence's (an encoder's states, with
+ * any number of rows).  A row that sees nothing gives zeros.  q and the weights enter the products with 22 bits, sums are f32; results
+ * do not depend on what else is in the batch as long as the sizes that the host knows are the same.  heads is a multiple of kv_heads.
+ * out may not share memory with q.  workspace: device memory of at least vtl_hip_attention_i8_workspace() bytes, 16-byte
+ * aligned, for the parts of long sequences; NULL (with size 0): the library's own (see above). */
+size_t vtl_hip_attention_i8_workspace(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, int heads);
+int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, const float *q, int64_t q_stride,
+                             int heads, float scale, int causal, float *out, int64_t out_stride, void *workspace,
+                             size_t workspace_bytes);
+
 /* ---- f32 / f64 matmul with f64 accumulation ------------------------------ */
 
 /* C[M,N] = op(A) . op(B) with every product and sum in f64 and one rounding

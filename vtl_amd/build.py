@@ -14,7 +14,7 @@ OBJ_DIR = os.path.join(PKG_DIR, "_build")
 # bench.py's measurement aid (an MFMA-only loop): a library of its own, no part of the product
 BENCH_PROBE_PATH = os.path.join(PKG_DIR, "libvtlbenchprobe.so")
 SOURCES = ["runtime.hip", "memory.hip", "host_copy.hip", "host_quant.hip", "quant.hip", "gemm_i8.hip", "matmul_f64acc.hip", "tensor_ops.hip",
-           "host_calls.hip"]
+           "host_calls.hip", "kv_cache.hip", "attention_i8.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

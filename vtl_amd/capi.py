@@ -36,6 +36,19 @@ class Watch(C.Structure):
     _fields_ = [("data", _vp), ("count", _i64), ("element_bytes", _i64), ("fingerprint", C.c_uint64)]
 
 
+class KVCache(C.Structure):
+    """`vtl_hip_kv_cache`: int8 keys and values in pages on the device."""
+    _fields_ = [("pages", _vp), ("num_pages", _ci), ("page_size", _ci), ("kv_heads", _ci), ("head_dim", _ci)]
+
+
+class KVBatch(C.Structure):
+    """`vtl_hip_kv_batch`: the sequences of one call on a cache."""
+    _fields_ = [("batch", _ci), ("max_pages", _ci), ("page_table", _vp), ("lengths", _vp), ("starts", _vp),
+                ("rows", _ci), ("most_rows", _ci), ("most_length", _ci)]
+
+
+_pc, _pb = C.POINTER(KVCache), C.POINTER(KVBatch)
+
 # name -> (restype, argtypes); kept in step with include/vtl_hip.h
 SIGNATURES = {
     "vtl_hip_device_count": (_ci, [C.POINTER(_ci)]),
@@ -97,6 +110,11 @@ SIGNATURES = {
     "vtl_hip_gemv_f64": (_ci, [_vp, _vp, _vp, _i64, _i64]),
     "vtl_hip_sigmoid_f32": (_ci, [_vp, _vp, _i64]),
     "vtl_hip_sigmoid_f64": (_ci, [_vp, _vp, _i64]),
+    "vtl_hip_kv_cache_bytes": (_sz, [_ci, _ci, _ci, _ci]),
+    "vtl_hip_kv_write_f32": (_ci, [_pc, _pb, _vp, _i64, _vp, _i64]),
+    "vtl_hip_kv_read_f32": (_ci, [_pc, _pb, _vp, _i64, _vp, _i64]),
+    "vtl_hip_attention_i8_workspace": (_sz, [_pc, _pb, _ci]),
+    "vtl_hip_attention_i8_f32": (_ci, [_pc, _pb, _vp, _i64, _ci, C.c_float, _ci, _vp, _i64, _vp, _sz]),
     "vtl_hip_strerror": (C.c_char_p, [_ci]),
     "vtl_hip_last_error": (C.c_char_p, []),
     "vtl_hip_version": (C.c_char_p, []),
