@@ -150,7 +150,9 @@ class Cache:
         A score's error: q has 22 bits and is scaled in f32 (2^-22 + 2^-23 of sum |q k|), dim products are added up in f32 (dim 2^-24 of the
         same sum), and the score is rounded three times (3 2^-24 of it) and once more when the maximum is taken off (the size of both).  A weight
         is off by twice the largest such error (its own and the sum's), relatively, and by 2^-20 for the exponential, the 22 bits of the weight
-        and the scales; adding up n tokens, 8 or more at a time, costs (n / 8 + 64) 2^-24."""
+        and the scales; adding up n tokens, 8 or more at a time, costs (n / 8 + 64) 2^-24.  The weight times the value's scale is two fp16 numbers once
+        the sequence's largest scale (up to 2^6 above the tile's) is brought to 2^13 at least: fp16 has no steps below 2^-24, so each such product is off by
+        up to 2^-25 / 2^13 of that scale, and n of them, times codes of up to 127, over a sum of weights that is 1 at least, by n 127 2^-38 of it."""
         out = np.zeros((q.shape[0], heads, self.dim))
         far = np.full(out.shape, 1e-30)
         group = heads // self.kv_heads
@@ -160,6 +162,7 @@ class Cache:
             if hi <= lo or n == 0:
                 continue
             k, v, there = self.tokens(b, np.arange(n))
+            finite = np.where(np.isfinite(v), np.abs(v), 0).max((0, 2))      # 127 times the largest scale, about, of each head
             k, v = k.astype(np.float64), v.astype(np.float64)
             last = np.arange(lo, hi) - hi + n if causal else np.full(hi - lo, n - 1)
             seen = there[None] & (np.arange(n)[None] <= last[:, None])
@@ -183,4 +186,5 @@ class Cache:
                     score_off = np.where(seen, size * (2.0 ** -22 + 2.0 ** -23 + self.dim * 2.0 ** -24) + 3 * 2.0 ** -24 * np.abs(s)
                                          + 2.0 ** -23 * (np.abs(s) + np.abs(top[:, None])), 0).max(1)
                     far[lo:hi, h] += (w @ np.abs(vg)) * (2 * score_off + 2.0 ** -20 + (n / 8 + 64) * 2.0 ** -24)[:, None]
+                    far[lo:hi, h] += n * 2.0 ** -38 * finite[g] * 127 / 64      # random codes come to half of 127 at least
         return out, far

@@ -58,7 +58,8 @@ def test_refused_tensors():
     assert calls(cache(), batch(), k=None)[0] == E and calls(cache(), batch(), v=None)[0] == E
     assert calls(cache(), batch(), stride=127)[:2] == [E, E]
     for more in ({"q": None}, {"out": None}, {"heads": 0}, {"heads": 3}, {"heads": -2}, {"q_stride": 255}, {"out_stride": 255},
-                 {"out": (1 << 20) + 512}):                                       # results over the queries
+                 {"out": (1 << 20) + 512},                                        # results over the queries
+                 {"ws": 20, "ws_bytes": 1 << 30}, {"ws": 16, "ws_bytes": 8}):    # not aligned, too small
         assert calls(cache(), batch(max_pages=4000, most_length=100000), **more)[2] == E, more
 
 
