@@ -151,8 +151,9 @@ class Cache:
         same sum), and the score is rounded three times (3 2^-24 of it) and once more when the maximum is taken off (the size of both).  A weight
         is off by twice the largest such error (its own and the sum's), relatively, and by 2^-20 for the exponential, the 22 bits of the weight
         and the scales; adding up n tokens, 8 or more at a time, costs (n / 8 + 64) 2^-24.  The weight times the value's scale is two fp16 numbers once
-        the sequence's largest scale (up to 2^6 above the tile's) is brought to 2^13 at least: fp16 has no steps below 2^-24, so each such product is off by
-        up to 2^-25 / 2^13 of that scale, and n of them, times codes of up to 127, over a sum of weights that is 1 at least, by n 127 2^-38 of it."""
+        the sequence's largest scale (up to 2^6 above the tile's) is brought to 2^9 at least, beside weights of up to 2^5: fp16 has no steps below 2^-24, so
+        each such product is off by up to 2^-25 / 2^9 of that scale, and n of them, times codes of up to 127, over a sum of weights that is 1 at least, by
+        n 127 2^-34 of it."""
         out = np.zeros((q.shape[0], heads, self.dim))
         far = np.full(out.shape, 1e-30)
         group = heads // self.kv_heads
@@ -186,5 +187,5 @@ class Cache:
                     score_off = np.where(seen, size * (2.0 ** -22 + 2.0 ** -23 + self.dim * 2.0 ** -24) + 3 * 2.0 ** -24 * np.abs(s)
                                          + 2.0 ** -23 * (np.abs(s) + np.abs(top[:, None])), 0).max(1)
                     far[lo:hi, h] += (w @ np.abs(vg)) * (2 * score_off + 2.0 ** -20 + (n / 8 + 64) * 2.0 ** -24)[:, None]
-                    far[lo:hi, h] += n * 2.0 ** -38 * finite[g] * 127 / 64      # random codes come to half of 127 at least
+                    far[lo:hi, h] += n * 2.0 ** -34 * finite[g] * 127 / 64      # random codes come to half of 127 at least
         return out, far

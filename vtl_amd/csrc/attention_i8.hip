@@ -200,15 +200,12 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
         const char *value_page;
         unsigned value_place;
         bool there;
+        const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
+        // Behind the last token: the last one's group, whose codes do as any, as those of page 0 where there is no page.
         auto page_for = [&](int token, unsigned &place, bool &ok) -> const char * {
-            const char *p = nullptr;
-            place = 0;
-            if (token < to)
-                p = kv_group(kv, b, (unsigned)token / 16, head, place);
-            ok = p != nullptr;
-            if (!ok)
-                place = 0;
-            return ok ? p : kv.pages;
+            const char *p = kv_group_or_any(kv, table, (unsigned)min(token, to - 1) / 16, head, place, ok);
+            ok = ok && token < to;
+            return p;
         };
         auto load_keys = [&](int j0) {
             unsigned place;
@@ -228,8 +225,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
             const char *p = value_page + kv_value_at(kv, value_place, 0);
 #pragma unroll
             for (int i = 0; i < DT / 16; i++)
-                if (16 * i < kv.padded)
-                    values[i] = *reinterpret_cast<const int4_t *>(p + (16 * i + col) * 16);
+                values[i] = *reinterpret_cast<const int4_t *>(p + ((16 * i < kv.padded ? 16 * i : 0) + col) * 16);
         };
 
         const int step = 64 * WAVES;
@@ -283,9 +279,10 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const bool is = mine < to - (4 * t + i);
-                    vs[t][i] = is ? vs[t][i] : 0.0f;
-                    most = fmaxf(most, fabsf(vs[t][i]) < INFINITY ? fabsf(vs[t][i]) : 0.0f);
+                    const bool finite = fabsf(vs[t][i]) < INFINITY;
+                    ks[t][i] = finite ? ks[t][i] : NAN;      // such a token is no number for the rows that see it, and out of the way of the others
+                    vs[t][i] = finite && mine < to - (4 * t + i) ? vs[t][i] : 0.0f;
+                    most = fmaxf(most, fabsf(vs[t][i]));
                 }
             most = max_across_32(max_across_16(most));      // the same in every lane of a column, and the columns hold the same
             const int moved = level.next(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(most))), fresh);
@@ -321,7 +318,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
                     for (int i = 0; i < 4; i++) {
                         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], unit_of[n], -off));
                         add += e;
-                        x[4 * t + i] = s[n][t][i] == -INFINITY ? 0.0f : e * vs[t][i];
+                        x[4 * t + i] = e * vs[t][i];
                     }
                 sum[n] = __builtin_fmaf(sum[n], keep, add);
                 split(x, p[n][0][0], p[n][0][1]);
@@ -334,16 +331,15 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
             // O^T: 64 tokens in two steps of 32, lane group g has 16 g + 8 step ..
 #pragma unroll
             for (int i = 0; i < DT / 16; i++)
-                if (16 * i < kv.padded)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const half8_t v = codes_to_half(values[i][2 * h], values[i][2 * h + 1]);
+                for (int h = 0; h < 2; h++) {
+                    const half8_t v = codes_to_half(values[i][2 * h], values[i][2 * h + 1]);
 #pragma unroll
-                        for (int n = 0; n < NB; n++)
+                    for (int n = 0; n < NB; n++)
 #pragma unroll
-                            for (int part = 0; part < 2; part++)
-                                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n][h][part], o[n][i], 0, 0, 0);
-                    }
+                        for (int part = 0; part < 2; part++)
+                            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n][h][part], o[n][i], 0, 0, 0);
+                }
         }
 
         // ---- the waves meet
@@ -400,35 +396,397 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
                         o[n][i] += *reinterpret_cast<const float4_t *>(&o_part[w][16 * n + col][16 * i + 4 * g]);
             __syncthreads();
         }
-        // one part, and it is the result; or the part of a split
+        // one part, and it is the result; or the part of a split: written row by row
         const bool alone = whole || chunk >= length;
+        const int64_t slot0 = ((int64_t)unit * parts.splits + split_at) * kRows;
         if (w == 0) {
 #pragma unroll
             for (int n = 0; n < NB; n++) {
-                const int row = row0 + 16 * n + col;
-                if (row >= rows)
-                    continue;
-                float *to_o;
-                float by;
-                if (alone) {
-                    to_o = out + (int64_t)(first + row / group) * out_stride + (head * group + row % group) * kv.head_dim;
-                    by = all_sum[n] == 0.0f ? 0.0f : 1.0f / all_sum[n];
-                } else {
-                    const int64_t slot = ((int64_t)unit * parts.splits + split_at) * kRows + 16 * n + col;
-                    to_o = parts.sums + slot * kv.head_dim;
-                    by = 1.0f;
-                    if (g == 0)
-                        parts.tops[slot] = float2_t{all_top[n], all_sum[n]};
+                const float by = all_sum[n] == 0.0f ? 0.0f : alone ? 1.0f / all_sum[n] : 1.0f;
+#pragma unroll
+                for (int i = 0; i < DT / 16; i++) {
+                    float4_t v;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        v[k] = all_sum[n] == 0.0f ? 0.0f : __builtin_ldexpf(o[n][i][k] * by, high - 13);
+                    *reinterpret_cast<float4_t *>(&o_part[0][16 * n + col][16 * i + 4 * g]) = v;
                 }
+                if (!alone && g == 0 && row0 + 16 * n + col < rows)
+                    parts.tops[slot0 + 16 * n + col] = float2_t{all_top[n], all_sum[n]};
+            }
+        }
+        __syncthreads();
+        for (int r = w; r < min(kRows, rows - row0); r += WAVES) {
+            const int row = row0 + r;
+            float *to_o = alone ? out + (int64_t)(first + row / group) * out_stride + (head * group + row % group) * kv.head_dim
+                                : parts.sums + (slot0 + r) * kv.head_dim;
 #pragma unroll
-                for (int i = 0; i < DT / 16; i++)
+            for (int i = 0; i < DT / 64; i++)
+                if (lane + 64 * i < kv.head_dim)
+                    to_o[lane + 64 * i] = o_part[0][r][lane + 64 * i];
+        }
+        __syncthreads();
+    }
+}
+
+// ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
+//
+// Bound by the matrix units (and nearly so by the vector units: ten operations a score, four of them the exponential).  A tile of 64 tokens is
+// made fp16 once for all waves, on its way into LDS; a tile is worked on while the next is written to the other half of LDS and the one behind
+// it is on its way from memory.  Pieces of 8 dimensions (keys) and of 8 tokens (values) lie together there, [piece][token or dimension][8], so that
+// a wave's operand is 512 consecutive bytes for each half wave.
+//
+// The sums are brought to a new maximum only where a row's has risen by more than 2^kSlack: until then its weights are up to 2^kSlack, for
+// which the values' scales leave room (2^(kSlack + 10) is below fp16's largest number).
+constexpr int kManyRows = 32;     // of a wave
+constexpr float kSlack = 5.0f;
+constexpr int kManyLevel = 9;     // the largest scale of a tile is brought to 2^9 .. 2^10
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+// What the waves of a workgroup share of a tile.
+template <int DT, int TOKENS>
+struct alignas(16) ManyTile {
+    _Float16 keys[DT / 8][TOKENS][8];
+    _Float16 values[TOKENS / 8][DT][8];
+    float key_scale[TOKENS], value_scale[TOKENS];
+    float minus[TOKENS];              // added to a token's scores: -infinity where there is none, NaN where its values' scale is no finite number
+    int marked;                   // whether there is any such
+    int level;                    // the values' scales are in units of 2^(level - kManyLevel)
+};
+
+template <int DT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, int heads, float scale,
+                                                                    int causal, float *__restrict__ out, int64_t out_stride, Parts parts)
+{
+    constexpr int T = 64 * WAVES;
+    constexpr int TOKENS = DT > 128 ? 32 : 64;             // of a tile: what the registers have room for
+    constexpr int kPieces = DT / 16 * TOKENS;              // of 16 bytes: as many of keys as of values
+    constexpr int kUnits = (kPieces + T - 1) / T;          // that a thread brings
+    constexpr bool kWhole = kPieces % T == 0;
+    constexpr int kAhead = 4;                              // operands of the first product on their way from LDS
+    // Two tiles; before them the rows of q as halves, [piece of 8 dimensions][half][row][8], and behind them the results, a row and 4 floats.
+    constexpr int kRows = kManyRows * WAVES;
+    constexpr int kPitch = DT + 4;
+    constexpr size_t kBytes = 2 * sizeof(ManyTile<DT, TOKENS>) > kRows * kPitch * sizeof(float) ? 2 * sizeof(ManyTile<DT, TOKENS>) : kRows * kPitch * sizeof(float);
+    __shared__ __align__(16) char lds[kBytes];
+    __shared__ float q_unit[kRows];
+    ManyTile<DT, TOKENS> *const tiles = reinterpret_cast<ManyTile<DT, TOKENS> *>(lds);
+
+    const int group = heads / kv.kv_heads;
+    // heads vary fastest: workgroups of one head meet in one L2 where their number is a multiple of eight; of a sequence's rows the last, which see most, go first
+    unsigned unit = blockIdx.x;
+    const unsigned both = (unsigned)kv.batch * kv.kv_heads;
+    const unsigned bh = unit % both;
+    unit /= both;
+    const int split_at = unit % (unsigned)parts.splits;
+    int tile = parts.tiles - 1 - (int)(unit / (unsigned)parts.splits);
+    const int head = bh % (unsigned)kv.kv_heads, b = bh / (unsigned)kv.kv_heads;
+    const int length = kv_length(kv, b);
+    int first, count;
+    kv_rows_of(kv, b, first, count);
+    const int rows = count * group;
+
+    for (; tile * kRows < rows; tile += parts.tiles) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));      // what follows from it is not kept in registers from one tile of rows to the next, of which there hardly is one
+        const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int col = lane & 31, h = lane >> 5;
+        const int row0 = tile * kRows + w * kManyRows;
+        const bool whole = tile >= parts.tiles;
+        if (whole && split_at)
+            break;
+        const int last_row = min((tile + 1) * kRows, rows) - 1;
+        const int seen = causal ? max(length - count + last_row / group + 1, 0) : length;
+        const int chunk = whole ? 0x7fffffc0 : chunk_of(parts, length);
+        const int from = whole ? 0 : split_at * chunk;
+        if (from >= seen && split_at)
+            break;
+        const int to = min(seen, whole ? seen : from + chunk);
+
+        // ---- a tile on its way: which page, what piece
+        int4_t keys[kUnits], values[kUnits];
+        float key_scale, value_scale;
+        bool is, first_tile = true;
+        Level level;
+        // Where there is no token, or no dimension, any codes do: q or the weight is 0 there.
+        const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
+        auto fetch = [&](int j0) {
+            const int token = min(j0 + lane % TOKENS, to - 1);
+            unsigned place;
+            const char *p = kv_group_or_any(kv, table, (unsigned)token / 16, head, place, is);
+            const unsigned slot = place * 16 + (unsigned)token % 16;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int d = 16 * i + 4 * g + k;
-                        if (d < kv.head_dim)
-                            to_o[d] = all_sum[n] == 0.0f ? 0.0f : __builtin_ldexpf(o[n][i][k] * by, high - 13);
+            for (int i = 0; i < kUnits; i++)
+                if (kWhole || tid + T * i < kPieces) {
+                    const int c = (tid + T * i) / TOKENS;
+                    keys[i] = *reinterpret_cast<const int4_t *>(p + kv_key_at(kv, 16 * c < kv.padded ? c : 0, slot));
+                }
+            if (w == 0) {
+                const float *scales = reinterpret_cast<const float *>(p + kv_scales_at(kv)) + slot;
+                is = is && j0 + lane % TOKENS < to;
+                key_scale = scales[0];
+                value_scale = scales[kv.page_size];
+            }
+#pragma unroll
+            for (int i = 0; i < kUnits; i++)
+                if (kWhole || tid + T * i < kPieces) {
+                    const int g = (tid + T * i) / DT, d = (tid + T * i) % DT;
+                    const int of = (min(j0 + 16 * (DT % 64 ? g : __builtin_amdgcn_readfirstlane(g)), to - 1)) / 16;
+                    bool any;
+                    p = kv_group_or_any(kv, table, (unsigned)of, head, place, any);
+                    values[i] = *reinterpret_cast<const int4_t *>(p + kv_value_at(kv, place, d < kv.padded ? d : 0));
+                }
+        };
+        auto store = [&](ManyTile<DT, TOKENS> &t) {
+#pragma unroll
+            for (int i = 0; i < kUnits; i++) {
+                if (kWhole || tid + T * i < kPieces) {
+                    const int c = (tid + T * i) / TOKENS, token = lane % TOKENS;
+                    *reinterpret_cast<half8_t *>(&t.keys[2 * c][token][0]) = codes_to_half(keys[i][0], keys[i][1]);
+                    *reinterpret_cast<half8_t *>(&t.keys[2 * c + 1][token][0]) = codes_to_half(keys[i][2], keys[i][3]);
+                }
+                if (kWhole || tid + T * i < kPieces) {
+                    const int g = (tid + T * i) / DT, d = (tid + T * i) % DT;
+                    *reinterpret_cast<half8_t *>(&t.values[2 * g][d][0]) = codes_to_half(values[i][0], values[i][1]);
+                    *reinterpret_cast<half8_t *>(&t.values[2 * g + 1][d][0]) = codes_to_half(values[i][2], values[i][3]);
+                }
+            }
+            if (w == 0) {
+                // such a value makes its token's score no number for the rows that see it, and is out of the way of the others
+                const bool finite = fabsf(value_scale) < INFINITY;
+                t.key_scale[lane % TOKENS] = is ? key_scale : 0.0f;
+                value_scale = is && finite ? value_scale : 0.0f;
+                t.minus[lane % TOKENS] = !is ? -INFINITY : finite ? 0.0f : NAN;
+                level.next(wave_max(fabsf(value_scale)), first_tile);
+                first_tile = false;
+                t.value_scale[lane % TOKENS] = __builtin_ldexpf(value_scale, kManyLevel - level.at);
+                const int marked = __any(!is || !finite);
+                if (lane == 0) {
+                    t.marked = marked;
+                    t.level = level.at;
+                }
+            }
+        };
+        if (from < to)
+            fetch(from);
+
+        // ---- this wave's rows of q as halves, by way of LDS to registers: lane `col` gets 8 dimensions of every 16 of a row
+        _Float16(*const q_half)[2][kRows][8] = reinterpret_cast<_Float16(*)[2][kRows][8]>(lds);
+        for (int r0 = 0; r0 < kManyRows; r0 += 8) {
+            float v[8][(DT + 63) / 64];
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const int at = row0 + r0 + r;
+                const float *from_q = q + (int64_t)(first + at / group) * q_stride + (head * group + at % group) * kv.head_dim;
+#pragma unroll
+                for (int i = 0; i < (DT + 63) / 64; i++)
+                    v[r][i] = at < rows && lane + 64 * i < kv.head_dim ? from_q[lane + 64 * i] : 0.0f;
+            }
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                float most = 0.0f;
+#pragma unroll
+                for (int i = 0; i < (DT + 63) / 64; i++) {
+                    v[r][i] = v[r][i] * scale * kLog2e;
+                    most = fmaxf(most, fabsf(v[r][i]));
+                }
+                const int e = exponent_of(wave_max(most)), at = w * kManyRows + r0 + r;
+#pragma unroll
+                for (int i = 0; i < (DT + 63) / 64; i++) {
+                    const int d = lane + 64 * i;
+                    const float y = __builtin_ldexpf(v[r][i], 14 - e);
+                    const _Float16 hi = (_Float16)y;
+                    if (DT % 64 == 0 || d < DT) {
+                        q_half[d / 8][0][at][d % 8] = hi;
+                        q_half[d / 8][1][at][d % 8] = (_Float16)(y - (float)hi);
+                    }
+                }
+                if (lane == 0)
+                    q_unit[at] = __builtin_ldexpf(1.0f, e - 14);
+            }
+        }
+        __syncthreads();
+        half8_t x[DT / 16][2];
+#pragma unroll
+        for (int i = 0; i < DT / 16; i++)
+#pragma unroll
+            for (int part = 0; part < 2; part++)
+                x[i][part] = *reinterpret_cast<const half8_t *>(&q_half[2 * i + h][part][w * kManyRows + col][0]);
+        const float unit_of = q_unit[w * kManyRows + col];
+        __syncthreads();
+
+        const int row = min(row0 + col, rows - 1);
+        const int limit = causal ? min(length - count + row / group + 1, to) : to;
+        // tokens that all rows of the wave see, and that any does
+        const int all_see = causal ? min(length - count + row0 / group + 1, to) : to;
+        const int any_sees = row0 >= rows ? 0 : causal ? min(length - count + min(row0 + kManyRows - 1, rows - 1) / group + 1, to) : to;
+
+        float top = -INFINITY, sum = 0.0f;
+        float16_t o[DT / 32];
+#pragma unroll
+        for (int i = 0; i < DT / 32; i++)
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                o[i][k] = 0.0f;
+        int level_at = 0;
+        bool fresh = true;
+
+        if (from < to) {
+            store(tiles[0]);
+            if (from + TOKENS < to)
+                fetch(from + TOKENS);
+        }
+        int which = 0;
+        for (int j0 = from; j0 < to; j0 += TOKENS, which ^= 1) {
+            __syncthreads();
+            const ManyTile<DT, TOKENS> &t = tiles[which];
+            const bool mine = j0 < any_sees;
+            float16_t s[TOKENS / 32];
+            if (mine) {
+                // row r of a product is the token with bits 2 and 3 of r exchanged: a lane then has 8 consecutive tokens for a step of the second product
+                const int token = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
+                half8_t k[kAhead][TOKENS / 32];
+                auto operand = [&](int d) {
+#pragma unroll
+                    for (int i = 0; i < TOKENS / 32; i++)
+                        k[d % kAhead][i] = *reinterpret_cast<const half8_t *>(&t.keys[2 * d + h][32 * i + token][0]);
+                };
+#pragma unroll
+                for (int d = 0; d < kAhead - 1; d++)
+                    operand(d);
+#pragma unroll
+                for (int d = 0; d < DT / 16; d++) {
+                    if (d + kAhead - 1 < DT / 16)
+                        operand(d + kAhead - 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int part = 0; part < 2; part++)
+#pragma unroll
+                        for (int i = 0; i < TOKENS / 32; i++)
+                            s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[d % kAhead][i], x[d][part], d || part ? s[i] : float16_t{}, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (j0 + TOKENS < to)
+                store(tiles[which ^ 1]);
+            if (j0 + 2 * TOKENS < to)
+                fetch(j0 + 2 * TOKENS);
+            if (!mine)
+                continue;
+
+            // value k of block i is token 32 i + 16 (k / 8) + 8 h + k % 8
+            float best = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < TOKENS / 32; i++)
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    const float4_t ks = *reinterpret_cast<const float4_t *>(&t.key_scale[32 * i + 16 * (k / 8) + 8 * h + k % 8]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s[i][k + j] *= ks[j];
+                }
+            if (j0 + TOKENS > all_see || t.marked) {
+                const int until = limit - j0 - 8 * h;
+#pragma unroll
+                for (int i = 0; i < TOKENS / 32; i++)
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4) {
+                        const int at = 32 * i + 16 * (k / 8) + k % 8;
+                        const float4_t minus = *reinterpret_cast<const float4_t *>(&t.minus[at + 8 * h]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            s[i][k + j] = at + j < until ? s[i][k + j] + minus[j] : -INFINITY;
                     }
             }
+#pragma unroll
+            for (int i = 0; i < TOKENS / 32; i++)
+#pragma unroll
+                for (int k = 0; k < 16; k++)
+                    best = fmaxf(best, s[i][k]);
+            best = max_across_32(best) * unit_of;
+            const int moved = fresh ? 0 : level_at - t.level;
+            level_at = t.level;
+            if (__any(best > top + kSlack) || fresh || moved) {
+                const float now = best > top + kSlack || fresh ? fmaxf(top, best) : top;
+                const float keep = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+                top = now;
+                sum *= keep;
+                const float by = __builtin_ldexpf(keep, moved);
+#pragma unroll
+                for (int i = 0; i < DT / 32; i++)
+                    o[i] *= by;
+                fresh = false;
+            }
+            const float off = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int i = 0; i < TOKENS / 32; i++) {
+                half8_t p[2][2];
+                float add = 0.0f;
+#pragma unroll
+                for (int k8 = 0; k8 < 2; k8++) {
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        v[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][8 * k8 + k], unit_of, -off));
+                        add += v[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k += 4) {
+                        const float4_t vs = *reinterpret_cast<const float4_t *>(&t.value_scale[32 * i + 16 * k8 + 8 * h + k]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            v[k + j] *= vs[j];
+                    }
+                    split(v, p[k8][0], p[k8][1]);
+                }
+                sum += add;
+#pragma unroll
+                for (int k8 = 0; k8 < 2; k8++) {
+                    half8_t v[DT / 32];
+#pragma unroll
+                    for (int c = 0; c < DT / 32; c++)
+                        v[c] = *reinterpret_cast<const half8_t *>(&t.values[4 * i + 2 * k8 + h][32 * c + col][0]);
+#pragma unroll
+                    for (int part = 0; part < 2; part++)
+#pragma unroll
+                        for (int c = 0; c < DT / 32; c++)
+                            o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c], p[k8][part], o[c], 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads();      // the next tile of rows writes where this one reads
+
+        sum += __shfl_xor(sum, 32);
+        const bool alone = whole || chunk >= length;
+        // results by way of LDS, so that rows are written whole
+        float(*const result)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds) + w * kManyRows;
+        const float by = sum == 0.0f ? 0.0f : alone ? 1.0f / sum : 1.0f;
+#pragma unroll
+        for (int i = 0; i < DT / 32; i++)
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+                float4_t v;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    v[j] = sum == 0.0f ? 0.0f : __builtin_ldexpf(o[i][k + j] * by, level_at - kManyLevel);
+                *reinterpret_cast<float4_t *>(&result[col][32 * i + 2 * k + 4 * h]) = v;
+            }
+        const int64_t slot0 = (((int64_t)bh * parts.tiles + tile) * parts.splits + split_at) * kRows + w * kManyRows;
+        if (!alone && h == 0 && row0 + col < rows)
+            parts.tops[slot0 + col] = float2_t{top, sum};
+        __syncthreads();
+#pragma unroll 4
+        for (int r = 0; r < kManyRows; r++) {
+            const int at = row0 + r;
+            if (at >= rows)
+                break;
+            float *to_o = alone ? out + (int64_t)(first + at / group) * out_stride + (head * group + at % group) * kv.head_dim
+                                : parts.sums + (slot0 + r) * kv.head_dim;
+#pragma unroll
+            for (int i = 0; i < (DT + 63) / 64; i++)
+                if (lane + 64 * i < kv.head_dim)
+                    to_o[lane + 64 * i] = result[r][lane + 64 * i];
         }
         __syncthreads();
     }
@@ -483,6 +841,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Kv kv, int heads, i
 
 // How a call is cut: rows in tiles, tokens in splits.
 struct Plan {
+    bool many;
     int tile_rows, tiles, splits, chunk;
     int64_t units;      // (sequence, key/value head, tile)
     size_t sums_bytes, tops_bytes;
@@ -493,16 +852,17 @@ Plan plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads)
 {
     Plan p{};
     const int64_t most_rows = kv.starts ? (b.most_rows ? std::min(b.most_rows, kv.rows) : kv.rows) : 1;
-    const int64_t most_length = b.most_length ? std::min(b.most_length, kv.most_tokens) : kv.most_tokens;
+    const int64_t most_length = std::max(b.most_length ? std::min(b.most_length, kv.most_tokens) : kv.most_tokens, 1);
     const int64_t rows = most_rows * (heads / kv.kv_heads);
-    p.tile_rows = rows <= 16 || kv.padded > 128 ? 16 : 32;
+    p.many = rows > (kv.padded > 128 ? 16 : 32);
+    p.tile_rows = p.many ? kManyRows * 4 : rows <= 16 ? 16 : 32;
     p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     p.units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
-    const int64_t wanted = std::max<int64_t>(1, 1024 / p.units);
-    p.splits = (int)std::min(wanted, (most_length + 511) / 512);
-    p.splits = std::max(p.splits, 1);
-    p.chunk = (int)((((most_length + p.splits - 1) / p.splits) + 511) / 512 * 512);
-    p.splits = (int)std::max<int64_t>(1, (most_length + p.chunk - 1) / p.chunk);
+    const int64_t wanted = std::max<int64_t>(1, (p.many ? 512 : 1024) / p.units);
+    const int least = p.many ? 256 : 512;
+    p.splits = (int)std::min(wanted, (most_length + least - 1) / least);
+    p.chunk = (int)((((most_length + p.splits - 1) / p.splits) + least - 1) / least * least);
+    p.splits = (int)((most_length + p.chunk - 1) / p.chunk);
     if (p.splits > 1) {
         const size_t rows_in = (size_t)p.units * p.splits * p.tile_rows;
         p.sums_bytes = (rows_in * kv.head_dim * sizeof(float) + 255) & ~(size_t)255;
@@ -511,12 +871,44 @@ Plan plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads)
     return p;
 }
 
+// The arguments that both kernels share.
+struct Call {
+    Kv kv;
+    const float *q;
+    int64_t q_stride;
+    int heads;
+    float scale;
+    int causal;
+    float *out;
+    int64_t out_stride;
+    Parts parts;
+    unsigned blocks;
+};
+
 template <int DT, int NB, int WAVES>
-void launch_few(const Kv &kv, const float *q, int64_t q_stride, int heads, float scale, int causal, float *out, int64_t out_stride,
-                const Parts &parts, unsigned blocks)
+int launch_few(const Call &c)
 {
-    hipLaunchKernelGGL((attention_few_kernel<DT, NB, WAVES>), dim3(blocks), dim3(64 * WAVES), 0, current_stream(), kv, q, q_stride, heads, scale, causal,
-                       out, out_stride, parts);
+    hipLaunchKernelGGL((attention_few_kernel<DT, NB, WAVES>), dim3(c.blocks), dim3(64 * WAVES), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale,
+                       c.causal, c.out, c.out_stride, c.parts);
+    return check_launch("attention_few_kernel");
+}
+
+template <int DT>
+int launch_many(const Call &c)
+{
+    hipLaunchKernelGGL((attention_many_kernel<DT, 4>), dim3(c.blocks), dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale, c.causal,
+                       c.out, c.out_stride, c.parts);
+    return check_launch("attention_many_kernel");
+}
+
+int launch_attention(const Call &c, const Plan &plan)
+{
+    const int padded = c.kv.padded;
+    if (plan.many)
+        return padded <= 64 ? launch_many<64>(c) : padded <= 96 ? launch_many<96>(c) : padded <= 128 ? launch_many<128>(c) : launch_many<256>(c);
+    if (plan.tile_rows == 16)
+        return padded <= 64 ? launch_few<64, 1, 8>(c) : padded <= 128 ? launch_few<128, 1, 8>(c) : launch_few<256, 1, 4>(c);
+    return padded <= 64 ? launch_few<64, 2, 8>(c) : launch_few<128, 2, 4>(c);
 }
 
 bool attention_sizes_ok(const Kv &kv, int heads) { return heads >= 1 && heads % kv.kv_heads == 0; }
@@ -561,21 +953,8 @@ int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_bat
         parts.sums = static_cast<float *>(workspace);
         parts.tops = reinterpret_cast<float2_t *>(static_cast<char *>(workspace) + plan.sums_bytes);
     }
-    const unsigned blocks = (unsigned)(plan.units * plan.splits);
-    if (kv.padded <= 64) {
-        if (plan.tile_rows == 16)
-            launch_few<64, 1, 8>(kv, q, q_stride, heads, scale, causal, out, out_stride, parts, blocks);
-        else
-            launch_few<64, 2, 8>(kv, q, q_stride, heads, scale, causal, out, out_stride, parts, blocks);
-    } else if (kv.padded <= 128) {
-        if (plan.tile_rows == 16)
-            launch_few<128, 1, 8>(kv, q, q_stride, heads, scale, causal, out, out_stride, parts, blocks);
-        else
-            launch_few<128, 2, 4>(kv, q, q_stride, heads, scale, causal, out, out_stride, parts, blocks);
-    } else {
-        launch_few<256, 1, 4>(kv, q, q_stride, heads, scale, causal, out, out_stride, parts, blocks);
-    }
-    const int launched = check_launch("attention_few_kernel");
+    const Call call{kv, q, q_stride, heads, scale, causal, out, out_stride, parts, (unsigned)(plan.units * plan.splits)};
+    const int launched = launch_attention(call, plan);
     if (launched != VTL_HIP_OK || plan.splits == 1)
         return launched;
     hipLaunchKernelGGL(attention_join_kernel, dim3((unsigned)((row_heads + 3) / 4)), dim3(256), 0, current_stream(), kv, heads, causal, out, out_stride,

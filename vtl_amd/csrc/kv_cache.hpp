@@ -98,6 +98,16 @@ __device__ __forceinline__ char *kv_group(const Kv &kv, int b, unsigned g, int h
     return kv.pages + ((int64_t)page * kv.kv_heads + head) * kv.head_bytes;
 }
 
+// The same without a way around the loads, for a group that the sequence has (its page may be none): where there is no page, page 0.
+__device__ __forceinline__ const char *kv_group_or_any(const Kv &kv, const int32_t *table, unsigned g, int head, unsigned &at, bool &there)
+{
+    const unsigned p = kv_page_of(kv, g);
+    at = g - p * kv.page_groups;
+    const int page = table[p];
+    there = (unsigned)page < (unsigned)kv.num_pages;
+    return kv.pages + ((int64_t)(there ? page : 0) * kv.kv_heads + head) * kv.head_bytes;
+}
+
 // Where things are in one head of a page.
 __device__ __forceinline__ unsigned kv_key_at(const Kv &kv, unsigned dim16, unsigned slot) { return (dim16 * kv.page_size + slot) * 16u; }
 __device__ __forceinline__ unsigned kv_value_at(const Kv &kv, unsigned group, unsigned dim)
