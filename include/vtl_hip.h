@@ -303,7 +303,7 @@ int vtl_hip_linear_backward_host_f64(const double *grad, const double *x, const 
  *   scales of the keys   f32 [P],
  *   scales of the values f32 [P]:
  * the order in which the matrix units take both.  page_size is a multiple of 16 up to 4096, head_dim 1 to
- * 256; `pages` (device memory, 16-byte aligned) need not be initialised.  The library keeps nothing about a cache. */
+ * 256, a page has less than 4 GiB; `pages` (device memory, 16-byte aligned) need not be initialised.  The library keeps nothing about a cache. */
 typedef struct {
     void *pages;
     int num_pages, page_size;

@@ -5,8 +5,8 @@
 // The codes K and V are whole numbers below 128, which fp16 holds exactly, so both products run on the fp16 matrix units with f32 sums.  What
 // meets them is no whole number: q (with scale and log2 e) and w_j sv_j, two halves of 11 bits each, hi = f16(x), lo = f16(x - hi), one product
 // for each.  So 22 bits of the operands enter, where one half alone would leave an error of 2^-11, and a third would cost half as much again.
-// Rows of q are scaled by a power of two to a largest value between 2^14 and 2^15; the values' scales of a tile likewise (`Level`): lo keeps
-// its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.
+// q is scaled by a power of two to a largest value between 2^14 and 2^15 (the rows of a workgroup that shares tiles by one, else each row by its
+// own); the values' scales of a tile likewise (`Level`): lo keeps its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.
 //
 // One pass over the tokens, with the running maximum and sum of the softmax, in powers of two.  Products are transposed, tokens as the
 // rows of S^T = K Q^T and dimensions as those of O^T = V^T W^T: a lane then holds what belongs to one row of q, maximum and sum are taken within the
@@ -41,6 +41,20 @@ __device__ __forceinline__ half8_t codes_to_half(int a, int b)
     return r.h - (_Float16)1152.0f;
 }
 
+// The two halves of two numbers, as elements 2 i and 2 i + 1 of each: one product with each half is one with 22 bits.
+__device__ __forceinline__ void split_two(float x, float y, half8_t &hi, half8_t &lo, int i)
+{
+    unsigned minus = 0xbc00;      // -1, unknown to the compiler (see split)
+    asm("" : "+s"(minus));
+    const float one = (float)__builtin_bit_cast(half2_t, minus)[0];
+    const half2_t a = __builtin_convertvector((float2_t{x, y}), half2_t);
+    const half2_t b = __builtin_convertvector((float2_t{__builtin_fmaf((float)a[0], one, x), __builtin_fmaf((float)a[1], one, y)}), half2_t);
+    hi[2 * i] = a[0];
+    hi[2 * i + 1] = a[1];
+    lo[2 * i] = b[0];
+    lo[2 * i + 1] = b[1];
+}
+
 // The two halves of eight numbers.
 __device__ __forceinline__ void split(const float *x, half8_t &hi, half8_t &lo)
 {
@@ -48,10 +62,14 @@ __device__ __forceinline__ void split(const float *x, half8_t &hi, half8_t &lo)
         half2_t p[4];
         half8_t h;
     } a, b;
+    // x - f32(hi) in one instruction, which multiplies a half and adds an f32; a -1 that the compiler sees it would make two of
+    unsigned minus = 0xbc00;
+    asm("" : "+s"(minus));
+    const float one = (float)__builtin_bit_cast(half2_t, minus)[0];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         a.p[i] = __builtin_convertvector((float2_t{x[2 * i], x[2 * i + 1]}), half2_t);
-        b.p[i] = __builtin_convertvector((float2_t{__builtin_fmaf((float)a.p[i][0], -1.0f, x[2 * i]), __builtin_fmaf((float)a.p[i][1], -1.0f, x[2 * i + 1])}),
+        b.p[i] = __builtin_convertvector((float2_t{__builtin_fmaf((float)a.p[i][0], one, x[2 * i]), __builtin_fmaf((float)a.p[i][1], one, x[2 * i + 1])}),
                                          half2_t);
     }
     hi = a.h;
@@ -62,6 +80,16 @@ __device__ __forceinline__ float max_across_16(float v)
 {
     const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float sum_across_16(float v)
+{
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float sum_across_32(float v)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 __device__ __forceinline__ float max_across_32(float v)
 {
@@ -134,9 +162,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
     int tile = unit % (unsigned)parts.tiles;
     const int head = (unit / (unsigned)parts.tiles) % (unsigned)kv.kv_heads;
     const int b = unit / (unsigned)parts.tiles / (unsigned)kv.kv_heads;
-    const int length = kv_length(kv, b);
-    int first, count;
-    kv_rows_of(kv, b, first, count);
+    int length, first, count;
+    kv_sequence(kv, b, length, first, count);
     const int rows = count * group;      // the host has checked that all rows of all heads are below 2^31
 
     for (; tile * kRows < rows; tile += parts.tiles) {
@@ -201,9 +228,10 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
         unsigned value_place;
         bool there;
         const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
+        const char *const first_page = kv.pages + (uint64_t)head * kv.head_bytes;
         // Behind the last token: the last one's group, whose codes do as any, as those of page 0 where there is no page.
         auto page_for = [&](int token, unsigned &place, bool &ok) -> const char * {
-            const char *p = kv_group_or_any(kv, table, (unsigned)min(token, to - 1) / 16, head, place, ok);
+            const char *p = kv_group_or_any(kv, table, (unsigned)min(token, to - 1) / 16, first_page, place, ok);
             ok = ok && token < to;
             return p;
         };
@@ -347,8 +375,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
             level_part[w] = fresh ? -1000 : level.at;
 #pragma unroll
         for (int n = 0; n < NB; n++) {
-            sum[n] += __shfl_xor(sum[n], 16);
-            sum[n] += __shfl_xor(sum[n], 32);
+            sum[n] = sum_across_32(sum_across_16(sum[n]));
             if (g == 0) {
                 top_part[w][16 * n + col] = top[n];
                 sum_part[w][16 * n + col] = sum[n];
@@ -455,6 +482,9 @@ struct alignas(16) ManyTile {
     int level;                    // the values' scales are in units of 2^(level - kManyLevel)
 };
 
+// What __builtin_amdgcn_sched_group_barrier calls them.
+constexpr int kSchedVector = 0x2, kSchedProduct = 0x8, kSchedRead = 0x100;
+
 template <int DT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, int heads, float scale,
                                                                     int causal, float *__restrict__ out, int64_t out_stride, Parts parts)
@@ -464,14 +494,17 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     constexpr int kPieces = DT / 16 * TOKENS;              // of 16 bytes: as many of keys as of values
     constexpr int kUnits = (kPieces + T - 1) / T;          // that a thread brings
     constexpr bool kWhole = kPieces % T == 0;
-    constexpr int kAhead = 4;                              // operands of the first product on their way from LDS
-    // Two tiles; before them the rows of q as halves, [piece of 8 dimensions][half][row][8], and behind them the results, a row and 4 floats.
+    constexpr int kBlocks = TOKENS / 32, kSteps = TOKENS / 16;
+    // Two tiles, in arrays of their own so that the compiler knows which of them is read and which written.  Before them each wave's rows of q as
+    // halves, [piece of 8 dimensions][half][row][8], and behind them its results, a row and 4 floats: half of the waves in either.
+    typedef ManyTile<DT, TOKENS> Tile;
     constexpr int kRows = kManyRows * WAVES;
     constexpr int kPitch = DT + 4;
-    constexpr size_t kBytes = 2 * sizeof(ManyTile<DT, TOKENS>) > kRows * kPitch * sizeof(float) ? 2 * sizeof(ManyTile<DT, TOKENS>) : kRows * kPitch * sizeof(float);
-    __shared__ __align__(16) char lds[kBytes];
-    __shared__ float q_unit[kRows];
-    ManyTile<DT, TOKENS> *const tiles = reinterpret_cast<ManyTile<DT, TOKENS> *>(lds);
+    constexpr size_t kWaveBytes = kManyRows * kPitch * sizeof(float);
+    constexpr size_t kBytes = sizeof(Tile) > WAVES / 2 * kWaveBytes ? sizeof(Tile) : WAVES / 2 * kWaveBytes;
+    __shared__ __align__(16) char lds_even[kBytes], lds_odd[kBytes];
+    __shared__ float q_most[WAVES];
+    Tile &even = *reinterpret_cast<Tile *>(lds_even), &odd = *reinterpret_cast<Tile *>(lds_odd);
 
     const int group = heads / kv.kv_heads;
     // heads vary fastest: workgroups of one head meet in one L2 where their number is a multiple of eight; of a sequence's rows the last, which see most, go first
@@ -482,9 +515,8 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     const int split_at = unit % (unsigned)parts.splits;
     int tile = parts.tiles - 1 - (int)(unit / (unsigned)parts.splits);
     const int head = bh % (unsigned)kv.kv_heads, b = bh / (unsigned)kv.kv_heads;
-    const int length = kv_length(kv, b);
-    int first, count;
-    kv_rows_of(kv, b, first, count);
+    int length, first, count;
+    kv_sequence(kv, b, length, first, count);
     const int rows = count * group;
 
     for (; tile * kRows < rows; tile += parts.tiles) {
@@ -509,53 +541,67 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         float key_scale, value_scale;
         bool is, first_tile = true;
         Level level;
+        int unit_at;      // q is in units of 2^unit_at, which the keys' scales make up for
         // Where there is no token, or no dimension, any codes do: q or the weight is 0 there.
         const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
+        const char *const first_page = kv.pages + (uint64_t)head * kv.head_bytes;
+        int key_page, value_page[kUnits];      // looked up a tile before they are needed
+        auto key_token = [&](int j0) { return (unsigned)min(j0 + lane % TOKENS, to - 1); };
+        auto value_group = [&](int j0, int i) { return (unsigned)min(j0 + 16 * ((tid + T * i) / DT), to - 1) / 16; };
+        auto look_up = [&](int j0) {
+            key_page = table[kv_page_of(kv, key_token(j0) / 16)];
+#pragma unroll
+            for (int i = 0; i < kUnits; i++)
+                if (kWhole || tid + T * i < kPieces)
+                    value_page[i] = table[kv_page_of(kv, value_group(j0, i))];
+        };
         auto fetch = [&](int j0) {
-            const int token = min(j0 + lane % TOKENS, to - 1);
-            unsigned place;
-            const char *p = kv_group_or_any(kv, table, (unsigned)token / 16, head, place, is);
-            const unsigned slot = place * 16 + (unsigned)token % 16;
+            const unsigned token = key_token(j0), slot = token - kv_page_of(kv, token / 16) * kv.page_size;
+            const char *p = kv_page_or_any(kv, key_page, first_page, is);
 #pragma unroll
             for (int i = 0; i < kUnits; i++)
                 if (kWhole || tid + T * i < kPieces) {
                     const int c = (tid + T * i) / TOKENS;
                     keys[i] = *reinterpret_cast<const int4_t *>(p + kv_key_at(kv, 16 * c < kv.padded ? c : 0, slot));
                 }
-            if (w == 0) {
-                const float *scales = reinterpret_cast<const float *>(p + kv_scales_at(kv)) + slot;
-                is = is && j0 + lane % TOKENS < to;
-                key_scale = scales[0];
-                value_scale = scales[kv.page_size];
-            }
+            const float *scales = reinterpret_cast<const float *>(p + kv_scales_at(kv)) + slot;
+            is = is && j0 + lane % TOKENS < to;
+            key_scale = scales[0];
+            value_scale = scales[kv.page_size];
 #pragma unroll
             for (int i = 0; i < kUnits; i++)
                 if (kWhole || tid + T * i < kPieces) {
-                    const int g = (tid + T * i) / DT, d = (tid + T * i) % DT;
-                    const int of = (min(j0 + 16 * (DT % 64 ? g : __builtin_amdgcn_readfirstlane(g)), to - 1)) / 16;
+                    const int d = (tid + T * i) % DT;
+                    const unsigned g = value_group(j0, i), place = g - kv_page_of(kv, g) * kv.page_groups;
                     bool any;
-                    p = kv_group_or_any(kv, table, (unsigned)of, head, place, any);
+                    p = kv_page_or_any(kv, value_page[i], first_page, any);
                     values[i] = *reinterpret_cast<const int4_t *>(p + kv_value_at(kv, place, d < kv.padded ? d : 0));
                 }
         };
-        auto store = [&](ManyTile<DT, TOKENS> &t) {
-#pragma unroll
-            for (int i = 0; i < kUnits; i++) {
-                if (kWhole || tid + T * i < kPieces) {
-                    const int c = (tid + T * i) / TOKENS, token = lane % TOKENS;
-                    *reinterpret_cast<half8_t *>(&t.keys[2 * c][token][0]) = codes_to_half(keys[i][0], keys[i][1]);
-                    *reinterpret_cast<half8_t *>(&t.keys[2 * c + 1][token][0]) = codes_to_half(keys[i][2], keys[i][3]);
-                }
-                if (kWhole || tid + T * i < kPieces) {
+        // half `part` of the codes of a thread's piece i, of keys or values
+        auto store_part = [&](Tile &t, int i, int of_values, int part) {
+            if (kWhole || tid + T * i < kPieces) {
+                const int4_t &codes = of_values ? values[i] : keys[i];
+                const half8_t eight = codes_to_half(codes[2 * part], codes[2 * part + 1]);
+                if (of_values) {
                     const int g = (tid + T * i) / DT, d = (tid + T * i) % DT;
-                    *reinterpret_cast<half8_t *>(&t.values[2 * g][d][0]) = codes_to_half(values[i][0], values[i][1]);
-                    *reinterpret_cast<half8_t *>(&t.values[2 * g + 1][d][0]) = codes_to_half(values[i][2], values[i][3]);
+                    *reinterpret_cast<half8_t *>(&t.values[2 * g + part][d][0]) = eight;
+                } else {
+                    const int c = (tid + T * i) / TOKENS, token = lane % TOKENS;
+                    *reinterpret_cast<half8_t *>(&t.keys[2 * c + part][token][0]) = eight;
                 }
             }
-            if (w == 0) {
+        };
+        auto store = [&](Tile &t) {
+#pragma unroll
+            for (int i = 0; i < 4 * kUnits; i++)
+                store_part(t, i / 4, i / 2 % 2, i % 2);
+        };
+        auto store_scales = [&](Tile &t) {
+            {
                 // such a value makes its token's score no number for the rows that see it, and is out of the way of the others
                 const bool finite = fabsf(value_scale) < INFINITY;
-                t.key_scale[lane % TOKENS] = is ? key_scale : 0.0f;
+                t.key_scale[lane % TOKENS] = is ? __builtin_ldexpf(key_scale, unit_at) : 0.0f;
                 value_scale = is && finite ? value_scale : 0.0f;
                 t.minus[lane % TOKENS] = !is ? -INFINITY : finite ? 0.0f : NAN;
                 level.next(wave_max(fabsf(value_scale)), first_tile);
@@ -568,43 +614,57 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 }
             }
         };
-        if (from < to)
+        if (from < to) {
+            look_up(from);
             fetch(from);
+            look_up(from + TOKENS);
+        }
 
-        // ---- this wave's rows of q as halves, by way of LDS to registers: lane `col` gets 8 dimensions of every 16 of a row
-        _Float16(*const q_half)[2][kRows][8] = reinterpret_cast<_Float16(*)[2][kRows][8]>(lds);
-        for (int r0 = 0; r0 < kManyRows; r0 += 8) {
-            float v[8][(DT + 63) / 64];
+        // ---- rows of q as halves, all in one unit, by way of LDS to registers: lane `col` gets 8 dimensions of every 16 of a row
+        char *const own = (w < WAVES / 2 ? lds_even : lds_odd) + w % (WAVES / 2) * kWaveBytes;
+        _Float16(*const q_half)[2][kManyRows][8] = reinterpret_cast<_Float16(*)[2][kManyRows][8]>(own);
+        {
+            float v[kManyRows][(DT + 63) / 64], most = 0.0f;
+            int in_group = row0 % group;
+            const float *from_q = q + (int64_t)(first + row0 / group) * q_stride + (head * group + in_group) * kv.head_dim;
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const int at = row0 + r0 + r;
-                const float *from_q = q + (int64_t)(first + at / group) * q_stride + (head * group + at % group) * kv.head_dim;
+            for (int r = 0; r < kManyRows; r++) {
 #pragma unroll
-                for (int i = 0; i < (DT + 63) / 64; i++)
-                    v[r][i] = at < rows && lane + 64 * i < kv.head_dim ? from_q[lane + 64 * i] : 0.0f;
+                for (int i = 0; i < (DT + 63) / 64; i++) {
+                    v[r][i] = row0 + r < rows && lane + 64 * i < kv.head_dim ? from_q[lane + 64 * i] : 0.0f;
+                }
+                const bool wrap = ++in_group == group;
+                in_group = wrap ? 0 : in_group;
+                from_q += wrap ? q_stride - (int64_t)(group - 1) * kv.head_dim : kv.head_dim;
             }
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                float most = 0.0f;
+            for (int r = 0; r < kManyRows; r++)
 #pragma unroll
                 for (int i = 0; i < (DT + 63) / 64; i++) {
                     v[r][i] = v[r][i] * scale * kLog2e;
-                    most = fmaxf(most, fabsf(v[r][i]));
+                    const float size = fabsf(v[r][i]);
+                    most = fmaxf(most, size < INFINITY ? size : 0.0f);      // a row that is no number spoils no other
                 }
-                const int e = exponent_of(wave_max(most)), at = w * kManyRows + r0 + r;
+            most = wave_max(most);
+            if (lane == 0)
+                q_most[w] = most;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WAVES; i++)
+                most = fmaxf(most, q_most[i]);
+            unit_at = __builtin_amdgcn_readfirstlane(exponent_of(most)) - 14;
+#pragma unroll
+            for (int r = 0; r < kManyRows; r++)
 #pragma unroll
                 for (int i = 0; i < (DT + 63) / 64; i++) {
                     const int d = lane + 64 * i;
-                    const float y = __builtin_ldexpf(v[r][i], 14 - e);
+                    const float y = __builtin_ldexpf(v[r][i], -unit_at);
                     const _Float16 hi = (_Float16)y;
                     if (DT % 64 == 0 || d < DT) {
-                        q_half[d / 8][0][at][d % 8] = hi;
-                        q_half[d / 8][1][at][d % 8] = (_Float16)(y - (float)hi);
+                        q_half[d / 8][0][r][d % 8] = hi;
+                        q_half[d / 8][1][r][d % 8] = (_Float16)(y - (float)hi);
                     }
                 }
-                if (lane == 0)
-                    q_unit[at] = __builtin_ldexpf(1.0f, e - 14);
-            }
         }
         __syncthreads();
         half8_t x[DT / 16][2];
@@ -612,8 +672,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         for (int i = 0; i < DT / 16; i++)
 #pragma unroll
             for (int part = 0; part < 2; part++)
-                x[i][part] = *reinterpret_cast<const half8_t *>(&q_half[2 * i + h][part][w * kManyRows + col][0]);
-        const float unit_of = q_unit[w * kManyRows + col];
+                x[i][part] = *reinterpret_cast<const half8_t *>(&q_half[2 * i + h][part][col][0]);
         __syncthreads();
 
         const int row = min(row0 + col, rows - 1);
@@ -622,7 +681,9 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         const int all_see = causal ? min(length - count + row0 / group + 1, to) : to;
         const int any_sees = row0 >= rows ? 0 : causal ? min(length - count + min(row0 + kManyRows - 1, rows - 1) / group + 1, to) : to;
 
-        float top = -INFINITY, sum = 0.0f;
+        // `off` is what a row's scores are less than by 2^kSlack at most; before the row has seen a token it is so low that any score is above
+        constexpr float kNone = -0x1p100f;
+        float off = kNone, sum = 0.0f;
         float16_t o[DT / 32];
 #pragma unroll
         for (int i = 0; i < DT / 32; i++)
@@ -630,137 +691,204 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             for (int k = 0; k < 16; k++)
                 o[i][k] = 0.0f;
         int level_at = 0;
-        bool fresh = true;
 
         if (from < to) {
-            store(tiles[0]);
-            if (from + TOKENS < to)
-                fetch(from + TOKENS);
+            store(even);
+            if (w == 0)
+                store_scales(even);
+            fetch(from + TOKENS);
+            look_up(from + 2 * TOKENS);
         }
-        int which = 0;
-        for (int j0 = from; j0 < to; j0 += TOKENS, which ^= 1) {
+        auto work = [&](const Tile &t, Tile &next, int j0) {
             __syncthreads();
-            const ManyTile<DT, TOKENS> &t = tiles[which];
-            const bool mine = j0 < any_sees;
-            float16_t s[TOKENS / 32];
-            if (mine) {
-                // row r of a product is the token with bits 2 and 3 of r exchanged: a lane then has 8 consecutive tokens for a step of the second product
-                const int token = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
-                half8_t k[kAhead][TOKENS / 32];
+            if (w == 0)
+                store_scales(next);
+            if (j0 >= any_sees) {
+                store(next);
+                fetch(j0 + 2 * TOKENS);
+                look_up(j0 + 3 * TOKENS);
+                return;
+            }
+            const int marked = __builtin_amdgcn_readfirstlane(t.marked), level_here = __builtin_amdgcn_readfirstlane(t.level);
+            // S^T.  Row r of a product is the token with bits 2 and 3 of r exchanged: a lane then has 8 consecutive tokens for a step of the second
+            // product.  Value k of block i is token 32 i + 16 (k / 8) + 8 h + k % 8.
+            float16_t s[kBlocks];
+            const int token = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
+            // `beside` is what a step has beside its products; operands are a step ahead of them
+            auto products = [&](auto beside) {
+                half8_t k[2][kBlocks];
                 auto operand = [&](int d) {
 #pragma unroll
-                    for (int i = 0; i < TOKENS / 32; i++)
-                        k[d % kAhead][i] = *reinterpret_cast<const half8_t *>(&t.keys[2 * d + h][32 * i + token][0]);
+                    for (int i = 0; i < kBlocks; i++)
+                        k[d % 2][i] = *reinterpret_cast<const half8_t *>(&t.keys[2 * d + h][32 * i + token][0]);
                 };
-#pragma unroll
-                for (int d = 0; d < kAhead - 1; d++)
-                    operand(d);
+                operand(0);
 #pragma unroll
                 for (int d = 0; d < DT / 16; d++) {
-                    if (d + kAhead - 1 < DT / 16)
-                        operand(d + kAhead - 1);
                     __builtin_amdgcn_sched_barrier(0);
+                    if (d + 1 < DT / 16)
+                        operand(d + 1);
 #pragma unroll
                     for (int part = 0; part < 2; part++)
 #pragma unroll
-                        for (int i = 0; i < TOKENS / 32; i++)
-                            s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[d % kAhead][i], x[d][part], d || part ? s[i] : float16_t{}, 0, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);
+                        for (int i = 0; i < kBlocks; i++)
+                            s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[d % 2][i], x[d][part], d || part ? s[i] : float16_t{}, 0, 0, 0);
+                    beside(d);
+                    __builtin_amdgcn_sched_group_barrier(kSchedRead, kBlocks, 0);
+#pragma unroll
+                    for (int i = 0; i < 2 * kBlocks; i++) {
+                        __builtin_amdgcn_sched_group_barrier(kSchedProduct, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(kSchedVector, 3, 0);
+                    }
                 }
-            }
-            if (j0 + TOKENS < to)
-                store(tiles[which ^ 1]);
-            if (j0 + 2 * TOKENS < to)
-                fetch(j0 + 2 * TOKENS);
-            if (!mine)
-                continue;
-
-            // value k of block i is token 32 i + 16 (k / 8) + 8 h + k % 8
-            float best = -INFINITY;
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            // scores less `off`, and the largest of this lane's
+            auto exponents = [&](float less) {
 #pragma unroll
-            for (int i = 0; i < TOKENS / 32; i++)
-#pragma unroll
-                for (int k = 0; k < 16; k += 4) {
-                    const float4_t ks = *reinterpret_cast<const float4_t *>(&t.key_scale[32 * i + 16 * (k / 8) + 8 * h + k % 8]);
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        s[i][k + j] *= ks[j];
-                }
-            if (j0 + TOKENS > all_see || t.marked) {
-                const int until = limit - j0 - 8 * h;
-#pragma unroll
-                for (int i = 0; i < TOKENS / 32; i++)
+                for (int i = 0; i < kBlocks; i++)
 #pragma unroll
                     for (int k = 0; k < 16; k += 4) {
-                        const int at = 32 * i + 16 * (k / 8) + k % 8;
-                        const float4_t minus = *reinterpret_cast<const float4_t *>(&t.minus[at + 8 * h]);
+                        const float4_t ks = *reinterpret_cast<const float4_t *>(&t.key_scale[32 * i + 16 * (k / 8) + 8 * h + k % 8]);
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            s[i][k + j] = at + j < until ? s[i][k + j] + minus[j] : -INFINITY;
+                            s[i][k + j] = __builtin_fmaf(s[i][k + j], ks[j], -less);
                     }
-            }
+                if (j0 + TOKENS > all_see || marked) {
+                    const int until = limit - j0 - 8 * h;
 #pragma unroll
-            for (int i = 0; i < TOKENS / 32; i++)
+                    for (int i = 0; i < kBlocks; i++)
 #pragma unroll
-                for (int k = 0; k < 16; k++)
-                    best = fmaxf(best, s[i][k]);
-            best = max_across_32(best) * unit_of;
-            const int moved = fresh ? 0 : level_at - t.level;
-            level_at = t.level;
-            if (__any(best > top + kSlack) || fresh || moved) {
-                const float now = best > top + kSlack || fresh ? fmaxf(top, best) : top;
-                const float keep = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now);
-                top = now;
+                        for (int k = 0; k < 16; k += 4) {
+                            const int at = 32 * i + 16 * (k / 8) + k % 8;
+                            const float4_t minus = *reinterpret_cast<const float4_t *>(&t.minus[at + 8 * h]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                s[i][k + j] = at + j < until ? s[i][k + j] + minus[j] : -INFINITY;
+                        }
+                }
+                float best = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        best = fmaxf(best, s[i][k]);
+                return best;
+            };
+            // with the next tile's way into LDS beside them
+            products([&](int d) {
+#pragma unroll
+                for (int i = 0; i < 4 * kUnits; i++)
+                    if (i * (DT / 16) / (4 * kUnits) == d)
+                        store_part(next, i / 4, i / 2 % 2, i % 2);
+            });
+            if (__any(exponents(off) > kSlack) || level_here != level_at) {
+                // a new maximum: the products again, as there are no registers to keep them
+                products([](int) {});
+                const float best = max_across_32(exponents(0.0f));
+                const float now = best > off + kSlack ? best : off;
+                const float keep = __builtin_amdgcn_exp2f(off - now);
+                off = now;
                 sum *= keep;
-                const float by = __builtin_ldexpf(keep, moved);
+                const float by = __builtin_ldexpf(keep, level_at - level_here);
+                level_at = level_here;
 #pragma unroll
                 for (int i = 0; i < DT / 32; i++)
                     o[i] *= by;
-                fresh = false;
+#pragma unroll
+                for (int i = 0; i < TOKENS / 32; i++)
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        s[i][k] -= now;
             }
-            const float off = top == -INFINITY ? 0.0f : top;
+            // O^T, 16 tokens a step.  Beside each product, in this order, a part of the next step's weights, and beside the last step's the loads
+            // of a later tile: a product holds the vector units' issue for half of its time, which leaves room for four operations.
+            constexpr int kSlots = DT / 16;      // products of a step
+            half8_t p[2][2], v[2][DT / 32];
+            float e[8], vs[8];
+            auto operand = [&](int step) {
 #pragma unroll
-            for (int i = 0; i < TOKENS / 32; i++) {
-                half8_t p[2][2];
-                float add = 0.0f;
+                for (int c = 0; c < DT / 32; c++)
+                    v[step % 2][c] = *reinterpret_cast<const half8_t *>(&t.values[2 * step + h][32 * c + col][0]);
+            };
+            auto scales_of = [&](int step) {
 #pragma unroll
-                for (int k8 = 0; k8 < 2; k8++) {
-                    float v[8];
+                for (int k = 0; k < 8; k += 4) {
+                    const float4_t four = *reinterpret_cast<const float4_t *>(&t.value_scale[16 * step + 8 * h + k]);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        v[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][8 * k8 + k], unit_of, -off));
-                        add += v[k];
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; k += 4) {
-                        const float4_t vs = *reinterpret_cast<const float4_t *>(&t.value_scale[32 * i + 16 * k8 + 8 * h + k]);
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            v[k + j] *= vs[j];
-                    }
-                    split(v, p[k8][0], p[k8][1]);
+                    for (int j = 0; j < 4; j++)
+                        vs[k + j] = four[j];
                 }
-                sum += add;
+            };
+            // weight k of a step: first its exponential, and one slot later (its result takes a while) the rest
+            auto raise = [&](int step, int k) { e[k] = __builtin_amdgcn_exp2f(s[step / 2][8 * (step % 2) + k]); };
+            auto weigh = [&](int step, int k) {
+                sum += e[k];
+                e[k] *= vs[k];
+                if (k % 2)
+                    split_two(e[k - 1], e[k], p[step % 2][0], p[step % 2][1], k / 2);
+            };
+            operand(0);
+            scales_of(0);
 #pragma unroll
-                for (int k8 = 0; k8 < 2; k8++) {
-                    half8_t v[DT / 32];
+            for (int k = 0; k < 8; k++)
+                raise(0, k);
 #pragma unroll
-                    for (int c = 0; c < DT / 32; c++)
-                        v[c] = *reinterpret_cast<const half8_t *>(&t.values[4 * i + 2 * k8 + h][32 * c + col][0]);
+            for (int k = 0; k < 8; k++)
+                weigh(0, k);
 #pragma unroll
-                    for (int part = 0; part < 2; part++)
+            for (int step = 0; step < kSteps; step++) {
+                const bool last = step + 1 == kSteps;
+                __builtin_amdgcn_sched_barrier(0);
+                if (!last) {
+                    operand(step + 1);
+                    scales_of(step + 1);
+                }
 #pragma unroll
-                        for (int c = 0; c < DT / 32; c++)
-                            o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c], p[k8][part], o[c], 0, 0, 0);
+                for (int slot = 0; slot < kSlots; slot++) {
+                    const int part = slot / (DT / 32), c = slot % (DT / 32);
+                    o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[step % 2][c], p[step % 2][part], o[c], 0, 0, 0);
+                    if (!last) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            if (k * kSlots / 8 == slot)
+                                raise(step + 1, k);
+                            if (k * kSlots / 8 + 1 == slot)
+                                weigh(step + 1, k);
+                        }
+                        if (slot + 1 == kSlots)
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                if (k * kSlots / 8 + 1 == kSlots)
+                                    weigh(step + 1, k);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                if (last) {
+                    int from_here = __builtin_amdgcn_readfirstlane(j0);
+                    asm volatile("" : "+s"(from_here));      // addresses are not made any earlier
+                    fetch(from_here + 2 * TOKENS);
+                    look_up(from_here + 3 * TOKENS);
+#pragma unroll
+                    for (int i = 0; i < kSlots; i++) {
+                        __builtin_amdgcn_sched_group_barrier(kSchedProduct, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(kSchedVector, 5, 0);
+                    }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        for (int j0 = from; j0 < to; j0 += 2 * TOKENS) {
+            work(even, odd, j0);
+            if (j0 + TOKENS < to)
+                work(odd, even, j0 + TOKENS);
         }
         __syncthreads();      // the next tile of rows writes where this one reads
 
-        sum += __shfl_xor(sum, 32);
+        sum = sum_across_32(sum);
         const bool alone = whole || chunk >= length;
         // results by way of LDS, so that rows are written whole
-        float(*const result)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds) + w * kManyRows;
+        float(*const result)[kPitch] = reinterpret_cast<float(*)[kPitch]>(own);
         const float by = sum == 0.0f ? 0.0f : alone ? 1.0f / sum : 1.0f;
 #pragma unroll
         for (int i = 0; i < DT / 32; i++)
@@ -774,7 +902,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             }
         const int64_t slot0 = (((int64_t)bh * parts.tiles + tile) * parts.splits + split_at) * kRows + w * kManyRows;
         if (!alone && h == 0 && row0 + col < rows)
-            parts.tops[slot0 + col] = float2_t{top, sum};
+            parts.tops[slot0 + col] = float2_t{off == kNone ? -INFINITY : off, sum};
         __syncthreads();
 #pragma unroll 4
         for (int r = 0; r < kManyRows; r++) {

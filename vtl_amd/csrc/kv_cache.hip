@@ -83,7 +83,7 @@ size_t vtl_hip_kv_cache_bytes(int num_pages, int page_size, int kv_heads, int he
         head_dim > kKvMostDim)
         return 0;
     const size_t page = (size_t)page_size * (2u * ((head_dim + 15) & ~15) + 8u) * (size_t)kv_heads;
-    if (page > ((size_t)1 << 62) / (size_t)num_pages)
+    if (page >> 32)
         return 0;
     return page * (size_t)num_pages;
 }

@@ -17,8 +17,9 @@ struct Kv {
     char *pages;
     int num_pages, page_size, kv_heads, head_dim;
     int padded;                   // head_dim rounded up to whole groups of 16
-    unsigned page_groups, magic;  // groups of 16 tokens in a page, and what divides by that (page_of)
-    unsigned head_bytes;          // of one head in one page
+    unsigned page_groups;         // groups of 16 tokens in a page
+    unsigned magic, one;          // what divides by that (kv_page_of)
+    unsigned head_bytes, page_bytes;
     const int32_t *table, *lengths, *starts;
     int batch, max_pages, rows;
     int most_tokens;              // max_pages * page_size, at most kKvMostTokens
@@ -42,8 +43,10 @@ inline int kv_sizes(const vtl_hip_kv_cache *c, const vtl_hip_kv_batch *b, Kv &kv
     kv.head_dim = c->head_dim;
     kv.padded = (c->head_dim + 15) & ~15;
     kv.page_groups = (unsigned)c->page_size / kKvGroup;
-    kv.magic = (unsigned)((((uint64_t)1 << 32) + kv.page_groups - 1) / kv.page_groups);
+    kv.magic = kv.page_groups == 1 ? 0 : (unsigned)((((uint64_t)1 << 32) + kv.page_groups - 1) / kv.page_groups);
+    kv.one = kv.page_groups == 1 ? ~0u : 0;
     kv.head_bytes = (unsigned)c->page_size * (2u * (unsigned)kv.padded + 8u);
+    kv.page_bytes = kv.head_bytes * (unsigned)c->kv_heads;
     kv.table = b->page_table;
     kv.lengths = b->lengths;
     kv.starts = b->starts;
@@ -66,10 +69,7 @@ inline size_t kv_span(const Kv &kv, int heads, int64_t stride)
 #ifdef __HIPCC__
 // Group `g` of 16 tokens is in page g / page_groups of its sequence.  Exact for g < 2^24, and so for every token below 2^28: the
 // product is off by less than g * page_groups / 2^32 <= 1 / page_groups.
-__device__ __forceinline__ unsigned kv_page_of(const Kv &kv, unsigned g)
-{
-    return kv.page_groups == 1 ? g : __umulhi(g, kv.magic);
-}
+__device__ __forceinline__ unsigned kv_page_of(const Kv &kv, unsigned g) { return __umulhi(g, kv.magic) + (g & kv.one); }
 
 __device__ __forceinline__ int kv_length(const Kv &kv, int b) { return min(max(kv.lengths[b], 0), kv.most_tokens); }
 
@@ -85,6 +85,15 @@ __device__ __forceinline__ void kv_rows_of(const Kv &kv, int b, int &first, int 
     count = max(min(max(kv.starts[b + 1], 0), kv.rows) - first, 0);
 }
 
+// The same for a sequence that the whole wave works on.
+__device__ __forceinline__ void kv_sequence(const Kv &kv, int b, int &length, int &first, int &count)
+{
+    kv_rows_of(kv, b, first, count);
+    length = __builtin_amdgcn_readfirstlane(kv_length(kv, b));
+    first = __builtin_amdgcn_readfirstlane(first);
+    count = __builtin_amdgcn_readfirstlane(count);
+}
+
 // One head of the page that group g of sequence b is in, and the group's place there; nullptr: there is no such page.
 __device__ __forceinline__ char *kv_group(const Kv &kv, int b, unsigned g, int head, unsigned &at)
 {
@@ -95,17 +104,22 @@ __device__ __forceinline__ char *kv_group(const Kv &kv, int b, unsigned g, int h
     const int page = kv.table[(int64_t)b * kv.max_pages + p];
     if ((unsigned)page >= (unsigned)kv.num_pages)
         return nullptr;
-    return kv.pages + ((int64_t)page * kv.kv_heads + head) * kv.head_bytes;
+    return kv.pages + (uint64_t)(unsigned)page * kv.page_bytes + (uint64_t)head * kv.head_bytes;
 }
 
-// The same without a way around the loads, for a group that the sequence has (its page may be none): where there is no page, page 0.
-__device__ __forceinline__ const char *kv_group_or_any(const Kv &kv, const int32_t *table, unsigned g, int head, unsigned &at, bool &there)
+// The same without a way around the loads: one head (first_page: that of page 0) of page `page`, or of page 0 where there is no such page.
+__device__ __forceinline__ const char *kv_page_or_any(const Kv &kv, int page, const char *first_page, bool &there)
+{
+    there = (unsigned)page < (unsigned)kv.num_pages;
+    return first_page + (uint64_t)(there ? (unsigned)page : 0u) * kv.page_bytes;
+}
+
+// And for a group that the sequence has (its page may be none).
+__device__ __forceinline__ const char *kv_group_or_any(const Kv &kv, const int32_t *table, unsigned g, const char *first_page, unsigned &at, bool &there)
 {
     const unsigned p = kv_page_of(kv, g);
     at = g - p * kv.page_groups;
-    const int page = table[p];
-    there = (unsigned)page < (unsigned)kv.num_pages;
-    return kv.pages + ((int64_t)(there ? page : 0) * kv.kv_heads + head) * kv.head_bytes;
+    return kv_page_or_any(kv, table[p], first_page, there);
 }
 
 // Where things are in one head of a page.
