@@ -126,7 +126,7 @@ struct Parts {
     int splits;     // of the tokens
     int chunk;      // tokens of a split; more where a sequence is longer than the host knew
     float *sums;    // [unit][split][row][head_dim]
-    float2_t *tops; // [unit][split][row]: maximum, sum of weights
+    float (*tops)[2];   // [unit][split][row]: maximum, sum of weights
 };
 
 // Tokens of a split of a sequence of which `seen` are of use.
@@ -135,73 +135,335 @@ __device__ __forceinline__ int chunk_of(const Parts &parts, int seen)
     return max(parts.chunk, ((seen + parts.splits - 1) / parts.splits + 63) & ~63);
 }
 
+// Parts of a row are made on one XCD and read on another: past the L2 caches, which are not coherent with each other.
+__device__ __forceinline__ void store_far(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float load_far(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Over each 16 lanes.
+__device__ __forceinline__ float row_max_16(float v)
+{
+#pragma unroll
+    for (int i = 1; i < 16; i *= 2)
+        v = fmaxf(v, __shfl_xor(v, i));
+    return v;
+}
+__device__ __forceinline__ float row_sum_16(float v)
+{
+#pragma unroll
+    for (int i = 1; i < 16; i *= 2)
+        v += __shfl_xor(v, i);
+    return v;
+}
+
+// One row's parts, n of them, put together by a wave: the first is at `first`, the others at `second` and on, `apart` rows from each other.
+template <int DT>
+__device__ __forceinline__ void join_row(const Kv &kv, const float *sums, const float (*tops)[2], int64_t first, int64_t second, int apart, int n, float *y)
+{
+    auto slot = [&](int i) { return i ? second + (int64_t)(i - 1) * apart : first; };
+    const int lane = threadIdx.x & 63;
+    // every lane has the maximum and the sum of a part
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = lane; i < n; i += 64)
+        top = fmaxf(top, load_far(&tops[slot(i)][0]));
+    top = max_across_32(max_across_16(row_max_16(top)));
+    const float off = top == -INFINITY ? 0.0f : top;
+    float o[DT / 64] = {};
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const int i = i0 + lane;
+        float by = 0.0f;
+        if (i < n) {
+            const float t = load_far(&tops[slot(i)][0]), v = load_far(&tops[slot(i)][1]);
+            by = v == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(t - off);
+            sum += v == 0.0f ? 0.0f : v * by;
+        }
+        const int few = min(n - i0, 64);
+        constexpr int kAtOnce = 1024 / DT;      // parts on their way from memory
+        for (int k0 = 0; k0 < few; k0 += kAtOnce) {
+            float v[kAtOnce][DT / 64];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++) {
+                const float *from = sums + slot(i0 + min(k0 + k, few - 1)) * kv.head_dim;
+#pragma unroll
+                for (int c = 0; c < DT / 64; c++)
+                    v[k][c] = lane + 64 * c < kv.head_dim ? load_far(from + lane + 64 * c) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++) {
+                const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), k0 + k));      // 0 behind the last part
+#pragma unroll
+                for (int c = 0; c < DT / 64; c++)
+                    o[c] = weight == 0.0f ? o[c] : __builtin_fmaf(v[k][c], weight, o[c]);
+            }
+        }
+    }
+    sum = sum_across_32(sum_across_16(row_sum_16(sum)));
+#pragma unroll
+    for (int c = 0; c < DT / 64; c++)
+        if (lane + 64 * c < kv.head_dim)
+            y[lane + 64 * c] = sum == 0.0f ? 0.0f : o[c] / sum;
+}
+
 // ---- few rows: a tile's rows are 16 or 32, all of a sequence's that read one key/value head ------------
 //
 // Bound by the cache's bytes (2 D + 8 a token and head): so every wave takes tiles of 64 tokens for itself, straight from memory into the registers in
-// the order in which the matrix units take them, a tile of keys on its way while the one before is worked on and its values behind it.
-// Waves of a workgroup meet once, at the end.
+// the order in which the matrix units take them; keys of the next tile are on their way while the weights of one are made, its values while the next
+// one's scores are, and the pages of both are looked up a tile before.
+//
+// A unit is a tile of rows and a key/value head; its tokens are cut into rounds, in which every wave of a workgroup has a tile of 64.  All
+// rounds of all units, behind each other, are dealt out evenly, as many workgroups as the chip takes at once: so ragged lengths cost nothing, and a
+// workgroup has parts of at most two units, its first and its last.  The workgroups that share a unit meet in the launch where
+// they have a counter: each writes its part through to memory and counts itself, and the last one adds the parts up and
+// leaves the counter at zero.  Else a launch of their own adds them up.
+constexpr int kMostShares = 512;
+__device__ unsigned g_arrived[kStreamSlots][2 * kMostShares];
+
+struct Shares {
+    int count;          // workgroups
+    int counters;       // which set of counters; -1: parts are added up by a launch of their own
+    float *sums;        // [2 count][rows of a tile][head_dim]: parts of the first unit and of the last of each workgroup
+    float (*tops)[2];   // [2 count][rows of a tile]
+};
+
+// What a workgroup has, and where others' begins: q or q + 1 rounds each.
+struct Deal {
+    int each, more;
+    __device__ __forceinline__ Deal(int total, int shares) : each(total / shares), more(total % shares) {}
+    __device__ __forceinline__ int start(int share) const { return share * each + min(share, more); }
+    __device__ __forceinline__ int of(int round) const
+    {
+        const int mark = more * (each + 1);
+        return round < mark ? round / (each + 1) : more + (round - mark) / max(each, 1);
+    }
+};
+
+// Over the lanes up to each.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int scan_step(int v)
+{
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xF, false);
+}
+__device__ __forceinline__ int scan_add(int v)
+{
+    v = scan_step<0x111, 0xF>(v);      // row_shr:1, 2, 4, 8
+    v = scan_step<0x112, 0xF>(v);
+    v = scan_step<0x114, 0xF>(v);
+    v = scan_step<0x118, 0xF>(v);
+    v = scan_step<0x142, 0xA>(v);      // row_bcast:15 into rows 1 and 3
+    return scan_step<0x143, 0xC>(v);   // row_bcast:31 into rows 2 and 3
+}
+
+// 64 sequences from `base` on, one a lane, and the rounds of all units of each: how many, and how many there are up to and with it.
+template <int ROWS, int STEP>
+struct Sequences {
+    int base, length, first, count, rounds, upto;
+    __device__ __forceinline__ Sequences(const Kv &kv, int group, int base_) : base(base_), length(0), first(0), count(0), rounds(0)
+    {
+        const int b = base + (int)(threadIdx.x & 63);
+        if (b < kv.batch) {
+            kv_rows_of(kv, b, first, count);
+            length = kv_length(kv, b);
+            rounds = (count * group + ROWS - 1) / ROWS * max((length + STEP - 1) / STEP, 1) * kv.kv_heads;
+        }
+        upto = scan_add(rounds);
+    }
+    __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(upto, 63); }
+};
+
+// The rounds of all sequences.  The host has seen to it that they are kMostRounds at most as long as `starts` ascends; where it does not, and they are
+// more than 32 bits count, there is nothing to do.
+constexpr int kMostRounds = 1 << 30;
+template <int ROWS, int STEP>
+__device__ __forceinline__ int all_rounds(const Kv &kv, int group, const Sequences<ROWS, STEP> &begin)
+{
+    int all = begin.all();
+    float size = (float)begin.rounds;
+    for (int base = 64; base < kv.batch; base += 64) {
+        const Sequences<ROWS, STEP> s(kv, group, base);
+        all += s.all();
+        size += (float)s.rounds;
+    }
+    const unsigned long long lots = __ballot(size > 1.5f * kMostRounds / 64.0f);      // of one lane's
+    if (!lots)
+        return all;
+    size = sum_across_32(sum_across_16(row_sum_16(size)));
+    return __builtin_amdgcn_readfirstlane(size > 1.5f * kMostRounds) ? 0 : all;
+}
+
+// Finds the sequences whose rounds a workgroup has, one behind the other.
+template <int ROWS, int STEP>
+struct Finder {
+    Sequences<ROWS, STEP> in;
+    int before;      // the rounds of all before in.base
+    __device__ __forceinline__ Finder(const Sequences<ROWS, STEP> &begin) : in(begin), before(0) {}
+    // The lane that has the sequence of `round`.
+    __device__ __forceinline__ int lane_of(const Kv &kv, int group, int round)
+    {
+        for (;;) {
+            const unsigned long long past = __ballot(before + in.upto > round);
+            if (past)
+                return __builtin_ctzll(past);
+            if (in.base + 64 >= kv.batch)
+                return 63;      // not reached: the rounds of all sequences are more
+            before += in.all();
+            in = Sequences<ROWS, STEP>(kv, group, in.base + 64);
+        }
+    }
+};
+
+// The part of a unit that a workgroup has: rounds begin .. end - 1 of its `rounds`, which are first_round .. of all.
+struct Part {
+    int b, length, first, count;      // the sequence and its rows of the call
+    int head, row0, here;             // key/value head; rows of the tile
+    int begin, end, rounds, first_round;
+};
+template <int ROWS, int STEP>
+__device__ __forceinline__ Part part_of(const Kv &kv, int group, Finder<ROWS, STEP> &find, int round, int stop)
+{
+    Part u;
+    const int at = find.lane_of(kv, group, round);
+    u.b = find.in.base + at;
+    u.length = __builtin_amdgcn_readlane(find.in.length, at);
+    u.first = __builtin_amdgcn_readlane(find.in.first, at);
+    u.count = __builtin_amdgcn_readlane(find.in.count, at);
+    const int before = find.before + __builtin_amdgcn_readlane(find.in.upto - find.in.rounds, at);
+    u.rounds = max((u.length + STEP - 1) / STEP, 1);
+    const int in = round - before, unit = in / u.rounds;
+    u.head = unit % kv.kv_heads;
+    u.row0 = unit / kv.kv_heads * ROWS;
+    u.here = min(ROWS, u.count * group - u.row0);
+    u.first_round = before + unit * u.rounds;
+    u.begin = round - u.first_round;
+    u.end = min(u.rounds, stop - u.first_round);
+    return u;
+}
+
+// Where a workgroup leaves its part of a unit that begins with `first_round`.
+__device__ __forceinline__ int part_slot(const Deal &deal, int share, int first_round) { return 2 * share + (first_round > deal.start(share) ? 1 : 0); }
+
+// Adds up a unit's parts: a wave for a row.
+template <int DT, int ROWS>
+__device__ __forceinline__ void join_unit(const Kv &kv, const Shares &shares, const Deal &deal, const Part &u, int share0, int share1, int group, int heads_first,
+                                          float *out, int64_t out_stride, int wave, int waves)
+{
+    // the first workgroup's part may be its second; the others' are their first
+    const int64_t slot0 = part_slot(deal, share0, u.first_round);
+    for (int r = wave; r < u.here; r += waves) {
+        const int row = u.row0 + r;
+        join_row<DT>(kv, shares.sums, shares.tops, slot0 * ROWS + r, (int64_t)2 * (share0 + 1) * ROWS + r, 2 * ROWS, share1 - share0 + 1,
+                     out + (int64_t)(u.first + row / group) * out_stride + (heads_first + row % group) * kv.head_dim);
+    }
+}
 
 template <int DT, int NB, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, int heads, float scale,
-                                                                     int causal, float *__restrict__ out, int64_t out_stride, Parts parts)
+__global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_few_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, int heads,
+                                                                                         float scale, int causal, float *__restrict__ out,
+                                                                                         int64_t out_stride, Shares shares)
 {
-    constexpr int kRows = 16 * NB;
-    constexpr int kPitch = DT + 4;
+    constexpr int kRows = 16 * NB, kPitch = DT + 4, kStep = 64 * WAVES;
     __shared__ __align__(16) _Float16 q_half[DT / 8][2][kRows][8];
     __shared__ float q_unit[kRows];
-    __shared__ __align__(16) float o_part[WAVES / 2][kRows][kPitch];
+    __shared__ __align__(16) float o_part[WAVES][kRows][kPitch];
     __shared__ float top_part[WAVES][kRows], sum_part[WAVES][kRows];
     __shared__ int level_part[WAVES];
+    __shared__ int is_last;
 
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int group = heads / kv.kv_heads;
-    unsigned unit = blockIdx.x;
-    const int split_at = unit % (unsigned)parts.splits;
-    unit /= (unsigned)parts.splits;
-    int tile = unit % (unsigned)parts.tiles;
-    const int head = (unit / (unsigned)parts.tiles) % (unsigned)kv.kv_heads;
-    const int b = unit / (unsigned)parts.tiles / (unsigned)kv.kv_heads;
-    int length, first, count;
-    kv_sequence(kv, b, length, first, count);
-    const int rows = count * group;      // the host has checked that all rows of all heads are below 2^31
-
-    for (; tile * kRows < rows; tile += parts.tiles) {
-        const int row0 = tile * kRows;
-        const bool whole = tile >= parts.tiles;      // beyond what the host knew: in one piece
-        if (whole && split_at)
-            break;
+    const int group = heads / kv.kv_heads, share = blockIdx.x;
+    const Sequences<kRows, kStep> begin(kv, group, 0);
+    const Deal deal(all_rounds(kv, group, begin), shares.count);
+    const int stop = deal.start(share + 1);
+    Finder<kRows, kStep> find(begin);
+    for (int round = deal.start(share); round < stop;) {
+        const Part u = part_of(kv, group, find, round, stop);
+        const int b = u.b, length = u.length, first = u.first, count = u.count, head = u.head, row0 = u.row0, here = u.here, rows = count * group;
         // the last token that the tile's last row sees
-        const int last_row = min(row0 + kRows, rows) - 1;
-        const int seen = causal ? max(length - count + last_row / group + 1, 0) : length;
-        const int chunk = whole ? 0x7fffffc0 : chunk_of(parts, length);
-        const int from = whole ? 0 : split_at * chunk;
-        if (from >= seen && split_at)
-            break;                                   // later tiles of the sequence see more, but they are beyond parts.tiles
-        const int to = min(seen, whole ? seen : from + chunk);
+        const int seen = causal ? max(length - count + (row0 + here - 1) / group + 1, 0) : length;
+        const int from = u.begin * kStep, to = min(seen, u.end * kStep);
+        const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
+        const char *const first_page = kv.pages + (uint64_t)head * kv.head_bytes;
 
-        // ---- rows of q as halves
-        for (int r = w; r < kRows; r += WAVES) {
-            const int row = row0 + r;
-            float x[DT / 64], most = 0.0f;
+        // Pages of the 16 tokens whose keys, and of those whose scales and values, this lane takes.
+        int key_page, value_page;
+        auto look_up = [&](int j0) {
+            key_page = table[kv_page_of(kv, (unsigned)min(j0 + 16 * (col >> 2), to - 1) / 16)];
+            value_page = table[kv_page_of(kv, (unsigned)min(j0 + 16 * g, to - 1) / 16)];
+        };
+        int j0 = from + 64 * w;
+        if (j0 < to)
+            look_up(j0);
+        // the wave's rows of q
+        constexpr int kMine = kRows / WAVES;
+        float q_row[kMine][DT / 64];
+#pragma unroll
+        for (int r = 0; r < kMine; r++) {
+            const int row = row0 + w + r * WAVES;
             const float *from_q = q + (int64_t)(first + row / group) * q_stride + (head * group + row % group) * kv.head_dim;
 #pragma unroll
-            for (int i = 0; i < DT / 64; i++) {
-                const int d = lane + 64 * i;
-                x[i] = row < rows && d < kv.head_dim ? from_q[d] * scale * kLog2e : 0.0f;
-                most = fmaxf(most, fabsf(x[i]));
+            for (int i = 0; i < DT / 64; i++)
+                q_row[r][i] = row < rows && lane + 64 * i < kv.head_dim ? from_q[lane + 64 * i] : 0.0f;
+        }
+
+        int4_t keys[4][DT / 64], values[DT / 16];
+        float4_t ks[4], vs[4];
+        bool there;
+        auto load_keys = [&](int j0) {
+            const unsigned group16 = (unsigned)min(j0 + 16 * (col >> 2), to - 1) / 16;
+            bool any;      // where there is no token, or no dimension, any codes do: q or the weight is 0 there
+            const char *page = kv_page_or_any(kv, key_page, first_page, any);
+            const unsigned slot = (group16 - kv_page_of(kv, group16) * kv.page_groups) * 16 + (col & 3);
+#pragma unroll
+            for (int u = 0; u < DT / 64; u++) {
+                const unsigned c = 16 * (4 * u + g) < kv.padded ? 4 * u + g : 0;
+                const char *p = page + kv_key_at(kv, c, slot);
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    keys[t][u] = *reinterpret_cast<const int4_t *>(p + 64 * t);
             }
-            const int e = exponent_of(wave_max(most));
+        };
+        auto load_values = [&](int j0) {
+            const unsigned group16 = (unsigned)min(j0 + 16 * g, to - 1) / 16;
+            const char *page = kv_page_or_any(kv, value_page, first_page, there);
+            there = there && j0 + 16 * g < to;
+            const unsigned place = group16 - kv_page_of(kv, group16) * kv.page_groups;
+            const float *scales = reinterpret_cast<const float *>(page + kv_scales_at(kv)) + place * 16;
+            const char *p = page + kv_value_at(kv, place, 0);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                ks[t] = reinterpret_cast<const float4_t *>(scales)[t];
+                vs[t] = reinterpret_cast<const float4_t *>(scales + kv.page_size)[t];
+            }
+#pragma unroll
+            for (int i = 0; i < DT / 16; i++)
+                values[i] = *reinterpret_cast<const int4_t *>(p + ((16 * i < kv.padded ? 16 * i : 0) + col) * 16);
+        };
+        if (j0 < to) {
+            load_keys(j0);
+            load_values(j0);
+            if (j0 + kStep < to)
+                look_up(j0 + kStep);
+        }
+
+        // ---- rows of q as halves
+#pragma unroll
+        for (int r = 0; r < kMine; r++) {
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DT / 64; i++) {
+                q_row[r][i] = q_row[r][i] * scale * kLog2e;
+                most = fmaxf(most, fabsf(q_row[r][i]));
+            }
+            const int e = exponent_of(wave_max(most)), at = w + r * WAVES;
 #pragma unroll
             for (int i = 0; i < DT / 64; i++) {
                 const int d = lane + 64 * i;
-                const float v = __builtin_ldexpf(x[i], 14 - e);
+                const float v = __builtin_ldexpf(q_row[r][i], 14 - e);
                 const _Float16 hi = (_Float16)v;
-                q_half[d / 8][0][r][d % 8] = hi;
-                q_half[d / 8][1][r][d % 8] = (_Float16)(v - (float)hi);
+                q_half[d / 8][0][at][d % 8] = hi;
+                q_half[d / 8][1][at][d % 8] = (_Float16)(v - (float)hi);
             }
             if (lane == 0)
-                q_unit[r] = __builtin_ldexpf(1.0f, e - 14);
+                q_unit[at] = __builtin_ldexpf(1.0f, e - 14);
         }
         __syncthreads();
 
@@ -222,56 +484,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
         Level level;
         bool fresh = true;
 
-        // Loads of a tile: pages of the 16 tokens whose keys, and whose scales and values, this lane takes.
-        int4_t keys[4][DT / 64], values[DT / 16];
-        const char *value_page;
-        unsigned value_place;
-        bool there;
-        const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
-        const char *const first_page = kv.pages + (uint64_t)head * kv.head_bytes;
-        // Behind the last token: the last one's group, whose codes do as any, as those of page 0 where there is no page.
-        auto page_for = [&](int token, unsigned &place, bool &ok) -> const char * {
-            const char *p = kv_group_or_any(kv, table, (unsigned)min(token, to - 1) / 16, first_page, place, ok);
-            ok = ok && token < to;
-            return p;
-        };
-        auto load_keys = [&](int j0) {
-            unsigned place;
-            bool ok;
-            const char *page = page_for(j0 + 16 * (col >> 2), place, ok);
-            const unsigned slot = place * 16 + (col & 3);
-#pragma unroll
-            for (int u = 0; u < DT / 64; u++) {
-                const unsigned c = 16 * (4 * u + g) < kv.padded ? 4 * u + g : 0;     // behind the dimensions: any codes, q is 0 there
-                const char *p = page + kv_key_at(kv, c, slot);
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-                    keys[t][u] = *reinterpret_cast<const int4_t *>(p + 64 * t);
-            }
-        };
-        auto load_values = [&] {
-            const char *p = value_page + kv_value_at(kv, value_place, 0);
-#pragma unroll
-            for (int i = 0; i < DT / 16; i++)
-                values[i] = *reinterpret_cast<const int4_t *>(p + ((16 * i < kv.padded ? 16 * i : 0) + col) * 16);
-        };
-
-        const int step = 64 * WAVES;
-        int j0 = from + 64 * w;
-        if (j0 < to)
-            load_keys(j0);
-        for (; j0 < to; j0 += step) {
+        for (; j0 < to; j0 += kStep) {
             asm volatile("" ::: "memory");      // q's halves are read again for every tile, not kept in registers
-            value_page = page_for(j0 + 16 * g, value_place, there);
-            load_values();
-            const float *scales = reinterpret_cast<const float *>(value_page + kv_scales_at(kv)) + value_place * 16;
-            float4_t ks[4], vs[4];
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                ks[t] = reinterpret_cast<const float4_t *>(scales)[t];
-                vs[t] = reinterpret_cast<const float4_t *>(scales + kv.page_size)[t];
-            }
-
             // S^T: row r of product t is token j0 + 16 (r / 4) + 4 t + r % 4, so that this lane's are 16 g .. 16 g + 15
             float4_t s[NB][4];
 #pragma unroll
@@ -297,8 +511,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
                                 s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], x, s[n][t], 0, 0, 0);
                         }
                 }
-            if (j0 + step < to)
-                load_keys(j0 + step);
+            if (j0 + kStep < to)
+                load_keys(j0 + kStep);
 
             // scales of tokens that are none count for nothing
             const int mine = there ? j0 + 16 * g : 0x7fffffff;
@@ -368,9 +582,13 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
                         for (int part = 0; part < 2; part++)
                             o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n][h][part], o[n][i], 0, 0, 0);
                 }
+            if (j0 + kStep < to)
+                load_values(j0 + kStep);
+            if (j0 + 2 * kStep < to)
+                look_up(j0 + 2 * kStep);
         }
 
-        // ---- the waves meet
+        // ---- the waves meet: what each has of the rows that there are, in its own units
         if (lane == 0)
             level_part[w] = fresh ? -1000 : level.at;
 #pragma unroll
@@ -380,80 +598,87 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_kernel(Kv kv, const 
                 top_part[w][16 * n + col] = top[n];
                 sum_part[w][16 * n + col] = sum[n];
             }
+            if (16 * n + col < here)
+#pragma unroll
+                for (int i = 0; i < DT / 16; i++)
+                    *reinterpret_cast<float4_t *>(&o_part[w][16 * n + col][16 * i + 4 * g]) = o[n][i];
         }
         __syncthreads();
-        int high = -1000;
-#pragma unroll
-        for (int i = 0; i < WAVES; i++)
-            high = max(high, level_part[i]);
-        float all_top[NB], all_sum[NB];
-#pragma unroll
-        for (int n = 0; n < NB; n++) {
-            all_top[n] = -INFINITY;
-            all_sum[n] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < WAVES; i++)
-                all_top[n] = fmaxf(all_top[n], top_part[i][16 * n + col]);
-            const float off = all_top[n] == -INFINITY ? 0.0f : all_top[n];
+        const bool alone = u.begin == 0 && u.end == u.rounds;
+        const int64_t slot0 = (int64_t)part_slot(deal, share, u.first_round) * kRows;
+        for (int r = w; r < here; r += WAVES) {
+            float t = -INFINITY, total = 0.0f, by[WAVES];
+            int high = -1000;
 #pragma unroll
             for (int i = 0; i < WAVES; i++) {
-                const float t = top_part[i][16 * n + col], v = sum_part[i][16 * n + col];
-                all_sum[n] += v == 0.0f ? 0.0f : v * __builtin_amdgcn_exp2f(t - off);
+                t = fmaxf(t, top_part[i][r]);
+                high = max(high, level_part[i]);
             }
-            const float by = fresh ? 0.0f : __builtin_ldexpf(__builtin_amdgcn_exp2f(top[n] - off), level.at - high);
+            const float off = t == -INFINITY ? 0.0f : t;
 #pragma unroll
-            for (int i = 0; i < DT / 16; i++)
-                o[n][i] = fresh ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : o[n][i] * by;
-        }
-        // half of them hand over to the other half, and so on
-#pragma unroll
-        for (int half = WAVES / 2; half; half /= 2) {
-            if (w >= half && w < 2 * half)
-#pragma unroll
-                for (int n = 0; n < NB; n++)
-#pragma unroll
-                    for (int i = 0; i < DT / 16; i++)
-                        *reinterpret_cast<float4_t *>(&o_part[w - half][16 * n + col][16 * i + 4 * g]) = o[n][i];
-            __syncthreads();
-            if (w < half)
-#pragma unroll
-                for (int n = 0; n < NB; n++)
-#pragma unroll
-                    for (int i = 0; i < DT / 16; i++)
-                        o[n][i] += *reinterpret_cast<const float4_t *>(&o_part[w][16 * n + col][16 * i + 4 * g]);
-            __syncthreads();
-        }
-        // one part, and it is the result; or the part of a split: written row by row
-        const bool alone = whole || chunk >= length;
-        const int64_t slot0 = ((int64_t)unit * parts.splits + split_at) * kRows;
-        if (w == 0) {
-#pragma unroll
-            for (int n = 0; n < NB; n++) {
-                const float by = all_sum[n] == 0.0f ? 0.0f : alone ? 1.0f / all_sum[n] : 1.0f;
-#pragma unroll
-                for (int i = 0; i < DT / 16; i++) {
-                    float4_t v;
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        v[k] = all_sum[n] == 0.0f ? 0.0f : __builtin_ldexpf(o[n][i][k] * by, high - 13);
-                    *reinterpret_cast<float4_t *>(&o_part[0][16 * n + col][16 * i + 4 * g]) = v;
-                }
-                if (!alone && g == 0 && row0 + 16 * n + col < rows)
-                    parts.tops[slot0 + 16 * n + col] = float2_t{all_top[n], all_sum[n]};
+            for (int i = 0; i < WAVES; i++) {
+                const float e = __builtin_amdgcn_exp2f(top_part[i][r] - off), v = sum_part[i][r];
+                total += v == 0.0f ? 0.0f : v * e;
+                by[i] = v == 0.0f ? 0.0f : __builtin_ldexpf(e, level_part[i] - high);
             }
-        }
-        __syncthreads();
-        for (int r = w; r < min(kRows, rows - row0); r += WAVES) {
             const int row = row0 + r;
             float *to_o = alone ? out + (int64_t)(first + row / group) * out_stride + (head * group + row % group) * kv.head_dim
-                                : parts.sums + (slot0 + r) * kv.head_dim;
+                                : shares.sums + (slot0 + r) * kv.head_dim;
+            const float over = total == 0.0f ? 0.0f : alone ? 1.0f / total : 1.0f;
 #pragma unroll
-            for (int i = 0; i < DT / 64; i++)
-                if (lane + 64 * i < kv.head_dim)
-                    to_o[lane + 64 * i] = o_part[0][r][lane + 64 * i];
+            for (int i = 0; i < DT / 64; i++) {
+                const int d = lane + 64 * i;
+                float v = 0.0f;
+#pragma unroll
+                for (int k = 0; k < WAVES; k++)
+                    if (by[k] != 0.0f)
+                        v = __builtin_fmaf(o_part[k][r][d], by[k], v);
+                v = total == 0.0f ? 0.0f : __builtin_ldexpf(v * over, high - 13);
+                if (d < kv.head_dim) {
+                    if (alone)
+                        to_o[d] = v;
+                    else
+                        store_far(to_o + d, v);
+                }
+            }
+            if (!alone && lane < 2)
+                store_far(&shares.tops[slot0 + r][lane], lane ? total : t);
         }
-        __syncthreads();
+        if (shares.counters >= 0 && !alone) {
+            // the parts are complete in memory before the workgroup counts itself
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int share0 = deal.of(u.first_round), share1 = deal.of(u.first_round + u.rounds - 1);
+            unsigned *const counter = &g_arrived[shares.counters][part_slot(deal, share0, u.first_round)];
+            if (threadIdx.x == 0)
+                is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == (unsigned)(share1 - share0 + 1);
+            __syncthreads();
+            if (is_last) {
+                if (threadIdx.x == 0)
+                    __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                join_unit<DT, kRows>(kv, shares, deal, u, share0, share1, group, head * group, out, out_stride, w, WAVES);
+            }
+        }
+        round = u.first_round + u.end;
     }
+}
+
+// The parts of the units that several workgroups have: a workgroup for each that may have the first part of one.
+template <int DT, int NB, int WAVES>
+__global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, int heads, float *__restrict__ out, int64_t out_stride, Shares shares)
+{
+    constexpr int kRows = 16 * NB, kStep = 64 * WAVES;
+    const int group = heads / kv.kv_heads, share = blockIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Sequences<kRows, kStep> begin(kv, group, 0);
+    const Deal deal(all_rounds(kv, group, begin), shares.count);
+    const int stop = deal.start(share + 1);
+    if (deal.start(share) >= stop)
+        return;
+    Finder<kRows, kStep> find(begin);
+    const Part u = part_of(kv, group, find, stop - 1, stop);
+    if (u.end == u.rounds || deal.of(u.first_round) != share)
+        return;
+    join_unit<DT, kRows>(kv, shares, deal, u, share, deal.of(u.first_round + u.rounds - 1), group, u.head * group, out, out_stride, w, 4);
 }
 
 // ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
@@ -902,7 +1127,10 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             }
         const int64_t slot0 = (((int64_t)bh * parts.tiles + tile) * parts.splits + split_at) * kRows + w * kManyRows;
         if (!alone && h == 0 && row0 + col < rows)
-            parts.tops[slot0 + col] = float2_t{off == kNone ? -INFINITY : off, sum};
+            {
+            parts.tops[slot0 + col][0] = off == kNone ? -INFINITY : off;
+            parts.tops[slot0 + col][1] = sum;
+        }
         __syncthreads();
 #pragma unroll 4
         for (int r = 0; r < kManyRows; r++) {
@@ -921,13 +1149,12 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 }
 
 // The parts of the rows whose tokens are split: a wave for each row and head.
-__global__ __launch_bounds__(256) void attention_join_kernel(Kv kv, int heads, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
+__global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, int heads, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
                                                              int tile_rows, unsigned units)
 {
     const unsigned unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (unit >= units)
         return;
-    const int lane = threadIdx.x & 63;
     const int h = unit % (unsigned)heads, row = unit / (unsigned)heads;
     int b, position;
     if (!kv_row(kv, row, b, position))
@@ -943,63 +1170,60 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Kv kv, int heads, i
     const int seen = causal ? max(length - count + last_row / group + 1, 0) : length;
     const int n = max((seen + chunk - 1) / chunk, 1);
     const int64_t slot = (((int64_t)b * kv.kv_heads + h / group) * parts.tiles + tile) * parts.splits * tile_rows + mine % tile_rows;
-    float top = -INFINITY;
-    for (int i = 0; i < n; i++)
-        top = fmaxf(top, parts.tops[slot + (int64_t)i * tile_rows][0]);
-    const float off = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o[kKvMostDim / 64] = {};
-    for (int i = 0; i < n; i++) {
-        const int64_t at = slot + (int64_t)i * tile_rows;
-        const float2_t t = parts.tops[at];
-        const float by = __builtin_amdgcn_exp2f(t[0] - off);
-        if (t[1] == 0.0f)
-            continue;
-        sum = __builtin_fmaf(t[1], by, sum);
-#pragma unroll
-        for (int k = 0; k < kKvMostDim / 64; k++)
-            if (lane + 64 * k < kv.head_dim)
-                o[k] = __builtin_fmaf(parts.sums[at * kv.head_dim + lane + 64 * k], by, o[k]);
-    }
-    float *y = out + (int64_t)row * out_stride + h * kv.head_dim;
-#pragma unroll
-    for (int k = 0; k < kKvMostDim / 64; k++)
-        if (lane + 64 * k < kv.head_dim)
-            y[lane + 64 * k] = sum == 0.0f ? 0.0f : o[k] / sum;
+    join_row<kKvMostDim>(kv, parts.sums, parts.tops, slot, slot + tile_rows, tile_rows, n, out + (int64_t)row * out_stride + h * kv.head_dim);
 }
 
-// How a call is cut: rows in tiles, tokens in splits.
+// How a call is cut.
 struct Plan {
     bool many;
-    int tile_rows, tiles, splits, chunk;
-    int64_t units;      // (sequence, key/value head, tile)
+    int tile_rows, tiles;
+    int splits, chunk;      // many rows: of the tokens of a tile
+    int waves, shares;      // few rows
+    int64_t blocks;
     size_t sums_bytes, tops_bytes;
     size_t bytes() const { return sums_bytes + tops_bytes; }
 };
 
-Plan plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads)
+// VTL_HIP_OK and how, or why not.
+int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
 {
-    Plan p{};
+    p = Plan{};
     const int64_t most_rows = kv.starts ? (b.most_rows ? std::min(b.most_rows, kv.rows) : kv.rows) : 1;
     const int64_t most_length = std::max(b.most_length ? std::min(b.most_length, kv.most_tokens) : kv.most_tokens, 1);
-    const int64_t rows = most_rows * (heads / kv.kv_heads);
+    const int64_t group = heads / kv.kv_heads, rows = most_rows * group;
+    if ((int64_t)kv.rows * heads > 0x7fffffc0)
+        return VTL_HIP_ERR_UNSUPPORTED;
     p.many = rows > (kv.padded > 128 ? 16 : 32);
     p.tile_rows = p.many ? kManyRows * 4 : rows <= 16 ? 16 : 32;
     p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
-    p.units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
-    const int64_t wanted = std::max<int64_t>(1, (p.many ? 512 : 1024) / p.units);
-    const int least = p.many ? 256 : 512;
-    p.splits = (int)std::min(wanted, (most_length + least - 1) / least);
-    p.chunk = (int)((((most_length + p.splits - 1) / p.splits) + least - 1) / least * least);
-    p.splits = (int)((most_length + p.chunk - 1) / p.chunk);
-    if (p.splits > 1) {
-        const size_t rows_in = (size_t)p.units * p.splits * p.tile_rows;
-        p.sums_bytes = (rows_in * kv.head_dim * sizeof(float) + 255) & ~(size_t)255;
-        p.tops_bytes = rows_in * sizeof(float2_t);
+    const int64_t units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
+    int64_t parts = 0;      // of rows that meet
+    if (p.many) {
+        const int64_t wanted = std::max<int64_t>(1, 512 / units);
+        p.splits = (int)std::min(wanted, (most_length + 255) / 256);
+        p.chunk = (int)((((most_length + p.splits - 1) / p.splits) + 255) / 256 * 256);
+        p.splits = (int)((most_length + p.chunk - 1) / p.chunk);
+        p.blocks = units * p.splits;
+        parts = p.splits > 1 ? p.blocks : 0;
+    } else {
+        p.waves = kv.padded <= 128 && (p.tile_rows == 16 || kv.padded <= 64) && units * ((most_length + 511) / 512) <= 256 ? 8 : 4;
+        const int64_t step = 64 * p.waves;
+        // what the device counts in 32 bits
+        if (((int64_t)kv.rows * group / p.tile_rows + kv.batch) * kv.kv_heads > kMostRounds / (kv.most_tokens / step + 1))
+            return VTL_HIP_ERR_UNSUPPORTED;
+        const int64_t at_once = p.waves == 8 || kv.padded > 128 || (kv.padded > 64 && p.tile_rows == 32) ? 256 : kMostShares;
+        p.shares = (int)std::min(at_once, units * ((most_length + step - 1) / step));
+        p.blocks = p.shares;
+        parts = p.shares > 1 ? 2 * p.shares : 0;
     }
-    return p;
+    if (p.blocks > 0x7fffffff)
+        return VTL_HIP_ERR_UNSUPPORTED;
+    p.sums_bytes = ((size_t)parts * p.tile_rows * kv.head_dim * sizeof(float) + 255) & ~(size_t)255;
+    p.tops_bytes = (size_t)parts * p.tile_rows * 2 * sizeof(float);
+    return VTL_HIP_OK;
 }
 
-// The arguments that both kernels share.
+// The arguments that the kernels share.
 struct Call {
     Kv kv;
     const float *q;
@@ -1009,34 +1233,53 @@ struct Call {
     int causal;
     float *out;
     int64_t out_stride;
-    Parts parts;
-    unsigned blocks;
+    Plan plan;
+    float *sums;
+    float (*tops)[2];
 };
 
 template <int DT, int NB, int WAVES>
 int launch_few(const Call &c)
 {
-    hipLaunchKernelGGL((attention_few_kernel<DT, NB, WAVES>), dim3(c.blocks), dim3(64 * WAVES), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale,
-                       c.causal, c.out, c.out_stride, c.parts);
-    return check_launch("attention_few_kernel");
+    const Shares shares{c.plan.shares, c.sums ? stream_slot(current_stream()) : -1, c.sums, c.tops};
+    const dim3 blocks((unsigned)c.plan.blocks);
+    hipLaunchKernelGGL((attention_few_kernel<DT, NB, WAVES>), blocks, dim3(64 * WAVES), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale, c.causal,
+                       c.out, c.out_stride, shares);
+    const int st = check_launch("attention_few_kernel");
+    if (st != VTL_HIP_OK || !c.sums || shares.counters >= 0)
+        return st;
+    hipLaunchKernelGGL((attention_few_join_kernel<DT, NB, WAVES>), blocks, dim3(256), 0, current_stream(), c.kv, c.heads, c.out, c.out_stride, shares);
+    return check_launch("attention_few_join_kernel");
 }
 
 template <int DT>
 int launch_many(const Call &c)
 {
-    hipLaunchKernelGGL((attention_many_kernel<DT, 4>), dim3(c.blocks), dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale, c.causal,
-                       c.out, c.out_stride, c.parts);
-    return check_launch("attention_many_kernel");
+    const Parts parts{c.plan.tiles, c.plan.splits, c.plan.chunk, c.sums, c.tops};
+    hipLaunchKernelGGL((attention_many_kernel<DT, 4>), dim3((unsigned)c.plan.blocks), dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale,
+                       c.causal, c.out, c.out_stride, parts);
+    const int st = check_launch("attention_many_kernel");
+    if (st != VTL_HIP_OK || !c.sums)
+        return st;
+    const int64_t row_heads = (int64_t)c.kv.rows * c.heads;
+    hipLaunchKernelGGL(attention_many_join_kernel, dim3((unsigned)((row_heads + 3) / 4)), dim3(256), 0, current_stream(), c.kv, c.heads, c.causal, c.out,
+                       c.out_stride, parts, c.plan.tile_rows, (unsigned)row_heads);
+    return check_launch("attention_many_join_kernel");
 }
 
-int launch_attention(const Call &c, const Plan &plan)
+int launch_attention(const Call &c)
 {
     const int padded = c.kv.padded;
-    if (plan.many)
+    if (c.plan.many)
         return padded <= 64 ? launch_many<64>(c) : padded <= 96 ? launch_many<96>(c) : padded <= 128 ? launch_many<128>(c) : launch_many<256>(c);
-    if (plan.tile_rows == 16)
-        return padded <= 64 ? launch_few<64, 1, 8>(c) : padded <= 128 ? launch_few<128, 1, 8>(c) : launch_few<256, 1, 4>(c);
-    return padded <= 64 ? launch_few<64, 2, 8>(c) : launch_few<128, 2, 4>(c);
+    if (c.plan.tile_rows == 16) {
+        if (c.plan.waves == 8)
+            return padded <= 64 ? launch_few<64, 1, 8>(c) : launch_few<128, 1, 8>(c);
+        return padded <= 64 ? launch_few<64, 1, 4>(c) : padded <= 128 ? launch_few<128, 1, 4>(c) : launch_few<256, 1, 4>(c);
+    }
+    if (c.plan.waves == 8)
+        return launch_few<64, 2, 8>(c);
+    return padded <= 64 ? launch_few<64, 2, 4>(c) : launch_few<128, 2, 4>(c);
 }
 
 bool attention_sizes_ok(const Kv &kv, int heads) { return heads >= 1 && heads % kv.kv_heads == 0; }
@@ -1050,7 +1293,8 @@ size_t vtl_hip_attention_i8_workspace(const vtl_hip_kv_cache *cache, const vtl_h
     Kv kv;
     if (kv_sizes(cache, batch, kv) != VTL_HIP_OK || !attention_sizes_ok(kv, heads) || kv.rows == 0 || kv.batch == 0)
         return 0;
-    return plan_of(kv, *batch, heads).bytes();
+    Plan plan;
+    return plan_of(kv, *batch, heads, plan) == VTL_HIP_OK ? plan.bytes() : 0;
 }
 
 int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, const float *q, int64_t q_stride, int heads,
@@ -1066,28 +1310,22 @@ int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_bat
         return VTL_HIP_OK;
     if (!q || !out || meet(q, kv_span(kv, heads, q_stride), out, kv_span(kv, heads, out_stride)))
         return VTL_HIP_ERR_INVALID_ARG;
-    const int64_t row_heads = (int64_t)kv.rows * heads;
-    const Plan plan = plan_of(kv, *batch, heads);
-    if (row_heads > 0x7fffffc0 || plan.units * plan.splits > 0x7fffffff)
-        return VTL_HIP_ERR_UNSUPPORTED;
-    if (workspace && ((reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes()))
+    Call call{kv, q, q_stride, heads, scale, causal, out, out_stride, {}, nullptr, nullptr};
+    const int planned = plan_of(kv, *batch, heads, call.plan);
+    if (planned != VTL_HIP_OK)
+        return planned;
+    const size_t need = call.plan.bytes();
+    if (workspace && ((reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need))
         return VTL_HIP_ERR_INVALID_ARG;
-    Parts parts{plan.tiles, plan.splits, plan.chunk, nullptr, nullptr};
-    if (plan.splits > 1) {
+    if (need) {
         if (!workspace)
-            workspace = library_workspace(plan.bytes());
+            workspace = library_workspace(need);
         if (!workspace)
             return workspace_status();
-        parts.sums = static_cast<float *>(workspace);
-        parts.tops = reinterpret_cast<float2_t *>(static_cast<char *>(workspace) + plan.sums_bytes);
+        call.sums = static_cast<float *>(workspace);
+        call.tops = reinterpret_cast<float(*)[2]>(static_cast<char *>(workspace) + call.plan.sums_bytes);
     }
-    const Call call{kv, q, q_stride, heads, scale, causal, out, out_stride, parts, (unsigned)(plan.units * plan.splits)};
-    const int launched = launch_attention(call, plan);
-    if (launched != VTL_HIP_OK || plan.splits == 1)
-        return launched;
-    hipLaunchKernelGGL(attention_join_kernel, dim3((unsigned)((row_heads + 3) / 4)), dim3(256), 0, current_stream(), kv, heads, causal, out, out_stride,
-                       parts, plan.tile_rows, (unsigned)row_heads);
-    return check_launch("attention_join_kernel");
+    return launch_attention(call);
 }
 
 }  // extern "C"
