@@ -99,6 +99,23 @@ __device__ __forceinline__ float max_across_32(float v)
 
 __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255) - 127; }
 
+// Rows of a tile are tokens of `size` heads each: which token and which of its heads a row is, given those of the tile's first row and how far behind it
+// (less than 128) the row is.
+struct Group {
+    int size;
+    float part;
+    __device__ __forceinline__ explicit Group(int n) : size(n), part(1.0f / (float)n) {}
+    __device__ __forceinline__ void row(int token0, int head0, int behind, int &token, int &head) const
+    {
+        const unsigned n = (unsigned)head0 + (unsigned)behind;
+        int more = (int)((float)n * part);      // at most 128: no further off than by one
+        head = (int)(n - (unsigned)more * (unsigned)size);
+        more += head < 0 ? -1 : head >= size ? 1 : 0;
+        head += head < 0 ? size : head >= size ? -size : 0;
+        token = token0 + more;
+    }
+};
+
 // The power of two that the values' scales are divided by, uniform in a wave: that of the largest of the tile's at hand.  It stays while the tile's
 // is at most 2^6 below it (a change costs a pass over the sums), and rises no further than the sums, which grow when it falls, have room for.
 struct Level {
@@ -369,7 +386,8 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
 
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int group = heads / kv.kv_heads, share = blockIdx.x;
+    const Group of(heads / kv.kv_heads);
+    const int group = of.size, share = blockIdx.x;
     const Sequences<kRows, kStep> begin(kv, group, 0);
     const Deal deal(all_rounds(kv, group, begin), shares.count);
     const int stop = deal.start(share + 1);
@@ -377,8 +395,10 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
     for (int round = deal.start(share); round < stop;) {
         const Part u = part_of(kv, group, find, round, stop);
         const int b = u.b, length = u.length, first = u.first, count = u.count, head = u.head, row0 = u.row0, here = u.here, rows = count * group;
-        // the last token that the tile's last row sees
-        const int seen = causal ? max(length - count + (row0 + here - 1) / group + 1, 0) : length;
+        const int token0 = row0 / group, head0 = row0 - token0 * group;      // of the tile's first row
+        int token, of_token;
+        of.row(token0, head0, here - 1, token, of_token);
+        const int seen = causal ? max(length - count + token + 1, 0) : length;      // by its last
         const int from = u.begin * kStep, to = min(seen, u.end * kStep);
         const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
         const char *const first_page = kv.pages + (uint64_t)head * kv.head_bytes;
@@ -398,7 +418,8 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
 #pragma unroll
         for (int r = 0; r < kMine; r++) {
             const int row = row0 + w + r * WAVES;
-            const float *from_q = q + (int64_t)(first + row / group) * q_stride + (head * group + row % group) * kv.head_dim;
+            of.row(token0, head0, w + r * WAVES, token, of_token);
+            const float *from_q = q + (int64_t)(first + token) * q_stride + (head * group + of_token) * kv.head_dim;
 #pragma unroll
             for (int i = 0; i < DT / 64; i++)
                 q_row[r][i] = row < rows && lane + 64 * i < kv.head_dim ? from_q[lane + 64 * i] : 0.0f;
@@ -472,9 +493,9 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
         float4_t o[NB][DT / 16];
 #pragma unroll
         for (int n = 0; n < NB; n++) {
-            const int row = min(row0 + 16 * n + col, rows - 1);
             unit_of[n] = q_unit[16 * n + col];
-            limit[n] = causal ? min(length - count + row / group + 1, to) : to;
+            of.row(token0, head0, min(16 * n + col, here - 1), token, of_token);
+            limit[n] = causal ? min(length - count + token + 1, to) : to;
             top[n] = -INFINITY;
             sum[n] = 0.0f;
 #pragma unroll
@@ -621,8 +642,8 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
                 total += v == 0.0f ? 0.0f : v * e;
                 by[i] = v == 0.0f ? 0.0f : __builtin_ldexpf(e, level_part[i] - high);
             }
-            const int row = row0 + r;
-            float *to_o = alone ? out + (int64_t)(first + row / group) * out_stride + (head * group + row % group) * kv.head_dim
+            of.row(token0, head0, r, token, of_token);
+            float *to_o = alone ? out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim
                                 : shares.sums + (slot0 + r) * kv.head_dim;
             const float over = total == 0.0f ? 0.0f : alone ? 1.0f / total : 1.0f;
 #pragma unroll
@@ -712,7 +733,7 @@ constexpr int kSchedVector = 0x2, kSchedProduct = 0x8, kSchedRead = 0x100;
 
 template <int DT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, int heads, float scale,
-                                                                    int causal, float *__restrict__ out, int64_t out_stride, Parts parts)
+                                                                    int causal, float *__restrict__ out, int64_t out_stride, Parts parts, int aligned)
 {
     constexpr int T = 64 * WAVES;
     constexpr int TOKENS = DT > 128 ? 32 : 64;             // of a tile: what the registers have room for
@@ -720,18 +741,18 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     constexpr int kUnits = (kPieces + T - 1) / T;          // that a thread brings
     constexpr bool kWhole = kPieces % T == 0;
     constexpr int kBlocks = TOKENS / 32, kSteps = TOKENS / 16;
-    // Two tiles, in arrays of their own so that the compiler knows which of them is read and which written.  Before them each wave's rows of q as
-    // halves, [piece of 8 dimensions][half][row][8], and behind them its results, a row and 4 floats: half of the waves in either.
+    // Two tiles.  Before them each wave's rows of q, and behind them its results: rows of DT + 4 floats.
     typedef ManyTile<DT, TOKENS> Tile;
     constexpr int kRows = kManyRows * WAVES;
     constexpr int kPitch = DT + 4;
     constexpr size_t kWaveBytes = kManyRows * kPitch * sizeof(float);
-    constexpr size_t kBytes = sizeof(Tile) > WAVES / 2 * kWaveBytes ? sizeof(Tile) : WAVES / 2 * kWaveBytes;
-    __shared__ __align__(16) char lds_even[kBytes], lds_odd[kBytes];
+    constexpr size_t kBytes = 2 * sizeof(Tile) > WAVES * kWaveBytes ? 2 * sizeof(Tile) : WAVES * kWaveBytes;
+    __shared__ __align__(16) char lds[kBytes];
     __shared__ float q_most[WAVES];
-    Tile &even = *reinterpret_cast<Tile *>(lds_even), &odd = *reinterpret_cast<Tile *>(lds_odd);
+    Tile *const tiles = reinterpret_cast<Tile *>(lds);
 
-    const int group = heads / kv.kv_heads;
+    const Group of(heads / kv.kv_heads);
+    const int group = of.size;
     // heads vary fastest: workgroups of one head meet in one L2 where their number is a multiple of eight; of a sequence's rows the last, which see most, go first
     unsigned unit = blockIdx.x;
     const unsigned both = (unsigned)kv.batch * kv.kv_heads;
@@ -750,6 +771,8 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int col = lane & 31, h = lane >> 5;
         const int row0 = tile * kRows + w * kManyRows;
+        const int row1 = min(row0, rows - 1), token0 = row1 / group, head0 = row1 - token0 * group;      // of the wave's first row
+        const int behind = max(min(kManyRows, rows - row0) - 1, 0);                                      // and how far behind it its last one is
         const bool whole = tile >= parts.tiles;
         if (whole && split_at)
             break;
@@ -845,66 +868,82 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             look_up(from + TOKENS);
         }
 
-        // ---- rows of q as halves, all in one unit, by way of LDS to registers: lane `col` gets 8 dimensions of every 16 of a row
-        char *const own = (w < WAVES / 2 ? lds_even : lds_odd) + w % (WAVES / 2) * kWaveBytes;
-        _Float16(*const q_half)[2][kManyRows][8] = reinterpret_cast<_Float16(*)[2][kManyRows][8]>(own);
+        // ---- rows of q as halves, all in one unit: rows into LDS as they are, and from there to the lanes, of which lane `col` gets 8 dimensions of
+        // every 16 of a row
+        float(*const own)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds + w * kWaveBytes);
+        float most = 0.0f;
         {
-            float v[kManyRows][(DT + 63) / 64], most = 0.0f;
-            int in_group = row0 % group;
-            const float *from_q = q + (int64_t)(first + row0 / group) * q_stride + (head * group + in_group) * kv.head_dim;
+            // as many lanes side by side as have a row in vectors of 16 bytes
+            constexpr int kLanes = DT / 4, kTogether = 64 / kLanes, kLoads = kManyRows / (kTogether ? kTogether : 1);
+            static_assert(DT / 4 <= 64, "a row in one instruction");
+            const int lane_row = lane / kLanes, d = lane % kLanes * 4;
+            if (aligned) {
+                float4_t v[kLoads];
 #pragma unroll
-            for (int r = 0; r < kManyRows; r++) {
-#pragma unroll
-                for (int i = 0; i < (DT + 63) / 64; i++) {
-                    v[r][i] = row0 + r < rows && lane + 64 * i < kv.head_dim ? from_q[lane + 64 * i] : 0.0f;
+                for (int i = 0; i < kLoads; i++) {
+                    const int r = i * kTogether + lane_row;
+                    int token, of_token;      // of the last row, or of the first dimensions, where there is none
+                    of.row(token0, head0, min(r, behind), token, of_token);
+                    v[i] = *reinterpret_cast<const float4_t *>(q + (int64_t)(first + token) * q_stride + (head * group + of_token) * kv.head_dim +
+                                                               (d < kv.head_dim ? d : 0));
                 }
-                const bool wrap = ++in_group == group;
-                in_group = wrap ? 0 : in_group;
-                from_q += wrap ? q_stride - (int64_t)(group - 1) * kv.head_dim : kv.head_dim;
-            }
 #pragma unroll
-            for (int r = 0; r < kManyRows; r++)
+                for (int i = 0; i < kLoads; i++) {
+                    if (row0 + i * kTogether + lane_row >= rows || d >= kv.head_dim)
+                        v[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < (DT + 63) / 64; i++) {
-                    v[r][i] = v[r][i] * scale * kLog2e;
-                    const float size = fabsf(v[r][i]);
-                    most = fmaxf(most, size < INFINITY ? size : 0.0f);      // a row that is no number spoils no other
+                    for (int j = 0; j < 4; j++)
+                        most = fmaxf(most, fabsf(v[i][j]) < INFINITY ? fabsf(v[i][j]) : 0.0f);      // a row that is no number spoils no other
+                    if (lane_row < kTogether)
+                        *reinterpret_cast<float4_t *>(&own[i * kTogether + lane_row][d]) = v[i];
                 }
-            most = wave_max(most);
-            if (lane == 0)
-                q_most[w] = most;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < WAVES; i++)
-                most = fmaxf(most, q_most[i]);
-            unit_at = __builtin_amdgcn_readfirstlane(exponent_of(most)) - 14;
-#pragma unroll
-            for (int r = 0; r < kManyRows; r++)
-#pragma unroll
-                for (int i = 0; i < (DT + 63) / 64; i++) {
-                    const int d = lane + 64 * i;
-                    const float y = __builtin_ldexpf(v[r][i], -unit_at);
-                    const _Float16 hi = (_Float16)y;
-                    if (DT % 64 == 0 || d < DT) {
-                        q_half[d / 8][0][r][d % 8] = hi;
-                        q_half[d / 8][1][r][d % 8] = (_Float16)(y - (float)hi);
+            } else {
+#pragma unroll 1
+                for (int r = 0; r < kManyRows; r++) {
+                    int token, of_token;
+                    of.row(token0, head0, min(r, behind), token, of_token);
+                    const float *from_q = q + (int64_t)(first + token) * q_stride + (head * group + of_token) * kv.head_dim;
+#pragma unroll 1
+                    for (int at = lane; at < DT; at += 64) {
+                        const float one = row0 + r < rows && at < kv.head_dim ? from_q[at] : 0.0f;
+                        own[r][at] = one;
+                        most = fmaxf(most, fabsf(one) < INFINITY ? fabsf(one) : 0.0f);
                     }
                 }
+            }
         }
+        const float to_exponents = scale * kLog2e;
+        most = wave_max(most);
+        if (lane == 0)
+            q_most[w] = most;
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; i++)
+            most = fmaxf(most, q_most[i]);
+        unit_at = __builtin_amdgcn_readfirstlane(exponent_of(fminf(most * fabsf(to_exponents), 0x1.fffffep127f))) - 14;
         half8_t x[DT / 16][2];
 #pragma unroll
-        for (int i = 0; i < DT / 16; i++)
+        for (int i = 0; i < DT / 16; i++) {
+            float v[8];
 #pragma unroll
-            for (int part = 0; part < 2; part++)
-                x[i][part] = *reinterpret_cast<const half8_t *>(&q_half[2 * i + h][part][col][0]);
+            for (int k = 0; k < 8; k += 4) {
+                const float4_t four = *reinterpret_cast<const float4_t *>(&own[col][16 * i + 8 * h + k]);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    v[k + j] = __builtin_ldexpf(four[j] * to_exponents, -unit_at);
+            }
+            split(v, x[i][0], x[i][1]);
+        }
         __syncthreads();
 
-        const int row = min(row0 + col, rows - 1);
-        const int limit = causal ? min(length - count + row / group + 1, to) : to;
-        // tokens that all rows of the wave see, and that any does
-        const int all_see = causal ? min(length - count + row0 / group + 1, to) : to;
-        const int any_sees = row0 >= rows ? 0 : causal ? min(length - count + min(row0 + kManyRows - 1, rows - 1) / group + 1, to) : to;
+        int token, of_token, limit = to, all_see = to, any_sees = row0 >= rows ? 0 : to;      // tokens that a row, all rows of the wave, and any see
+        if (causal) {
+            of.row(token0, head0, min(col, behind), token, of_token);
+            limit = min(length - count + token + 1, to);
+            all_see = min(length - count + token0 + 1, to);
+            of.row(token0, head0, behind, token, of_token);
+            any_sees = row0 >= rows ? 0 : min(length - count + token + 1, to);
+        }
 
         // `off` is what a row's scores are less than by 2^kSlack at most; before the row has seen a token it is so low that any score is above
         constexpr float kNone = -0x1p100f;
@@ -918,13 +957,16 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         int level_at = 0;
 
         if (from < to) {
-            store(even);
+            store(tiles[0]);
             if (w == 0)
-                store_scales(even);
+                store_scales(tiles[0]);
             fetch(from + TOKENS);
             look_up(from + 2 * TOKENS);
         }
-        auto work = [&](const Tile &t, Tile &next, int j0) {
+        int which = 0;
+        for (int j0 = from; j0 < to; j0 += TOKENS, which ^= 1) {
+            const Tile &t = tiles[which];
+            Tile &next = tiles[which ^ 1];
             __syncthreads();
             if (w == 0)
                 store_scales(next);
@@ -932,20 +974,20 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 store(next);
                 fetch(j0 + 2 * TOKENS);
                 look_up(j0 + 3 * TOKENS);
-                return;
+                continue;
             }
             const int marked = __builtin_amdgcn_readfirstlane(t.marked), level_here = __builtin_amdgcn_readfirstlane(t.level);
             // S^T.  Row r of a product is the token with bits 2 and 3 of r exchanged: a lane then has 8 consecutive tokens for a step of the second
             // product.  Value k of block i is token 32 i + 16 (k / 8) + 8 h + k % 8.
             float16_t s[kBlocks];
-            const int token = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
-            // `beside` is what a step has beside its products; operands are a step ahead of them
-            auto products = [&](auto beside) {
+            const int of_row = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
+            // With the next tile's way into LDS beside them; operands are a step ahead of the products.
+            {
                 half8_t k[2][kBlocks];
                 auto operand = [&](int d) {
 #pragma unroll
                     for (int i = 0; i < kBlocks; i++)
-                        k[d % 2][i] = *reinterpret_cast<const half8_t *>(&t.keys[2 * d + h][32 * i + token][0]);
+                        k[d % 2][i] = *reinterpret_cast<const half8_t *>(&t.keys[2 * d + h][32 * i + of_row][0]);
                 };
                 operand(0);
 #pragma unroll
@@ -958,7 +1000,10 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 #pragma unroll
                         for (int i = 0; i < kBlocks; i++)
                             s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[d % 2][i], x[d][part], d || part ? s[i] : float16_t{}, 0, 0, 0);
-                    beside(d);
+#pragma unroll
+                    for (int i = 0; i < 4 * kUnits; i++)
+                        if (i * (DT / 16) / (4 * kUnits) == d)
+                            store_part(next, i / 4, i / 2 % 2, i % 2);
                     __builtin_amdgcn_sched_group_barrier(kSchedRead, kBlocks, 0);
 #pragma unroll
                     for (int i = 0; i < 2 * kBlocks; i++) {
@@ -967,52 +1012,41 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
-            };
-            // scores less `off`, and the largest of this lane's
-            auto exponents = [&](float less) {
+            }
+            // scores less `off`, and the largest of this lane's; a row's first scores are taken as they are
+            const float less = off == kNone ? 0.0f : off;
+#pragma unroll
+            for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    const float4_t ks = *reinterpret_cast<const float4_t *>(&t.key_scale[32 * i + 16 * (k / 8) + 8 * h + k % 8]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s[i][k + j] = __builtin_fmaf(s[i][k + j], ks[j], -less);
+                }
+            if (j0 + TOKENS > all_see || marked) {
+                const int until = limit - j0 - 8 * h;
 #pragma unroll
                 for (int i = 0; i < kBlocks; i++)
 #pragma unroll
                     for (int k = 0; k < 16; k += 4) {
-                        const float4_t ks = *reinterpret_cast<const float4_t *>(&t.key_scale[32 * i + 16 * (k / 8) + 8 * h + k % 8]);
+                        const int at = 32 * i + 16 * (k / 8) + k % 8;
+                        const float4_t minus = *reinterpret_cast<const float4_t *>(&t.minus[at + 8 * h]);
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            s[i][k + j] = __builtin_fmaf(s[i][k + j], ks[j], -less);
+                            s[i][k + j] = at + j < until ? s[i][k + j] + minus[j] : -INFINITY;
                     }
-                if (j0 + TOKENS > all_see || marked) {
-                    const int until = limit - j0 - 8 * h;
+            }
+            float best = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < kBlocks; i++)
+            for (int i = 0; i < kBlocks; i++)
 #pragma unroll
-                        for (int k = 0; k < 16; k += 4) {
-                            const int at = 32 * i + 16 * (k / 8) + k % 8;
-                            const float4_t minus = *reinterpret_cast<const float4_t *>(&t.minus[at + 8 * h]);
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                s[i][k + j] = at + j < until ? s[i][k + j] + minus[j] : -INFINITY;
-                        }
-                }
-                float best = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < kBlocks; i++)
-#pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        best = fmaxf(best, s[i][k]);
-                return best;
-            };
-            // with the next tile's way into LDS beside them
-            products([&](int d) {
-#pragma unroll
-                for (int i = 0; i < 4 * kUnits; i++)
-                    if (i * (DT / 16) / (4 * kUnits) == d)
-                        store_part(next, i / 4, i / 2 % 2, i % 2);
-            });
-            if (__any(exponents(off) > kSlack) || level_here != level_at) {
-                // a new maximum: the products again, as there are no registers to keep them
-                products([](int) {});
-                const float best = max_across_32(exponents(0.0f));
-                const float now = best > off + kSlack ? best : off;
-                const float keep = __builtin_amdgcn_exp2f(off - now);
+                for (int k = 0; k < 16; k++)
+                    best = fmaxf(best, s[i][k]);
+            if (__any(best > (off == kNone ? -INFINITY : kSlack)) || level_here != level_at) {
+                // A new maximum.  The scores are rounded once where they are brought to it by a difference, by 2^-24 of how far it has risen at most.
+                const float top = max_across_32(best), rise = off == kNone || top > kSlack ? top : 0.0f;
+                const float now = top == -INFINITY ? off : less + rise, keep = __builtin_amdgcn_exp2f(off - now), further = now - less;
                 off = now;
                 sum *= keep;
                 const float by = __builtin_ldexpf(keep, level_at - level_here);
@@ -1021,10 +1055,10 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 for (int i = 0; i < DT / 32; i++)
                     o[i] *= by;
 #pragma unroll
-                for (int i = 0; i < TOKENS / 32; i++)
+                for (int i = 0; i < kBlocks; i++)
 #pragma unroll
                     for (int k = 0; k < 16; k++)
-                        s[i][k] -= now;
+                        s[i][k] -= further;
             }
             // O^T, 16 tokens a step.  Beside each product, in this order, a part of the next step's weights, and beside the last step's the loads
             // of a later tile: a product holds the vector units' issue for half of its time, which leaves room for four operations.
@@ -1102,18 +1136,12 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-        };
-        for (int j0 = from; j0 < to; j0 += 2 * TOKENS) {
-            work(even, odd, j0);
-            if (j0 + TOKENS < to)
-                work(odd, even, j0 + TOKENS);
         }
         __syncthreads();      // the next tile of rows writes where this one reads
 
         sum = sum_across_32(sum);
         const bool alone = whole || chunk >= length;
         // results by way of LDS, so that rows are written whole
-        float(*const result)[kPitch] = reinterpret_cast<float(*)[kPitch]>(own);
         const float by = sum == 0.0f ? 0.0f : alone ? 1.0f / sum : 1.0f;
 #pragma unroll
         for (int i = 0; i < DT / 32; i++)
@@ -1123,7 +1151,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     v[j] = sum == 0.0f ? 0.0f : __builtin_ldexpf(o[i][k + j] * by, level_at - kManyLevel);
-                *reinterpret_cast<float4_t *>(&result[col][32 * i + 2 * k + 4 * h]) = v;
+                *reinterpret_cast<float4_t *>(&own[col][32 * i + 2 * k + 4 * h]) = v;
             }
         const int64_t slot0 = (((int64_t)bh * parts.tiles + tile) * parts.splits + split_at) * kRows + w * kManyRows;
         if (!alone && h == 0 && row0 + col < rows)
@@ -1132,17 +1160,15 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             parts.tops[slot0 + col][1] = sum;
         }
         __syncthreads();
-#pragma unroll 4
-        for (int r = 0; r < kManyRows; r++) {
-            const int at = row0 + r;
-            if (at >= rows)
-                break;
-            float *to_o = alone ? out + (int64_t)(first + at / group) * out_stride + (head * group + at % group) * kv.head_dim
+#pragma unroll 2
+        for (int r = 0; r < min(kManyRows, rows - row0); r++) {
+            of.row(token0, head0, r, token, of_token);
+            float *to_o = alone ? out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim
                                 : parts.sums + (slot0 + r) * kv.head_dim;
 #pragma unroll
             for (int i = 0; i < (DT + 63) / 64; i++)
                 if (lane + 64 * i < kv.head_dim)
-                    to_o[lane + 64 * i] = result[r][lane + 64 * i];
+                    to_o[lane + 64 * i] = own[r][lane + 64 * i];
         }
         __syncthreads();
     }
@@ -1257,7 +1283,8 @@ int launch_many(const Call &c)
 {
     const Parts parts{c.plan.tiles, c.plan.splits, c.plan.chunk, c.sums, c.tops};
     hipLaunchKernelGGL((attention_many_kernel<DT, 4>), dim3((unsigned)c.plan.blocks), dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale,
-                       c.causal, c.out, c.out_stride, parts);
+                       c.causal, c.out, c.out_stride, parts,
+                       c.kv.head_dim % 4 == 0 && c.q_stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(c.q) & 15));
     const int st = check_launch("attention_many_kernel");
     if (st != VTL_HIP_OK || !c.sums)
         return st;
