@@ -173,15 +173,17 @@ __device__ __forceinline__ float row_sum_16(float v)
 }
 
 // One row's parts, n of them, put together by a wave: the first is at `first`, the others at `second` and on, `apart` rows from each other.
-template <int DT>
+// THERE: they were written by an earlier launch, so the caches have nothing older.
+template <int DT, bool THERE>
 __device__ __forceinline__ void join_row(const Kv &kv, const float *sums, const float (*tops)[2], int64_t first, int64_t second, int apart, int n, float *y)
 {
     auto slot = [&](int i) { return i ? second + (int64_t)(i - 1) * apart : first; };
+    auto load = [](const float *at) { return THERE ? *at : load_far(at); };
     const int lane = threadIdx.x & 63;
     // every lane has the maximum and the sum of a part
     float top = -INFINITY, sum = 0.0f;
     for (int i = lane; i < n; i += 64)
-        top = fmaxf(top, load_far(&tops[slot(i)][0]));
+        top = fmaxf(top, load(&tops[slot(i)][0]));
     top = max_across_32(max_across_16(row_max_16(top)));
     const float off = top == -INFINITY ? 0.0f : top;
     float o[DT / 64] = {};
@@ -189,7 +191,7 @@ __device__ __forceinline__ void join_row(const Kv &kv, const float *sums, const 
         const int i = i0 + lane;
         float by = 0.0f;
         if (i < n) {
-            const float t = load_far(&tops[slot(i)][0]), v = load_far(&tops[slot(i)][1]);
+            const float t = load(&tops[slot(i)][0]), v = load(&tops[slot(i)][1]);
             by = v == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(t - off);
             sum += v == 0.0f ? 0.0f : v * by;
         }
@@ -202,7 +204,7 @@ __device__ __forceinline__ void join_row(const Kv &kv, const float *sums, const 
                 const float *from = sums + slot(i0 + min(k0 + k, few - 1)) * kv.head_dim;
 #pragma unroll
                 for (int c = 0; c < DT / 64; c++)
-                    v[k][c] = lane + 64 * c < kv.head_dim ? load_far(from + lane + 64 * c) : 0.0f;
+                    v[k][c] = lane + 64 * c < kv.head_dim ? load(from + lane + 64 * c) : 0.0f;
             }
 #pragma unroll
             for (int k = 0; k < kAtOnce; k++) {
@@ -358,7 +360,7 @@ __device__ __forceinline__ Part part_of(const Kv &kv, int group, Finder<ROWS, ST
 __device__ __forceinline__ int part_slot(const Deal &deal, int share, int first_round) { return 2 * share + (first_round > deal.start(share) ? 1 : 0); }
 
 // Adds up a unit's parts: a wave for a row.
-template <int DT, int ROWS>
+template <int DT, int ROWS, bool THERE>
 __device__ __forceinline__ void join_unit(const Kv &kv, const Shares &shares, const Deal &deal, const Part &u, int share0, int share1, int group, int heads_first,
                                           float *out, int64_t out_stride, int wave, int waves)
 {
@@ -366,8 +368,8 @@ __device__ __forceinline__ void join_unit(const Kv &kv, const Shares &shares, co
     const int64_t slot0 = part_slot(deal, share0, u.first_round);
     for (int r = wave; r < u.here; r += waves) {
         const int row = u.row0 + r;
-        join_row<DT>(kv, shares.sums, shares.tops, slot0 * ROWS + r, (int64_t)2 * (share0 + 1) * ROWS + r, 2 * ROWS, share1 - share0 + 1,
-                     out + (int64_t)(u.first + row / group) * out_stride + (heads_first + row % group) * kv.head_dim);
+        join_row<DT, THERE>(kv, shares.sums, shares.tops, slot0 * ROWS + r, (int64_t)2 * (share0 + 1) * ROWS + r, 2 * ROWS, share1 - share0 + 1,
+                            out + (int64_t)(u.first + row / group) * out_stride + (heads_first + row % group) * kv.head_dim);
     }
 }
 
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
             if (is_last) {
                 if (threadIdx.x == 0)
                     __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                join_unit<DT, kRows>(kv, shares, deal, u, share0, share1, group, head * group, out, out_stride, w, WAVES);
+                join_unit<DT, kRows, false>(kv, shares, deal, u, share0, share1, group, head * group, out, out_stride, w, WAVES);
             }
         }
         round = u.first_round + u.end;
@@ -699,7 +701,7 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, int head
     const Part u = part_of(kv, group, find, stop - 1, stop);
     if (u.end == u.rounds || deal.of(u.first_round) != share)
         return;
-    join_unit<DT, kRows>(kv, shares, deal, u, share, deal.of(u.first_round + u.rounds - 1), group, u.head * group, out, out_stride, w, 4);
+    join_unit<DT, kRows, true>(kv, shares, deal, u, share, deal.of(u.first_round + u.rounds - 1), group, u.head * group, out, out_stride, w, 4);
 }
 
 // ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
@@ -1175,6 +1177,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 }
 
 // The parts of the rows whose tokens are split: a wave for each row and head.
+template <int DT>
 __global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, int heads, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
                                                              int tile_rows, unsigned units)
 {
@@ -1196,7 +1199,7 @@ __global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, int hea
     const int seen = causal ? max(length - count + last_row / group + 1, 0) : length;
     const int n = max((seen + chunk - 1) / chunk, 1);
     const int64_t slot = (((int64_t)b * kv.kv_heads + h / group) * parts.tiles + tile) * parts.splits * tile_rows + mine % tile_rows;
-    join_row<kKvMostDim>(kv, parts.sums, parts.tops, slot, slot + tile_rows, tile_rows, n, out + (int64_t)row * out_stride + h * kv.head_dim);
+    join_row<DT, true>(kv, parts.sums, parts.tops, slot, slot + tile_rows, tile_rows, n, out + (int64_t)row * out_stride + h * kv.head_dim);
 }
 
 // How a call is cut.
@@ -1225,9 +1228,16 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     const int64_t units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
     int64_t parts = 0;      // of rows that meet
     if (p.many) {
-        const int64_t wanted = std::max<int64_t>(1, 512 / units);
-        p.splits = (int)std::min(wanted, (most_length + 255) / 256);
-        p.chunk = (int)((((most_length + p.splits - 1) / p.splits) + 255) / 256 * 256);
+        // A workgroup for each compute unit or two, whichever has less to do one after the other: two on a unit take turns with its matrix units.
+        // With 48 tiles of rows over 1500 tokens 5 splits take 25.0 us and 8 take 26.2; with 96 over 1777 tokens 2 take 54.2 us and 5 take 47.5.
+        int64_t least = 0;
+        for (int each = 1; each <= 2; each++) {
+            const int64_t n = std::max<int64_t>(1, 256 * each / units), chunk = ((most_length + n - 1) / n + 63) / 64 * 64;
+            if (each == 1 || each * chunk < least) {
+                least = each * chunk;
+                p.chunk = (int)chunk;
+            }
+        }
         p.splits = (int)((most_length + p.chunk - 1) / p.chunk);
         p.blocks = units * p.splits;
         parts = p.splits > 1 ? p.blocks : 0;
@@ -1289,7 +1299,7 @@ int launch_many(const Call &c)
     if (st != VTL_HIP_OK || !c.sums)
         return st;
     const int64_t row_heads = (int64_t)c.kv.rows * c.heads;
-    hipLaunchKernelGGL(attention_many_join_kernel, dim3((unsigned)((row_heads + 3) / 4)), dim3(256), 0, current_stream(), c.kv, c.heads, c.causal, c.out,
+    hipLaunchKernelGGL(attention_many_join_kernel<(DT + 63) / 64 * 64>, dim3((unsigned)((row_heads + 3) / 4)), dim3(256), 0, current_stream(), c.kv, c.heads, c.causal, c.out,
                        c.out_stride, parts, c.plan.tile_rows, (unsigned)row_heads);
     return check_launch("attention_many_join_kernel");
 }
