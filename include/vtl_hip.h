@@ -32,8 +32,8 @@
  *     K-split partial sums of the matmuls, with f32 and f64 operands from
  *     K = 2048 on (for the gradients the dimension that is summed over, for
  *     column sums 128 rows), vtl_hip_linear_i8_requant,
- *     vtl_hip_linear_f32_dynquant with workspace == NULL, int8 operands that
- *     need repacking).  There is one such buffer per purpose and device,
+ *     vtl_hip_linear_f32_dynquant and vtl_hip_attention_i8_f32 with workspace ==
+ *     NULL, int8 operands that need repacking).  There is one such buffer per purpose and device,
  *     shared by every stream: calls that use it must not overlap on a device,
  *     i.e. issue them on one stream (or order the streams yourself).  Calls
  *     on whole host tensors have blocks of their own instead while no stream
@@ -316,7 +316,8 @@ typedef struct {
  * sequence b (rows == batch).  Rows of no sequence are left as they are.
  * What the device finds there is taken as follows, and nothing is read or written outside the cache and the call's tensors:
  * lengths below 0 and above max_pages * page_size (at most 2^28) count as these; starts outside 0 .. rows as the nearest of
- * these; a page number outside 0 .. num_pages - 1 is no page: tokens there are not written, are read as zeros and
+ * these, and they ascend (where they do not, a sequence has no rows or some that others have too, and what those get is
+ * undefined); a page number outside 0 .. num_pages - 1 is no page: tokens there are not written, are read as zeros and
  * are not attended to.  The same holds for rows in front of a sequence's first token (more rows than tokens): not
  * written, read as zeros, and attending to nothing where causal.
  * most_rows and most_length are the largest number of rows and the largest length of any sequence, for the host's choice of
@@ -347,10 +348,19 @@ int vtl_hip_kv_read_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *b
 /* Attention of the rows q [rows, heads, head_dim] over their sequences' keys and values (which hold the rows' own tokens
  * already): out[r, h] = sum_j w_j v_j, w = softmax over j of scale * q[r, h] . k_j, with head h reading key/value head
  * h / (heads / kv_heads).  causal: a row sees the tokens up to its own; otherwise all of its sequence's (an encoder's states, with
- * any number of rows).  A row that sees nothing gives zeros.  q and the weights enter the products with 22 bits, sums are f32; results
- * do not depend on what else is in the batch as long as the sizes that the host knows are the same.  heads is a multiple of kv_heads.
- * out may not share memory with q.  workspace: device memory of at least vtl_hip_attention_i8_workspace() bytes, 16-byte
- * aligned, for the parts of long sequences; NULL (with size 0): the library's own (see above). */
+ * any number of rows).  A row that sees nothing gives zeros, and one that sees a token with an infinite or NaN scale gives NaN.
+ * heads is a multiple of kv_heads; a batch of which 2^30 or more tiles would have to be counted is refused
+ * (VTL_HIP_ERR_UNSUPPORTED).  out may not share memory with q.
+ *
+ * q and the weights enter the products with 22 bits below the largest of q that are worked on together (up to 128 rows), sums
+ * are f32.  How sums are cut depends on the lengths and rows of the whole batch and on most_rows and most_length: the same call gives the same
+ * bits, a sequence in another batch need not.
+ *
+ * workspace: device memory of at least vtl_hip_attention_i8_workspace() bytes, 16-byte aligned, for the parts of sequences that
+ * several workgroups share; NULL (with size 0): the library's own (see above).  Calls that may overlap on a device need one each.  With few rows a
+ * sequence (heads / kv_heads times most_rows up to 32, or 16 above 128 dimensions) these parts meet in the same launch on
+ * counters kept per stream, for the first 16 streams of a device that make such a call; calls on further streams, and
+ * calls recorded into a graph, take a second launch and give the same bits, as all calls with more rows do. */
 size_t vtl_hip_attention_i8_workspace(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, int heads);
 int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, const float *q, int64_t q_stride,
                              int heads, float scale, int causal, float *out, int64_t out_stride, void *workspace,

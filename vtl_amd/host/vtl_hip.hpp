@@ -341,6 +341,105 @@ inline void relu_hip(HipTensor<T> &t)
         hip_check(vtl_hip_relu_f64((double *)t.data.ptr, (int64_t)t.size), "vtl_hip_relu_f64");
 }
 
+// `HipKVCache{pages; num_pages; page_size; kv_heads; head_dim}`: pages for the int8 keys and values of sequences.
+class HipKVCache {
+public:
+    HipStorage<uint8_t> pages;
+    int num_pages = 0, page_size = 0, kv_heads = 0, head_dim = 0;
+
+    HipKVCache(int num_pages_, int page_size_, int kv_heads_, int head_dim_, HipParams p = {})
+        : num_pages(num_pages_), page_size(page_size_), kv_heads(kv_heads_), head_dim(head_dim_)
+    {
+        const size_t bytes = vtl_hip_kv_cache_bytes(num_pages, page_size, kv_heads, head_dim);
+        if (!bytes)
+            throw std::invalid_argument("HipKVCache: no cache has these sizes");
+        pages = HipStorage<uint8_t>(bytes, p);
+    }
+    vtl_hip_kv_cache handle() const { return {pages.ptr, num_pages, page_size, kv_heads, head_dim}; }
+    void release() { pages.release(); }
+};
+
+// `HipKVBatch{page_table; lengths; starts; rows; most_rows; most_length}`: the sequences of a call, device tensors
+// that outlive it.  starts may be null: row b is then the last token of sequence b.
+class HipKVBatch {
+public:
+    const HipTensor<int32_t> *page_table, *lengths, *starts;
+    int rows, most_rows = 0, most_length = 0;
+
+    HipKVBatch(const HipTensor<int32_t> &page_table_, const HipTensor<int32_t> &lengths_, const HipTensor<int32_t> *starts_ = nullptr, int rows_ = 0,
+               int most_rows_ = 0, int most_length_ = 0)
+        : page_table(&page_table_), lengths(&lengths_), starts(starts_), rows(rows_), most_rows(most_rows_), most_length(most_length_)
+    {
+        if (!page_table->is_matrix() || lengths->size != (size_t)page_table->shape[0])
+            throw std::invalid_argument("HipKVBatch: a length for each row of the page table expected");
+        if (starts && starts->size != lengths->size + 1)
+            throw std::invalid_argument("HipKVBatch: one start more than lengths expected");
+        if (!starts)
+            rows = page_table->shape[0];
+    }
+    vtl_hip_kv_batch handle() const
+    {
+        return {page_table->shape[0], page_table->shape[1], (const int32_t *)page_table->data.ptr, (const int32_t *)lengths->data.ptr,
+                starts ? (const int32_t *)starts->data.ptr : nullptr, rows, most_rows, most_length};
+    }
+};
+
+// Address of column `first` of the f32 rows of t, and the elements from one row to the next.
+inline const float *kv_rows(const HipTensor<float> &t, const HipKVBatch &batch, size_t width, size_t first, int64_t &stride)
+{
+    if (t.rank() < 2 || t.shape[0] != batch.rows)
+        throw std::invalid_argument("a row for each of the batch expected");
+    const size_t columns = t.shape[0] ? t.size / (size_t)t.shape[0] : first + width;
+    if (first + width > columns)
+        throw std::invalid_argument("rows have fewer columns than the heads take");
+    stride = (int64_t)columns;
+    return t.data.ptr ? (const float *)t.data.ptr + first : nullptr;
+}
+
+// `kv_write_hip(cache, batch, k, v) !`: rows of keys and values, which may be columns of one tensor from k_first and
+// v_first on, quantized into the cache.
+inline void kv_write_hip(const HipKVCache &cache, const HipKVBatch &batch, const HipTensor<float> &k, const HipTensor<float> &v, size_t k_first = 0,
+                         size_t v_first = 0)
+{
+    const size_t width = (size_t)cache.kv_heads * cache.head_dim;
+    int64_t ks, vs;
+    const float *kp = kv_rows(k, batch, width, k_first, ks), *vp = kv_rows(v, batch, width, v_first, vs);
+    const vtl_hip_kv_cache c = cache.handle();
+    const vtl_hip_kv_batch b = batch.handle();
+    hip_check(vtl_hip_kv_write_f32(&c, &b, kp, ks, vp, vs), "vtl_hip_kv_write_f32");
+}
+
+// `kv_read_hip(cache, batch) !(&HipTensor[f32], &HipTensor[f32])`: the rows back, [rows, kv_heads, head_dim] each.
+inline std::pair<HipTensor<float>, HipTensor<float>> kv_read_hip(const HipKVCache &cache, const HipKVBatch &batch)
+{
+    const HipParams p{cache.pages.device_id};
+    HipTensor<float> k({batch.rows, cache.kv_heads, cache.head_dim}, p), v({batch.rows, cache.kv_heads, cache.head_dim}, p);
+    const int64_t stride = (int64_t)cache.kv_heads * cache.head_dim;
+    const vtl_hip_kv_cache c = cache.handle();
+    const vtl_hip_kv_batch b = batch.handle();
+    hip_check(vtl_hip_kv_read_f32(&c, &b, (float *)k.data.ptr, stride, (float *)v.data.ptr, stride), "vtl_hip_kv_read_f32");
+    return {std::move(k), std::move(v)};
+}
+
+// `attention_i8_hip(cache, batch, q, heads, scale, causal, workspace) !&HipTensor[f32]`: softmax(scale * q . k^T) . v of every
+// row over its sequence, [rows, heads, head_dim]; workspace may be null.
+inline HipTensor<float> attention_i8_hip(const HipKVCache &cache, const HipKVBatch &batch, const HipTensor<float> &q, int heads, float scale, bool causal,
+                                         const HipStorage<uint8_t> *workspace = nullptr, size_t q_first = 0)
+{
+    if (heads < 1)
+        throw std::invalid_argument("attention_i8_hip: a head at least");
+    int64_t stride;
+    const size_t width = (size_t)heads * cache.head_dim;
+    const float *qp = kv_rows(q, batch, width, q_first, stride);
+    HipTensor<float> out({batch.rows, heads, cache.head_dim}, HipParams{q.data.device_id});
+    const vtl_hip_kv_cache c = cache.handle();
+    const vtl_hip_kv_batch b = batch.handle();
+    hip_check(vtl_hip_attention_i8_f32(&c, &b, qp, stride, heads, scale, causal, (float *)out.data.ptr, (int64_t)width, workspace ? workspace->ptr : nullptr,
+                                       workspace ? workspace->size : 0),
+              "vtl_hip_attention_i8_f32");
+    return out;
+}
+
 // `linear_backward_hip_f32(grad, input, weight, bias_needs_grad) ![]&vtl.Tensor[f32]`
 // (cf. linear_backward_vulkan_f32, nn/internal/linear_vulkan_backward_d_vulkan.v:9-38):
 // host tensors in, {d_input[M,K], d_weight[N,K], d_bias[1,N]} out; d_bias is zeros
