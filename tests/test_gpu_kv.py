@@ -274,15 +274,15 @@ def test_same_results_twice_and_on_a_stream(stream):
         assert all(np.array_equal(got[0], g) for g in got[1:])
 
 
-@pytest.mark.parametrize("counts", [None, [4, 4, 4]])
+@pytest.mark.parametrize("counts", [None, [4, 4, 4], [20, 20, 20]])
 def test_recorded_into_a_graph(stream, counts):
     """Write and attention recorded once; between the replays the lengths and the new tokens change on the device, and the program
     makes calls of its own."""
     st, hiprt = stream
     heads, kv_heads, dim, n = 8, 2, 128, 3
-    most = [1400, 900, 64]
+    most = [1400, 900, 200]
     c = Cache(most, 32, kv_heads, dim, seed=14)
-    rows = 1 if counts is None else 4
+    rows = 1 if counts is None else counts[0]
     c.to_device()
     b = c.batch(counts)
     first = [1000, 500, 10]
@@ -347,6 +347,115 @@ def test_workspace_of_the_callers():
     if need > 16:
         with pytest.raises(capi.VtlHipError):
             attention_i8_hip(c.cache, b, t, 8, workspace=HipStorage.empty(need - 16, np.uint8))
+
+
+@pytest.mark.parametrize("lengths,counts,heads,kv_heads,dim", [([40, 900], None, 200, 1, 32), ([90], [2], 200, 1, 64), ([65], [3], 1000, 2, 16),
+                                                              ([400], None, 129, 1, 256)])
+def test_heads_that_share_keys(lengths, counts, heads, kv_heads, dim):
+    """More query heads on one key/value head than a tile has rows: a token's rows are in several tiles."""
+    test_attention(None, lengths, counts, 16, heads, kv_heads, dim, True)
+
+
+@pytest.mark.parametrize("counts", [1, 3, 9])
+def test_many_sequences(counts):
+    """More sequences than a wave has lanes, among them empty ones and ones with no rows."""
+    rng = np.random.default_rng(counts)
+    lengths = np.where(rng.random(150) < 0.2, 0, rng.integers(1, 150, 150))
+    each = None if counts == 1 else rng.integers(0, counts + 1, 150)
+    c = Cache(lengths, 16, 2, 64, seed=17, fill=False)
+    _, _, ks, vs = c.parts()
+    ks[:], vs[:] = rng.uniform(0.01, 0.05, ks.shape), rng.uniform(0.01, 0.05, vs.shape)      # codes are any
+    c.to_device()
+    b = c.batch(each)
+    q = normal(18, b.rows, 8, 64)
+    want, far = c.attend(q, 8, np.float32(0.125), True)
+    out = attention_i8_hip(c.cache, b, HipTensor.from_host(q), 8).cpu()
+    assert (np.abs(out - want) <= far).all()
+
+
+@pytest.mark.parametrize("counts,most_rows,most_length", [([50, 7, 300], 1, 10), ([50, 7, 300], 40, 64), ([3, 1, 2], 1, 1), ([600, 0, 1], 33, 100)])
+@pytest.mark.parametrize("dim", [64, 200])
+def test_more_than_the_host_knows(counts, most_rows, most_length, dim):
+    c = Cache([700, 90, 300], 32, 2, dim, seed=19).to_device()
+    b = c.batch(counts)
+    b.handle.most_rows, b.handle.most_length = most_rows, most_length
+    q = normal(20, b.rows, 4, dim)
+    want, far = c.attend(q, 4, np.float32(dim ** -0.5), True)
+    out = attention_i8_hip(c.cache, b, HipTensor.from_host(q), 4).cpu()
+    assert (np.abs(out - want) <= far).all()
+
+
+@pytest.mark.parametrize("counts", [[3, 2], [70, 40]])
+@pytest.mark.parametrize("dim", [64, 80, 33])
+@pytest.mark.parametrize("first", [0, 1, 4])
+def test_columns_of_wider_rows(counts, dim, first):
+    """q and the result in rows that are wider than they, from any column on."""
+    c = Cache([300, 90], 16, 2, dim, seed=22).to_device()
+    b = c.batch(counts)
+    q = normal(23, b.rows, 4, dim)
+    columns = 4 * dim + 7
+    wide = normal(24, b.rows, columns)
+    wide[:, first:first + 4 * dim] = q.reshape(b.rows, -1)
+    kept = normal(25, b.rows, columns + 2)
+    want, far = c.attend(q, 4, np.float32(0.125), True)
+    hq, ho = HipTensor.from_host(wide), HipTensor.from_host(kept)
+    capi.call("vtl_hip_attention_i8_f32", C.byref(c.cache.handle), C.byref(b.handle), hq.ptr + 4 * first, columns, 4, 0.125, 1, ho.ptr + 4 * first,
+              columns + 2, None, 0)
+    got = ho.cpu()
+    mine = np.zeros(columns + 2, bool)
+    mine[first:first + 4 * dim] = True
+    assert np.array_equal(got[:, ~mine], kept[:, ~mine])
+    assert (np.abs(got[:, mine].reshape(want.shape) - want) <= far).all()
+
+
+@pytest.mark.parametrize("counts", [[5, 4, 3], [90, 70, 40]])
+def test_starts_that_descend(guard_bands, counts):
+    """What such rows get is undefined, but nothing else is touched, and the next call finds everything as it was."""
+    c = Cache([900, 300, 500], 16, 2, 64, seed=26).to_device()
+    good = c.batch(counts)
+    rows = good.rows
+    q = HipTensor.from_host(normal(27, rows, 8, 64))
+    want = attention_i8_hip(c.cache, good, q, 8).cpu()
+    for starts in ([rows, 0, rows, 2], [2, rows, 1, rows], [rows, rows - 1, 1, 0], [0, -3, rows + 9, 0]):
+        bad = HipKVBatch(good.page_table, good.lengths, HipTensor.from_host(np.array(starts, np.int32)), rows)
+        for causal in (True, False):
+            attention_i8_hip(c.cache, bad, q, 8, causal=causal).release()
+        k, v = kv_read_hip(c.cache, bad)
+        k.release()
+        v.release()
+        assert np.array_equal(c.fetch(), c.host)
+        assert np.array_equal(attention_i8_hip(c.cache, good, q, 8).cpu(), want)
+
+
+@pytest.mark.parametrize("counts", [None, [33, 40, 2]])
+def test_two_streams_at_once(stream, counts):
+    """Calls on two streams, none waited for, each with a workspace of its own."""
+    st, hiprt = stream
+    c = Cache([3000, 700, 150], 64, 2, 128, seed=28).to_device()
+    b = c.batch(counts)
+    need = capi.lib().vtl_hip_attention_i8_workspace(C.byref(c.cache.handle), C.byref(b.handle), 16)
+    q = [HipTensor.from_host(normal(29 + i, b.rows, 16, 128)) for i in range(2)]
+    want = [attention_i8_hip(c.cache, b, t, 16).cpu() for t in q]
+    ws = [HipStorage.empty(max(need, 16), np.uint8) for _ in q]
+    other = C.c_void_p()
+    assert hiprt.hipStreamCreate(C.byref(other)) == 0
+    out = [[HipTensor.empty([b.rows, 16, 128], np.float32) for _ in range(8)] for _ in q]
+    try:
+        capi.call("vtl_hip_set_stream", other)
+        capi.call("vtl_hip_sync")
+        for turn in range(8):
+            for i, s in enumerate((st, other)):
+                capi.call("vtl_hip_set_stream", s)
+                capi.call("vtl_hip_attention_i8_f32", C.byref(c.cache.handle), C.byref(b.handle), q[i].ptr, 16 * 128, 16, 128 ** -0.5, 1,
+                          out[i][turn].ptr, 16 * 128, ws[i].ptr, ws[i].size)
+        for s in (other, st):
+            capi.call("vtl_hip_set_stream", s)
+            capi.call("vtl_hip_sync")
+        for i in range(2):
+            assert all(np.array_equal(t.cpu(), want[i]) for t in out[i])
+    finally:
+        capi.call("vtl_hip_set_stream", st)
+        hiprt.hipStreamDestroy(other)
 
 
 # -- as a decoder uses them ------------------------------------------------------------------------------
