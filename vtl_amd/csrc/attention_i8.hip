@@ -104,7 +104,7 @@ __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_u
 struct Group {
     int size;
     float part;
-    __device__ __forceinline__ explicit Group(int n) : size(n), part(1.0f / (float)n) {}
+    explicit Group(int n) : size(n), part(1.0f / (float)n) {}
     __device__ __forceinline__ void row(int token0, int head0, int behind, int &token, int &head) const
     {
         const unsigned n = (unsigned)head0 + (unsigned)behind;
@@ -149,7 +149,7 @@ struct Parts {
 // Tokens of a split of a sequence of which `seen` are of use.
 __device__ __forceinline__ int chunk_of(const Parts &parts, int seen)
 {
-    return max(parts.chunk, ((seen + parts.splits - 1) / parts.splits + 63) & ~63);
+    return max(parts.chunk, (int)((((unsigned)seen + parts.splits - 1) / (unsigned)parts.splits + 63) & ~63u));
 }
 
 // Parts of a row are made on one XCD and read on another: past the L2 caches, which are not coherent with each other.
@@ -246,12 +246,12 @@ struct Shares {
 // What a workgroup has, and where others' begins: q or q + 1 rounds each.
 struct Deal {
     int each, more;
-    __device__ __forceinline__ Deal(int total, int shares) : each(total / shares), more(total % shares) {}
+    __device__ __forceinline__ Deal(int total, int shares) : each((int)((unsigned)total / (unsigned)shares)), more(total - each * shares) {}
     __device__ __forceinline__ int start(int share) const { return share * each + min(share, more); }
     __device__ __forceinline__ int of(int round) const
     {
         const int mark = more * (each + 1);
-        return round < mark ? round / (each + 1) : more + (round - mark) / max(each, 1);
+        return round < mark ? (int)((unsigned)round / (unsigned)(each + 1)) : more + (int)((unsigned)(round - mark) / (unsigned)max(each, 1));
     }
 };
 
@@ -346,11 +346,12 @@ __device__ __forceinline__ Part part_of(const Kv &kv, int group, Finder<ROWS, ST
     u.count = __builtin_amdgcn_readlane(find.in.count, at);
     const int before = find.before + __builtin_amdgcn_readlane(find.in.upto - find.in.rounds, at);
     u.rounds = max((u.length + STEP - 1) / STEP, 1);
-    const int in = round - before, unit = in / u.rounds;
-    u.head = unit % kv.kv_heads;
-    u.row0 = unit / kv.kv_heads * ROWS;
+    // none is negative: a division of signs costs twice the code
+    const unsigned unit = (unsigned)(round - before) / (unsigned)u.rounds, tile = unit / (unsigned)kv.kv_heads;
+    u.head = (int)(unit - tile * (unsigned)kv.kv_heads);
+    u.row0 = (int)tile * ROWS;
     u.here = min(ROWS, u.count * group - u.row0);
-    u.first_round = before + unit * u.rounds;
+    u.first_round = before + (int)unit * u.rounds;
     u.begin = round - u.first_round;
     u.end = min(u.rounds, stop - u.first_round);
     return u;
@@ -374,7 +375,7 @@ __device__ __forceinline__ void join_unit(const Kv &kv, const Shares &shares, co
 }
 
 template <int DT, int NB, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_few_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, int heads,
+__global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_few_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, Group of,
                                                                                          float scale, int causal, float *__restrict__ out,
                                                                                          int64_t out_stride, Shares shares)
 {
@@ -386,18 +387,25 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
     __shared__ int level_part[WAVES];
     __shared__ int is_last;
 
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4;
-    const Group of(heads / kv.kv_heads);
-    const int group = of.size, share = blockIdx.x;
-    const Sequences<kRows, kStep> begin(kv, group, 0);
-    const Deal deal(all_rounds(kv, group, begin), shares.count);
+    const int share = blockIdx.x;
+    const Sequences<kRows, kStep> begin(kv, of.size, 0);
+    const Deal deal(all_rounds(kv, of.size, begin), shares.count);
     const int stop = deal.start(share + 1);
     Finder<kRows, kStep> find(begin);
+    // Opaque: what follows from it is worked out in each turn of the loop, of which there hardly are two, and not kept in registers that there are none of.
+    auto opaque = [](int v) {
+        asm volatile("" : "+s"(v));
+        return v;
+    };
     for (int round = deal.start(share); round < stop;) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int col = lane & 15, g = lane >> 4;
+        const int group = opaque(of.size);
         const Part u = part_of(kv, group, find, round, stop);
         const int b = u.b, length = u.length, first = u.first, count = u.count, head = u.head, row0 = u.row0, here = u.here, rows = count * group;
-        const int token0 = row0 / group, head0 = row0 - token0 * group;      // of the tile's first row
+        const int token0 = (int)((unsigned)row0 / (unsigned)group), head0 = row0 - token0 * group;      // of the tile's first row
         int token, of_token;
         of.row(token0, head0, here - 1, token, of_token);
         const int seen = causal ? max(length - count + token + 1, 0) : length;      // by its last
@@ -431,13 +439,14 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
         float4_t ks[4], vs[4];
         bool there;
         auto load_keys = [&](int j0) {
+            const int padded = opaque(kv.padded);
             const unsigned group16 = (unsigned)min(j0 + 16 * (col >> 2), to - 1) / 16;
             bool any;      // where there is no token, or no dimension, any codes do: q or the weight is 0 there
             const char *page = kv_page_or_any(kv, key_page, first_page, any);
             const unsigned slot = (group16 - kv_page_of(kv, group16) * kv.page_groups) * 16 + (col & 3);
 #pragma unroll
             for (int u = 0; u < DT / 64; u++) {
-                const unsigned c = 16 * (4 * u + g) < kv.padded ? 4 * u + g : 0;
+                const unsigned c = 16 * (4 * u + g) < padded ? 4 * u + g : 0;
                 const char *p = page + kv_key_at(kv, c, slot);
 #pragma unroll
                 for (int t = 0; t < 4; t++)
@@ -451,6 +460,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
             const unsigned place = group16 - kv_page_of(kv, group16) * kv.page_groups;
             const float *scales = reinterpret_cast<const float *>(page + kv_scales_at(kv)) + place * 16;
             const char *p = page + kv_value_at(kv, place, 0);
+            const int padded = opaque(kv.padded);
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 ks[t] = reinterpret_cast<const float4_t *>(scales)[t];
@@ -458,7 +468,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
             }
 #pragma unroll
             for (int i = 0; i < DT / 16; i++)
-                values[i] = *reinterpret_cast<const int4_t *>(p + ((16 * i < kv.padded ? 16 * i : 0) + col) * 16);
+                values[i] = *reinterpret_cast<const int4_t *>(p + ((16 * i < padded ? 16 * i : 0) + col) * 16);
         };
         if (j0 < to) {
             load_keys(j0);
@@ -470,6 +480,8 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
         // ---- rows of q as halves
 #pragma unroll
         for (int r = 0; r < kMine; r++) {
+            if (w + r * WAVES >= here)
+                break;      // what lies there gives sums that no row has
             float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < DT / 64; i++) {
@@ -629,39 +641,36 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
         __syncthreads();
         const bool alone = u.begin == 0 && u.end == u.rounds;
         const int64_t slot0 = (int64_t)part_slot(deal, share, u.first_round) * kRows;
+        const int part = min(lane & 15, WAVES - 1);      // lane i of 16 has what wave i knows of a row
+        const float level_mine = (float)level_part[part];
+        const int high = (int)row_max_16(level_mine);
         for (int r = w; r < here; r += WAVES) {
-            float t = -INFINITY, total = 0.0f, by[WAVES];
-            int high = -1000;
-#pragma unroll
-            for (int i = 0; i < WAVES; i++) {
-                t = fmaxf(t, top_part[i][r]);
-                high = max(high, level_part[i]);
-            }
-            const float off = t == -INFINITY ? 0.0f : t;
-#pragma unroll
-            for (int i = 0; i < WAVES; i++) {
-                const float e = __builtin_amdgcn_exp2f(top_part[i][r] - off), v = sum_part[i][r];
-                total += v == 0.0f ? 0.0f : v * e;
-                by[i] = v == 0.0f ? 0.0f : __builtin_ldexpf(e, level_part[i] - high);
-            }
+            const float top_mine = top_part[part][r], sum_mine = (lane & 15) < WAVES ? sum_part[part][r] : 0.0f;
+            const float t = row_max_16(top_mine), off = t == -INFINITY ? 0.0f : t, e = __builtin_amdgcn_exp2f(top_mine - off);
+            const float total = row_sum_16(sum_mine == 0.0f ? 0.0f : sum_mine * e);
+            const float over = total == 0.0f ? 0.0f : alone ? 1.0f / total : 1.0f;
+            // nothing: of a wave that had no tokens, or of a row that sees none
+            const float by = sum_mine == 0.0f ? 0.0f : __builtin_ldexpf(e, (int)level_mine - high);
             of.row(token0, head0, r, token, of_token);
             float *to_o = alone ? out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim
                                 : shares.sums + (slot0 + r) * kv.head_dim;
-            const float over = total == 0.0f ? 0.0f : alone ? 1.0f / total : 1.0f;
+            float v[DT / 64] = {};
+#pragma unroll
+            for (int k = 0; k < WAVES; k++) {
+                const float by_wave = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), k));
+#pragma unroll
+                for (int i = 0; i < DT / 64; i++)
+                    v[i] = __builtin_fmaf(o_part[k][r][lane + 64 * i], by_wave, v[i]);
+            }
 #pragma unroll
             for (int i = 0; i < DT / 64; i++) {
                 const int d = lane + 64 * i;
-                float v = 0.0f;
-#pragma unroll
-                for (int k = 0; k < WAVES; k++)
-                    if (by[k] != 0.0f)
-                        v = __builtin_fmaf(o_part[k][r][d], by[k], v);
-                v = total == 0.0f ? 0.0f : __builtin_ldexpf(v * over, high - 13);
+                v[i] = total == 0.0f ? 0.0f : __builtin_ldexpf(v[i] * over, high - 13);
                 if (d < kv.head_dim) {
                     if (alone)
-                        to_o[d] = v;
+                        to_o[d] = v[i];
                     else
-                        store_far(to_o + d, v);
+                        store_far(to_o + d, v[i]);
                 }
             }
             if (!alone && lane < 2)
@@ -734,7 +743,7 @@ struct alignas(16) ManyTile {
 constexpr int kSchedVector = 0x2, kSchedProduct = 0x8, kSchedRead = 0x100;
 
 template <int DT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, int heads, float scale,
+__global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, Group of, float scale,
                                                                     int causal, float *__restrict__ out, int64_t out_stride, Parts parts, int aligned)
 {
     constexpr int T = 64 * WAVES;
@@ -753,33 +762,30 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     __shared__ float q_most[WAVES];
     Tile *const tiles = reinterpret_cast<Tile *>(lds);
 
-    const Group of(heads / kv.kv_heads);
     const int group = of.size;
     // heads vary fastest: workgroups of one head meet in one L2 where their number is a multiple of eight; of a sequence's rows the last, which see most, go first
-    unsigned unit = blockIdx.x;
-    const unsigned both = (unsigned)kv.batch * kv.kv_heads;
-    const unsigned bh = unit % both;
-    unit /= both;
-    const int split_at = unit % (unsigned)parts.splits;
-    int tile = parts.tiles - 1 - (int)(unit / (unsigned)parts.splits);
-    const int head = bh % (unsigned)kv.kv_heads, b = bh / (unsigned)kv.kv_heads;
+    const unsigned bh = blockIdx.x;
+    const int split_at = blockIdx.y, b = (int)(bh / (unsigned)kv.kv_heads), head = (int)(bh - (unsigned)b * (unsigned)kv.kv_heads);
+    int tile = parts.tiles - 1 - (int)blockIdx.z;
     int length, first, count;
     kv_sequence(kv, b, length, first, count);
-    const int rows = count * group;
+    const int rows = count * group, tiles_here = (int)(((unsigned)rows + kRows - 1) / kRows);
 
-    for (; tile * kRows < rows; tile += parts.tiles) {
+    for (; tile < tiles_here; tile += parts.tiles) {
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));      // what follows from it is not kept in registers from one tile of rows to the next, of which there hardly is one
         const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int col = lane & 31, h = lane >> 5;
         const int row0 = tile * kRows + w * kManyRows;
-        const int row1 = min(row0, rows - 1), token0 = row1 / group, head0 = row1 - token0 * group;      // of the wave's first row
-        const int behind = max(min(kManyRows, rows - row0) - 1, 0);                                      // and how far behind it its last one is
+        const int tile_token = (int)((unsigned)(tile * kRows) / (unsigned)group), tile_head = tile * kRows - tile_token * group;      // of the first row
+        int token0, head0, last_token, of_last;      // of the wave's first row (where it has none, of the tile's last), and of the tile's last
+        of.row(tile_token, tile_head, min(w * kManyRows, rows - tile * kRows - 1), token0, head0);
+        of.row(tile_token, tile_head, min(kRows, rows - tile * kRows) - 1, last_token, of_last);
+        const int behind = max(min(kManyRows, rows - row0) - 1, 0);      // how far behind its first the wave's last row is
         const bool whole = tile >= parts.tiles;
         if (whole && split_at)
             break;
-        const int last_row = min((tile + 1) * kRows, rows) - 1;
-        const int seen = causal ? max(length - count + last_row / group + 1, 0) : length;
+        const int seen = causal ? max(length - count + last_token + 1, 0) : length;
         const int chunk = whole ? 0x7fffffc0 : chunk_of(parts, length);
         const int from = whole ? 0 : split_at * chunk;
         if (from >= seen && split_at)
@@ -1179,27 +1185,28 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 // The parts of the rows whose tokens are split: a wave for each row and head.
 template <int DT>
 __global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, int heads, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
-                                                             int tile_rows, unsigned units)
+                                                                  unsigned units)
 {
-    const unsigned unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (unit >= units)
-        return;
-    const int h = unit % (unsigned)heads, row = unit / (unsigned)heads;
-    int b, position;
-    if (!kv_row(kv, row, b, position))
-        return;
-    int first, count;
-    kv_rows_of(kv, b, first, count);
-    const int group = heads / kv.kv_heads, length = kv_length(kv, b);
-    const int mine = (row - first) * group + h % group, tile = mine / tile_rows;
-    const int chunk = chunk_of(parts, length);
-    if (tile >= parts.tiles || chunk >= length)
-        return;                                         // there already
-    const int last_row = min((tile + 1) * tile_rows, count * group) - 1;
-    const int seen = causal ? max(length - count + last_row / group + 1, 0) : length;
-    const int n = max((seen + chunk - 1) / chunk, 1);
-    const int64_t slot = (((int64_t)b * kv.kv_heads + h / group) * parts.tiles + tile) * parts.splits * tile_rows + mine % tile_rows;
-    join_row<DT, true>(kv, parts.sums, parts.tops, slot, slot + tile_rows, tile_rows, n, out + (int64_t)row * out_stride + h * kv.head_dim);
+    constexpr int tile_rows = kManyRows * 4;
+    const int group = heads / kv.kv_heads;
+    for (unsigned unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); unit < units; unit += gridDim.x * 4) {
+        const int row = (int)(unit / (unsigned)heads), h = (int)(unit - (unsigned)row * (unsigned)heads);
+        int b, position;
+        if (!kv_row(kv, row, b, position))
+            continue;
+        int first, count;
+        kv_rows_of(kv, b, first, count);
+        const int length = kv_length(kv, b), kv_head = (int)((unsigned)h / (unsigned)group);
+        const int mine = (row - first) * group + h - kv_head * group, tile = mine / tile_rows;
+        const int chunk = chunk_of(parts, length);
+        if (tile >= parts.tiles || chunk >= length)
+            continue;                                       // there already
+        const int last_row = min((tile + 1) * tile_rows, count * group) - 1;
+        const int seen = causal ? max(length - count + (int)((unsigned)last_row / (unsigned)group) + 1, 0) : length;
+        const int n = max((int)((unsigned)(seen + chunk - 1) / (unsigned)chunk), 1);
+        const int64_t slot = (((int64_t)b * kv.kv_heads + kv_head) * parts.tiles + tile) * parts.splits * tile_rows + mine % tile_rows;
+        join_row<DT, true>(kv, parts.sums, parts.tops, slot, slot + tile_rows, tile_rows, n, out + (int64_t)row * out_stride + h * kv.head_dim);
+    }
 }
 
 // How a call is cut.
@@ -1208,7 +1215,6 @@ struct Plan {
     int tile_rows, tiles;
     int splits, chunk;      // many rows: of the tokens of a tile
     int waves, shares;      // few rows
-    int64_t blocks;
     size_t sums_bytes, tops_bytes;
     size_t bytes() const { return sums_bytes + tops_bytes; }
 };
@@ -1225,9 +1231,15 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     p.many = rows > (kv.padded > 128 ? 16 : 32);
     p.tile_rows = p.many ? kManyRows * 4 : rows <= 16 ? 16 : 32;
     p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
-    const int64_t units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
+    int64_t units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
     int64_t parts = 0;      // of rows that meet
     if (p.many) {
+        // what a grid may have, and no more than a launch's worth where most_rows is not known; a workgroup goes on to the tiles behind
+        const int64_t both = (int64_t)kv.batch * kv.kv_heads;
+        if (both > 0xffffff)
+            return VTL_HIP_ERR_UNSUPPORTED;
+        p.tiles = (int)std::min<int64_t>(p.tiles, std::min<int64_t>(0xffff, std::max<int64_t>(1, (1 << 22) / both)));
+        units = both * p.tiles;
         // A workgroup for each compute unit or two, whichever has less to do one after the other: two on a unit take turns with its matrix units.
         // With 48 tiles of rows over 1500 tokens 5 splits take 25.0 us and 8 take 26.2; with 96 over 1777 tokens 2 take 54.2 us and 5 take 47.5.
         int64_t least = 0;
@@ -1239,8 +1251,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
             }
         }
         p.splits = (int)((most_length + p.chunk - 1) / p.chunk);
-        p.blocks = units * p.splits;
-        parts = p.splits > 1 ? p.blocks : 0;
+        parts = p.splits > 1 ? units * p.splits : 0;
     } else {
         p.waves = kv.padded <= 128 && (p.tile_rows == 16 || kv.padded <= 64) && units * ((most_length + 511) / 512) <= 256 ? 8 : 4;
         const int64_t step = 64 * p.waves;
@@ -1249,11 +1260,8 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
             return VTL_HIP_ERR_UNSUPPORTED;
         const int64_t at_once = p.waves == 8 || kv.padded > 128 || (kv.padded > 64 && p.tile_rows == 32) ? 256 : kMostShares;
         p.shares = (int)std::min(at_once, units * ((most_length + step - 1) / step));
-        p.blocks = p.shares;
         parts = p.shares > 1 ? 2 * p.shares : 0;
     }
-    if (p.blocks > 0x7fffffff)
-        return VTL_HIP_ERR_UNSUPPORTED;
     p.sums_bytes = ((size_t)parts * p.tile_rows * kv.head_dim * sizeof(float) + 255) & ~(size_t)255;
     p.tops_bytes = (size_t)parts * p.tile_rows * 2 * sizeof(float);
     return VTL_HIP_OK;
@@ -1278,9 +1286,9 @@ template <int DT, int NB, int WAVES>
 int launch_few(const Call &c)
 {
     const Shares shares{c.plan.shares, c.sums ? stream_slot(current_stream()) : -1, c.sums, c.tops};
-    const dim3 blocks((unsigned)c.plan.blocks);
-    hipLaunchKernelGGL((attention_few_kernel<DT, NB, WAVES>), blocks, dim3(64 * WAVES), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale, c.causal,
-                       c.out, c.out_stride, shares);
+    const dim3 blocks((unsigned)c.plan.shares);
+    hipLaunchKernelGGL((attention_few_kernel<DT, NB, WAVES>), blocks, dim3(64 * WAVES), 0, current_stream(), c.kv, c.q, c.q_stride,
+                       Group(c.heads / c.kv.kv_heads), c.scale, c.causal, c.out, c.out_stride, shares);
     const int st = check_launch("attention_few_kernel");
     if (st != VTL_HIP_OK || !c.sums || shares.counters >= 0)
         return st;
@@ -1292,15 +1300,16 @@ template <int DT>
 int launch_many(const Call &c)
 {
     const Parts parts{c.plan.tiles, c.plan.splits, c.plan.chunk, c.sums, c.tops};
-    hipLaunchKernelGGL((attention_many_kernel<DT, 4>), dim3((unsigned)c.plan.blocks), dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, c.heads, c.scale,
+    const dim3 blocks((unsigned)(c.kv.batch * c.kv.kv_heads), (unsigned)c.plan.splits, (unsigned)c.plan.tiles);
+    hipLaunchKernelGGL((attention_many_kernel<DT, 4>), blocks, dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, Group(c.heads / c.kv.kv_heads), c.scale,
                        c.causal, c.out, c.out_stride, parts,
                        c.kv.head_dim % 4 == 0 && c.q_stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(c.q) & 15));
     const int st = check_launch("attention_many_kernel");
     if (st != VTL_HIP_OK || !c.sums)
         return st;
-    const int64_t row_heads = (int64_t)c.kv.rows * c.heads;
-    hipLaunchKernelGGL(attention_many_join_kernel<(DT + 63) / 64 * 64>, dim3((unsigned)((row_heads + 3) / 4)), dim3(256), 0, current_stream(), c.kv, c.heads, c.causal, c.out,
-                       c.out_stride, parts, c.plan.tile_rows, (unsigned)row_heads);
+    const unsigned row_heads = (unsigned)c.kv.rows * (unsigned)c.heads;
+    hipLaunchKernelGGL(attention_many_join_kernel<(DT + 63) / 64 * 64>, dim3(std::min((row_heads + 3) / 4, 1u << 20)), dim3(256), 0, current_stream(), c.kv,
+                       c.heads, c.causal, c.out, c.out_stride, parts, row_heads);
     return check_launch("attention_many_join_kernel");
 }
 
