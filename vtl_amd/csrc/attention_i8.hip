@@ -142,7 +142,7 @@ struct Parts {
     int tiles;      // of rows, in the sequence with the most
     int splits;     // of the tokens
     int chunk;      // tokens of a split; more where a sequence is longer than the host knew
-    float *sums;    // [unit][split][row][head_dim]
+    float *sums;    // [unit][split][row][padded head_dim]
     float (*tops)[2];   // [unit][split][row]: maximum, sum of weights
 };
 
@@ -727,6 +727,7 @@ constexpr float kSlack = 5.0f;
 constexpr int kManyLevel = 9;     // the largest scale of a tile is brought to 2^9 .. 2^10
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
 
 // What the waves of a workgroup share of a tile.
 template <int DT, int TOKENS>
@@ -885,7 +886,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             constexpr int kLanes = DT / 4, kTogether = 64 / kLanes, kLoads = kManyRows / (kTogether ? kTogether : 1);
             static_assert(DT / 4 <= 64, "a row in one instruction");
             const int lane_row = lane / kLanes, d = lane % kLanes * 4;
-            if (aligned) {
+            if (aligned & 1) {
                 float4_t v[kLoads];
 #pragma unroll
                 for (int i = 0; i < kLoads; i++) {
@@ -928,7 +929,9 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 #pragma unroll
         for (int i = 0; i < WAVES; i++)
             most = fmaxf(most, q_most[i]);
-        unit_at = __builtin_amdgcn_readfirstlane(exponent_of(fminf(most * fabsf(to_exponents), 0x1.fffffep127f))) - 14;
+        // one multiplication for the scale and the unit, which is as large as to have that finite
+        unit_at = __builtin_amdgcn_readfirstlane(max(exponent_of(fminf(most * fabsf(to_exponents), 0x1.fffffep127f)) - 14, exponent_of(fabsf(to_exponents)) - 100));
+        const float to_unit = __builtin_ldexpf(to_exponents, -unit_at);
         half8_t x[DT / 16][2];
 #pragma unroll
         for (int i = 0; i < DT / 16; i++) {
@@ -938,7 +941,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 const float4_t four = *reinterpret_cast<const float4_t *>(&own[col][16 * i + 8 * h + k]);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    v[k + j] = __builtin_ldexpf(four[j] * to_exponents, -unit_at);
+                    v[k + j] = four[j] * to_unit;
             }
             split(v, x[i][0], x[i][1]);
         }
@@ -1149,8 +1152,8 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 
         sum = sum_across_32(sum);
         const bool alone = whole || chunk >= length;
-        // results by way of LDS, so that rows are written whole
-        const float by = sum == 0.0f ? 0.0f : alone ? 1.0f / sum : 1.0f;
+        // results by way of LDS, so that rows are written whole, in vectors where they are aligned (parts always are)
+        const float by = sum == 0.0f ? 0.0f : __builtin_ldexpf(alone ? 1.0f / sum : 1.0f, level_at - kManyLevel);
 #pragma unroll
         for (int i = 0; i < DT / 32; i++)
 #pragma unroll
@@ -1158,55 +1161,132 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 float4_t v;
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    v[j] = sum == 0.0f ? 0.0f : __builtin_ldexpf(o[i][k + j] * by, level_at - kManyLevel);
+                    v[j] = o[i][k + j] * by;
                 *reinterpret_cast<float4_t *>(&own[col][32 * i + 2 * k + 4 * h]) = v;
             }
         const int64_t slot0 = (((int64_t)bh * parts.tiles + tile) * parts.splits + split_at) * kRows + w * kManyRows;
-        if (!alone && h == 0 && row0 + col < rows)
-            {
+        if (!alone && h == 0 && row0 + col < rows) {
             parts.tops[slot0 + col][0] = off == kNone ? -INFINITY : off;
             parts.tops[slot0 + col][1] = sum;
         }
         __syncthreads();
-#pragma unroll 2
-        for (int r = 0; r < min(kManyRows, rows - row0); r++) {
-            of.row(token0, head0, r, token, of_token);
-            float *to_o = alone ? out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim
-                                : parts.sums + (slot0 + r) * kv.head_dim;
-#pragma unroll
-            for (int i = 0; i < (DT + 63) / 64; i++)
-                if (lane + 64 * i < kv.head_dim)
-                    to_o[lane + 64 * i] = own[r][lane + 64 * i];
+        if (!alone || aligned & 2) {
+            constexpr int kLanes = DT / 4, kTogether = 64 / kLanes;
+            const int lane_row = lane / kLanes, d = lane % kLanes * 4;
+            if (lane_row < kTogether && d < kv.head_dim)
+#pragma unroll 4
+                for (int r = lane_row; r < kManyRows; r += kTogether) {
+                    if (row0 + r >= rows)
+                        break;
+                    of.row(token0, head0, r, token, of_token);
+                    float *to_o = alone ? out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim
+                                        : parts.sums + (slot0 + r) * kv.padded;
+                    *reinterpret_cast<float4_t *>(to_o + d) = *reinterpret_cast<const float4_t *>(&own[r][d]);
+                }
+        } else {
+#pragma unroll 1
+            for (int r = 0; r < min(kManyRows, rows - row0); r++) {
+                of.row(token0, head0, r, token, of_token);
+                float *to_o = out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim;
+#pragma unroll 1
+                for (int at = lane; at < kv.head_dim; at += 64)
+                    to_o[at] = own[r][at];
+            }
         }
         __syncthreads();
     }
 }
 
-// The parts of the rows whose tokens are split: a wave for each row and head.
-template <int DT>
-__global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, int heads, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
-                                                                  unsigned units)
+// Where the tokens of a tile of rows are split: a row's parts put together, by as many lanes as have one of them in vectors.  The parts of a row
+// are all on their way at once (8 of them, which is most that there are), so that what bounds this is two trips to memory, one for the
+// sequence and one for the parts.  SHARE waves have the same rows and take turns with the parts where there are many.
+template <int DT, int SHARE>
+__global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, Group of, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
+                                                                  int aligned)
 {
-    constexpr int tile_rows = kManyRows * 4;
-    const int group = heads / kv.kv_heads;
-    for (unsigned unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); unit < units; unit += gridDim.x * 4) {
-        const int row = (int)(unit / (unsigned)heads), h = (int)(unit - (unsigned)row * (unsigned)heads);
-        int b, position;
-        if (!kv_row(kv, row, b, position))
-            continue;
-        int first, count;
-        kv_rows_of(kv, b, first, count);
-        const int length = kv_length(kv, b), kv_head = (int)((unsigned)h / (unsigned)group);
-        const int mine = (row - first) * group + h - kv_head * group, tile = mine / tile_rows;
-        const int chunk = chunk_of(parts, length);
-        if (tile >= parts.tiles || chunk >= length)
-            continue;                                       // there already
-        const int last_row = min((tile + 1) * tile_rows, count * group) - 1;
-        const int seen = causal ? max(length - count + (int)((unsigned)last_row / (unsigned)group) + 1, 0) : length;
-        const int n = max((int)((unsigned)(seen + chunk - 1) / (unsigned)chunk), 1);
-        const int64_t slot = (((int64_t)b * kv.kv_heads + kv_head) * parts.tiles + tile) * parts.splits * tile_rows + mine % tile_rows;
-        join_row<DT, true>(kv, parts.sums, parts.tops, slot, slot + tile_rows, tile_rows, n, out + (int64_t)row * out_stride + h * kv.head_dim);
+    constexpr int kRows = kManyRows * 4, kLanes = DT / 4, kTogether = 64 / kLanes, kAtOnce = 8;
+    const unsigned bh = blockIdx.x;
+    const int b = (int)(bh / (unsigned)kv.kv_heads), head = (int)(bh - (unsigned)b * (unsigned)kv.kv_heads), tile = blockIdx.z;
+    int length, first, count;
+    kv_sequence(kv, b, length, first, count);
+    const int group = of.size, rows = count * group, chunk = chunk_of(parts, length);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane_row = lane / kLanes, d = lane % kLanes * 4;
+    const int r = ((int)blockIdx.y * (4 / SHARE) + (SHARE == 1 ? w : 0)) * kTogether + lane_row, behind = min(kRows, rows - tile * kRows) - 1;
+    if (chunk >= length || tile * kRows >= rows || r - lane_row > behind)
+        return;      // there already, or no rows
+    const int tile_token = (int)((unsigned)(tile * kRows) / (unsigned)group), tile_head = tile * kRows - tile_token * group;
+    int token, of_token;
+    of.row(tile_token, tile_head, behind, token, of_token);
+    const int seen = causal ? max(length - count + token + 1, 0) : length;
+    const int n = max((int)((unsigned)(seen + chunk - 1) / (unsigned)chunk), 1);
+    const bool mine = lane_row < kTogether && r <= behind && d < kv.head_dim;
+    const int64_t slot = ((int64_t)bh * parts.tiles + tile) * parts.splits * kRows + min(r, behind);
+    const float *const sums = parts.sums + slot * kv.padded + (mine ? d : 0);
+    const float2_t *const tops = reinterpret_cast<const float2_t *>(parts.tops) + slot;
+    float top = -INFINITY, sum = 0.0f;
+    float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = SHARE == 1 ? 0 : w * kAtOnce; i0 < n; i0 += kAtOnce * SHARE) {
+        float2_t t[kAtOnce];
+        float4_t v[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            const int64_t at = (int64_t)min(i0 + k, n - 1) * kRows;
+            t[k] = tops[at];
+            v[k] = *reinterpret_cast<const float4_t *>(sums + at * kv.padded);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++)
+            now = fmaxf(now, t[k][0]);
+        const float off = now == -INFINITY ? 0.0f : now, keep = __builtin_amdgcn_exp2f(top - off);
+        top = now;
+        sum *= keep;
+        o *= keep;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            const float more = i0 + k < n ? t[k][1] : 0.0f, weight = more == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(t[k][0] - off);
+            sum = more == 0.0f ? sum : __builtin_fmaf(more, weight, sum);      // also where the weight is 0: a sum that is no number stays none
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                o[j] = weight == 0.0f ? o[j] : __builtin_fmaf(v[k][j], weight, o[j]);
+        }
     }
+    if (SHARE > 1) {
+        __shared__ float4_t o_part[SHARE][64];
+        __shared__ float top_part[SHARE][64], sum_part[SHARE][64];
+        o_part[w][lane] = o;
+        top_part[w][lane] = top;
+        sum_part[w][lane] = sum;
+        __syncthreads();
+        if (w)
+            return;
+        top = -INFINITY;
+        for (int i = 0; i < SHARE; i++)
+            top = fmaxf(top, top_part[i][lane]);
+        const float off = top == -INFINITY ? 0.0f : top;
+        sum = 0.0f;
+        o = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < SHARE; i++) {
+            const float more = sum_part[i][lane], weight = more == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top_part[i][lane] - off);
+            sum = more == 0.0f ? sum : __builtin_fmaf(more, weight, sum);
+            if (weight != 0.0f)
+                o += o_part[i][lane] * weight;
+        }
+    }
+    o = sum == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : o / sum;
+    of.row(tile_token, tile_head, min(r, behind), token, of_token);
+    float *const y = out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim + d;
+    if (!mine)
+        return;
+    if (aligned & 2) {
+        *reinterpret_cast<float4_t *>(y) = o;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (d + j < kv.head_dim)
+            y[j] = o[j];
 }
 
 // How a call is cut.
@@ -1262,7 +1342,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         p.shares = (int)std::min(at_once, units * ((most_length + step - 1) / step));
         parts = p.shares > 1 ? 2 * p.shares : 0;
     }
-    p.sums_bytes = ((size_t)parts * p.tile_rows * kv.head_dim * sizeof(float) + 255) & ~(size_t)255;
+    p.sums_bytes = ((size_t)parts * p.tile_rows * (p.many ? kv.padded : kv.head_dim) * sizeof(float) + 255) & ~(size_t)255;
     p.tops_bytes = (size_t)parts * p.tile_rows * 2 * sizeof(float);
     return VTL_HIP_OK;
 }
@@ -1301,15 +1381,24 @@ int launch_many(const Call &c)
 {
     const Parts parts{c.plan.tiles, c.plan.splits, c.plan.chunk, c.sums, c.tops};
     const dim3 blocks((unsigned)(c.kv.batch * c.kv.kv_heads), (unsigned)c.plan.splits, (unsigned)c.plan.tiles);
+    // rows that vectors of 16 bytes read, 1, and write, 2
+    auto vectors = [&](const float *p, int64_t stride) { return c.kv.head_dim % 4 == 0 && stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(p) & 15); };
+    const int aligned = (vectors(c.q, c.q_stride) ? 1 : 0) | (vectors(c.out, c.out_stride) ? 2 : 0);
     hipLaunchKernelGGL((attention_many_kernel<DT, 4>), blocks, dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, Group(c.heads / c.kv.kv_heads), c.scale,
                        c.causal, c.out, c.out_stride, parts,
-                       c.kv.head_dim % 4 == 0 && c.q_stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(c.q) & 15));
+                       aligned);
     const int st = check_launch("attention_many_kernel");
     if (st != VTL_HIP_OK || !c.sums)
         return st;
-    const unsigned row_heads = (unsigned)c.kv.rows * (unsigned)c.heads;
-    hipLaunchKernelGGL(attention_many_join_kernel<(DT + 63) / 64 * 64>, dim3(std::min((row_heads + 3) / 4, 1u << 20)), dim3(256), 0, current_stream(), c.kv,
-                       c.heads, c.causal, c.out, c.out_stride, parts, row_heads);
+    constexpr int kTogether = 256 / DT;      // rows of a wave
+    auto join = [&](auto kernel, int at_once) {
+        hipLaunchKernelGGL(kernel, dim3(blocks.x, (unsigned)(kManyRows * 4 / at_once), blocks.z), dim3(256), 0, current_stream(), c.kv,
+                           Group(c.heads / c.kv.kv_heads), c.causal, c.out, c.out_stride, parts, aligned);
+    };
+    if (c.plan.splits > 16)
+        join(attention_many_join_kernel<DT, 4>, kTogether);
+    else
+        join(attention_many_join_kernel<DT, 1>, 4 * kTogether);
     return check_launch("attention_many_join_kernel");
 }
 
