@@ -154,7 +154,6 @@ __device__ __forceinline__ int chunk_of(const Parts &parts, int seen)
 
 // Parts of a row are made on one XCD and read on another: past the L2 caches, which are not coherent with each other.
 __device__ __forceinline__ void store_far(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float load_far(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // Over each 16 lanes.
 __device__ __forceinline__ float row_max_16(float v)
@@ -172,55 +171,66 @@ __device__ __forceinline__ float row_sum_16(float v)
     return v;
 }
 
-// One row's parts, n of them, put together by a wave: the first is at `first`, the others at `second` and on, `apart` rows from each other.
-// THERE: they were written by an earlier launch, so the caches have nothing older.
-template <int DT, bool THERE>
-__device__ __forceinline__ void join_row(const Kv &kv, const float *sums, const float (*tops)[2], int64_t first, int64_t second, int apart, int n, float *y)
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+// Two of a part's numbers.  THERE: an earlier launch wrote them, so the caches have nothing older.
+template <bool THERE>
+__device__ __forceinline__ float2_t load_two(const float *p)
 {
-    auto slot = [&](int i) { return i ? second + (int64_t)(i - 1) * apart : first; };
-    auto load = [](const float *at) { return THERE ? *at : load_far(at); };
-    const int lane = threadIdx.x & 63;
-    // every lane has the maximum and the sum of a part
+    if (THERE)
+        return *reinterpret_cast<const float2_t *>(p);
+    return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Parts of a row put together: numbers begin .. begin + AT_ONCE - 1, then `step` further on, as long as there are any of n.  A lane has four values of the row;
+// they and the maxima and sums of AT_ONCE parts are on their way at once, so that what bounds this is a trip to memory for so many.
+struct Joined {
     float top = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < n; i += 64)
-        top = fmaxf(top, load(&tops[slot(i)][0]));
-    top = max_across_32(max_across_16(row_max_16(top)));
-    const float off = top == -INFINITY ? 0.0f : top;
-    float o[DT / 64] = {};
-    for (int i0 = 0; i0 < n; i0 += 64) {
-        const int i = i0 + lane;
-        float by = 0.0f;
-        if (i < n) {
-            const float t = load(&tops[slot(i)][0]), v = load(&tops[slot(i)][1]);
-            by = v == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(t - off);
-            sum += v == 0.0f ? 0.0f : v * by;
-        }
-        const int few = min(n - i0, 64);
-        constexpr int kAtOnce = 1024 / DT;      // parts on their way from memory
-        for (int k0 = 0; k0 < few; k0 += kAtOnce) {
-            float v[kAtOnce][DT / 64];
+    float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    template <int AT_ONCE, bool THERE, typename SLOT>
+    __device__ __forceinline__ void add(int begin, int n, int step, const float *sums, int pitch, const float (*tops)[2], SLOT slot)
+    {
+        for (int i0 = begin; i0 < n; i0 += step) {
+            float2_t t[AT_ONCE], v[AT_ONCE][2];
 #pragma unroll
-            for (int k = 0; k < kAtOnce; k++) {
-                const float *from = sums + slot(i0 + min(k0 + k, few - 1)) * kv.head_dim;
-#pragma unroll
-                for (int c = 0; c < DT / 64; c++)
-                    v[k][c] = lane + 64 * c < kv.head_dim ? load(from + lane + 64 * c) : 0.0f;
+            for (int k = 0; k < AT_ONCE; k++) {
+                const int64_t at = slot(min(i0 + k, n - 1));
+                t[k] = load_two<THERE>(tops[at]);
+                v[k][0] = load_two<THERE>(sums + at * pitch);
+                v[k][1] = load_two<THERE>(sums + at * pitch + 2);
             }
+            float now = top;
 #pragma unroll
-            for (int k = 0; k < kAtOnce; k++) {
-                const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), k0 + k));      // 0 behind the last part
+            for (int k = 0; k < AT_ONCE; k++)
+                now = fmaxf(now, t[k][0]);
+            const float off = now == -INFINITY ? 0.0f : now, keep = __builtin_amdgcn_exp2f(top - off);
+            top = now;
+            sum *= keep;
+            o *= keep;
 #pragma unroll
-                for (int c = 0; c < DT / 64; c++)
-                    o[c] = weight == 0.0f ? o[c] : __builtin_fmaf(v[k][c], weight, o[c]);
+            for (int k = 0; k < AT_ONCE; k++) {
+                const float more = i0 + k < n ? t[k][1] : 0.0f, weight = more == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(t[k][0] - off);
+                sum = more == 0.0f ? sum : __builtin_fmaf(more, weight, sum);      // also where the weight is 0: a sum that is no number stays none
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[j] = weight == 0.0f ? o[j] : __builtin_fmaf(v[k][j / 2][j % 2], weight, o[j]);
             }
         }
     }
-    sum = sum_across_32(sum_across_16(row_sum_16(sum)));
+    // The row's values d .. d + 3, of which there are `dims` at all.
+    __device__ __forceinline__ void store(float *y, int d, int dims, bool vectors) const
+    {
+        const float4_t v = sum == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : o / sum;
+        if (vectors)
+            *reinterpret_cast<float4_t *>(y + d) = v;
+        else
 #pragma unroll
-    for (int c = 0; c < DT / 64; c++)
-        if (lane + 64 * c < kv.head_dim)
-            y[lane + 64 * c] = sum == 0.0f ? 0.0f : o[c] / sum;
-}
+            for (int j = 0; j < 4; j++)
+                if (d + j < dims)
+                    y[d + j] = v[j];
+    }
+};
 
 // ---- few rows: a tile's rows are 16 or 32, all of a sequence's that read one key/value head ------------
 //
@@ -239,8 +249,9 @@ __device__ unsigned g_arrived[kStreamSlots][2 * kMostShares];
 struct Shares {
     int count;          // workgroups
     int counters;       // which set of counters; -1: parts are added up by a launch of their own
-    float *sums;        // [2 count][rows of a tile][head_dim]: parts of the first unit and of the last of each workgroup
+    float *sums;        // [2 count][rows of a tile][padded head_dim]: parts of the first unit and of the last of each workgroup
     float (*tops)[2];   // [2 count][rows of a tile]
+    int vectors;        // whether a row of the result is written in vectors of 16 bytes
 };
 
 // What a workgroup has, and where others' begins: q or q + 1 rounds each.
@@ -360,17 +371,25 @@ __device__ __forceinline__ Part part_of(const Kv &kv, int group, Finder<ROWS, ST
 // Where a workgroup leaves its part of a unit that begins with `first_round`.
 __device__ __forceinline__ int part_slot(const Deal &deal, int share, int first_round) { return 2 * share + (first_round > deal.start(share) ? 1 : 0); }
 
-// Adds up a unit's parts: a wave for a row.
+// Adds up a unit's parts: the first workgroup's may be its second, the others' are their first.
 template <int DT, int ROWS, bool THERE>
-__device__ __forceinline__ void join_unit(const Kv &kv, const Shares &shares, const Deal &deal, const Part &u, int share0, int share1, int group, int heads_first,
-                                          float *out, int64_t out_stride, int wave, int waves)
+__device__ __forceinline__ void join_unit(const Kv &kv, const Shares &shares, const Deal &deal, const Part &u, int share0, int share1, const Group &of, float *out,
+                                          int64_t out_stride, int wave, int waves)
 {
-    // the first workgroup's part may be its second; the others' are their first
+    constexpr int kLanes = DT / 4, kTogether = 64 / kLanes;
     const int64_t slot0 = part_slot(deal, share0, u.first_round);
-    for (int r = wave; r < u.here; r += waves) {
-        const int row = u.row0 + r;
-        join_row<DT, THERE>(kv, shares.sums, shares.tops, slot0 * ROWS + r, (int64_t)2 * (share0 + 1) * ROWS + r, 2 * ROWS, share1 - share0 + 1,
-                            out + (int64_t)(u.first + row / group) * out_stride + (heads_first + row % group) * kv.head_dim);
+    const int lane = threadIdx.x & 63, d = lane % kLanes * 4;
+    const int token0 = (int)((unsigned)u.row0 / (unsigned)of.size), head0 = u.row0 - token0 * of.size;
+    for (int r0 = wave * kTogether; r0 < u.here; r0 += waves * kTogether) {
+        const int r = min(r0 + lane / kLanes, u.here - 1);
+        const bool mine = r0 + lane / kLanes < u.here && d < kv.head_dim;
+        Joined row;
+        row.add<(DT > 128 ? 8 : 16), THERE>(0, share1 - share0 + 1, DT > 128 ? 8 : 16, shares.sums + (mine ? d : 0), kv.padded, shares.tops,
+                                           [&](int i) { return (i ? 2 * (share0 + i) : slot0) * ROWS + r; });
+        int token, of_token;
+        of.row(token0, head0, r, token, of_token);
+        if (mine)
+            row.store(out + (int64_t)(u.first + token) * out_stride + (u.head * of.size + of_token) * kv.head_dim, d, kv.head_dim, shares.vectors);
     }
 }
 
@@ -653,7 +672,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
             const float by = sum_mine == 0.0f ? 0.0f : __builtin_ldexpf(e, (int)level_mine - high);
             of.row(token0, head0, r, token, of_token);
             float *to_o = alone ? out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim
-                                : shares.sums + (slot0 + r) * kv.head_dim;
+                                : shares.sums + (slot0 + r) * kv.padded;
             float v[DT / 64] = {};
 #pragma unroll
             for (int k = 0; k < WAVES; k++) {
@@ -688,7 +707,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
             if (is_last) {
                 if (threadIdx.x == 0)
                     __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                join_unit<DT, kRows, false>(kv, shares, deal, u, share0, share1, group, head * group, out, out_stride, w, WAVES);
+                join_unit<DT, kRows, false>(kv, shares, deal, u, share0, share1, of, out, out_stride, w, WAVES);
             }
         }
         round = u.first_round + u.end;
@@ -697,10 +716,10 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
 
 // The parts of the units that several workgroups have: a workgroup for each that may have the first part of one.
 template <int DT, int NB, int WAVES>
-__global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, int heads, float *__restrict__ out, int64_t out_stride, Shares shares)
+__global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of, float *__restrict__ out, int64_t out_stride, Shares shares)
 {
     constexpr int kRows = 16 * NB, kStep = 64 * WAVES;
-    const int group = heads / kv.kv_heads, share = blockIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = of.size, share = blockIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Sequences<kRows, kStep> begin(kv, group, 0);
     const Deal deal(all_rounds(kv, group, begin), shares.count);
     const int stop = deal.start(share + 1);
@@ -710,7 +729,7 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, int head
     const Part u = part_of(kv, group, find, stop - 1, stop);
     if (u.end == u.rounds || deal.of(u.first_round) != share)
         return;
-    join_unit<DT, kRows, true>(kv, shares, deal, u, share, deal.of(u.first_round + u.rounds - 1), group, u.head * group, out, out_stride, w, 4);
+    join_unit<DT, kRows, true>(kv, shares, deal, u, share, deal.of(u.first_round + u.rounds - 1), of, out, out_stride, w, 4);
 }
 
 // ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
@@ -727,7 +746,6 @@ constexpr float kSlack = 5.0f;
 constexpr int kManyLevel = 9;     // the largest scale of a tile is brought to 2^9 .. 2^10
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
-typedef float float2_t __attribute__((ext_vector_type(2)));
 
 // What the waves of a workgroup share of a tile.
 template <int DT, int TOKENS>
@@ -1197,9 +1215,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     }
 }
 
-// Where the tokens of a tile of rows are split: a row's parts put together, by as many lanes as have one of them in vectors.  The parts of a row
-// are all on their way at once (8 of them, which is most that there are), so that what bounds this is two trips to memory, one for the
-// sequence and one for the parts.  SHARE waves have the same rows and take turns with the parts where there are many.
+// Where the tokens of a tile of rows are split: what bounds it is two trips to memory, one for the sequence and one for the parts.  SHARE waves have the same rows and take turns with the parts where there are many.
 template <int DT, int SHARE>
 __global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, Group of, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
                                                                   int aligned)
@@ -1222,71 +1238,33 @@ __global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, Group o
     const int n = max((int)((unsigned)(seen + chunk - 1) / (unsigned)chunk), 1);
     const bool mine = lane_row < kTogether && r <= behind && d < kv.head_dim;
     const int64_t slot = ((int64_t)bh * parts.tiles + tile) * parts.splits * kRows + min(r, behind);
-    const float *const sums = parts.sums + slot * kv.padded + (mine ? d : 0);
-    const float2_t *const tops = reinterpret_cast<const float2_t *>(parts.tops) + slot;
-    float top = -INFINITY, sum = 0.0f;
-    float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i0 = SHARE == 1 ? 0 : w * kAtOnce; i0 < n; i0 += kAtOnce * SHARE) {
-        float2_t t[kAtOnce];
-        float4_t v[kAtOnce];
-#pragma unroll
-        for (int k = 0; k < kAtOnce; k++) {
-            const int64_t at = (int64_t)min(i0 + k, n - 1) * kRows;
-            t[k] = tops[at];
-            v[k] = *reinterpret_cast<const float4_t *>(sums + at * kv.padded);
-        }
-        float now = top;
-#pragma unroll
-        for (int k = 0; k < kAtOnce; k++)
-            now = fmaxf(now, t[k][0]);
-        const float off = now == -INFINITY ? 0.0f : now, keep = __builtin_amdgcn_exp2f(top - off);
-        top = now;
-        sum *= keep;
-        o *= keep;
-#pragma unroll
-        for (int k = 0; k < kAtOnce; k++) {
-            const float more = i0 + k < n ? t[k][1] : 0.0f, weight = more == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(t[k][0] - off);
-            sum = more == 0.0f ? sum : __builtin_fmaf(more, weight, sum);      // also where the weight is 0: a sum that is no number stays none
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                o[j] = weight == 0.0f ? o[j] : __builtin_fmaf(v[k][j], weight, o[j]);
-        }
-    }
+    Joined joined;
+    joined.add<kAtOnce, true>(SHARE == 1 ? 0 : w * kAtOnce, n, kAtOnce * SHARE, parts.sums + (mine ? d : 0), kv.padded, parts.tops,
+                              [&](int i) { return slot + (int64_t)i * kRows; });
     if (SHARE > 1) {
         __shared__ float4_t o_part[SHARE][64];
         __shared__ float top_part[SHARE][64], sum_part[SHARE][64];
-        o_part[w][lane] = o;
-        top_part[w][lane] = top;
-        sum_part[w][lane] = sum;
+        o_part[w][lane] = joined.o;
+        top_part[w][lane] = joined.top;
+        sum_part[w][lane] = joined.sum;
         __syncthreads();
         if (w)
             return;
-        top = -INFINITY;
+        float top = -INFINITY;
         for (int i = 0; i < SHARE; i++)
             top = fmaxf(top, top_part[i][lane]);
         const float off = top == -INFINITY ? 0.0f : top;
-        sum = 0.0f;
-        o = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        joined = Joined();
         for (int i = 0; i < SHARE; i++) {
             const float more = sum_part[i][lane], weight = more == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top_part[i][lane] - off);
-            sum = more == 0.0f ? sum : __builtin_fmaf(more, weight, sum);
+            joined.sum = more == 0.0f ? joined.sum : __builtin_fmaf(more, weight, joined.sum);
             if (weight != 0.0f)
-                o += o_part[i][lane] * weight;
+                joined.o += o_part[i][lane] * weight;
         }
     }
-    o = sum == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : o / sum;
     of.row(tile_token, tile_head, min(r, behind), token, of_token);
-    float *const y = out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim + d;
-    if (!mine)
-        return;
-    if (aligned & 2) {
-        *reinterpret_cast<float4_t *>(y) = o;
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (d + j < kv.head_dim)
-            y[j] = o[j];
+    if (mine)
+        joined.store(out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim, d, kv.head_dim, aligned & 2);
 }
 
 // How a call is cut.
@@ -1342,7 +1320,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         p.shares = (int)std::min(at_once, units * ((most_length + step - 1) / step));
         parts = p.shares > 1 ? 2 * p.shares : 0;
     }
-    p.sums_bytes = ((size_t)parts * p.tile_rows * (p.many ? kv.padded : kv.head_dim) * sizeof(float) + 255) & ~(size_t)255;
+    p.sums_bytes = ((size_t)parts * p.tile_rows * kv.padded * sizeof(float) + 255) & ~(size_t)255;
     p.tops_bytes = (size_t)parts * p.tile_rows * 2 * sizeof(float);
     return VTL_HIP_OK;
 }
@@ -1360,19 +1338,22 @@ struct Call {
     Plan plan;
     float *sums;
     float (*tops)[2];
+    // Whether rows can be read and written in vectors of 16 bytes.
+    bool vectors(const float *p, int64_t stride) const { return kv.head_dim % 4 == 0 && stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(p) & 15); }
 };
 
 template <int DT, int NB, int WAVES>
 int launch_few(const Call &c)
 {
-    const Shares shares{c.plan.shares, c.sums ? stream_slot(current_stream()) : -1, c.sums, c.tops};
+    const Shares shares{c.plan.shares, c.sums ? stream_slot(current_stream()) : -1, c.sums, c.tops, c.vectors(c.out, c.out_stride)};
     const dim3 blocks((unsigned)c.plan.shares);
     hipLaunchKernelGGL((attention_few_kernel<DT, NB, WAVES>), blocks, dim3(64 * WAVES), 0, current_stream(), c.kv, c.q, c.q_stride,
                        Group(c.heads / c.kv.kv_heads), c.scale, c.causal, c.out, c.out_stride, shares);
     const int st = check_launch("attention_few_kernel");
     if (st != VTL_HIP_OK || !c.sums || shares.counters >= 0)
         return st;
-    hipLaunchKernelGGL((attention_few_join_kernel<DT, NB, WAVES>), blocks, dim3(256), 0, current_stream(), c.kv, c.heads, c.out, c.out_stride, shares);
+    hipLaunchKernelGGL((attention_few_join_kernel<DT, NB, WAVES>), blocks, dim3(256), 0, current_stream(), c.kv,
+                       Group(c.heads / c.kv.kv_heads), c.out, c.out_stride, shares);
     return check_launch("attention_few_join_kernel");
 }
 
@@ -1382,8 +1363,7 @@ int launch_many(const Call &c)
     const Parts parts{c.plan.tiles, c.plan.splits, c.plan.chunk, c.sums, c.tops};
     const dim3 blocks((unsigned)(c.kv.batch * c.kv.kv_heads), (unsigned)c.plan.splits, (unsigned)c.plan.tiles);
     // rows that vectors of 16 bytes read, 1, and write, 2
-    auto vectors = [&](const float *p, int64_t stride) { return c.kv.head_dim % 4 == 0 && stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(p) & 15); };
-    const int aligned = (vectors(c.q, c.q_stride) ? 1 : 0) | (vectors(c.out, c.out_stride) ? 2 : 0);
+    const int aligned = (c.vectors(c.q, c.q_stride) ? 1 : 0) | (c.vectors(c.out, c.out_stride) ? 2 : 0);
     hipLaunchKernelGGL((attention_many_kernel<DT, 4>), blocks, dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, Group(c.heads / c.kv.kv_heads), c.scale,
                        c.causal, c.out, c.out_stride, parts,
                        aligned);
