@@ -1311,7 +1311,13 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         p.splits = (int)((most_length + p.chunk - 1) / p.chunk);
         parts = p.splits > 1 ? units * p.splits : 0;
     } else {
-        p.waves = kv.padded <= 128 && (p.tile_rows == 16 || kv.padded <= 64) && units * ((most_length + 511) / 512) <= 256 ? 8 : 4;
+        // Eight waves, of which a unit has one workgroup, where they save the meeting of several (up to 512 tokens: 20 sequences with 8 heads of 128 values
+        // and 500 tokens take 11.5 us, with four waves 15.5), where the parts to meet are many (a sequence of 20000: 22.9 and 25.3) or a tile has
+        // half the bytes (8 sequences of 3001, 16 heads of 64 values: 18.7 and 20.0).  Else four, of which a compute unit has two workgroups that are not
+        // in step (48 sequences of 6000: 64.5 and 73.2; 2 of 3000: 11.8 and 13.0).
+        const bool eight = kv.padded <= 128 && (p.tile_rows == 16 || kv.padded <= 64);
+        const bool better = most_length <= 512 || kv.padded <= 64 ? units <= 256 : units <= 32 && most_length > 15 * 256;
+        p.waves = eight && better ? 8 : 4;
         const int64_t step = 64 * p.waves;
         // what the device counts in 32 bits
         if (((int64_t)kv.rows * group / p.tile_rows + kv.batch) * kv.kv_heads > kMostRounds / (kv.most_tokens / step + 1))
