@@ -120,7 +120,9 @@ ATTENDS = [  # lengths, rows of each (None: one, without starts), page, heads, k
     ([5, 200, 90], [5, 5, 5], 16, 16, 16, 64), ([900, 33], [8, 3], 32, 8, 2, 128), ([400, 64, 64], [2, 1, 4], 64, 16, 4, 72),
     ([64], [64], 64, 4, 2, 64), ([300], [300], 16, 8, 2, 128), ([1777, 1000, 201], [201, 90, 201], 32, 20, 4, 80),
     ([700], [130], 128, 6, 1, 256), ([257, 31], [257, 31], 16, 3, 3, 96), ([129, 500, 0, 64], [40, 33, 17, 65], 16, 4, 2, 128),
-    ([1500, 1500], [77, 77], 64, 12, 12, 64), ([5000], [35], 64, 1, 1, 64), ([4000, 70], [33, 1], 128, 2, 2, 100), ([2600], [20], 64, 1, 1, 256), ([333], [333], 48, 5, 1, 100), ([20], [65], 16, 2, 2, 16), ([2100], [65], 64, 8, 8, 128)]
+    ([1500, 1500], [77, 77], 64, 12, 12, 64), ([5000], [35], 64, 1, 1, 64), ([4000, 70], [33, 1], 128, 2, 2, 100), ([2600], [20], 64, 1, 1, 256),
+    ([3000, 2500], [20, 17], 64, 16, 16, 64), ([3000, 2500], [20, 17], 64, 16, 16, 128), (list(range(190, 230)), [18] * 40, 16, 8, 8, 64),
+    ([333], [333], 48, 5, 1, 100), ([20], [65], 16, 2, 2, 16), ([2100], [65], 64, 8, 8, 128)]
 
 
 @pytest.mark.parametrize("lengths,counts,page,heads,kv_heads,dim", ATTENDS)

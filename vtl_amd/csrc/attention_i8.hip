@@ -234,7 +234,9 @@ struct Joined {
 
 // ---- few rows: a tile's rows are 16 or 32, all of a sequence's that read one key/value head ------------
 //
-// Bound by the cache's bytes (2 D + 8 a token and head): so every wave takes tiles of 64 tokens for itself, straight from memory into the registers in
+// Bound by the cache's bytes (2 D + 8 a token and head; 2 sequences of 65000 tokens, 8 heads of 128: 275 MB in 60.6 us, 4.5 TB/s, where a copy of 2 GiB
+// moves 4.9; 48 of up to 6000: 64.5 us) and, where those are few, by the latencies behind each other and the code read for the first time (one of 300:
+// 8.7 us; 8 of 3001 with 5 rows each, 16 heads of 64: 18.7 us, 1.8 TB/s).  So every wave takes tiles of 64 tokens for itself, straight from memory into the registers in
 // the order in which the matrix units take them; keys of the next tile are on their way while the weights of one are made, its values while the next
 // one's scores are, and the pages of both are looked up a tile before.
 //
@@ -734,10 +736,14 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of
 
 // ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
 //
-// Bound by the matrix units (and nearly so by the vector units: ten operations a score, four of them the exponential).  A tile of 64 tokens is
-// made fp16 once for all waves, on its way into LDS; a tile is worked on while the next is written to the other half of LDS and the one behind
-// it is on its way from memory.  Pieces of 8 dimensions (keys) and of 8 tokens (values) lie together there, [piece][token or dimension][8], so that
-// a wave's operand is 512 consecutive bytes for each half wave.
+// Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 927 us, 1.11 PFLOP/s of fp16 products
+// (two halves for each), where the library's product of 8192 x 8192 x 8192 makes 1.22; the clock is down to 1.6 GHz then, and nothing but
+// those products, on such operands, takes 605 us.  A prompt of 4096: 282 us.  Vector work is nearly as much (ten operations a score, four of them the
+// exponential) and goes on beside the products.  A tile of 64 tokens (32 above 128 dimensions, where registers are short) is made fp16 once for all
+// waves, on its way into LDS; a tile is worked on while the next is written to the other half of LDS and the one behind it is on its way from
+// memory.  Pieces of 8 dimensions (keys) and of 8 tokens (values) lie together there, [piece][token or dimension][8], so that a wave's operand is 512
+// consecutive bytes for each half wave.  Where there are few tiles a workgroup's start and end are what counts (code read for the first time, q's way
+// in, the results' out): 4 x 77 rows over 1500 tokens, 12 heads of 64, take 18.2 us, 3 x 201 rows over up to 1777, 20 heads of 80, 37.
 //
 // The sums are brought to a new maximum only where a row's has risen by more than 2^kSlack: until then its weights are up to 2^kSlack, for
 // which the values' scales leave room (2^(kSlack + 10) is below fp16's largest number).
@@ -1286,7 +1292,10 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     const int64_t group = heads / kv.kv_heads, rows = most_rows * group;
     if ((int64_t)kv.rows * heads > 0x7fffffc0)
         return VTL_HIP_ERR_UNSUPPORTED;
-    p.many = rows > (kv.padded > 128 ? 16 : 32);
+    // Up to 32 rows are few (16 above 128 dimensions, as many as the registers hold): 8 sequences of 3001 tokens with 16 heads of 64 values take 27.3 us with
+    // 32 rows each, where the other kernel takes 46.9 with any number up to 128; of 128 values 49.1 and 64.1.  But 17 and more are many where there
+    // are no more than 256 tokens for a compute unit: 8 sequences of 300 take 19.0 us and 26.6, one of 3001 15.0 and 17.2.
+    p.many = rows > (kv.padded > 128 ? 16 : 32) || (rows > 16 && (int64_t)kv.batch * kv.kv_heads * most_length <= 256 * 256);
     p.tile_rows = p.many ? kManyRows * 4 : rows <= 16 ? 16 : 32;
     p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     int64_t units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
@@ -1299,7 +1308,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         p.tiles = (int)std::min<int64_t>(p.tiles, std::min<int64_t>(0xffff, std::max<int64_t>(1, (1 << 22) / both)));
         units = both * p.tiles;
         // A workgroup for each compute unit or two, whichever has less to do one after the other: two on a unit take turns with its matrix units.
-        // With 48 tiles of rows over 1500 tokens 5 splits take 25.0 us and 8 take 26.2; with 96 over 1777 tokens 2 take 54.2 us and 5 take 47.5.
+        // With 48 tiles of rows over 1500 tokens 5 splits take 18.4 us, 8 take 18.2 and 12 take 23; with 96 over 1777 tokens 2 take 44.8 us and 5 take 37.0.
         int64_t least = 0;
         for (int each = 1; each <= 2; each++) {
             const int64_t n = std::max<int64_t>(1, 256 * each / units), chunk = ((most_length + n - 1) / n + 63) / 64 * 64;
@@ -1381,6 +1390,7 @@ int launch_many(const Call &c)
         hipLaunchKernelGGL(kernel, dim3(blocks.x, (unsigned)(kManyRows * 4 / at_once), blocks.z), dim3(256), 0, current_stream(), c.kv,
                            Group(c.heads / c.kv.kv_heads), c.causal, c.out, c.out_stride, parts, aligned);
     };
+    // many parts: 128 rows over 8000 tokens with one head of 64 are done after 16.0 us, with a wave for a row's parts after 25.6
     if (c.plan.splits > 16)
         join(attention_many_join_kernel<DT, 4>, kTogether);
     else
