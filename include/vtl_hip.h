@@ -313,7 +313,8 @@ typedef struct {
 /* Which sequences a call works on.  page_table, lengths and starts are device pointers.  Sequence b has lengths[b] tokens
  * in the cache, the call's among them; token i is in slot i % page_size of page page_table[b, i / page_size].  Rows starts[b] ..
  * starts[b + 1] - 1 of the call's tensors are the LAST tokens of sequence b, in order; starts == NULL: row b is the last token of
- * sequence b (rows == batch).  Rows of no sequence are left as they are.
+ * sequence b (rows == batch).  Rows of no sequence are left as they are.  Up to 2^30 rows and sequences, and of these times heads
+ * as many as a launch can count: VTL_HIP_ERR_UNSUPPORTED beyond.
  * What the device finds there is taken as follows, and nothing is read or written outside the cache and the call's tensors:
  * lengths below 0 and above max_pages * page_size (at most 2^28) count as these; starts outside 0 .. rows as the nearest of
  * these, and they ascend (where they do not, a sequence has no rows or some that others have too, and what those get is
@@ -349,8 +350,7 @@ int vtl_hip_kv_read_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *b
  * already): out[r, h] = sum_j w_j v_j, w = softmax over j of scale * q[r, h] . k_j, with head h reading key/value head
  * h / (heads / kv_heads).  causal: a row sees the tokens up to its own; otherwise all of its sequence's (an encoder's states, with
  * any number of rows).  A row that sees nothing gives zeros, and one that sees a token with an infinite or NaN scale gives NaN.
- * heads is a multiple of kv_heads; a batch of which 2^30 or more tiles would have to be counted is refused
- * (VTL_HIP_ERR_UNSUPPORTED).  out may not share memory with q.
+ * heads is a multiple of kv_heads; rows times heads are below 2^31 - 64 (VTL_HIP_ERR_UNSUPPORTED beyond).  out may not share memory with q.
  *
  * q and the weights enter the products with 22 bits below the largest of q that are worked on together (up to 128 rows), sums
  * are f32.  How sums are cut depends on the lengths and rows of the whole batch and on most_rows and most_length: the same call gives the same

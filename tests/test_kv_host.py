@@ -63,6 +63,13 @@ def test_refused_tensors():
         assert calls(cache(), batch(max_pages=4000, most_length=100000), **more)[2] == E, more
 
 
+def test_more_than_is_counted():
+    u = capi.ERR_UNSUPPORTED
+    assert calls(cache(), batch(rows=(1 << 30) + 1, starts=ONE), q_stride=256, out=1 << 60) == [u] * 3
+    assert calls(cache(), batch(batch=(1 << 30) + 1, rows=(1 << 30) + 1), out=1 << 60) == [u] * 3
+    assert calls(cache(kv_heads=1000), batch(batch=1 << 24, rows=1 << 24), stride=64000, heads=1000, q_stride=64000, out_stride=64000, out=1 << 60) == [u] * 3
+
+
 def test_nothing_to_do():
     assert calls(cache(), batch(batch=0, rows=0, page_table=None, lengths=None), k=None, v=None, q=None, out=None) == [OK] * 3
     assert calls(cache(), batch(rows=0, starts=ONE)) == [OK] * 3

@@ -1305,7 +1305,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         const int64_t both = (int64_t)kv.batch * kv.kv_heads;
         if (both > 0xffffff)
             return VTL_HIP_ERR_UNSUPPORTED;
-        p.tiles = (int)std::min<int64_t>(p.tiles, std::min<int64_t>(0xffff, std::max<int64_t>(1, (1 << 22) / both)));
+        p.tiles = (int)std::min<int64_t>(p.tiles, std::min<int64_t>(0xffff, std::max<int64_t>(1, kKvMostBlocks / both)));
         units = both * p.tiles;
         // A workgroup for each compute unit or two, whichever has less to do one after the other: two on a unit take turns with its matrix units.
         // With 48 tiles of rows over 1500 tokens 5 splits take 18.4 us, 8 take 18.2 and 12 take 23; with 96 over 1777 tokens 2 take 44.8 us and 5 take 37.0.

@@ -263,9 +263,11 @@ int grid_of(const Kv &kv, const vtl_hip_kv_batch &b, int items, Rows &rows, unsi
     rows.groups = kv.starts ? (int)((most + 2 * kKvGroup - 2) / kKvGroup) : 1;
     const int seg = kv.padded <= 64 ? 16 : kv.padded <= 128 ? 32 : 64, at_once = 256 / seg;
     rows.parts = (items + at_once - 1) / at_once;
-    const int64_t all = (int64_t)rows.groups * kv.batch * rows.parts;
-    if (all > 0x7fffffff)
+    const int64_t a_group_each = (int64_t)kv.batch * rows.parts;
+    if (a_group_each > 0xffffff)      // workgroups of 256 that a grid may have
         return VTL_HIP_ERR_UNSUPPORTED;
+    rows.groups = (int)std::min<int64_t>(rows.groups, std::max<int64_t>(1, kKvMostBlocks / a_group_each));
+    const int64_t all = rows.groups * a_group_each;
     blocks = (unsigned)all;
     return VTL_HIP_OK;
 }

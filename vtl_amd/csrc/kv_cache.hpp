@@ -11,6 +11,8 @@ constexpr int kKvGroup = 16;                  // tokens that lie together for a 
 constexpr int kKvMostPage = 4096;
 constexpr int kKvMostDim = 256;
 constexpr int64_t kKvMostTokens = 1 << 28;    // of a sequence
+constexpr int kKvMostRows = 1 << 30;          // of a call, and sequences: what is counted past the last one fits 32 bits
+constexpr int kKvMostBlocks = 1 << 22;        // of a launch; what is behind is theirs too
 
 // A cache and the sequences of a call, by value.
 struct Kv {
@@ -36,6 +38,8 @@ inline int kv_sizes(const vtl_hip_kv_cache *c, const vtl_hip_kv_batch *b, Kv &kv
         return VTL_HIP_ERR_INVALID_ARG;
     if (b->batch > 0 && (!b->page_table || !b->lengths || (!b->starts && b->rows != b->batch)))
         return VTL_HIP_ERR_INVALID_ARG;
+    if (b->batch > kKvMostRows || b->rows > kKvMostRows)
+        return VTL_HIP_ERR_UNSUPPORTED;
     kv.pages = static_cast<char *>(c->pages);
     kv.num_pages = c->num_pages;
     kv.page_size = c->page_size;
