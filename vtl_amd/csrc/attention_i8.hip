@@ -945,7 +945,9 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 }
             }
         }
-        const float to_exponents = scale * kLog2e;
+        float to_exponents = scale;
+        asm volatile("" : "+s"(to_exponents));      // nor this
+        to_exponents *= kLog2e;
         most = wave_max(most);
         if (lane == 0)
             q_most[w] = most;
@@ -1099,7 +1101,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             // of a later tile: a product holds the vector units' issue for half of its time, which leaves room for four operations.
             constexpr int kSlots = DT / 16;      // products of a step
             half8_t p[2][2], v[2][DT / 32];
-            float e[8], vs[8];
+            float e[8], vs[8], of_tile = 0.0f;      // the tile's sum by itself: a long sequence's is rounded once a tile
             auto operand = [&](int step) {
 #pragma unroll
                 for (int c = 0; c < DT / 32; c++)
@@ -1117,7 +1119,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             // weight k of a step: first its exponential, and one slot later (its result takes a while) the rest
             auto raise = [&](int step, int k) { e[k] = __builtin_amdgcn_exp2f(s[step / 2][8 * (step % 2) + k]); };
             auto weigh = [&](int step, int k) {
-                sum += e[k];
+                of_tile += e[k];
                 e[k] *= vs[k];
                 if (k % 2)
                     split_two(e[k - 1], e[k], p[step % 2][0], p[step % 2][1], k / 2);
@@ -1171,6 +1173,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
+            sum += of_tile;
         }
         __syncthreads();      // the next tile of rows writes where this one reads
 
