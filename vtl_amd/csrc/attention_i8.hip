@@ -806,6 +806,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         int token0, head0, last_token, of_last;      // of the wave's first row (where it has none, of the tile's last), and of the tile's last
         of.row(tile_token, tile_head, min(w * kManyRows, rows - tile * kRows - 1), token0, head0);
         of.row(tile_token, tile_head, min(kRows, rows - tile * kRows) - 1, last_token, of_last);
+        const int keeper = rows - tile * kRows <= kRows - kManyRows ? WAVES - 1 : 0;      // makes the scales: the wave that has no rows, if there is one
         const int behind = max(min(kManyRows, rows - row0) - 1, 0);      // how far behind its first the wave's last row is
         const bool whole = tile >= parts.tiles;
         if (whole && split_at)
@@ -995,7 +996,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 
         if (from < to) {
             store(tiles[0]);
-            if (w == 0)
+            if (w == keeper)
                 store_scales(tiles[0]);
             fetch(from + TOKENS);
             look_up(from + 2 * TOKENS);
@@ -1005,7 +1006,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             const Tile &t = tiles[which];
             Tile &next = tiles[which ^ 1];
             __syncthreads();
-            if (w == 0)
+            if (w == keeper)
                 store_scales(next);
             if (j0 >= any_sees) {
                 store(next);
