@@ -736,14 +736,14 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of
 
 // ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
 //
-// Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 927 us, 1.11 PFLOP/s of fp16 products
+// Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 922 us, 1.12 PFLOP/s of fp16 products
 // (two halves for each), where the library's product of 8192 x 8192 x 8192 makes 1.22; the clock is down to 1.6 GHz then, and nothing but
-// those products, on such operands, takes 605 us.  A prompt of 4096: 282 us.  Vector work is nearly as much (ten operations a score, four of them the
+// those products, on such operands, takes 605 us.  A prompt of 4096: 279 us.  Vector work is nearly as much (ten operations a score, four of them the
 // exponential) and goes on beside the products.  A tile of 64 tokens (32 above 128 dimensions, where registers are short) is made fp16 once for all
 // waves, on its way into LDS; a tile is worked on while the next is written to the other half of LDS and the one behind it is on its way from
 // memory.  Pieces of 8 dimensions (keys) and of 8 tokens (values) lie together there, [piece][token or dimension][8], so that a wave's operand is 512
 // consecutive bytes for each half wave.  Where there are few tiles a workgroup's start and end are what counts (code read for the first time, q's way
-// in, the results' out): 4 x 77 rows over 1500 tokens, 12 heads of 64, take 18.2 us, 3 x 201 rows over up to 1777, 20 heads of 80, 37.
+// in, the results' out): 4 x 77 rows over 1500 tokens, 12 heads of 64, take 17.2 us, 3 x 201 rows over up to 1777, 20 heads of 80, 37.
 //
 // The sums are brought to a new maximum only where a row's has risen by more than 2^kSlack: until then its weights are up to 2^kSlack, for
 // which the values' scales leave room (2^(kSlack + 10) is below fp16's largest number).
@@ -767,7 +767,8 @@ struct alignas(16) ManyTile {
 // What __builtin_amdgcn_sched_group_barrier calls them.
 constexpr int kSchedVector = 0x2, kSchedProduct = 0x8, kSchedRead = 0x100;
 
-template <int DT, int WAVES>
+// SPLIT: whether tokens are split (a variant of its own: without, the prompt of 4096 takes 279 us for 282).
+template <int DT, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, Group of, float scale,
                                                                     int causal, float *__restrict__ out, int64_t out_stride, Parts parts, int aligned)
 {
@@ -790,7 +791,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     const int group = of.size;
     // heads vary fastest: workgroups of one head meet in one L2 where their number is a multiple of eight; of a sequence's rows the last, which see most, go first
     const unsigned bh = blockIdx.x;
-    const int split_at = blockIdx.y, b = (int)(bh / (unsigned)kv.kv_heads), head = (int)(bh - (unsigned)b * (unsigned)kv.kv_heads);
+    const int split_at = SPLIT ? blockIdx.y : 0, b = (int)(bh / (unsigned)kv.kv_heads), head = (int)(bh - (unsigned)b * (unsigned)kv.kv_heads);
     int tile = parts.tiles - 1 - (int)blockIdx.z;
     int length, first, count;
     kv_sequence(kv, b, length, first, count);
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         of.row(tile_token, tile_head, min(kRows, rows - tile * kRows) - 1, last_token, of_last);
         const int keeper = rows - tile * kRows <= kRows - kManyRows ? WAVES - 1 : 0;      // makes the scales: the wave that has no rows, if there is one
         const int behind = max(min(kManyRows, rows - row0) - 1, 0);      // how far behind its first the wave's last row is
-        const bool whole = tile >= parts.tiles;
+        const bool whole = !SPLIT || tile >= parts.tiles;
         if (whole && split_at)
             break;
         const int seen = causal ? max(length - count + last_token + 1, 0) : length;
@@ -1312,7 +1313,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         p.tiles = (int)std::min<int64_t>(p.tiles, std::min<int64_t>(0xffff, std::max<int64_t>(1, kKvMostBlocks / both)));
         units = both * p.tiles;
         // A workgroup for each compute unit or two, whichever has less to do one after the other: two on a unit take turns with its matrix units.
-        // With 48 tiles of rows over 1500 tokens 5 splits take 18.4 us, 8 take 18.2 and 12 take 23; with 96 over 1777 tokens 2 take 44.8 us and 5 take 37.0.
+        // With 48 tiles of rows over 1500 tokens 5 splits take 17.3 us, 8 take 18.2 and 12 take 23; with 96 over 1777 tokens 2 take 44.8 us and 5 take 37.0.
         int64_t least = 0;
         for (int each = 1; each <= 2; each++) {
             const int64_t n = std::max<int64_t>(1, 256 * each / units), chunk = ((most_length + n - 1) / n + 63) / 64 * 64;
@@ -1383,7 +1384,7 @@ int launch_many(const Call &c)
     const dim3 blocks((unsigned)(c.kv.batch * c.kv.kv_heads), (unsigned)c.plan.splits, (unsigned)c.plan.tiles);
     // rows that vectors of 16 bytes read, 1, and write, 2
     const int aligned = (c.vectors(c.q, c.q_stride) ? 1 : 0) | (c.vectors(c.out, c.out_stride) ? 2 : 0);
-    hipLaunchKernelGGL((attention_many_kernel<DT, 4>), blocks, dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, Group(c.heads / c.kv.kv_heads), c.scale,
+    hipLaunchKernelGGL((c.sums ? attention_many_kernel<DT, 4, true> : attention_many_kernel<DT, 4, false>), blocks, dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, Group(c.heads / c.kv.kv_heads), c.scale,
                        c.causal, c.out, c.out_stride, parts,
                        aligned);
     const int st = check_launch("attention_many_kernel");
