@@ -352,7 +352,7 @@ int vtl_hip_kv_read_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *b
  * any number of rows).  A row that sees nothing gives zeros, and one that sees a token with an infinite or NaN scale gives NaN.
  * heads is a multiple of kv_heads; rows times heads are below 2^31 - 64 (VTL_HIP_ERR_UNSUPPORTED beyond).  out may not share memory with q.
  *
- * q and the weights enter the products with 22 bits below the largest of q that are worked on together (up to 128 rows), sums
+ * q and the weights enter the products with 22 bits below the largest of q that are worked on together (up to 256 rows), sums
  * are f32.  How sums are cut depends on the lengths and rows of the whole batch and on most_rows and most_length: the same call gives the same
  * bits, a sequence in another batch need not.
  *

@@ -100,7 +100,7 @@ __device__ __forceinline__ float max_across_32(float v)
 __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255) - 127; }
 
 // Rows of a tile are tokens of `size` heads each: which token and which of its heads a row is, given those of the tile's first row and how far behind it
-// (less than 128) the row is.
+// (less than 256) the row is.
 struct Group {
     int size;
     float part;
@@ -108,7 +108,7 @@ struct Group {
     __device__ __forceinline__ void row(int token0, int head0, int behind, int &token, int &head) const
     {
         const unsigned n = (unsigned)head0 + (unsigned)behind;
-        int more = (int)((float)n * part);      // at most 128: no further off than by one
+        int more = (int)((float)n * part);      // at most 256: no further off than by one
         head = (int)(n - (unsigned)more * (unsigned)size);
         more += head < 0 ? -1 : head >= size ? 1 : 0;
         head += head < 0 ? size : head >= size ? -size : 0;
@@ -736,14 +736,14 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of
 
 // ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
 //
-// Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 922 us, 1.12 PFLOP/s of fp16 products
+// Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 871 us, 1.18 PFLOP/s of fp16 products
 // (two halves for each), where the library's product of 8192 x 8192 x 8192 makes 1.22; the clock is down to 1.6 GHz then, and nothing but
-// those products, on such operands, takes 605 us.  A prompt of 4096: 279 us.  Vector work is nearly as much (ten operations a score, four of them the
+// those products, on such operands, takes 605 us.  A prompt of 4096: 256 us.  Vector work is nearly as much (ten operations a score, four of them the
 // exponential) and goes on beside the products.  A tile of 64 tokens (32 above 128 dimensions, where registers are short) is made fp16 once for all
 // waves, on its way into LDS; a tile is worked on while the next is written to the other half of LDS and the one behind it is on its way from
 // memory.  Pieces of 8 dimensions (keys) and of 8 tokens (values) lie together there, [piece][token or dimension][8], so that a wave's operand is 512
 // consecutive bytes for each half wave.  Where there are few tiles a workgroup's start and end are what counts (code read for the first time, q's way
-// in, the results' out): 4 x 77 rows over 1500 tokens, 12 heads of 64, take 17.2 us, 3 x 201 rows over up to 1777, 20 heads of 80, 37.
+// in, the results' out): 4 x 77 rows over 1500 tokens, 12 heads of 64, take 17.2 us, 3 x 201 rows over up to 1777, 20 heads of 80, 35.
 //
 // The sums are brought to a new maximum only where a row's has risen by more than 2^kSlack: until then its weights are up to 2^kSlack, for
 // which the values' scales leave room (2^(kSlack + 10) is below fp16's largest number).
@@ -767,7 +767,7 @@ struct alignas(16) ManyTile {
 // What __builtin_amdgcn_sched_group_barrier calls them.
 constexpr int kSchedVector = 0x2, kSchedProduct = 0x8, kSchedRead = 0x100;
 
-// SPLIT: whether tokens are split (a variant of its own: without, the prompt of 4096 takes 279 us for 282).
+// SPLIT: whether tokens are split (a variant of its own: without, a prompt of 4096 takes a hundredth less).
 template <int DT, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, Group of, float scale,
                                                                     int causal, float *__restrict__ out, int64_t out_stride, Parts parts, int aligned)
@@ -1227,11 +1227,11 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 }
 
 // Where the tokens of a tile of rows are split: what bounds it is two trips to memory, one for the sequence and one for the parts.  SHARE waves have the same rows and take turns with the parts where there are many.
-template <int DT, int SHARE>
+template <int DT, int WAVES, int SHARE>
 __global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, Group of, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
                                                                   int aligned)
 {
-    constexpr int kRows = kManyRows * 4, kLanes = DT / 4, kTogether = 64 / kLanes, kAtOnce = 8;
+    constexpr int kRows = kManyRows * WAVES, kLanes = DT / 4, kTogether = 64 / kLanes, kAtOnce = 8;
     const unsigned bh = blockIdx.x;
     const int b = (int)(bh / (unsigned)kv.kv_heads), head = (int)(bh - (unsigned)b * (unsigned)kv.kv_heads), tile = blockIdx.z;
     int length, first, count;
@@ -1283,7 +1283,8 @@ struct Plan {
     bool many;
     int tile_rows, tiles;
     int splits, chunk;      // many rows: of the tokens of a tile
-    int waves, shares;      // few rows
+    int waves;              // of a workgroup
+    int shares;             // few rows
     size_t sums_bytes, tops_bytes;
     size_t bytes() const { return sums_bytes + tops_bytes; }
 };
@@ -1301,7 +1302,14 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     // 32 rows each, where the other kernel takes 46.9 with any number up to 128; of 128 values 49.1 and 64.1.  But 17 and more are many where there
     // are no more than 256 tokens for a compute unit: 8 sequences of 300 take 19.0 us and 26.6, one of 3001 15.0 and 17.2.
     p.many = rows > (kv.padded > 128 ? 16 : 32) || (rows > 16 && (int64_t)kv.batch * kv.kv_heads * most_length <= 256 * 256);
-    p.tile_rows = p.many ? kManyRows * 4 : rows <= 16 ? 16 : 32;
+    // Many rows: eight waves share the codes that are made fp16 and brought to LDS once, and have a compute unit for themselves, where there is enough to do, four
+    // tiles of tokens for each of them (a row sees half of its sequence's new tokens), and their rows do not lie idle.  2048 rows behind 14336 tokens, 32 heads of
+    // 128 on 8: 908 us and 958 with four waves on the same card, a prompt of 4096 266 and 286, 512 rows behind 29500 442 and 518; but a prompt of
+    // 1000 48.4 and 44.7, 40 rows over 3000 23.0 and 20.5, 4 x 70 with 8 x 4 heads of 64 (three halves of tiles) 36.9 and 34.2.
+    const int64_t halves = (rows + kManyRows * 4 - 1) / (kManyRows * 4);      // tiles of four waves' rows
+    const bool enough = (int64_t)kv.batch * kv.kv_heads * ((halves + 1) / 2) * (most_length - std::min(most_rows, most_length) / 2) >= 256 * 256;
+    p.waves = p.many && kv.padded <= 128 && enough && (halves % 2 == 0 || halves > 8) ? 8 : 4;
+    p.tile_rows = p.many ? kManyRows * p.waves : rows <= 16 ? 16 : 32;
     p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     int64_t units = (int64_t)kv.batch * kv.kv_heads * p.tiles;
     int64_t parts = 0;      // of rows that meet
@@ -1315,7 +1323,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         // A workgroup for each compute unit or two, whichever has less to do one after the other: two on a unit take turns with its matrix units.
         // With 48 tiles of rows over 1500 tokens 5 splits take 17.3 us, 8 take 18.2 and 12 take 23; with 96 over 1777 tokens 2 take 44.8 us and 5 take 37.0.
         int64_t least = 0;
-        for (int each = 1; each <= 2; each++) {
+        for (int each = 1; each <= 8 / p.waves; each++) {
             const int64_t n = std::max<int64_t>(1, 256 * each / units), chunk = ((most_length + n - 1) / n + 63) / 64 * 64;
             if (each == 1 || each * chunk < least) {
                 least = each * chunk;
@@ -1377,37 +1385,39 @@ int launch_few(const Call &c)
     return check_launch("attention_few_join_kernel");
 }
 
-template <int DT>
+template <int DT, int WAVES>
 int launch_many(const Call &c)
 {
     const Parts parts{c.plan.tiles, c.plan.splits, c.plan.chunk, c.sums, c.tops};
+    const Group of(c.heads / c.kv.kv_heads);
     const dim3 blocks((unsigned)(c.kv.batch * c.kv.kv_heads), (unsigned)c.plan.splits, (unsigned)c.plan.tiles);
     // rows that vectors of 16 bytes read, 1, and write, 2
     const int aligned = (c.vectors(c.q, c.q_stride) ? 1 : 0) | (c.vectors(c.out, c.out_stride) ? 2 : 0);
-    hipLaunchKernelGGL((c.sums ? attention_many_kernel<DT, 4, true> : attention_many_kernel<DT, 4, false>), blocks, dim3(256), 0, current_stream(), c.kv, c.q, c.q_stride, Group(c.heads / c.kv.kv_heads), c.scale,
-                       c.causal, c.out, c.out_stride, parts,
-                       aligned);
+    hipLaunchKernelGGL((c.sums ? attention_many_kernel<DT, WAVES, true> : attention_many_kernel<DT, WAVES, false>), blocks, dim3(64 * WAVES), 0,
+                       current_stream(), c.kv, c.q, c.q_stride, of, c.scale, c.causal, c.out, c.out_stride, parts, aligned);
     const int st = check_launch("attention_many_kernel");
     if (st != VTL_HIP_OK || !c.sums)
         return st;
     constexpr int kTogether = 256 / DT;      // rows of a wave
     auto join = [&](auto kernel, int at_once) {
-        hipLaunchKernelGGL(kernel, dim3(blocks.x, (unsigned)(kManyRows * 4 / at_once), blocks.z), dim3(256), 0, current_stream(), c.kv,
-                           Group(c.heads / c.kv.kv_heads), c.causal, c.out, c.out_stride, parts, aligned);
+        hipLaunchKernelGGL(kernel, dim3(blocks.x, (unsigned)(kManyRows * WAVES / at_once), blocks.z), dim3(256), 0, current_stream(), c.kv, of, c.causal,
+                           c.out, c.out_stride, parts, aligned);
     };
     // many parts: 128 rows over 8000 tokens with one head of 64 are done after 16.0 us, with a wave for a row's parts after 25.6
     if (c.plan.splits > 16)
-        join(attention_many_join_kernel<DT, 4>, kTogether);
+        join(attention_many_join_kernel<DT, WAVES, 4>, kTogether);
     else
-        join(attention_many_join_kernel<DT, 1>, 4 * kTogether);
+        join(attention_many_join_kernel<DT, WAVES, 1>, 4 * kTogether);
     return check_launch("attention_many_join_kernel");
 }
 
 int launch_attention(const Call &c)
 {
     const int padded = c.kv.padded;
+    if (c.plan.many && c.plan.waves == 8)
+        return padded <= 64 ? launch_many<64, 8>(c) : padded <= 96 ? launch_many<96, 8>(c) : launch_many<128, 8>(c);
     if (c.plan.many)
-        return padded <= 64 ? launch_many<64>(c) : padded <= 96 ? launch_many<96>(c) : padded <= 128 ? launch_many<128>(c) : launch_many<256>(c);
+        return padded <= 64 ? launch_many<64, 4>(c) : padded <= 96 ? launch_many<96, 4>(c) : padded <= 128 ? launch_many<128, 4>(c) : launch_many<256, 4>(c);
     if (c.plan.tile_rows == 16) {
         if (c.plan.waves == 8)
             return padded <= 64 ? launch_few<64, 1, 8>(c) : launch_few<128, 1, 8>(c);
