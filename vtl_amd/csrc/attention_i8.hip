@@ -1320,16 +1320,26 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
             return VTL_HIP_ERR_UNSUPPORTED;
         p.tiles = (int)std::min<int64_t>(p.tiles, std::min<int64_t>(0xffff, std::max<int64_t>(1, kKvMostBlocks / both)));
         units = both * p.tiles;
-        // A workgroup for each compute unit or two, whichever has less to do one after the other: two on a unit take turns with its matrix units.
-        // With 48 tiles of rows over 1500 tokens 5 splits take 17.3 us, 8 take 18.2 and 12 take 23; with 96 over 1777 tokens 2 take 44.8 us and 5 take 37.0.
+        // Whatever has least to do one after the other.  Four waves: a workgroup for each compute unit or two, which take turns with its matrix units
+        // (48 tiles of rows over 1500 tokens: 5 splits take 17.3 us, 8 take 18.2 and 12 take 23; 96 over 1777: 2 take 44.8 and 5 take 37.0).  Where a compute
+        // unit has one, as many splits as fill them once or, of few, whose rounds leave fewer idle; a round's start and end count as 512 tokens
+        // (1826 rows behind 11564 tokens, 20 heads of 64 on 4, 144 tiles: 413 us without splits, 308 with 5).  Not from 256
+        // tiles on: as many short ones as long ones fill the last round where a prompt is causal.
+        const bool alone = p.waves == 8 || kv.padded > 128;
         int64_t least = 0;
-        for (int each = 1; each <= 8 / p.waves; each++) {
-            const int64_t n = std::max<int64_t>(1, 256 * each / units), chunk = ((most_length + n - 1) / n + 63) / 64 * 64;
-            if (each == 1 || each * chunk < least) {
-                least = each * chunk;
+        auto consider = [&](int64_t n, int64_t turns, int64_t more) {
+            const int64_t chunk = ((most_length + n - 1) / n + 63) / 64 * 64, cost = turns * (chunk + more);
+            if (!least || cost < least) {
+                least = cost;
                 p.chunk = (int)chunk;
             }
-        }
+        };
+        if (alone && units > 32 && units < 256)
+            for (int64_t n = 1; n <= 8; n++)
+                consider(n, (units * n + 255) / 256, 512);
+        else
+            for (int each = 1; each <= (alone ? 1 : 2); each++)
+                consider(std::max<int64_t>(1, 256 * each / units), each, 0);
         p.splits = (int)((most_length + p.chunk - 1) / p.chunk);
         parts = p.splits > 1 ? units * p.splits : 0;
     } else {
