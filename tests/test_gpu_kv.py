@@ -121,7 +121,8 @@ ATTENDS = [  # lengths, rows of each (None: one, without starts), page, heads, k
     ([64], [64], 64, 4, 2, 64), ([300], [300], 16, 8, 2, 128), ([1777, 1000, 201], [201, 90, 201], 32, 20, 4, 80),
     ([700], [130], 128, 6, 1, 256), ([257, 31], [257, 31], 16, 3, 3, 96), ([129, 500, 0, 64], [40, 33, 17, 65], 16, 4, 2, 128),
     ([1500, 1500], [77, 77], 64, 12, 12, 64), ([5000], [35], 64, 1, 1, 64), ([4000, 70], [33, 1], 128, 2, 2, 100), ([2600], [20], 64, 1, 1, 256),
-    ([3000, 2500], [20, 17], 64, 16, 16, 64), ([3000, 2500], [20, 17], 64, 16, 16, 128), (list(range(190, 230)), [18] * 40, 16, 8, 8, 64),
+    ([3000, 2500], [20, 17], 64, 16, 16, 64), ([3000, 2500], [20, 17], 64, 16, 16, 128), ([8300, 8200], [20, 17], 64, 16, 16, 128),
+    (list(range(190, 230)), [18] * 40, 16, 8, 8, 64),
     ([9000], [64], 64, 32, 8, 64), ([3000, 2999, 40], [64, 63, 40], 64, 32, 8, 80), ([4100, 4000], [64, 64], 32, 32, 8, 128),
     ([700] * 5, [512] * 5, 64, 16, 16, 100), ([700, 1, 699, 0, 720], [512, 1, 511, 0, 512], 32, 16, 16, 64), ([1500], [1100], 64, 16, 16, 96),
     ([333], [333], 48, 5, 1, 100), ([20], [65], 16, 2, 2, 16), ([2100], [65], 64, 8, 8, 128)]

@@ -1298,10 +1298,12 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     const int64_t group = heads / kv.kv_heads, rows = most_rows * group;
     if ((int64_t)kv.rows * heads > 0x7fffffc0)
         return VTL_HIP_ERR_UNSUPPORTED;
-    // Up to 32 rows are few (16 above 128 dimensions, as many as the registers hold): 8 sequences of 3001 tokens with 16 heads of 64 values take 27.3 us with
+    // Up to 32 rows are few (16 above 128 dimensions, as many as the registers hold): 8 sequences of up to 3001 tokens with 16 heads of 64 values take 27.3 us with
     // 32 rows each, where the other kernel takes 46.9 with any number up to 128; of 128 values 49.1 and 64.1.  But 17 and more are many where there
-    // are no more than 256 tokens for a compute unit: 8 sequences of 300 take 19.0 us and 26.6, one of 3001 15.0 and 17.2.
-    p.many = rows > (kv.padded > 128 ? 16 : 32) || (rows > 16 && (int64_t)kv.batch * kv.kv_heads * most_length <= 256 * 256);
+    // is little to read for a compute unit, 256 tokens or, above 64 dimensions, where half as many waves have room, 1024: 20 sequences of 333, 24 rows each, 8 heads
+    // of 128, take 20.9 us and 23.8, 20 of 1000 29.7 and 40.5, 45 of 1000 49.5 and 53.8; of 64 values 21.8 and 17.6.
+    p.many = rows > (kv.padded > 128 ? 16 : 32) ||
+             (rows > 16 && (int64_t)kv.batch * kv.kv_heads * most_length <= 256 * (kv.padded > 64 ? 1024 : 256));
     // Many rows: eight waves share the codes that are made fp16 and brought to LDS once, and have a compute unit for themselves, where there is enough to do, four
     // tiles of tokens for each of them (a row sees half of its sequence's new tokens), and their rows do not lie idle.  2048 rows behind 14336 tokens, 32 heads of
     // 128 on 8: 908 us and 958 with four waves on the same card, a prompt of 4096 266 and 286, 512 rows behind 29500 442 and 518; but a prompt of
