@@ -350,7 +350,8 @@ int vtl_hip_kv_read_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *b
  * already): out[r, h] = sum_j w_j v_j, w = softmax over j of scale * q[r, h] . k_j, with head h reading key/value head
  * h / (heads / kv_heads).  causal: a row sees the tokens up to its own; otherwise all of its sequence's (an encoder's states, with
  * any number of rows).  A row that sees nothing gives zeros, and one that sees a token with an infinite or NaN scale gives NaN.
- * heads is a multiple of kv_heads; rows times heads are below 2^31 - 64 (VTL_HIP_ERR_UNSUPPORTED beyond).  out may not share memory with q.
+ * heads is a multiple of kv_heads; rows times heads are 2^31 - 64 at most, as are the
+ * values of a row (VTL_HIP_ERR_UNSUPPORTED beyond).  out may not share memory with q.
  *
  * q and the weights enter the products with 22 bits below the largest of q that are worked on together (up to 256 rows), sums
  * are f32.  How sums are cut depends on the lengths and rows of the whole batch and on most_rows and most_length: the same call gives the same

@@ -70,6 +70,12 @@ def test_more_than_is_counted():
     assert calls(cache(kv_heads=1000), batch(batch=1 << 24, rows=1 << 24), stride=64000, heads=1000, q_stride=64000, out_stride=64000, out=1 << 60) == [u] * 3
 
 
+def test_rows_of_more_than_32_bits():
+    wide = {"q_stride": 1 << 32, "out_stride": 1 << 32, "out": 1 << 60}
+    assert calls(cache(kv_heads=1, head_dim=256), batch(batch=1, rows=1), stride=256, heads=1 << 23, **wide)[2] == capi.ERR_UNSUPPORTED
+    assert calls(cache(kv_heads=1), batch(), stride=64, heads=1 << 30, q_stride=1 << 40, out_stride=1 << 40, out=1 << 60)[2] == capi.ERR_UNSUPPORTED
+
+
 def test_nothing_to_do():
     assert calls(cache(), batch(batch=0, rows=0, page_table=None, lengths=None), k=None, v=None, q=None, out=None) == [OK] * 3
     assert calls(cache(), batch(rows=0, starts=ONE)) == [OK] * 3

@@ -770,7 +770,8 @@ constexpr int kSchedVector = 0x2, kSchedProduct = 0x8, kSchedRead = 0x100;
 // SPLIT: whether tokens are split (a variant of its own: without, a prompt of 4096 takes a hundredth less).
 template <int DT, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, Group of, float scale,
-                                                                    int causal, float *__restrict__ out, int64_t out_stride, Parts parts, int aligned)
+                                                                                     int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
+                                                                                     int aligned)
 {
     constexpr int T = 64 * WAVES;
     constexpr int TOKENS = DT > 128 ? 32 : 64;             // of a tile: what the registers have room for
@@ -881,20 +882,18 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 store_part(t, i / 4, i / 2 % 2, i % 2);
         };
         auto store_scales = [&](Tile &t) {
-            {
-                // such a value makes its token's score no number for the rows that see it, and is out of the way of the others
-                const bool finite = fabsf(value_scale) < INFINITY;
-                t.key_scale[lane % TOKENS] = is ? __builtin_ldexpf(key_scale, unit_at) : 0.0f;
-                value_scale = is && finite ? value_scale : 0.0f;
-                t.minus[lane % TOKENS] = !is ? -INFINITY : finite ? 0.0f : NAN;
-                level.next(wave_max(fabsf(value_scale)), first_tile);
-                first_tile = false;
-                t.value_scale[lane % TOKENS] = __builtin_ldexpf(value_scale, kManyLevel - level.at);
-                const int marked = __any(!is || !finite);
-                if (lane == 0) {
-                    t.marked = marked;
-                    t.level = level.at;
-                }
+            // a value's scale that is no finite number makes its token's score no number for the rows that see it, and is out of the way of the others
+            const bool finite = fabsf(value_scale) < INFINITY;
+            t.key_scale[lane % TOKENS] = is ? __builtin_ldexpf(key_scale, unit_at) : 0.0f;
+            value_scale = is && finite ? value_scale : 0.0f;
+            t.minus[lane % TOKENS] = !is ? -INFINITY : finite ? 0.0f : NAN;
+            level.next(wave_max(fabsf(value_scale)), first_tile);
+            first_tile = false;
+            t.value_scale[lane % TOKENS] = __builtin_ldexpf(value_scale, kManyLevel - level.at);
+            const int marked = __any(!is || !finite);
+            if (lane == 0) {
+                t.marked = marked;
+                t.level = level.at;
             }
         };
         if (from < to) {
@@ -1226,7 +1225,8 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     }
 }
 
-// Where the tokens of a tile of rows are split: what bounds it is two trips to memory, one for the sequence and one for the parts.  SHARE waves have the same rows and take turns with the parts where there are many.
+// Where the tokens of a tile of rows are split: what bounds it is two trips to memory, one for the sequence and one for the parts.  SHARE waves have
+// the same rows and take turns with the parts where there are many.
 template <int DT, int WAVES, int SHARE>
 __global__ __launch_bounds__(256) void attention_many_join_kernel(Kv kv, Group of, int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
                                                                   int aligned)
@@ -1296,7 +1296,7 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     const int64_t most_rows = kv.starts ? (b.most_rows ? std::min(b.most_rows, kv.rows) : kv.rows) : 1;
     const int64_t most_length = std::max(b.most_length ? std::min(b.most_length, kv.most_tokens) : kv.most_tokens, 1);
     const int64_t group = heads / kv.kv_heads, rows = most_rows * group;
-    if ((int64_t)kv.rows * heads > 0x7fffffc0)
+    if ((int64_t)kv.rows * heads > 0x7fffffc0 || (int64_t)heads * kv.head_dim > 0x7fffffc0)
         return VTL_HIP_ERR_UNSUPPORTED;
     // Up to 32 rows are few (16 above 128 dimensions, as many as the registers hold): 8 sequences of up to 3001 tokens with 16 heads of 64 values take 27.3 us with
     // 32 rows each, where the other kernel takes 46.9 with any number up to 128; of 128 values 49.1 and 64.1.  But 17 and more are many where there
