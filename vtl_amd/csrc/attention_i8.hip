@@ -600,11 +600,12 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
                 for (int t = 0; t < 4; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float v = s[n][t][i] * ks[t][i];
+                        // the unit goes to the key's scale first: either may be far from 1 where their product is not
+                        const float v = s[n][t][i] * (ks[t][i] * unit_of[n]);
                         s[n][t][i] = mine < until - (4 * t + i) ? v : -INFINITY;
                         best = fmaxf(best, s[n][t][i]);
                     }
-                best = max_across_32(max_across_16(best)) * unit_of[n];
+                best = max_across_32(max_across_16(best));
                 const float now = fmaxf(top[n], best);
                 const float off = now == -INFINITY ? 0.0f : now;
                 const float keep = __builtin_amdgcn_exp2f(top[n] - off);
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
                 for (int t = 0; t < 4; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], unit_of[n], -off));
+                        const float e = __builtin_amdgcn_exp2f(s[n][t][i] - off);
                         add += e;
                         x[4 * t + i] = e * vs[t][i];
                     }
@@ -956,9 +957,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 #pragma unroll
         for (int i = 0; i < WAVES; i++)
             most = fmaxf(most, q_most[i]);
-        // one multiplication for the scale and the unit, which is as large as to have that finite
-        unit_at = __builtin_amdgcn_readfirstlane(max(exponent_of(fminf(most * fabsf(to_exponents), 0x1.fffffep127f)) - 14, exponent_of(fabsf(to_exponents)) - 100));
-        const float to_unit = __builtin_ldexpf(to_exponents, -unit_at);
+        unit_at = __builtin_amdgcn_readfirstlane(exponent_of(fminf(most * fabsf(to_exponents), 0x1.fffffep127f)) - 14);
         half8_t x[DT / 16][2];
 #pragma unroll
         for (int i = 0; i < DT / 16; i++) {
@@ -968,7 +967,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 const float4_t four = *reinterpret_cast<const float4_t *>(&own[col][16 * i + 8 * h + k]);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    v[k + j] = four[j] * to_unit;
+                    v[k + j] = __builtin_ldexpf(four[j] * to_exponents, -unit_at);
             }
             split(v, x[i][0], x[i][1]);
         }
