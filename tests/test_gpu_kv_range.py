@@ -39,3 +39,25 @@ def test_scales_of_keys_far_from_one(counts, dim, power):
     q = normal(5, rows_of(counts), 4, dim, std=2.0) * np.float32(2.0 ** -power)
     out, want, far = attend(c, counts, q, 4, dim ** -0.5)
     assert (np.abs(out - want) <= far).all()
+
+
+@pytest.mark.parametrize("counts", ROWS)
+@pytest.mark.parametrize("target", [0, 70])
+def test_scores_far_below_zero(counts, target):
+    """All scores are below -2^100, one token's by a factor of three less than the others': its values are what comes out."""
+    c = Cache([300, 180], 16, 2, 64, seed=4)
+    kc, _, ks, _ = c.parts()
+    kc[:], ks[c.table[c.table >= 0]] = -127, np.float32(3 * 2.0 ** 36)
+    for b in range(2):
+        page, slot = c.place(b, target)
+        ks[page, :, slot] = np.float32(2.0 ** 36)
+    c.to_device()
+    q = np.random.default_rng(6).uniform(1, 2, (rows_of(counts), 4, 64)).astype(np.float32) * np.float32(2.0 ** 58)
+    b = c.batch(counts)
+    out = attention_i8_hip(c.cache, b, HipTensor.from_host(q), 4, scale=1.0).cpu()
+    for b in range(2):
+        lo, hi = c.rows_of(b)
+        _, v, _ = c.tokens(b, [target])
+        want = np.repeat(v[0], 2, axis=0)
+        # the weight is 1, the value's scale two halves of fp16 (22 bits), and sum and quotient are rounded once each
+        assert (np.abs(out[lo:hi] - want) <= np.abs(want) * 2.0 ** -20).all()

@@ -982,8 +982,8 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             any_sees = row0 >= rows ? 0 : min(length - count + token + 1, to);
         }
 
-        // `off` is what a row's scores are less than by 2^kSlack at most; before the row has seen a token it is so low that any score is above
-        constexpr float kNone = -0x1p100f;
+        // `off` is what a row's scores are more than by kSlack at most; kNone before the row has seen a token
+        constexpr float kNone = -INFINITY;
         float off = kNone, sum = 0.0f;
         float16_t o[DT / 32];
 #pragma unroll
@@ -1083,7 +1083,9 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             if (__any(best > (off == kNone ? -INFINITY : kSlack)) || level_here != level_at) {
                 // A new maximum.  The scores are rounded once where they are brought to it by a difference, by 2^-24 of how far it has risen at most.
                 const float top = max_across_32(best), rise = off == kNone || top > kSlack ? top : 0.0f;
-                const float now = top == -INFINITY ? off : less + rise, keep = __builtin_amdgcn_exp2f(off - now), further = now - less;
+                // a row that has not seen a token has sums of 0 and scores of -infinity, and keeps them
+                const float now = top == -INFINITY ? off : less + rise, keep = off == kNone ? 1.0f : __builtin_amdgcn_exp2f(off - now);
+                const float further = now == kNone ? 0.0f : now - less;
                 off = now;
                 sum *= keep;
                 const float by = __builtin_ldexpf(keep, level_at - level_here);
@@ -1193,7 +1195,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             }
         const int64_t slot0 = (((int64_t)bh * parts.tiles + tile) * parts.splits + split_at) * kRows + w * kManyRows;
         if (!alone && h == 0 && row0 + col < rows) {
-            parts.tops[slot0 + col][0] = off == kNone ? -INFINITY : off;
+            parts.tops[slot0 + col][0] = off;
             parts.tops[slot0 + col][1] = sum;
         }
         __syncthreads();
