@@ -61,3 +61,22 @@ def test_scores_far_below_zero(counts, target):
         want = np.repeat(v[0], 2, axis=0)
         # the weight is 1, the value's scale two halves of fp16 (22 bits), and sum and quotient are rounded once each
         assert (np.abs(out[lo:hi] - want) <= np.abs(want) * 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("counts", [None, [6], [30], [90]])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_scales_that_are_no_numbers(bad, counts, dim):
+    """Whatever the token's codes are, and so whatever sign a score has: the rows that see it are no numbers, and no other."""
+    c = Cache([200], 16, 2, dim, seed=6)
+    rows = 1 if counts is None else counts[0]
+    page, slot = c.place(0, 150 if rows > 49 else 200 - (rows + 1) // 2)
+    ks = c.parts()[2]
+    ks[page, 0, slot] = bad
+    c.to_device()
+    q = normal(8, rows, 4, dim)
+    out, want, far = attend(c, counts, q, 4, 0.125)
+    spoiled = np.isnan(want)
+    assert spoiled[-1, :2].all() and not spoiled[:, 2:].any() and (rows < 3 or not spoiled[0].any())
+    assert np.isnan(out[spoiled]).all()
+    assert (np.abs(out - want)[~spoiled] <= far[~spoiled]).all()

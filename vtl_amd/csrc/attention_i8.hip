@@ -572,14 +572,28 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
 
             // scales of tokens that are none count for nothing
             const int mine = there ? j0 + 16 * g : 0x7fffffff;
+            float4_t zeros = ks[0] * 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    zeros[i] = __builtin_fmaf(vs[t][i], 0.0f, t ? __builtin_fmaf(ks[t][i], 0.0f, zeros[i]) : zeros[i]);
+            if (__any(!(zeros[0] + zeros[1] + zeros[2] + zeros[3] == 0.0f)))
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // a token with such a scale is no number for the rows that see it, and out of the way of the others
+                        const bool finite = fabsf(vs[t][i]) < INFINITY && fabsf(ks[t][i]) < INFINITY;
+                        ks[t][i] = finite ? ks[t][i] : NAN;
+                        vs[t][i] = finite ? vs[t][i] : 0.0f;
+                    }
             float most = 0.0f;
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const bool finite = fabsf(vs[t][i]) < INFINITY;
-                    ks[t][i] = finite ? ks[t][i] : NAN;      // such a token is no number for the rows that see it, and out of the way of the others
-                    vs[t][i] = finite && mine < to - (4 * t + i) ? vs[t][i] : 0.0f;
+                    vs[t][i] = mine < to - (4 * t + i) ? vs[t][i] : 0.0f;
                     most = fmaxf(most, fabsf(vs[t][i]));
                 }
             most = max_across_32(max_across_16(most));      // the same in every lane of a column, and the columns hold the same
@@ -760,7 +774,7 @@ struct alignas(16) ManyTile {
     _Float16 keys[DT / 8][TOKENS][8];
     _Float16 values[TOKENS / 8][DT][8];
     float key_scale[TOKENS], value_scale[TOKENS];
-    float minus[TOKENS];              // added to a token's scores: -infinity where there is none, NaN where its values' scale is no finite number
+    float minus[TOKENS];              // added to a token's scores: -infinity where there is none, NaN where a scale of it is no finite number
     int marked;                   // whether there is any such
     int level;                    // the values' scales are in units of 2^(level - kManyLevel)
 };
@@ -883,8 +897,8 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 store_part(t, i / 4, i / 2 % 2, i % 2);
         };
         auto store_scales = [&](Tile &t) {
-            // a value's scale that is no finite number makes its token's score no number for the rows that see it, and is out of the way of the others
-            const bool finite = fabsf(value_scale) < INFINITY;
+            // a scale that is no finite number makes its token's score no number for the rows that see it, and is out of the way of the others
+            const bool finite = fabsf(value_scale) < INFINITY && fabsf(key_scale) < INFINITY;
             t.key_scale[lane % TOKENS] = is ? __builtin_ldexpf(key_scale, unit_at) : 0.0f;
             value_scale = is && finite ? value_scale : 0.0f;
             t.minus[lane % TOKENS] = !is ? -INFINITY : finite ? 0.0f : NAN;
