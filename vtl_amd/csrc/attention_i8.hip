@@ -6,7 +6,9 @@
 // meets them is no whole number: q (with scale and log2 e) and w_j sv_j, two halves of 11 bits each, hi = f16(x), lo = f16(x - hi), one product
 // for each.  So 22 bits of the operands enter, where one half alone would leave an error of 2^-11, and a third would cost half as much again.
 // q is scaled by a power of two to a largest value between 2^14 and 2^15 (the rows of a workgroup that shares tiles by one, else each row by its
-// own); the values' scales of a tile likewise (`Level`): lo keeps its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.
+// own): lo keeps its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.  The products w_j sv_j are kept between 2^13 and 2^14
+// likewise, by the largest that the row itself has had: a token that a row gives no weight takes nothing from it, however large its values.  (Few rows take
+// the largest of each tile; many rows take the values' scales for it and look at the products only where those are far apart, `kNear`.)
 //
 // One pass over the tokens, with the running maximum and sum of the softmax, in powers of two.  Products are transposed, tokens as the
 // rows of S^T = K Q^T and dimensions as those of O^T = V^T W^T: a lane then holds what belongs to one row of q, maximum and sum are taken within the
@@ -113,27 +115,6 @@ struct Group {
         more += head < 0 ? -1 : head >= size ? 1 : 0;
         head += head < 0 ? size : head >= size ? -size : 0;
         token = token0 + more;
-    }
-};
-
-// The power of two that the values' scales are divided by, uniform in a wave: that of the largest of the tile's at hand.  It stays while the tile's
-// is at most 2^6 below it (a change costs a pass over the sums), and rises no further than the sums, which grow when it falls, have room for.
-struct Level {
-    int at = -100;
-    int room = 0;      // powers of two that the sums may have grown by
-
-    // The new level for a tile whose largest scale is `most`; what the sums are multiplied by is 2^(old - new).
-    __device__ __forceinline__ int next(float most, bool first)
-    {
-        const int tile = max(exponent_of(most), -100);
-        if (first) {
-            at = tile;
-            return 0;
-        }
-        int by = tile > at ? tile - at : tile < at - 6 ? max(tile - at, room - 60) : 0;
-        at += by;
-        room = max(room - by, 0);
-        return -by;
     }
 };
 
@@ -405,7 +386,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
     __shared__ float q_unit[kRows];
     __shared__ __align__(16) float o_part[WAVES][kRows][kPitch];
     __shared__ float top_part[WAVES][kRows], sum_part[WAVES][kRows];
-    __shared__ int level_part[WAVES];
+    __shared__ float level_part[WAVES][kRows];
     __shared__ int is_last;
 
     const int share = blockIdx.x;
@@ -524,7 +505,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
         __syncthreads();
 
         float unit_of[NB], top[NB], sum[NB];
-        int limit[NB];
+        int limit[NB], level[NB];      // sums of values are in units of 2^(level - 13)
         float4_t o[NB][DT / 16];
 #pragma unroll
         for (int n = 0; n < NB; n++) {
@@ -533,12 +514,11 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
             limit[n] = causal ? min(length - count + token + 1, to) : to;
             top[n] = -INFINITY;
             sum[n] = 0.0f;
+            level[n] = -127;
 #pragma unroll
             for (int i = 0; i < DT / 16; i++)
                 o[n][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        Level level;
-        bool fresh = true;
 
         for (; j0 < to; j0 += kStep) {
             asm volatile("" ::: "memory");      // q's halves are read again for every tile, not kept in registers
@@ -588,22 +568,6 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
                         ks[t][i] = finite ? ks[t][i] : NAN;
                         vs[t][i] = finite ? vs[t][i] : 0.0f;
                     }
-            float most = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    vs[t][i] = mine < to - (4 * t + i) ? vs[t][i] : 0.0f;
-                    most = fmaxf(most, fabsf(vs[t][i]));
-                }
-            most = max_across_32(max_across_16(most));      // the same in every lane of a column, and the columns hold the same
-            const int moved = level.next(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(most))), fresh);
-            fresh = false;
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    vs[t][i] = __builtin_ldexpf(vs[t][i], 13 - level.at);
 
             half8_t p[NB][2][2];
 #pragma unroll
@@ -624,7 +588,7 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
                 const float off = now == -INFINITY ? 0.0f : now;
                 const float keep = __builtin_amdgcn_exp2f(top[n] - off);
                 top[n] = now;
-                float x[16], add = 0.0f;
+                float x[16], add = 0.0f, most = 0.0f;
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -632,11 +596,19 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
                         const float e = __builtin_amdgcn_exp2f(s[n][t][i] - off);
                         add += e;
                         x[4 * t + i] = e * vs[t][i];
+                        most = fmaxf(most, fabsf(x[4 * t + i]));
                     }
                 sum[n] = __builtin_fmaf(sum[n], keep, add);
+                // the row's level is the largest power of two that a weight times its value's scale has had, brought to the present maximum
+                most = max_across_32(max_across_16(most));
+                const int before = level[n];
+                level[n] = max(before + exponent_of(keep), exponent_of(most));
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    x[i] = __builtin_ldexpf(x[i], 13 - level[n]);
                 split(x, p[n][0][0], p[n][0][1]);
                 split(x + 8, p[n][1][0], p[n][1][1]);
-                const float by = __builtin_ldexpf(keep, moved);
+                const float by = __builtin_ldexpf(keep, before - level[n]);
 #pragma unroll
                 for (int i = 0; i < DT / 16; i++)
                     o[n][i] *= by;
@@ -660,12 +632,11 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
         }
 
         // ---- the waves meet: what each has of the rows that there are, in its own units
-        if (lane == 0)
-            level_part[w] = fresh ? -1000 : level.at;
 #pragma unroll
         for (int n = 0; n < NB; n++) {
             sum[n] = sum_across_32(sum_across_16(sum[n]));
             if (g == 0) {
+                level_part[w][16 * n + col] = (float)level[n];
                 top_part[w][16 * n + col] = top[n];
                 sum_part[w][16 * n + col] = sum[n];
             }
@@ -678,15 +649,15 @@ __global__ __launch_bounds__(64 * WAVES, DT * NB > 128 ? 1 : 2) void attention_f
         const bool alone = u.begin == 0 && u.end == u.rounds;
         const int64_t slot0 = (int64_t)part_slot(deal, share, u.first_round) * kRows;
         const int part = min(lane & 15, WAVES - 1);      // lane i of 16 has what wave i knows of a row
-        const float level_mine = (float)level_part[part];
-        const int high = (int)row_max_16(level_mine);
         for (int r = w; r < here; r += WAVES) {
-            const float top_mine = top_part[part][r], sum_mine = (lane & 15) < WAVES ? sum_part[part][r] : 0.0f;
+            const float level_mine = level_part[part][r], top_mine = top_part[part][r], sum_mine = (lane & 15) < WAVES ? sum_part[part][r] : 0.0f;
             const float t = row_max_16(top_mine), off = t == -INFINITY ? 0.0f : t, e = __builtin_amdgcn_exp2f(top_mine - off);
             const float total = row_sum_16(sum_mine == 0.0f ? 0.0f : sum_mine * e);
             const float over = total == 0.0f ? 0.0f : alone ? 1.0f / total : 1.0f;
             // nothing: of a wave that had no tokens, or of a row that sees none
-            const float by = sum_mine == 0.0f ? 0.0f : __builtin_ldexpf(e, (int)level_mine - high);
+            const bool none = sum_mine == 0.0f || e == 0.0f;
+            const int high = (int)row_max_16(none ? -1000.0f : level_mine + (float)exponent_of(e));
+            const float by = none ? 0.0f : __builtin_ldexpf(e, (int)level_mine - high);
             of.row(token0, head0, r, token, of_token);
             float *to_o = alone ? out + (int64_t)(first + token) * out_stride + (head * group + of_token) * kv.head_dim
                                 : shares.sums + (slot0 + r) * kv.padded;
@@ -764,7 +735,11 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of
 // which the values' scales leave room (2^(kSlack + 10) is below fp16's largest number).
 constexpr int kManyRows = 32;     // of a wave
 constexpr float kSlack = 5.0f;
-constexpr int kManyLevel = 9;     // the largest scale of a tile is brought to 2^9 .. 2^10
+constexpr int kManyLevel = 9;     // the largest scale so far is brought to 2^9 .. 2^10
+// Scales further below the largest than 2^kNear, or a largest one that has risen by more than 2^kRise, leave fp16 few bits for the rows that have no weight
+// where the large ones are.  In such a tile each row is brought to where the largest product of a weight and a scale that it sees there is 2^14, as far as its
+// sums stay within f32, for which 2^kMost leaves room.
+constexpr int kNear = 10, kRise = 2, kMost = 110;
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
@@ -775,7 +750,7 @@ struct alignas(16) ManyTile {
     _Float16 values[TOKENS / 8][DT][8];
     float key_scale[TOKENS], value_scale[TOKENS];
     float minus[TOKENS];              // added to a token's scores: -infinity where there is none, NaN where a scale of it is no finite number
-    int marked;                   // whether there is any such
+    int marked;                   // whether there is any such, 1; whether the values' scales are far apart, 2
     int level;                    // the values' scales are in units of 2^(level - kManyLevel)
 };
 
@@ -839,7 +814,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
         int4_t keys[kUnits], values[kUnits];
         float key_scale, value_scale;
         bool is, first_tile = true;
-        Level level;
+        int level = -100, base = 127;      // the values' level, and what it was when all rows were last brought to it
         int unit_at;      // q is in units of 2^unit_at, which the keys' scales make up for
         // Where there is no token, or no dimension, any codes do: q or the weight is 0 there.
         const int32_t *const table = kv.table + (int64_t)b * kv.max_pages;
@@ -902,13 +877,17 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             t.key_scale[lane % TOKENS] = is ? __builtin_ldexpf(key_scale, unit_at) : 0.0f;
             value_scale = is && finite ? value_scale : 0.0f;
             t.minus[lane % TOKENS] = !is ? -INFINITY : finite ? 0.0f : NAN;
-            level.next(wave_max(fabsf(value_scale)), first_tile);
+            const float size = fabsf(value_scale);
+            level = max(level, exponent_of(wave_max(size)));
+            t.value_scale[lane % TOKENS] = __builtin_ldexpf(value_scale, kManyLevel - level);
+            base = first_tile ? level : base;
             first_tile = false;
-            t.value_scale[lane % TOKENS] = __builtin_ldexpf(value_scale, kManyLevel - level.at);
-            const int marked = __any(!is || !finite);
+            const bool apart = __any(size != 0.0f && exponent_of(size) < level - kNear) || level > base + kRise;
+            base = apart ? level : base;
+            const int marked = (__any(!is || !finite) ? 1 : 0) | (apart ? 2 : 0);
             if (lane == 0) {
                 t.marked = marked;
-                t.level = level.at;
+                t.level = level;
             }
         };
         if (from < to) {
@@ -1075,7 +1054,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                     for (int j = 0; j < 4; j++)
                         s[i][k + j] = __builtin_fmaf(s[i][k + j], ks[j], -less);
                 }
-            if (j0 + TOKENS > all_see || marked) {
+            if (j0 + TOKENS > all_see || marked & 1) {
                 const int until = limit - j0 - 8 * h;
 #pragma unroll
                 for (int i = 0; i < kBlocks; i++)
@@ -1094,11 +1073,37 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 #pragma unroll
                 for (int k = 0; k < 16; k++)
                     best = fmaxf(best, s[i][k]);
-            if (__any(best > (off == kNone ? -INFINITY : kSlack)) || level_here != level_at) {
+            const bool apart = marked & 2;
+            if (__any(best > (off == kNone ? -INFINITY : kSlack)) || level_here != level_at || apart) {
                 // A new maximum.  The scores are rounded once where they are brought to it by a difference, by 2^-24 of how far it has risen at most.
-                const float top = max_across_32(best), rise = off == kNone || top > kSlack ? top : 0.0f;
+                const float top = max_across_32(best);
+                float rise = off == kNone || top > kSlack ? top : 0.0f;
+                if (__builtin_expect(apart, 0)) {
+                    // what its scores are taken less is what a row's products want, not its weights: below the maximum where its values are small
+                    float most = -INFINITY, size = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4) {
+                            const float4_t vs = *reinterpret_cast<const float4_t *>(&t.value_scale[32 * i + 16 * (k / 8) + 8 * h + k % 8]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                most = fmaxf(most, s[i][k + j] + __builtin_amdgcn_logf(fabsf(vs[j])));
+                        }
+#pragma unroll
+                    for (int i = 0; i < DT / 32; i++)
+#pragma unroll
+                        for (int k = 0; k < 16; k++)
+                            size = fmaxf(size, fabsf(o[i][k]));
+                    const int up = level_here - level_at;
+                    most = max_across_32(most);
+                    most = most == -INFINITY ? (float)-up : most - (float)min(14, kMost - level_here);
+                    const int least = max(exponent_of(max_across_32(sum)) - kMost,
+                                          exponent_of(max_across_32(size)) - up - min(kMost, kMost + 17 - level_here));
+                    rise = fmaxf(fmaxf(most, top - kMost), (float)least);
+                }
                 // a row that has not seen a token has sums of 0 and scores of -infinity, and keeps them
-                const float now = top == -INFINITY ? off : less + rise, keep = off == kNone ? 1.0f : __builtin_amdgcn_exp2f(off - now);
+                const float now = off == kNone && top == -INFINITY ? off : less + rise, keep = off == kNone ? 1.0f : __builtin_amdgcn_exp2f(off - now);
                 const float further = now == kNone ? 0.0f : now - less;
                 off = now;
                 sum *= keep;
