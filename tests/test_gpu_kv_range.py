@@ -166,3 +166,19 @@ def test_values_that_grow_and_shrink(counts):
         want, far = attend_alone(c, q, 8, 1.0, True)
         off = np.abs(out - want)
         assert (off <= far).all(), float((off / far).max())
+
+
+@pytest.mark.parametrize("counts", ROWS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("power", [20, 26, 40, 90])
+def test_scores_far_above_one(counts, dim, power):
+    """Scores so large that f32 has steps of more than 1 there: which of the largest a row takes is the rounding's choice, but its weights are
+    none above their sum."""
+    c = Cache([700, 330], 32, 2, dim, seed=14).to_device()
+    q = normal(15, rows_of(counts), 4, dim) * np.float32(2.0 ** power)
+    for out in results(c, counts, q, 4, 1.0):
+        for b in range(2):
+            lo, hi = c.rows_of(b)
+            _, v, _ = c.tokens(b, np.arange(c.length(b)))
+            most = np.repeat(np.abs(v).max(0), 2, axis=0)
+            assert (np.abs(out[lo:hi]) <= most * (1 + 2.0 ** -12)).all()

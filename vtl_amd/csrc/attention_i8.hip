@@ -1104,7 +1104,8 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 }
                 // a row that has not seen a token has sums of 0 and scores of -infinity, and keeps them
                 const float now = off == kNone && top == -INFINITY ? off : less + rise, keep = off == kNone ? 1.0f : __builtin_amdgcn_exp2f(off - now);
-                const float further = now == kNone ? 0.0f : now - less;
+                // as much as `off` moves, but of scores with steps of more than 1 as much as the largest is above
+                const float moves = now - less, further = now == kNone ? 0.0f : fabsf(moves - rise) < 1.0f ? moves : rise;
                 off = now;
                 sum *= keep;
                 const float by = __builtin_ldexpf(keep, level_at - level_here);
