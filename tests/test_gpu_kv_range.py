@@ -182,3 +182,19 @@ def test_scores_far_above_one(counts, dim, power):
             _, v, _ = c.tokens(b, np.arange(c.length(b)))
             most = np.repeat(np.abs(v).max(0), 2, axis=0)
             assert (np.abs(out[lo:hi]) <= most * (1 + 2.0 ** -12)).all()
+
+
+@pytest.mark.parametrize("counts", [[4, 5], [30, 20], [90, 70], [250, 300]])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("power", [14, 30, 60, 90])
+def test_large_queries_beside_a_row(counts, dim, power):
+    """Some rows' queries are 2^power as large as the others': nothing to those."""
+    c = Cache([400, 330], 32, 2, dim, seed=9).to_device()
+    q = normal(11, sum(counts), 4, dim)
+    large = np.zeros(q.shape[:2], bool)
+    large[1::7, 1], large[counts[0] - 1, 3] = True, True
+    q[large] *= np.float32(2.0 ** power)
+    for out in results(c, counts, q, 4, 0.125):
+        want, far = c.attend(q, 4, np.float32(0.125), True)
+        assert (np.abs(out - want)[~large] <= far[~large]).all()
+        assert np.isfinite(out).all()

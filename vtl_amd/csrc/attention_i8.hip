@@ -5,8 +5,8 @@
 // The codes K and V are whole numbers below 128, which fp16 holds exactly, so both products run on the fp16 matrix units with f32 sums.  What
 // meets them is no whole number: q (with scale and log2 e) and w_j sv_j, two halves of 11 bits each, hi = f16(x), lo = f16(x - hi), one product
 // for each.  So 22 bits of the operands enter, where one half alone would leave an error of 2^-11, and a third would cost half as much again.
-// q is scaled by a power of two to a largest value between 2^14 and 2^15 (the rows of a workgroup that shares tiles by one, else each row by its
-// own): lo keeps its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.  The products w_j sv_j are kept between 2^13 and 2^14
+// q is scaled by a power of two to a largest value between 2^14 and 2^15 (the rows of a workgroup that shares tiles by one, but for those more than
+// 2^kNear below, and else each row by its own): lo keeps its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.  The products w_j sv_j are kept between 2^13 and 2^14
 // likewise, by the largest that the row itself has had: a token that a row gives no weight takes nothing from it, however large its values.  (Few rows take
 // the largest of each tile; many rows take the values' scales for it and look at the products only where those are far apart, `kNear`.)
 //
@@ -777,6 +777,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
     constexpr size_t kBytes = 2 * sizeof(Tile) > WAVES * kWaveBytes ? 2 * sizeof(Tile) : WAVES * kWaveBytes;
     __shared__ __align__(16) char lds[kBytes];
     __shared__ float q_most[WAVES];
+    __shared__ int q_below[kRows];      // how many powers of two a row's unit is below the workgroup's
     Tile *const tiles = reinterpret_cast<Tile *>(lds);
 
     const int group = of.size;
@@ -896,10 +897,10 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             look_up(from + TOKENS);
         }
 
-        // ---- rows of q as halves, all in one unit: rows into LDS as they are, and from there to the lanes, of which lane `col` gets 8 dimensions of
+        // ---- rows of q as halves, all in one unit but for small ones: rows into LDS as they are, and from there to the lanes, of which lane `col` gets 8 dimensions of
         // every 16 of a row
         float(*const own)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds + w * kWaveBytes);
-        float most = 0.0f;
+        float most = 0.0f, least = INFINITY;      // of four values of a row that are not all 0, the largest
         {
             // as many lanes side by side as have a row in vectors of 16 bytes
             constexpr int kLanes = DT / 4, kTogether = 64 / kLanes, kLoads = kManyRows / (kTogether ? kTogether : 1);
@@ -919,13 +920,17 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 for (int i = 0; i < kLoads; i++) {
                     if (row0 + i * kTogether + lane_row >= rows || d >= kv.head_dim)
                         v[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                    float size = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        most = fmaxf(most, fabsf(v[i][j]) < INFINITY ? fabsf(v[i][j]) : 0.0f);      // a row that is no number spoils no other
+                        size = fmaxf(size, fabsf(v[i][j]) < INFINITY ? fabsf(v[i][j]) : 0.0f);      // a row that is no number spoils no other
+                    most = fmaxf(most, size);
+                    least = size == 0.0f ? least : fminf(least, size);
                     if (lane_row < kTogether)
                         *reinterpret_cast<float4_t *>(&own[i * kTogether + lane_row][d]) = v[i];
                 }
             } else {
+                least = 0.0f;
 #pragma unroll 1
                 for (int r = 0; r < kManyRows; r++) {
                     int token, of_token;
@@ -950,7 +955,27 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
 #pragma unroll
         for (int i = 0; i < WAVES; i++)
             most = fmaxf(most, q_most[i]);
-        unit_at = __builtin_amdgcn_readfirstlane(exponent_of(fminf(most * fabsf(to_exponents), 0x1.fffffep127f)) - 14);
+        auto unit_for = [&](float size) { return exponent_of(fminf(size * fabsf(to_exponents), 0x1.fffffep127f)) - 14; };
+        unit_at = __builtin_amdgcn_readfirstlane(unit_for(most));
+        int below = 0;
+        bool rows_apart = false;
+        if (__builtin_expect(__any(exponent_of(least) < exponent_of(most) - kNear), 0)) {
+            float size = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DT / 16; i++)
+#pragma unroll
+                for (int k = 0; k < 8; k += 4) {
+                    const float4_t four = *reinterpret_cast<const float4_t *>(&own[col][16 * i + 8 * h + k]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        size = fmaxf(size, fabsf(four[j]));
+                }
+            size = max_across_32(size);
+            below = size == 0.0f ? 0 : unit_at - unit_for(size);
+            below = below > kNear ? below : 0;
+            rows_apart = __any(below);
+            q_below[w * kManyRows + col] = below;
+        }
         half8_t x[DT / 16][2];
 #pragma unroll
         for (int i = 0; i < DT / 16; i++) {
@@ -960,7 +985,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                 const float4_t four = *reinterpret_cast<const float4_t *>(&own[col][16 * i + 8 * h + k]);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    v[k + j] = __builtin_ldexpf(four[j] * to_exponents, -unit_at);
+                    v[k + j] = __builtin_ldexpf(four[j] * to_exponents, below - unit_at);
             }
             split(v, x[i][0], x[i][1]);
         }
@@ -1042,6 +1067,15 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if (__builtin_expect(rows_apart, 0)) {
+                // the lane counted anew, for want of registers
+                const int below = q_below[w * kManyRows + __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)) % kManyRows];
+#pragma unroll
+                for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        s[i][k] = __builtin_ldexpf(s[i][k], -below);
             }
             // scores less `off`, and the largest of this lane's; a row's first scores are taken as they are
             const float less = off == kNone ? 0.0f : off;
