@@ -1,0 +1,60 @@
+"""What the calls on the int8 key/value cache enqueue, without a GPU: on a HIP runtime that keeps count and runs no kernel
+(tests/host_runtime/fake_runtime.cpp)."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+ROOT = os.path.dirname(HERE)
+
+_PRELUDE = r"""
+import ctypes as C, re, sys
+fake = C.CDLL(sys.argv[2], mode=C.RTLD_GLOBAL)
+sys.path.insert(0, sys.argv[1])
+from vtl_amd import capi
+fake.fake_set(1, 0, 0, 0)
+ONE = 1 << 20                  # an address that nothing here reads
+
+def launches():
+    buf = C.create_string_buffer(1 << 20)
+    n = fake.fake_log(buf, C.c_size_t(len(buf)))
+    lines = [l.split() for l in buf.raw[:n].decode().splitlines()]
+    return [(l[4], int(l[3])) for l in lines if l[0] == "launch"]
+
+def attention(kv_heads, heads, dim, batch, rows, starts=ONE, most_rows=0, most_length=0, max_pages=4, page=16):
+    cache = capi.KVCache(ONE, 4, page, kv_heads, dim)
+    b = capi.KVBatch(batch, max_pages, ONE, ONE, starts, rows, most_rows, most_length)
+    launches()
+    st = capi.status("vtl_hip_attention_i8_f32", C.byref(cache), C.byref(b), 1 << 30, heads * dim, heads, 0.125, 1, 1 << 50, heads * dim, ONE, 1 << 40)
+    return st, launches()
+"""
+
+
+@pytest.fixture(scope="module")
+def fake_runtime(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("runtime") / "libfake_runtime.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    os.path.join(HERE, "host_runtime", "fake_runtime.cpp"), "-o", out], check=True)
+    return out
+
+
+def _run(fake, program):
+    res = subprocess.run([sys.executable, "-c", _PRELUDE + program, ROOT, fake], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
+    assert res.returncode == 0 and res.stdout.strip().endswith("done"), res.stdout[-3000:]
+
+
+def test_grids_of_very_many_sequences(fake_runtime):
+    """A grid has less than 2^32 threads in a row, whatever number of waves a workgroup would have."""
+    _run(fake_runtime, r"""
+for batch in (1 << 19, (1 << 20) - 1, 1 << 20, (1 << 21) - 1):
+    st, log = attention(8, 8, 64, batch, batch)
+    assert st == capi.OK and len(log) >= 1, (batch, st)
+    name, blocks = log[0]
+    waves = int(re.search(r"attention_many_kernelILi64ELi(\d)E", name).group(1))
+    assert blocks % (8 * batch) == 0 and 8 * batch * 64 * waves < 1 << 32, (batch, waves)
+    assert waves == (8 if batch < 1 << 20 else 4), (batch, waves)
+assert attention(8, 8, 64, 1 << 21, 1 << 21)[0] == capi.ERR_UNSUPPORTED
+print("done")
+""")

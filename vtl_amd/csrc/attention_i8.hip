@@ -1358,14 +1358,16 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     // is little to read for a compute unit, 256 tokens or, above 64 dimensions, where half as many waves have room, 1024: 20 sequences of 333, 24 rows each, 8 heads
     // of 128, take 20.9 us and 23.8, 20 of 1000 29.7 and 40.5, 45 of 1000 49.5 and 53.8; of 64 values 21.8 and 17.6.
     p.many = rows > (kv.padded > 128 ? 16 : 32) ||
-             (rows > 16 && (int64_t)kv.batch * kv.kv_heads * most_length <= 256 * (kv.padded > 64 ? 1024 : 256));
+             (rows > 16 && (double)kv.batch * kv.kv_heads * (double)most_length <= 256.0 * (kv.padded > 64 ? 1024 : 256));
     // Many rows: eight waves share the codes that are made fp16 and brought to LDS once, and have a compute unit for themselves, where there is enough to do, four
     // tiles of tokens for each of them (a row sees half of its sequence's new tokens), and their rows do not lie idle.  2048 rows behind 14336 tokens, 32 heads of
     // 128 on 8: 908 us and 958 with four waves on the same card, a prompt of 4096 266 and 286, 512 rows behind 29500 442 and 518; but a prompt of
     // 1000 48.4 and 44.7, 40 rows over 3000 23.0 and 20.5, 4 x 70 with 8 x 4 heads of 64 (three halves of tiles) 36.9 and 34.2.
     const int64_t halves = (rows + kManyRows * 4 - 1) / (kManyRows * 4);      // tiles of four waves' rows
-    const bool enough = (int64_t)kv.batch * kv.kv_heads * ((halves + 1) / 2) * (most_length - std::min(most_rows, most_length) / 2) >= 256 * 256;
-    p.waves = p.many && kv.padded <= 128 && enough && (halves % 2 == 0 || halves > 8) ? 8 : 4;
+    const double work = (double)kv.batch * kv.kv_heads * (double)((halves + 1) / 2) * (double)(most_length - std::min(most_rows, most_length) / 2);
+    // a grid has less than 2^32 threads in a row
+    const bool fits = (int64_t)kv.batch * kv.kv_heads * 64 * 8 <= 0xffffffff;
+    p.waves = p.many && kv.padded <= 128 && fits && work >= 256 * 256 && (halves % 2 == 0 || halves > 8) ? 8 : 4;
     p.tile_rows = p.many ? kManyRows * p.waves : rows <= 16 ? 16 : 32;
     p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     int64_t units = (int64_t)kv.batch * kv.kv_heads * p.tiles;

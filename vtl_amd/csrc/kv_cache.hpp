@@ -12,7 +12,7 @@ constexpr int kKvMostPage = 4096;
 constexpr int kKvMostDim = 256;
 constexpr int64_t kKvMostTokens = 1 << 28;    // of a sequence
 constexpr int kKvMostRows = 1 << 30;          // of a call, and sequences: what is counted past the last one fits 32 bits
-constexpr int kKvMostBlocks = 1 << 22;        // of a launch; what is behind is theirs too
+constexpr int kKvMostBlocks = 1 << 22;        // of a launch, or one for each sequence and head where those are more; what is behind is theirs too
 
 // A cache and the sequences of a call, by value.
 struct Kv {
