@@ -359,9 +359,9 @@ int vtl_hip_kv_read_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *b
  *
  * workspace: device memory of at least vtl_hip_attention_i8_workspace() bytes, 16-byte aligned, for the parts of sequences that
  * several workgroups share; NULL (with size 0): the library's own (see above).  Calls that may overlap on a device need one each.  With up to 16
- * rows a key/value head (heads / kv_heads times most_rows) these parts meet in the same launch on counters kept per stream, for the
- * first 16 streams of a device that make such a call; calls on further streams, calls recorded into a graph, and
- * calls with more rows take a second launch where there are such parts.  A call gives the same bits either way.
+ * rows a key/value head (heads / kv_heads times most_rows), or up to 32 of at most 128 dimensions where there is much to read, these parts meet in the
+ * same launch on counters kept per stream, for the first 16 streams of a device that make such a call; calls on further streams, calls
+ * recorded into a graph, and calls with more rows take a second launch where there are such parts.  A call gives the same bits either way.
  */
 size_t vtl_hip_attention_i8_workspace(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, int heads);
 int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *batch, const float *q, int64_t q_stride,

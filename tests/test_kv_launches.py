@@ -58,3 +58,28 @@ for batch in (1 << 19, (1 << 20) - 1, 1 << 20, (1 << 21) - 1):
 assert attention(8, 8, 64, 1 << 21, 1 << 21)[0] == capi.ERR_UNSUPPORTED
 print("done")
 """)
+
+
+def test_variants_for_few_rows(fake_runtime):
+    """Which of them a call takes, and that its parts are added up by a launch of their own while a graph is recorded and on streams without
+    counters, and within the launch on others."""
+    _run(fake_runtime, r"""
+sys.path.insert(0, sys.argv[1] + "/tests")
+from kv_cases import SHARED
+for variant, (lengths, counts, heads, kv_heads, dim) in SHARED.items():
+    rows = len(lengths) if counts is None else sum(counts)
+    def names(stream):
+        capi.call("vtl_hip_set_stream", stream)
+        st, log = attention(kv_heads, heads, dim, len(lengths), rows, ONE if counts else None, max(counts or [1]), max(lengths), 1 + max(lengths) // 16)
+        assert st == capi.OK
+        return [re.sub(r"Li(\d+)E", r"\1 ", re.search(r"attention_(\w+?_kernelI(?:Li\d+E)+)", n).group(1)) for n, _ in log]
+    few, join = ("%s_kernelI%d %d %d " % (what, *variant) for what in ("few", "few_join"))
+    assert names(None) == [few], (variant, names(None))
+    for stream in range(2, 17):       # the null stream is the first
+        assert names(stream) == [few]
+    assert names(17) == [few, join], (variant, names(17))
+    fake.fake_set(1, 1, 0, 0)
+    assert names(2) == [few, join]
+    fake.fake_set(1, 0, 0, 0)
+print("done")
+""")
