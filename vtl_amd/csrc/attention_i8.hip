@@ -152,8 +152,6 @@ __device__ __forceinline__ float row_sum_16(float v)
     return v;
 }
 
-typedef float float2_t __attribute__((ext_vector_type(2)));
-
 // Two of a part's numbers.  THERE: an earlier launch wrote them, so the caches have nothing older.
 template <bool THERE>
 __device__ __forceinline__ float2_t load_two(const float *p)

@@ -118,14 +118,6 @@ __device__ __forceinline__ const char *kv_page_or_any(const Kv &kv, int page, co
     return first_page + (uint64_t)(there ? (unsigned)page : 0u) * kv.page_bytes;
 }
 
-// And for a group that the sequence has (its page may be none).
-__device__ __forceinline__ const char *kv_group_or_any(const Kv &kv, const int32_t *table, unsigned g, const char *first_page, unsigned &at, bool &there)
-{
-    const unsigned p = kv_page_of(kv, g);
-    at = g - p * kv.page_groups;
-    return kv_page_or_any(kv, table[p], first_page, there);
-}
-
 // Where things are in one head of a page.
 __device__ __forceinline__ unsigned kv_key_at(const Kv &kv, unsigned dim16, unsigned slot) { return (dim16 * kv.page_size + slot) * 16u; }
 __device__ __forceinline__ unsigned kv_value_at(const Kv &kv, unsigned group, unsigned dim)
@@ -133,31 +125,6 @@ __device__ __forceinline__ unsigned kv_value_at(const Kv &kv, unsigned group, un
     return (unsigned)kv.padded * kv.page_size + (group * kv.padded + dim) * 16u;
 }
 __device__ __forceinline__ unsigned kv_scales_at(const Kv &kv) { return 2u * kv.padded * kv.page_size; }
-
-// The sequence of a row, and the row's position there; false: none.  Called by whole waves.
-__device__ __forceinline__ bool kv_row(const Kv &kv, int row, int &b, int &position)
-{
-    if (!kv.starts) {
-        b = row;
-        position = kv_length(kv, b) - 1;
-        return true;
-    }
-    const int lane = threadIdx.x & 63;
-    b = 0;
-    for (int base = 0; base < kv.batch; base += 64) {
-        const int i = base + lane;
-        const bool before = i < kv.batch && kv.starts[i + 1] <= row;
-        b += __popcll(__ballot(before));
-    }
-    if (b >= kv.batch)
-        return false;
-    int first, count;
-    kv_rows_of(kv, b, first, count);
-    if (row < first || row >= first + count)
-        return false;
-    position = kv_length(kv, b) - (first + count - row);
-    return true;
-}
 #endif
 
 }  // namespace vtlhip
