@@ -1,10 +1,14 @@
 """What the calls on the int8 key/value cache enqueue, without a GPU: on a HIP runtime that keeps count and runs no kernel
 (tests/host_runtime/fake_runtime.cpp)."""
+import ctypes as C
 import os
 import subprocess
 import sys
+from types import SimpleNamespace
 
 import pytest
+
+from vtl_amd import attention_i8_workspace, capi
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -83,3 +87,40 @@ for variant, (lengths, counts, heads, kv_heads, dim) in SHARED.items():
     fake.fake_set(1, 0, 0, 0)
 print("done")
 """)
+
+
+def test_workspace_of_the_python_mirror():
+    one = 1 << 20
+    cache = SimpleNamespace(handle=capi.KVCache(one, 400, 64, 8, 128))
+    some = SimpleNamespace(handle=capi.KVBatch(2, 150, one, one, None, 2, 1, 9000))
+    none = SimpleNamespace(handle=capi.KVBatch(2, 1, one, one, None, 2, 1, 60))
+    need = attention_i8_workspace(cache, some, 32)
+    assert need == capi.lib().vtl_hip_attention_i8_workspace(C.byref(cache.handle), C.byref(some.handle), 32) and need > 1 << 16
+    assert attention_i8_workspace(cache, none, 32) < need and attention_i8_workspace(cache, none, 31) == 0
+
+
+def test_workspace_of_the_cpp_mirror(fake_runtime, tmp_path):
+    """What the mirror says is enough for the call, and one byte less is refused."""
+    (tmp_path / "ws.cpp").write_text(r"""
+#include "vtl_hip.hpp"
+extern "C" int check()
+{
+    vtl::HipKVCache cache(400, 64, 8, 128);
+    vtl::HipTensor<int32_t> table({2, 150}), lengths({2});
+    vtl::HipKVBatch batch(table, lengths, nullptr, 0, 1, 9000);
+    vtl::HipTensor<float> q({2, 32 * 128});
+    const size_t need = vtl::attention_i8_workspace(cache, batch, 32);
+    vtl::HipStorage<uint8_t> enough(need), less(need - 1);
+    vtl::attention_i8_hip(cache, batch, q, 32, 0.1f, true, &enough);
+    try {
+        vtl::attention_i8_hip(cache, batch, q, 32, 0.1f, true, &less);
+    } catch (const vtl::HipError &) {
+        return need > 1 << 16;
+    }
+    return 0;
+}
+""")
+    lib, program = os.path.join(ROOT, "vtl_amd"), str(tmp_path / "ws.so")
+    subprocess.run(["g++", "-std=c++17", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I", os.path.join(lib, "host"), str(tmp_path / "ws.cpp"),
+                    "-o", program, "-L", lib, "-lvtlhip", "-Wl,-rpath," + lib], check=True)
+    _run(fake_runtime, f"assert C.CDLL({program!r}).check() == 1\nprint('done')\n")

@@ -6,7 +6,7 @@ the linear_forward_f32 hook, Sequential.linear); `kv_cache` has the
 int8 key/value cache and the attention over it.
 """
 from . import capi  # noqa: F401
-from .kv_cache import HipKVBatch, HipKVCache, attention_i8_hip, kv_read_hip, kv_write_hip  # noqa: F401
+from .kv_cache import HipKVBatch, HipKVCache, attention_i8_hip, attention_i8_workspace, kv_read_hip, kv_write_hip  # noqa: F401
 from .layers import (PER_CHANNEL, PER_TENSOR, HipSession, QuantLinearLayer,  # noqa: F401
                      QuantizedWeights, hip_backward_enabled, hip_linear_enabled,
                      hip_tests_enabled, linear_backward_hip_f32, linear_forward_f32_use_hip,

@@ -421,8 +421,17 @@ inline std::pair<HipTensor<float>, HipTensor<float>> kv_read_hip(const HipKVCach
     return {std::move(k), std::move(v)};
 }
 
+// `attention_i8_workspace(cache, batch, heads) !usize`: bytes of the workspace that the call takes for these arguments; 0: none
+// is needed.
+inline size_t attention_i8_workspace(const HipKVCache &cache, const HipKVBatch &batch, int heads)
+{
+    const vtl_hip_kv_cache c = cache.handle();
+    const vtl_hip_kv_batch b = batch.handle();
+    return vtl_hip_attention_i8_workspace(&c, &b, heads);
+}
+
 // `attention_i8_hip(cache, batch, q, heads, scale, causal, workspace) !&HipTensor[f32]`: softmax(scale * q . k^T) . v of every
-// row over its sequence, [rows, heads, head_dim]; workspace may be null.
+// row over its sequence, [rows, heads, head_dim]; workspace, of attention_i8_workspace bytes, may be null.
 inline HipTensor<float> attention_i8_hip(const HipKVCache &cache, const HipKVBatch &batch, const HipTensor<float> &q, int heads, float scale, bool causal,
                                          const HipStorage<uint8_t> *workspace = nullptr, size_t q_first = 0)
 {

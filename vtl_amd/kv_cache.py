@@ -88,11 +88,18 @@ def kv_read_hip(cache: HipKVCache, batch: HipKVBatch):
     return k, v
 
 
+def attention_i8_workspace(cache: HipKVCache, batch: HipKVBatch, heads: int) -> int:
+    """Bytes of the workspace that `attention_i8_hip` takes for these arguments (0: none is needed): for calls that may overlap on a device, and
+    for calls recorded into a graph, `HipStorage.empty(bytes, np.uint8)` each."""
+    return capi.lib().vtl_hip_attention_i8_workspace(C.byref(cache.handle), C.byref(batch.handle), heads)
+
+
 def attention_i8_hip(cache: HipKVCache, batch: HipKVBatch, q: HipTensor, heads: int, scale: float | None = None, causal: bool = True,
                      q_first: int = 0, workspace: HipStorage | None = None) -> HipTensor:
     """`attention_i8_hip(cache, batch, q, heads, scale, causal) !&HipTensor[f32]`: softmax(scale * q . k^T) . v of every row over
     its sequence, [rows, heads, head_dim]; scale is 1 / sqrt(head_dim) unless given.  The rows' own tokens have been written before.
-    q may be columns of a fused projection's output, from q_first on."""
+    q may be columns of a fused projection's output, from q_first on; workspace, of `attention_i8_workspace` bytes, is the library's own
+    unless given."""
     width = heads * cache.head_dim
     qp, qs = _rows(q, batch, width, q_first, "attention_i8_hip q")
     if scale is None:
