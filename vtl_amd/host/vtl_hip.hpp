@@ -409,7 +409,8 @@ inline void kv_write_hip(const HipKVCache &cache, const HipKVBatch &batch, const
     hip_check(vtl_hip_kv_write_f32(&c, &b, kp, ks, vp, vs), "vtl_hip_kv_write_f32");
 }
 
-// `kv_read_hip(cache, batch) !(&HipTensor[f32], &HipTensor[f32])`: the rows back, [rows, kv_heads, head_dim] each.
+// `kv_read_hip(cache, batch) !(&HipTensor[f32], &HipTensor[f32])`: the rows back, [rows, kv_heads, head_dim] each.  Rows of no
+// sequence are not written: what they hold is undefined.
 inline std::pair<HipTensor<float>, HipTensor<float>> kv_read_hip(const HipKVCache &cache, const HipKVBatch &batch)
 {
     const HipParams p{cache.pages.device_id};
@@ -431,7 +432,8 @@ inline size_t attention_i8_workspace(const HipKVCache &cache, const HipKVBatch &
 }
 
 // `attention_i8_hip(cache, batch, q, heads, scale, causal, workspace) !&HipTensor[f32]`: softmax(scale * q . k^T) . v of every
-// row over its sequence, [rows, heads, head_dim]; workspace, of attention_i8_workspace bytes, may be null.
+// row over its sequence, [rows, heads, head_dim]; workspace, of attention_i8_workspace bytes, may be null.  Rows of no sequence are
+// not written: what they hold is undefined.
 inline HipTensor<float> attention_i8_hip(const HipKVCache &cache, const HipKVBatch &batch, const HipTensor<float> &q, int heads, float scale, bool causal,
                                          const HipStorage<uint8_t> *workspace = nullptr, size_t q_first = 0)
 {

@@ -79,7 +79,8 @@ def kv_write_hip(cache: HipKVCache, batch: HipKVBatch, k: HipTensor, v: HipTenso
 
 
 def kv_read_hip(cache: HipKVCache, batch: HipKVBatch):
-    """`kv_read_hip(cache, batch) !(&HipTensor[f32], &HipTensor[f32])`: the rows' keys and values, [rows, kv_heads, head_dim] each."""
+    """`kv_read_hip(cache, batch) !(&HipTensor[f32], &HipTensor[f32])`: the rows' keys and values, [rows, kv_heads, head_dim] each.
+    Rows of no sequence are not written: what they hold is undefined."""
     p = cache.pages.params
     k = HipTensor.empty([batch.rows, cache.kv_heads, cache.head_dim], np.float32, p)
     v = HipTensor.empty(k.shape, np.float32, p)
@@ -99,7 +100,7 @@ def attention_i8_hip(cache: HipKVCache, batch: HipKVBatch, q: HipTensor, heads: 
     """`attention_i8_hip(cache, batch, q, heads, scale, causal) !&HipTensor[f32]`: softmax(scale * q . k^T) . v of every row over
     its sequence, [rows, heads, head_dim]; scale is 1 / sqrt(head_dim) unless given.  The rows' own tokens have been written before.
     q may be columns of a fused projection's output, from q_first on; workspace, of `attention_i8_workspace` bytes, is the library's own
-    unless given."""
+    unless given.  Rows of no sequence are not written: what they hold is undefined."""
     width = heads * cache.head_dim
     qp, qs = _rows(q, batch, width, q_first, "attention_i8_hip q")
     if scale is None:
