@@ -322,7 +322,8 @@ typedef struct {
  * are not attended to.  The same holds for rows in front of a sequence's first token (more rows than tokens): not
  * written, read as zeros, and attending to nothing where causal.
  * most_rows and most_length are the largest number of rows and the largest length of any sequence, for the host's choice of
- * launches: larger ones on the device are computed all the same, only slower.  0: not known. */
+ * launches: larger ones on the device are computed all the same, only slower.  0: not known; all rows, and the tokens that the table has
+ * room for, are taken for them, which is slow for many rows over much shorter sequences. */
 typedef struct {
     int batch, max_pages;
     const int32_t *page_table;   /* [batch, max_pages] */
@@ -353,9 +354,9 @@ int vtl_hip_kv_read_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_batch *b
  * heads is a multiple of kv_heads; rows times heads are 2^31 - 64 at most, as are the
  * values of a row (VTL_HIP_ERR_UNSUPPORTED beyond).  out may not share memory with q.
  *
- * q and the weights enter the products with 22 bits below the largest of q that are worked on together (up to 256 rows), sums
- * are f32.  How sums are cut depends on the lengths and rows of the whole batch and on most_rows and most_length: the same call gives the same
- * bits, a sequence in another batch need not.
+ * q enters the products with 22 bits, or to 2^-28 of the row's largest value where that is less, and a weight times its value's scale with 22
+ * bits, or to 2^-22 of the row's largest (2^-16 among values 2^120 apart); scores and sums are f32 and have its range and steps.  How sums are cut depends on the lengths and rows of the whole batch and on most_rows and
+ * most_length: the same call gives the same bits, a sequence in another batch need not.
  *
  * workspace: device memory of at least vtl_hip_attention_i8_workspace() bytes, 16-byte aligned, for the parts of sequences that
  * several workgroups share; NULL (with size 0): the library's own (see above).  Calls that may overlap on a device need one each.  With up to 16

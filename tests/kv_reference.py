@@ -151,7 +151,7 @@ class Cache:
         same sum), and the score is rounded three times (3 2^-24 of it) and once more when the maximum is taken off (the size of both).  A weight
         is off by twice the largest such error (its own and the sum's), relatively, and by 2^-20 for the exponential, the 22 bits of the weight
         and the scales; adding up n tokens, 8 or more at a time, costs (n / 8 + 64) 2^-24.  The weight times the value's scale is two fp16 numbers once
-        the sequence's largest scale (up to 2^6 above the tile's) is brought to 2^9 at least, beside weights of up to 2^5: fp16 has no steps below 2^-24, so
+        the sequence's largest scale so far is brought to 2^9 at least, beside weights of up to 2^5: fp16 has no steps below 2^-24, so
         each such product is off by up to 2^-25 / 2^9 of that scale, and n of them, times codes of up to 127, over a sum of weights that is 1 at least, by
         n 127 2^-34 of it."""
         out = np.zeros((q.shape[0], heads, self.dim))

@@ -213,9 +213,9 @@ struct Joined {
 
 // ---- few rows: a tile's rows are 16 or 32, all of a sequence's that read one key/value head ------------
 //
-// Bound by the cache's bytes (2 D + 8 a token and head; 2 sequences of 65000 tokens, 8 heads of 128: 275 MB in 60.6 us, 4.5 TB/s, where a copy of 2 GiB
-// moves 4.9; 48 of up to 6000: 64.5 us) and, where those are few, by the latencies behind each other and the code read for the first time (one of 300:
-// 8.7 us; 8 of 3001 with 5 rows each, 16 heads of 64: 18.7 us, 1.8 TB/s).  So every wave takes tiles of 64 tokens for itself, straight from memory into the registers in
+// Bound by the way of the cache's bytes into registers (2 D + 8 a token and head; 2 sequences of 65000 tokens, 8 heads of 128: 275 MB in 60.7 us, 4.5 TB/s,
+// where a stream that is only read has 7.3; 48 of up to 6000: 63.8 us) and, where those are few, by the latencies behind each other and the code read for the
+// first time (one of 300: 8.4 us; 8 of 3001 with 5 rows each, 16 heads of 64: 17.9 us, 1.9 TB/s).  So every wave takes tiles of 64 tokens for itself, straight from memory into the registers in
 // the order in which the matrix units take them; keys of the next tile are on their way while the weights of one are made, its values while the next
 // one's scores are, and the pages of both are looked up a tile before.
 //
@@ -720,14 +720,14 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of
 
 // ---- many rows: every wave has 32 of them, and the waves of a workgroup share the tokens -------------------
 //
-// Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 871 us, 1.18 PFLOP/s of fp16 products
-// (two halves for each), where the library's product of 8192 x 8192 x 8192 makes 1.22; the clock is down to 1.6 GHz then, and nothing but
-// those products, on such operands, takes 605 us.  A prompt of 4096: 256 us.  Vector work is nearly as much (ten operations a score, four of them the
+// Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 888 to 950 us from card to card, 1.09
+// to 1.16 PFLOP/s of fp16 products (two halves for each), where the library's product of 8192 x 8192 x 8192 makes 1.16 to 1.22; the clock is down to 1.6 GHz
+// then, and nothing but those products, on such operands, takes 605 to 647 us.  A prompt of 4096: 258 to 276 us.  Vector work is nearly as much (ten operations a score, four of them the
 // exponential) and goes on beside the products.  A tile of 64 tokens (32 above 128 dimensions, where registers are short) is made fp16 once for all
 // waves, on its way into LDS; a tile is worked on while the next is written to the other half of LDS and the one behind it is on its way from
 // memory.  Pieces of 8 dimensions (keys) and of 8 tokens (values) lie together there, [piece][token or dimension][8], so that a wave's operand is 512
 // consecutive bytes for each half wave.  Where there are few tiles a workgroup's start and end are what counts (code read for the first time, q's way
-// in, the results' out): 4 x 77 rows over 1500 tokens, 12 heads of 64, take 17.2 us, 3 x 201 rows over up to 1777, 20 heads of 80, 35.
+// in, the results' out): 4 x 77 rows over 1500 tokens, 12 heads of 64, take 18.1 us, 3 x 201 rows over up to 1777, 20 heads of 80, 36.
 //
 // The sums are brought to a new maximum only where a row's has risen by more than 2^kSlack: until then its weights are up to 2^kSlack, for
 // which the values' scales leave room (2^(kSlack + 10) is below fp16's largest number).
@@ -755,7 +755,7 @@ struct alignas(16) ManyTile {
 // What __builtin_amdgcn_sched_group_barrier calls them.
 constexpr int kSchedVector = 0x2, kSchedProduct = 0x8, kSchedRead = 0x100;
 
-// SPLIT: whether tokens are split (a variant of its own: without, a prompt of 4096 takes a hundredth less).
+// SPLIT: whether tokens are split (a variant of its own: without, two prompts of 2500 with 16 heads of 256 take 317 us and not 327, the chunk 900 and not 905).
 template <int DT, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_kernel(Kv kv, const float *__restrict__ q, int64_t q_stride, Group of, float scale,
                                                                                      int causal, float *__restrict__ out, int64_t out_stride, Parts parts,
@@ -1351,16 +1351,16 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
     const int64_t group = heads / kv.kv_heads, rows = most_rows * group;
     if ((int64_t)kv.rows * heads > 0x7fffffc0 || (int64_t)heads * kv.head_dim > 0x7fffffc0)
         return VTL_HIP_ERR_UNSUPPORTED;
-    // Up to 32 rows are few (16 above 128 dimensions, as many as the registers hold): 8 sequences of up to 3001 tokens with 16 heads of 64 values take 27.3 us with
-    // 32 rows each, where the other kernel takes 46.9 with any number up to 128; of 128 values 49.1 and 64.1.  But 17 and more are many where there
+    // Up to 32 rows are few (16 above 128 dimensions, as many as the registers hold): 8 sequences of 3001 tokens with 16 heads of 64 values take 27.4 us with
+    // 32 rows each, where the other kernel takes 47.6 with any number up to 128; of 128 values 50.4 and 65.5.  But 17 and more are many where there
     // is little to read for a compute unit, 256 tokens or, above 64 dimensions, where half as many waves have room, 1024: 20 sequences of 333, 24 rows each, 8 heads
-    // of 128, take 20.9 us and 23.8, 20 of 1000 29.7 and 40.5, 45 of 1000 49.5 and 53.8; of 64 values 21.8 and 17.6.
+    // of 128, take 21.8 us and 24.0, 20 of 1000 31.2 and 41.1, 45 of 1000 50.5 and 55.0; of 64 values 20 of 1000 22.3 and 17.8.
     p.many = rows > (kv.padded > 128 ? 16 : 32) ||
              (rows > 16 && (double)kv.batch * kv.kv_heads * (double)most_length <= 256.0 * (kv.padded > 64 ? 1024 : 256));
     // Many rows: eight waves share the codes that are made fp16 and brought to LDS once, and have a compute unit for themselves, where there is enough to do, four
     // tiles of tokens for each of them (a row sees half of its sequence's new tokens), and their rows do not lie idle.  2048 rows behind 14336 tokens, 32 heads of
-    // 128 on 8: 908 us and 958 with four waves on the same card, a prompt of 4096 266 and 286, 512 rows behind 29500 442 and 518; but a prompt of
-    // 1000 48.4 and 44.7, 40 rows over 3000 23.0 and 20.5, 4 x 70 with 8 x 4 heads of 64 (three halves of tiles) 36.9 and 34.2.
+    // 128 on 8: 905 us and 945 with four waves on the same card, a prompt of 4096 266 and 287, 512 rows behind 29500 442 and 519; but a prompt of
+    // 1000 49.0 and 44.3, 40 rows over 3000 23.1 and 20.7, 4 x 70 over 3000 with 8 x 4 heads of 64 (three halves of tiles) 38.9 and 36.8.
     const int64_t halves = (rows + kManyRows * 4 - 1) / (kManyRows * 4);      // tiles of four waves' rows
     const double work = (double)kv.batch * kv.kv_heads * (double)((halves + 1) / 2) * (double)(most_length - std::min(most_rows, most_length) / 2);
     // a grid has less than 2^32 threads in a row
@@ -1378,9 +1378,9 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         p.tiles = (int)std::min<int64_t>(p.tiles, std::min<int64_t>(0xffff, std::max<int64_t>(1, kKvMostBlocks / both)));
         units = both * p.tiles;
         // Whatever has least to do one after the other.  Four waves: a workgroup for each compute unit or two, which take turns with its matrix units
-        // (48 tiles of rows over 1500 tokens: 5 splits take 17.3 us, 8 take 18.2 and 12 take 23; 96 over 1777: 2 take 44.8 and 5 take 37.0).  Where a compute
+        // (48 tiles of rows over 1500 tokens: 5 splits take 18.5 us, 8 take 19.2 and 12 take 24.2; 96 over 1777: 2 take 45.1 and 5 take 38.8).  Where a compute
         // unit has one, as many splits as fill them once or, of few, whose rounds leave fewer idle; a round's start and end count as 512 tokens
-        // (1826 rows behind 11564 tokens, 20 heads of 64 on 4, 144 tiles: 413 us without splits, 308 with 5).  Not from 256
+        // (1826 rows behind 11564 tokens, 20 heads of 64 on 4, 144 tiles: 417 us without splits, 311 with 5).  Not from 256
         // tiles on: as many short ones as long ones fill the last round where a prompt is causal.
         const bool alone = p.waves == 8 || kv.padded > 128;
         int64_t least = 0;
@@ -1401,9 +1401,9 @@ int plan_of(const Kv &kv, const vtl_hip_kv_batch &b, int heads, Plan &p)
         parts = p.splits > 1 ? units * p.splits : 0;
     } else {
         // Eight waves, of which a unit has one workgroup, where they save the meeting of several (up to 512 tokens: 20 sequences with 8 heads of 128 values
-        // and 500 tokens take 11.5 us, with four waves 15.5), where the parts to meet are many (a sequence of 20000: 22.9 and 25.3) or a tile has
-        // half the bytes (8 sequences of 3001, 16 heads of 64 values: 18.7 and 20.0).  Else four, of which a compute unit has two workgroups that are not
-        // in step (48 sequences of 6000: 64.5 and 73.2; 2 of 3000: 11.8 and 13.0).
+        // and 500 tokens take 10.4 us, with four waves 13.7), where the parts to meet are many (a sequence of 20000: 22.1 and 23.5) or a tile has
+        // half the bytes (8 sequences of 3001, 16 heads of 64 values: 17.7 and 18.8).  Else four, of which a compute unit has two workgroups that are not
+        // in step (48 sequences of 6000: 64.7 and 69.6; 2 of 3000: 11.4 and 12.8).
         const bool eight = kv.padded <= 128 && (p.tile_rows == 16 || kv.padded <= 64);
         const bool better = most_length <= 512 || kv.padded <= 64 ? units <= 256 : units <= 32 && most_length > 15 * 256;
         p.waves = eight && better ? 8 : 4;
@@ -1470,7 +1470,7 @@ int launch_many(const Call &c)
         hipLaunchKernelGGL(kernel, dim3(blocks.x, (unsigned)(kManyRows * WAVES / at_once), blocks.z), dim3(256), 0, current_stream(), c.kv, of, c.causal,
                            c.out, c.out_stride, parts, aligned);
     };
-    // many parts: 128 rows over 8000 tokens with one head of 64 are done after 16.0 us, with a wave for a row's parts after 25.6
+    // many parts: 128 rows over 8000 tokens with one head of 64 are done after 16.2 us, with a wave for a row's parts after 25.9
     if (c.plan.splits > 16)
         join(attention_many_join_kernel<DT, WAVES, 4>, kTogether);
     else
