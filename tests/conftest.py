@@ -32,6 +32,15 @@ def _few_processors(request, monkeypatch):
         monkeypatch.setenv("VTL_HIP_HOST_QUANTIZE", "0")
 
 
+@pytest.fixture(autouse=True)
+def _no_idle_threads(request, monkeypatch):
+    """The programs that test_host_runtime.py runs measure processor time, which must not be that of numpy's library: its threads, made at
+    the import, look for work for half a second before they sleep (0.6 s of sleep right behind the import: 0.5 to 0.63 s of processor
+    time with eight of them, none with one)."""
+    if request.module.__name__ == "test_host_runtime":
+        monkeypatch.setenv("OPENBLAS_NUM_THREADS", "1")
+
+
 class _Knobs:
     """Environment switches of the library for one test: the library reads its
     VTL_HIP_* switches once, so every change here is followed by
