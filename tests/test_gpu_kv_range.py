@@ -152,6 +152,25 @@ def test_large_values_without_weight(counts, dim, power):
 
 
 @pytest.mark.parametrize("counts", ROWS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("mean", [-250, -500])
+def test_low_scores_beside_large_values(counts, dim, mean):
+    """All scores are far below zero, and values' scales 2^40 apart from the first token on."""
+    c = Cache([400, 330], 32, 2, dim, seed=16)
+    kc, _, ks, vs = c.parts()
+    rng = np.random.default_rng(17)
+    kc[:] = rng.integers(-103, -96, kc.shape)
+    written = c.table[c.table >= 0]
+    ks[written], vs[written] = np.float32(-mean / (100 * dim * 1.5)), np.exp2(rng.integers(-20, 20, vs[written].shape)).astype(np.float32)
+    c.to_device()
+    q = rng.uniform(1, 2, (rows_of(counts), 4, dim)).astype(np.float32)
+    for out in results(c, counts, q, 4, 1.0):
+        want, far = attend_alone(c, q, 4, 1.0, True)
+        off = np.abs(out - want)
+        assert (off <= far).all(), float((off / far).max())
+
+
+@pytest.mark.parametrize("counts", ROWS)
 def test_values_that_grow_and_shrink(counts):
     """Values' scales rise by 2^80 along a sequence and fall again, the scores against them: what counts is now here, now there."""
     c = Cache([700, 330], 32, 1, 64, seed=12)

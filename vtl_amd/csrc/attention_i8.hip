@@ -1129,10 +1129,10 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
                             size = fmaxf(size, fabsf(o[i][k]));
                     const int up = level_here - level_at;
                     most = max_across_32(most);
-                    most = most == -INFINITY ? (float)-up : most - (float)min(14, kMost - level_here);
+                    most = most == -INFINITY ? (rise == 0.0f ? (float)-up : rise) : most - (float)min(14, kMost - level_here);
                     const int least = max(exponent_of(max_across_32(sum)) - kMost,
                                           exponent_of(max_across_32(size)) - up - min(kMost, kMost + 17 - level_here));
-                    rise = fmaxf(fmaxf(most, top - kMost), (float)least);
+                    rise = fmaxf(fmaxf(most, top - kMost), off == kNone ? -INFINITY : (float)least);
                 }
                 // a row that has not seen a token has sums of 0 and scores of -infinity, and keeps them
                 const float now = off == kNone && top == -INFINITY ? off : less + rise, keep = off == kNone ? 1.0f : __builtin_amdgcn_exp2f(off - now);
