@@ -171,6 +171,26 @@ def test_low_scores_beside_large_values(counts, dim, mean):
 
 
 @pytest.mark.parametrize("counts", ROWS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("power", [16, 30, 80])
+def test_weight_on_tokens_without_values(counts, dim, power):
+    """A few tokens have all the weight and values of zero: what comes out is the others', by 2^power smaller and as exact as ever."""
+    c = Cache([400, 330], 32, 2, dim, seed=18)
+    kc, _, ks, vs = c.parts()
+    ks[c.table[c.table >= 0]] = np.float32(0.02 / dim ** 0.5)        # the others' scores are near 0
+    for b in range(2):
+        for token in (0, 70, 200):
+            page, slot = c.place(b, token)
+            kc[page, :, :, slot], ks[page, :, slot], vs[page, :, slot] = 100, np.float32(power * np.log(2) / (100 * dim * 1.5)), 0
+    c.to_device()
+    q = np.random.default_rng(19).uniform(1, 2, (rows_of(counts), 4, dim)).astype(np.float32)
+    for out in results(c, counts, q, 4, 1.0):
+        want, far = attend_alone(c, q, 4, 1.0, True)
+        off = np.abs(out - want)
+        assert (off <= far).all(), float((off / far).max())
+
+
+@pytest.mark.parametrize("counts", ROWS)
 def test_values_that_grow_and_shrink(counts):
     """Values' scales rise by 2^80 along a sequence and fall again, the scores against them: what counts is now here, now there."""
     c = Cache([700, 330], 32, 1, 64, seed=12)

@@ -734,8 +734,8 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of
 constexpr int kManyRows = 32;     // of a wave
 constexpr float kSlack = 5.0f;
 constexpr int kManyLevel = 9;     // the largest scale so far is brought to 2^9 .. 2^10
-// Scales further below the largest than 2^kNear, or a largest one that has risen by more than 2^kRise, leave fp16 few bits for the rows that have no weight
-// where the large ones are.  In such a tile each row is brought to where the largest product of a weight and a scale that it sees there is 2^14, as far as its
+// Scales further below the largest than 2^kNear, zeros among them, or a largest one that has risen by more than 2^kRise, leave fp16 few bits for the rows
+// that have no weight where the large ones are.  In such a tile each row is brought to where the largest product of a weight and a scale that it sees there is 2^14, as far as its
 // sums stay within f32, for which 2^kMost leaves room.
 constexpr int kNear = 10, kRise = 2, kMost = 110;
 
@@ -881,7 +881,7 @@ __global__ __launch_bounds__(64 * WAVES, DT > 128 ? 1 : 2) void attention_many_k
             t.value_scale[lane % TOKENS] = __builtin_ldexpf(value_scale, kManyLevel - level);
             base = first_tile ? level : base;
             first_tile = false;
-            const bool apart = __any(size != 0.0f && exponent_of(size) < level - kNear) || level > base + kRise;
+            const bool apart = __any(is && exponent_of(size) < level - kNear) || level > base + kRise;
             base = apart ? level : base;
             const int marked = (__any(!is || !finite) ? 1 : 0) | (apart ? 2 : 0);
             if (lane == 0) {
