@@ -6,9 +6,10 @@
 // meets them is no whole number: q (with scale and log2 e) and w_j sv_j, two halves of 11 bits each, hi = f16(x), lo = f16(x - hi), one product
 // for each.  So 22 bits of the operands enter, where one half alone would leave an error of 2^-11, and a third would cost half as much again.
 // q is scaled by a power of two to a largest value between 2^14 and 2^15 (the rows of a workgroup that shares tiles by one, but for those more than
-// 2^kNear below, and else each row by its own): lo keeps its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.  The products w_j sv_j are kept between 2^13 and 2^14
-// likewise, by the largest that the row itself has had: a token that a row gives no weight takes nothing from it, however large its values.  (Few rows take
-// the largest of each tile; many rows take the values' scales for it and look at the products only where those are far apart, `kNear`.)
+// 2^kNear below, and else each row by its own): lo keeps its bits down to 2^-16 of the largest, and is off by 2^-39 of it below that.  The products
+// w_j sv_j are kept between 2^13 and 2^14 likewise, by the largest that the row itself has had: a token that a row gives no weight takes nothing from
+// it, however large its values.  (Few rows take the largest of each tile; many rows take the values' scales for it and look at the products only where
+// those are far apart, `kNear`.)
 //
 // One pass over the tokens, with the running maximum and sum of the softmax, in powers of two.  Products are transposed, tokens as the
 // rows of S^T = K Q^T and dimensions as those of O^T = V^T W^T: a lane then holds what belongs to one row of q, maximum and sum are taken within the
@@ -722,8 +723,8 @@ __global__ __launch_bounds__(256) void attention_few_join_kernel(Kv kv, Group of
 //
 // Bound by the matrix units, and by the power that they take: 2048 rows behind 14336 tokens, 32 heads of 128 on 8, take 888 to 950 us from card to card, 1.09
 // to 1.16 PFLOP/s of fp16 products (two halves for each), where the library's product of 8192 x 8192 x 8192 makes 1.16 to 1.22; the clock is down to 1.6 GHz
-// then, and nothing but those products, on such operands, takes 605 to 647 us.  A prompt of 4096: 258 to 276 us.  Vector work is nearly as much (ten operations a score, four of them the
-// exponential) and goes on beside the products.  A tile of 64 tokens (32 above 128 dimensions, where registers are short) is made fp16 once for all
+// then, and nothing but those products, on such operands, takes 605 to 647 us.  A prompt of 4096: 258 to 276 us.  Vector work is nearly as much (ten
+// operations a score, four of them the exponential) and goes on beside the products.  A tile of 64 tokens (32 above 128 dimensions, where registers are short) is made fp16 once for all
 // waves, on its way into LDS; a tile is worked on while the next is written to the other half of LDS and the one behind it is on its way from
 // memory.  Pieces of 8 dimensions (keys) and of 8 tokens (values) lie together there, [piece][token or dimension][8], so that a wave's operand is 512
 // consecutive bytes for each half wave.  Where there are few tiles a workgroup's start and end are what counts (code read for the first time, q's way
