@@ -42,14 +42,15 @@ def test_two_threads_on_streams_of_their_own(hiprt):
         call = Call(c, counts, heads, 128, seed=i)
         call.enqueue()
         want.append(call.result())
-    wrong, streams = [], [new_stream(hiprt) for _ in range(2)]
+    wrong, streams, one_at_a_time = [], [new_stream(hiprt) for _ in range(2)], threading.Lock()
 
     def work(stream):
         try:
             capi.call("vtl_hip_set_device", 0)
             capi.call("vtl_hip_set_stream", stream)
-            calls = [Call(c, counts, heads, 128, seed=i) for i, (counts, heads) in enumerate(mixes)]
-            for _ in range(5):
+            with one_at_a_time:       # Cache.batch writes down the starts
+                calls = [Call(c, counts, heads, 128, seed=i) for i, (counts, heads) in enumerate(mixes)]
+            for _ in range(20):
                 for call in calls:
                     call.enqueue()
                 capi.call("vtl_hip_sync")
