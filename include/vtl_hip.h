@@ -369,6 +369,62 @@ int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_bat
                              int heads, float scale, int causal, float *out, int64_t out_stride, void *workspace,
                              size_t workspace_bytes);
 
+/* ---- microscaled 4-bit floating point (MXFP4) ------------------------------- */
+
+/* Rows of 4-bit codes with a scale for every 32 values.  A code (e2m1) is a sign (bit 3) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; a scale (e8m0) is a
+ * byte b for 2^(b - 127), 255 for no number; a value is their product.  A matrix [rows, cols] lies in rows padded to
+ * vtl_hip_mxfp4_padded_row(cols) values, cols rounded up to a multiple of 256 (0: no such row): codes [rows, padded / 2] bytes, the value with the even
+ * index in the low four bits, and scales [rows, padded / 32] bytes; codes are 16-byte aligned, scales 8-byte aligned.  Codes and scales behind the
+ * end of a row are zeros (as vtl_hip_quantize_f32_mxfp4 leaves them); where cols is a multiple of 256 this is the usual dense packing.
+ * cols is at most 2^24, and rows times padded / 256 less than 2^31 (VTL_HIP_ERR_UNSUPPORTED beyond). */
+int vtl_hip_mxfp4_padded_row(int cols);
+
+/* Rows of f32, x_stride elements from one to the next: b = max(0, e - 2) with e the exponent field of the block's largest magnitude, each code the
+ * nearest to x / 2^(b - 127), the even one of two, at most 6 in magnitude.  A block with an infinity or NaN gets b = 255 and zero codes. */
+int vtl_hip_quantize_f32_mxfp4(const float *x, int64_t x_stride, int64_t rows, int64_t cols, uint8_t *codes, uint8_t *scales);
+/* x = code * 2^(b - 127) in f32. */
+int vtl_hip_dequantize_mxfp4_f32(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, float *x, int64_t x_stride);
+
+/* Y[m,n] = x[m,:] . w[n,:] + bias[n], ReLU if relu != 0 (x < 0 -> 0), with both operands as codes, x [M, K] and w [N, K]; bias may be NULL.
+ * Sums of 32 products are exact, and added up in f32; in how many ranges K is cut depends on M, N and K alone, so the same
+ * call gives the same bits, a row among other rows need not.  A block without a number makes its row's or column's outputs NaN.
+ * workspace: device memory of vtl_hip_linear_mxfp4_workspace() bytes (0: none is needed), 16-byte aligned; NULL (with size 0): the library's own (see
+ * above).  Calls that may overlap on a device need one each. */
+size_t vtl_hip_linear_mxfp4_workspace(int M, int N, int K);
+int vtl_hip_linear_mxfp4_f32(const uint8_t *x, const uint8_t *x_scales, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M,
+                             int N, int K, int relu, void *workspace, size_t workspace_bytes);
+/* The same of f32 rows X[M, K], which become codes as vtl_hip_quantize_f32_mxfp4 makes them: in the product's own launch where they are few, else in
+ * one before it. */
+size_t vtl_hip_linear_f32_mxfp4_workspace(int M, int N, int K);
+int vtl_hip_linear_f32_mxfp4(const float *X, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M, int N, int K, int relu,
+                             void *workspace, size_t workspace_bytes);
+
+/* A layer of experts: a router gives each token a score for every expert, the top_k experts with the largest scores take part.
+ *   score[e]  = f32(sum of router[e,:] . x in f64) + router_bias[e]
+ *   p         = softmax of the scores, over all experts; renormalize: over the chosen ones
+ *   h_e       = SiLU(gate_e . x + bias) * (up_e . x + bias), SiLU(g) = g / (1 + exp(-g))
+ *   y         = sum over the chosen e of p[e] * (down_e . h_e + down_bias[e])
+ * Of equal scores the lower index is chosen, NaN behind all numbers.  gate_up has rows of dim values, for each expert those of its gate and then
+ * those of its up (hidden each); down has dim rows of hidden values for each expert.  The biases may be NULL. */
+enum { VTL_HIP_MOE_MOST_TOKENS = 64, VTL_HIP_MOE_MOST_EXPERTS = 512, VTL_HIP_MOE_MOST_TOP = 16, VTL_HIP_MOE_MOST_DIM = 65536 };
+typedef struct {
+    int experts, top_k, dim, hidden, renormalize;
+    const float *router;            /* [experts, dim] */
+    const float *router_bias;       /* [experts] */
+    const uint8_t *gate_up, *gate_up_scales;   /* [experts * 2 * hidden, dim] */
+    const float *gate_up_bias;      /* [experts, 2 * hidden] */
+    const uint8_t *down, *down_scales;         /* [experts * dim, hidden] */
+    const float *down_bias;         /* [experts, dim] */
+} vtl_hip_moe;
+
+/* Y[tokens, dim] of X[tokens, dim], for a few tokens: up to VTL_HIP_MOE_MOST_TOKENS, and experts, top_k, dim and hidden within the limits
+ * above (VTL_HIP_ERR_UNSUPPORTED beyond).  x, and p times the hidden values, enter the products with 24 bits of the largest among 32 (to 2^-128 where that is below
+ * 2^-103), sums are f32; the same call gives the same bits.  A token with an infinity or NaN, or without a finite score, gives NaN, and so does a
+ * chosen expert's block of weights without a number.  X and Y may not share memory.
+ * workspace: as above, of vtl_hip_moe_mxfp4_workspace() bytes (0: no such layer). */
+size_t vtl_hip_moe_mxfp4_workspace(const vtl_hip_moe *layer, int tokens);
+int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, int tokens, void *workspace, size_t workspace_bytes);
+
 /* ---- f32 / f64 matmul with f64 accumulation ------------------------------ */
 
 /* C[M,N] = op(A) . op(B) with every product and sum in f64 and one rounding

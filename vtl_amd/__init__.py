@@ -3,7 +3,8 @@
 `capi` binds the C ABI of libvtlhip.so; `storage`, `tensor`, `layers` and
 `models` mirror the V files that plug it into VTL (HipStorage, HipTensor,
 the linear_forward_f32 hook, Sequential.linear); `kv_cache` has the
-int8 key/value cache and the attention over it.
+int8 key/value cache and the attention over it, `mxfp4` rows of microscaled
+4-bit codes with linear layers and a layer of experts on them.
 """
 from . import capi  # noqa: F401
 from .kv_cache import HipKVBatch, HipKVCache, attention_i8_hip, attention_i8_workspace, kv_read_hip, kv_write_hip  # noqa: F401
@@ -14,6 +15,8 @@ from .layers import (PER_CHANNEL, PER_TENSOR, HipSession, QuantLinearLayer,  # n
                      linear_gate_use_hip_backward, matmul_gate_backward_hip, matmul_hip_host,
                      relu_forward_hip_f32,
                      sigmoid_forward_hip_f32)
+from .mxfp4 import (HipMoE, HipMxfp4, linear_f32_mxfp4_hip, linear_mxfp4_hip, linear_mxfp4_workspace, moe_mxfp4_hip,  # noqa: F401
+                    quantize_mxfp4_hip)
 from .models import Sequential  # noqa: F401
 from .storage import HipParams, HipStorage, hip_available  # noqa: F401
 from .tensor import (HipTensor, colsum_hip, gemm_i8_hip, linear_backward_hip,  # noqa: F401

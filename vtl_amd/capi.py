@@ -47,6 +47,13 @@ class KVBatch(C.Structure):
                 ("rows", _ci), ("most_rows", _ci), ("most_length", _ci)]
 
 
+class MoE(C.Structure):
+    """`vtl_hip_moe`: a layer of experts whose weights are MXFP4 rows on the device."""
+    _fields_ = [("experts", _ci), ("top_k", _ci), ("dim", _ci), ("hidden", _ci), ("renormalize", _ci),
+                ("router", _vp), ("router_bias", _vp), ("gate_up", _vp), ("gate_up_scales", _vp), ("gate_up_bias", _vp),
+                ("down", _vp), ("down_scales", _vp), ("down_bias", _vp)]
+
+
 _pc, _pb = C.POINTER(KVCache), C.POINTER(KVBatch)
 
 # name -> (restype, argtypes); kept in step with include/vtl_hip.h
@@ -115,6 +122,15 @@ SIGNATURES = {
     "vtl_hip_kv_read_f32": (_ci, [_pc, _pb, _vp, _i64, _vp, _i64]),
     "vtl_hip_attention_i8_workspace": (_sz, [_pc, _pb, _ci]),
     "vtl_hip_attention_i8_f32": (_ci, [_pc, _pb, _vp, _i64, _ci, C.c_float, _ci, _vp, _i64, _vp, _sz]),
+    "vtl_hip_mxfp4_padded_row": (_ci, [_ci]),
+    "vtl_hip_quantize_f32_mxfp4": (_ci, [_vp, _i64, _i64, _i64, _vp, _vp]),
+    "vtl_hip_dequantize_mxfp4_f32": (_ci, [_vp, _vp, _i64, _i64, _vp, _i64]),
+    "vtl_hip_linear_mxfp4_workspace": (_sz, [_ci, _ci, _ci]),
+    "vtl_hip_linear_mxfp4_f32": (_ci, [_vp, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp, _sz]),
+    "vtl_hip_linear_f32_mxfp4_workspace": (_sz, [_ci, _ci, _ci]),
+    "vtl_hip_linear_f32_mxfp4": (_ci, [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp, _sz]),
+    "vtl_hip_moe_mxfp4_workspace": (_sz, [C.POINTER(MoE), _ci]),
+    "vtl_hip_moe_mxfp4_f32": (_ci, [C.POINTER(MoE), _vp, _vp, _ci, _vp, _sz]),
     "vtl_hip_strerror": (C.c_char_p, [_ci]),
     "vtl_hip_last_error": (C.c_char_p, []),
     "vtl_hip_version": (C.c_char_p, []),

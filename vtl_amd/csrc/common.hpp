@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "vtl_hip.h"
 
 namespace vtlhip {
@@ -325,6 +327,24 @@ struct Tuning {
     int matmul_splits = -1;         // VTL_HIP_MATMUL_SPLITS: K ranges of the f64-accumulating matmul
 };
 const Tuning &tuning();
+
+// A flag per device: kernel attributes are per device, the library may serve several.  Atomic,
+// so that two host threads that meet at a kernel's first launch do not race on the flag itself
+// (setting the attribute twice is harmless).
+using DoneFlag = std::atomic<bool>;
+template <typename V>
+struct PerDevice {
+    V v[64] = {};
+    V &get()
+    {
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
+            (void)hipGetLastError();
+            dev = 0;
+        }
+        return v[dev];
+    }
+};
 
 constexpr int kWave = 64;
 

@@ -1997,24 +1997,6 @@ inline void attach_gemv_result(GemmArgs &g, unsigned blocks, bool one_batch)
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// A flag per device: kernel attributes are per device, the library may serve several.  Atomic,
-// so that two host threads that meet at a kernel's first launch do not race on the flag itself
-// (setting the attribute twice is harmless).
-using DoneFlag = std::atomic<bool>;
-template <typename V>
-struct PerDevice {
-    V v[64] = {};
-    V &get()
-    {
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
-            (void)hipGetLastError();
-            dev = 0;
-        }
-        return v[dev];
-    }
-};
-
 template <typename Kern>
 int launch_with_lds(Kern kern, DoneFlag &attr_done, int lds, int tiles, int threads, const GemmArgs &g,
                     hipStream_t st, const char *name)

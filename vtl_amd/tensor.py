@@ -174,6 +174,11 @@ class HipTensor:
         capi.call("vtl_hip_dequantize_i8_f32", self.ptr, scales.ptr, rows, cols, per_row, x.ptr)
         return x
 
+    def quantize_mxfp4(self):
+        """`quantize_mxfp4() !&HipMxfp4`: 4-bit codes with a scale for every 32 values of a row (mxfp4.py)."""
+        from .mxfp4 import quantize_mxfp4_hip
+        return quantize_mxfp4_hip(self)
+
     def relu_(self) -> "HipTensor":
         """In-place ReLU (x < 0 -> 0), cf. relu_cuda tensor_cuda_d_cuda.v:205-235."""
         sfx = _float_suffix(self, "relu_")
