@@ -19,11 +19,13 @@ namespace {
 constexpr int kMostTokens = VTL_HIP_MOE_MOST_TOKENS, kMostExperts = VTL_HIP_MOE_MOST_EXPERTS, kMostTop = VTL_HIP_MOE_MOST_TOP;
 constexpr int kDigits = 5, kTokensATile = 3;   // 15 of a tile's 16 columns
 
-// Which experts have tokens, in order, and which tokens: written by moe_plan_kernel.
+// Which experts have tokens, in order, and which tokens: pairs of an expert and a token.
+struct Entry {
+    int expert, offset, pairs, unused;      // the expert's first pair, and how many it has
+};
 struct Plan {
-    int count;                              // experts that somebody chose
-    int expert[kMostExperts];
-    int offset[kMostExperts + 1];           // their first (expert, token) pair
+    int count, unused[3];                   // experts that somebody chose
+    Entry entry[kMostExperts];
     int token[kMostTokens * kMostTop];      // of a pair
     float weight[kMostTokens * kMostTop];
 };
@@ -39,6 +41,8 @@ struct Args {
     Plan *plan;
     uint8_t *x_digits, *x_scales;           // [tokens, 5, dim padded], [tokens, dim padded / 32]
     uint8_t *h_digits, *h_scales;           // the same of each pair's hidden values
+    float *parts;                           // [splits, tokens, dim] where several workgroups share rows of the output
+    int splits;
 };
 
 __device__ __forceinline__ v4f mfma_digits(v4i w, v8i d, v4f c, int sw, int sd)
@@ -92,54 +96,83 @@ __device__ __forceinline__ void store_digits(uint8_t *digits, uint8_t *scales, i
 
 // ---- scores ---------------------------------------------------------------------------------
 
-// A workgroup has one expert's scores for up to eight tokens, sums in f64 (scores next to each other decide on experts), or, behind those, four
-// chunks of the tokens' digits.
-constexpr int kScoreTokens = 8;
+// Added up over the lanes of a wave within the vector unit; the last lane has the sum.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_from(double v)
+{
+    const long long bits = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)bits, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, ROWS, 0xF, false);
+    return v + __builtin_bit_cast(double, (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo));
+}
+__device__ __forceinline__ double wave_sum_f64(double v)
+{
+    v = add_from<0xB1, 0xF>(v);     // quad_perm [1,0,3,2]
+    v = add_from<0x4E, 0xF>(v);     // quad_perm [2,3,0,1]
+    v = add_from<0x141, 0xF>(v);    // row_half_mirror
+    v = add_from<0x140, 0xF>(v);    // row_mirror
+    v = add_from<0x142, 0xA>(v);    // lane 15 of a row into the next row
+    return add_from<0x143, 0xC>(v); // lane 31 into the upper half
+}
 
+// A workgroup has one expert's scores for NT tokens, sums in f64 (scores next to each other decide on experts), or, behind those, four
+// chunks of the tokens' digits.
+template <int NT, bool VEC>
 __global__ __launch_bounds__(256) void moe_scores_kernel(const Args g)
 {
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-    const int groups = (g.tokens + kScoreTokens - 1) / kScoreTokens;
-    int b = (int)blockIdx.x;
+    const int groups = (g.tokens + NT - 1) / NT;
+    const int b = (int)blockIdx.x;
+    auto four = [&](const float *row, int k) {
+        v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (VEC) {
+            if (k < g.dim)
+                v = *reinterpret_cast<const v4f *>(row + k);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (k + i < g.dim)
+                    v[i] = row[k + i];
+        }
+        return v;
+    };
     if (b >= g.experts * groups) {
         const int c = 4 * (b - g.experts * groups) + w;
         if (c >= g.tokens * g.dim_chunks)
             return;
-        const int t = c / g.dim_chunks, col = c % g.dim_chunks * kChunk + 4 * lane;
-        const float *const row = g.x + (size_t)t * g.dim;
-        v4f v;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            v[i] = col + i < g.dim ? row[col + i] : 0.0f;
-        const int padded = g.dim_chunks * kChunk;
+        const int t = c / g.dim_chunks, col = c % g.dim_chunks * kChunk + 4 * lane, padded = g.dim_chunks * kChunk;
+        const v4f v = four(g.x + (size_t)t * g.dim, col);
         store_digits(g.x_digits + (size_t)t * kDigits * padded, g.x_scales + (size_t)t * (padded / kBlock), padded, col, v);
         return;
     }
-    const int e = b % g.experts, t0 = b / g.experts * kScoreTokens, n = min(kScoreTokens, g.tokens - t0);
-    double sum[kScoreTokens];
+    const int e = b % g.experts, t0 = b / g.experts * NT;
+    double sum[NT];
 #pragma unroll
-    for (int t = 0; t < kScoreTokens; t++)
+    for (int t = 0; t < NT; t++)
         sum[t] = 0.0;
     const float *const router = g.router + (size_t)e * g.dim;
-    for (int k = (int)threadIdx.x; k < g.dim; k += 256) {
-        const double r = router[k];
+#pragma unroll 4
+    for (int k = 4 * (int)threadIdx.x; k < g.dim; k += 1024) {
+        const v4f r = four(router, k);
+        v4f x[NT];
 #pragma unroll
-        for (int t = 0; t < kScoreTokens; t++)
-            if (t < n)
-                sum[t] = fma((double)g.x[(size_t)(t0 + t) * g.dim + k], r, sum[t]);
+        for (int t = 0; t < NT; t++)
+            x[t] = four(g.x + (size_t)min(t0 + t, g.tokens - 1) * g.dim, k);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                sum[t] = fma((double)x[t][i], (double)r[i], sum[t]);
     }
-    __shared__ double part[4][kScoreTokens];
+    __shared__ double part[4][NT];
 #pragma unroll
-    for (int t = 0; t < kScoreTokens; t++)
-        if (t < n) {
-#pragma unroll
-            for (int step = 32; step; step >>= 1)
-                sum[t] += __shfl_xor(sum[t], step);
-            if (lane == 0)
-                part[w][t] = sum[t];
-        }
+    for (int t = 0; t < NT; t++) {
+        sum[t] = wave_sum_f64(sum[t]);
+        if (lane == kWave - 1)
+            part[w][t] = sum[t];
+    }
     __syncthreads();
-    if ((int)threadIdx.x < n) {
+    if (threadIdx.x < NT && t0 + (int)threadIdx.x < g.tokens) {
         float s = (float)(((part[0][threadIdx.x] + part[1][threadIdx.x]) + part[2][threadIdx.x]) + part[3][threadIdx.x]);
         if (g.router_bias)
             s = s + g.router_bias[e];
@@ -149,19 +182,35 @@ __global__ __launch_bounds__(256) void moe_scores_kernel(const Args g)
 
 // ---- the plan -------------------------------------------------------------------------------
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned max_from(unsigned v)
+{
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
+}
 __device__ __forceinline__ unsigned wave_max_u32(unsigned v)
 {
-#pragma unroll
-    for (int step = 32; step; step >>= 1)
-        v = max(v, (unsigned)__shfl_xor((int)v, step));
-    return v;
+    v = max_from<0xB1, 0xF>(v);
+    v = max_from<0x4E, 0xF>(v);
+    v = max_from<0x141, 0xF>(v);
+    v = max_from<0x140, 0xF>(v);
+    v = max_from<0x142, 0xA>(v);
+    v = max_from<0x143, 0xC>(v);
+    return (unsigned)__builtin_amdgcn_readlane((int)v, kWave - 1);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float sum_from(float v)
+{
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xF, false));
 }
 __device__ __forceinline__ float wave_sum_f32(float v)
 {
-#pragma unroll
-    for (int step = 32; step; step >>= 1)
-        v += __shfl_xor(v, step);
-    return v;
+    v = sum_from<0xB1, 0xF>(v);
+    v = sum_from<0x4E, 0xF>(v);
+    v = sum_from<0x141, 0xF>(v);
+    v = sum_from<0x140, 0xF>(v);
+    v = sum_from<0x142, 0xA>(v);
+    v = sum_from<0x143, 0xC>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kWave - 1));
 }
 
 // Numbers in their order, from 2 on; 1: NaN, behind all of them.
@@ -173,107 +222,130 @@ __device__ __forceinline__ unsigned order_of(float v)
     return max(b & 0x80000000u ? ~b : b | 0x80000000u, 2u);
 }
 
-// One workgroup: a wave has a token's scores, finds its `top` largest (the lower index of two that are equal) and notes the token with these experts;
-// then the experts that were noted are put in order.
-__global__ __launch_bounds__(1024) void moe_plan_kernel(const Args g)
+struct Choice {
+    Plan plan;
+    unsigned long long by[kMostExperts];    // the tokens that chose an expert, a bit each
+    float most[kMostTokens], total[kMostTokens];
+};
+
+// The plan, made in shared memory by the NW waves of a workgroup: a wave has a token's scores, EACH a lane, finds its `top` largest (the lower
+// index of two that are equal) and notes the token with these experts; then the experts that were noted are put in order.
+template <int EACH, int NW>
+__device__ __forceinline__ void make_plan(const Args &g, Choice &c)
 {
-    __shared__ unsigned long long chosen_by[kMostExperts];
-    __shared__ int place[kMostExperts], pairs[kMostExperts];
-    __shared__ float most[kMostTokens], total[kMostTokens];
-    constexpr int kEach = kMostExperts / kWave;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-    for (int e = (int)threadIdx.x; e < kMostExperts; e += 1024)
-        chosen_by[e] = 0;
+    for (int e = (int)threadIdx.x; e < EACH * kWave; e += NW * kWave)
+        c.by[e] = 0;
     __syncthreads();
-    for (int t = w; t < g.tokens; t += 16) {
-        float v[kEach];
-        unsigned key[kEach];
-        float high = -__builtin_inff();
+    for (int t = w; t < g.tokens; t += NW) {
+        float v[EACH];
+        unsigned key[EACH], top = 0;
 #pragma unroll
-        for (int i = 0; i < kEach; i++) {
+        for (int i = 0; i < EACH; i++) {
             const int e = lane + i * kWave;
             v[i] = e < g.experts ? g.scores[(size_t)t * g.experts + e] : -__builtin_inff();
-            key[i] = e < g.experts ? order_of(v[i]) : 0u;
-            high = fmaxf(high, v[i]);
         }
+        float high = -__builtin_inff();
 #pragma unroll
-        for (int step = 32; step; step >>= 1)
-            high = fmaxf(high, __shfl_xor(high, step));
-        float sum = 0.0f;
+        for (int i = 0; i < EACH; i++) {
+            key[i] = lane + i * kWave < g.experts ? order_of(v[i]) : 0u;
+            top = max(top, key[i]);
+        }
+        top = wave_max_u32(top);
+        // the largest score: NaN where there is nothing else, and then so is all that follows
+        high = top == 1u ? __builtin_nanf("") : __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
+        float sum = 0.0f, taken = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kEach; i++)
-            if (lane + i * kWave < g.experts)
-                sum += expf(v[i] - high);
+        for (int i = 0; i < EACH; i++) {
+            v[i] = lane + i * kWave < g.experts ? expf(v[i] - high) : 0.0f;
+            sum += v[i];
+        }
         sum = wave_sum_f32(sum);
-        float taken = 0.0f;
         for (int k = 0; k < g.top; k++) {
             unsigned m = 0;
 #pragma unroll
-            for (int i = 0; i < kEach; i++)
+            for (int i = 0; i < EACH; i++)
                 m = max(m, key[i]);
             m = wave_max_u32(m);
             bool found = false;
 #pragma unroll
-            for (int i = 0; i < kEach; i++) {
+            for (int i = 0; i < EACH; i++) {
                 const unsigned long long here = __ballot(key[i] == m);
                 if (!found && here) {
                     found = true;
                     const int at = __ffsll(here) - 1;
-                    taken += __shfl(expf(v[i] - high), at);
+                    taken += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[i]), at));
                     if (lane == at) {
                         key[i] = 0;
-                        atomicOr(&chosen_by[lane + i * kWave], 1ull << t);
+                        atomicOr(&c.by[lane + i * kWave], 1ull << t);
                     }
                 }
             }
         }
         if (lane == 0) {
-            most[t] = high;
-            total[t] = g.renormalize && sum == sum ? taken : sum;
+            c.most[t] = high;
+            c.total[t] = g.renormalize && sum == sum ? taken : sum;
         }
     }
     __syncthreads();
     if (w == 0) {
         int count = 0, at = 0;
-        for (int i = 0; i < g.experts; i += kWave) {
-            const int e = i + lane;
-            const unsigned long long who = e < g.experts ? chosen_by[e] : 0;
-            const unsigned long long some = __ballot(who != 0);
-            const int before = __popcll(some & ((1ull << lane) - 1));
-            int n = __popcll(who), first = n;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int e = i * kWave + lane;
+            const unsigned long long who = c.by[e], some = __ballot(who != 0);
+            const int n = __popcll(who);
+            int first = n;
 #pragma unroll
             for (int step = 1; step < kWave; step <<= 1) {
                 const int from = __shfl_up(first, step);
                 if (lane >= step)
                     first += from;
             }
-            const int all = __shfl(first, kWave - 1);
-            if (who) {
-                place[count + before] = e;
-                pairs[count + before] = at + first - n;
-            }
+            if (who)
+                c.plan.entry[count + __popcll(some & ((1ull << lane) - 1))] = Entry{e, at + first - n, n, 0};
             count += __popcll(some);
-            at += all;
+            at += __shfl(first, kWave - 1);
         }
-        if (lane == 0) {
-            g.plan->count = count;
-            g.plan->offset[count] = at;
-        }
-        for (int a = lane; a < count; a += kWave) {
-            g.plan->expert[a] = place[a];
-            g.plan->offset[a] = pairs[a];
-        }
-        __threadfence_block();
-        for (int a = lane; a < count; a += kWave) {
-            const int e = place[a];
-            unsigned long long who = chosen_by[e];
-            for (int i = pairs[a]; who; who &= who - 1, i++) {
-                const int t = __ffsll(who) - 1;
-                g.plan->token[i] = t;
-                g.plan->weight[i] = expf(g.scores[(size_t)t * g.experts + e] - most[t]) / total[t];
-            }
+        if (lane == 0)
+            c.plan.count = count;
+    }
+    __syncthreads();
+    for (int a = (int)threadIdx.x; a < c.plan.count; a += NW * kWave) {
+        const Entry entry = c.plan.entry[a];
+        unsigned long long who = c.by[entry.expert];
+        for (int i = entry.offset; who; who &= who - 1, i++) {
+            const int t = __ffsll(who) - 1;
+            c.plan.token[i] = t;
+            c.plan.weight[i] = expf(g.scores[(size_t)t * g.experts + entry.expert] - c.most[t]) / c.total[t];
         }
     }
+    __syncthreads();
+}
+
+// For the launches behind.
+template <int NW>
+__device__ __forceinline__ void publish(const Args &g, const Choice &c)
+{
+    const int pairs = g.tokens * g.top;
+    for (int i = (int)threadIdx.x; i < max(c.plan.count, pairs); i += NW * kWave) {
+        if (i < c.plan.count)
+            g.plan->entry[i] = c.plan.entry[i];
+        if (i < pairs) {
+            g.plan->token[i] = c.plan.token[i];
+            g.plan->weight[i] = c.plan.weight[i];
+        }
+    }
+    if (threadIdx.x == 0)
+        g.plan->count = c.plan.count;
+}
+
+template <int EACH>
+__global__ __launch_bounds__(1024) void moe_plan_kernel(const Args g)
+{
+    __shared__ Choice c;
+    make_plan<EACH, 16>(g, c);
+    publish<16>(g, c);
 }
 
 // ---- products -------------------------------------------------------------------------------
@@ -326,66 +398,92 @@ __device__ __forceinline__ float sum_digits(float v)
     return s + v;
 }
 
-constexpr int kProductWaves = 8;
+constexpr int kProductWaves = 8, kKWaves = 4;
 
-// 32 hidden values of an expert's tokens: 32 rows of its gate and as many of its up, K dealt out among the waves.  They go out as digits, already
-// times their weights, so that the next product adds experts up as it adds up K.
-template <int TILES>
+// Two 16-byte pieces of a row's chunk, and its scales.
+struct Weights {
+    v4i codes[2];
+    v2u scales;
+    __device__ __forceinline__ void load(const uint8_t *c, const uint8_t *s, int chunk)
+    {
+        codes[0] = *reinterpret_cast<const v4i *>(c + (size_t)chunk * kChunkCodes);
+        codes[1] = *reinterpret_cast<const v4i *>(c + (size_t)chunk * kChunkCodes + 64);
+        scales = *reinterpret_cast<const v2u *>(s + (size_t)chunk * kChunkScales);
+    }
+    __device__ __forceinline__ int scale(int step) const { return (int)(scales[step] >> ((int)(threadIdx.x % kWave) / 16 * 8)); }
+};
+
+// 32 hidden values of an expert's tokens: two times 16 rows of its gate and as many of its up, four waves each, which deal K out among them.
+// They go out as digits, already times their weights, so that the next product adds experts up as it adds up K.
+// EACH: every workgroup makes the plan for itself (a few tokens: less than a launch takes); 0: it is there.
+template <int TILES, int EACH>
 __global__ __launch_bounds__(64 * kProductWaves) void moe_gate_up_kernel(const Args g)
 {
-    __shared__ __attribute__((aligned(16))) float part[kProductWaves][TILES * kTokensATile][68];
+    __shared__ __attribute__((aligned(16))) float part[kProductWaves][TILES * kTokensATile][36];
     const int tiles = g.hidden_chunks * (kChunk / 32), a = (int)blockIdx.x / tiles, row0 = (int)blockIdx.x % tiles * 32;
-    if (a >= g.plan->count)
+    const Plan *plan = g.plan;
+    if constexpr (EACH != 0) {
+        __shared__ Choice c;
+        make_plan<EACH, kProductWaves>(g, c);
+        if (blockIdx.x == 0)
+            publish<kProductWaves>(g, c);
+        plan = &c.plan;
+    }
+    if (a >= plan->count)
         return;
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
-    const int e = g.plan->expert[a], offset = g.plan->offset[a], n = g.plan->offset[a + 1] - offset;
+    const int e = __builtin_amdgcn_readfirstlane(plan->entry[a].expert), offset = __builtin_amdgcn_readfirstlane(plan->entry[a].offset),
+              n = __builtin_amdgcn_readfirstlane(plan->entry[a].pairs);
     const size_t pitch = (size_t)g.dim_chunks * kChunkCodes, spitch = (size_t)g.dim_chunks * kChunkScales;
-    const uint8_t *wc[4], *ws[4];
+    const uint8_t *wc[2], *ws[2];
 #pragma unroll
-    for (int f = 0; f < 4; f++) {
-        const size_t row = (size_t)e * 2 * g.hidden + (f / 2) * (size_t)g.hidden + (size_t)min(row0 + f % 2 * 16 + r, g.hidden - 1);
+    for (int f = 0; f < 2; f++) {
+        const size_t row = ((size_t)e * 2 + f) * g.hidden + (size_t)min(row0 + w / kKWaves * 16 + r, g.hidden - 1);
         wc[f] = g.gate_up.codes + row * pitch + q * 16;
         ws[f] = g.gate_up.scales + row * spitch;
     }
-    const int begin = g.dim_chunks * w / kProductWaves, end = g.dim_chunks * (w + 1) / kProductWaves;
+    const int begin = g.dim_chunks * (w % kKWaves) / kKWaves, end = g.dim_chunks * (w % kKWaves + 1) / kKWaves;
     for (int first = 0; first < n; first += TILES * kTokensATile) {
         const int now = min(n - first, TILES * kTokensATile);
         if (row0 < g.hidden) {
             Columns<TILES> x;
-            x.at(g.x_digits, g.x_scales, g.dim_chunks * kChunk, g.plan->token, offset + first, now);
-            v4f acc[4][TILES];
+            x.at(g.x_digits, g.x_scales, g.dim_chunks * kChunk, plan->token, offset + first, now);
+            v4f acc[2][TILES];
 #pragma unroll
-            for (int f = 0; f < 4; f++)
+            for (int f = 0; f < 2; f++)
 #pragma unroll
                 for (int i = 0; i < TILES; i++)
                     acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            for (int c = begin; c < end; c++) {
-                v4i codes[4][2];
-                v2u scales[4];
+            for (int c = begin; c < end; c += 2) {
+                const bool two = c + 1 < end;
+                Weights weights[2][2];
 #pragma unroll
-                for (int f = 0; f < 4; f++) {
-                    codes[f][0] = *reinterpret_cast<const v4i *>(wc[f] + (size_t)c * kChunkCodes);
-                    codes[f][1] = *reinterpret_cast<const v4i *>(wc[f] + (size_t)c * kChunkCodes + 64);
-                    scales[f] = *reinterpret_cast<const v2u *>(ws[f] + (size_t)c * kChunkScales);
-                }
+                for (int h = 0; h < 2; h++)
+                    if (h == 0 || two)
 #pragma unroll
-                for (int i = 0; i < TILES; i++)
-                    if (i * kTokensATile < now) {
-                        const v2u xs = x.load_scales(i, c);
+                        for (int f = 0; f < 2; f++)
+                            weights[h][f].load(wc[f], ws[f], c + h);
 #pragma unroll
-                        for (int s = 0; s < 2; s++) {
-                            const v8i d = x.load(i, c, s);
-                            const int xb = x.scale(xs, s);
+                for (int h = 0; h < 2; h++)
+                    if (h == 0 || two)
 #pragma unroll
-                            for (int f = 0; f < 4; f++)
-                                acc[f][i] = mfma_digits(codes[f][s], d, acc[f][i], (int)(scales[f][s] >> (8 * q)), xb);
-                        }
-                    }
+                        for (int i = 0; i < TILES; i++)
+                            if (i * kTokensATile < now) {
+                                const v2u xs = x.load_scales(i, c + h);
+#pragma unroll
+                                for (int s = 0; s < 2; s++) {
+                                    const v8i d = x.load(i, c + h, s);
+                                    const int xb = x.scale(xs, s);
+#pragma unroll
+                                    for (int f = 0; f < 2; f++)
+                                        acc[f][i] = mfma_digits(weights[h][f].codes[s], d, acc[f][i], weights[h][f].scale(s), xb);
+                                }
+                            }
             }
 #pragma unroll
             for (int i = 0; i < TILES; i++)
 #pragma unroll
-                for (int f = 0; f < 4; f++) {
+                for (int f = 0; f < 2; f++) {
                     v4f v;
 #pragma unroll
                     for (int k = 0; k < 4; k++)
@@ -399,13 +497,14 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_gate_up_kernel(const A
             const int i = item / 8, row = item % 8 * 4, pair = offset + first + i;
             v4f h = {0.0f, 0.0f, 0.0f, 0.0f};
             if (row0 < g.hidden) {
-                v4f gate = *reinterpret_cast<const v4f *>(&part[0][i][row]), up = *reinterpret_cast<const v4f *>(&part[0][i][32 + row]);
+                const float(*const mine)[TILES * kTokensATile][36] = &part[row / 16 * kKWaves];
+                v4f gate = *reinterpret_cast<const v4f *>(&mine[0][i][row % 16]), up = *reinterpret_cast<const v4f *>(&mine[0][i][16 + row % 16]);
 #pragma unroll
-                for (int j = 1; j < kProductWaves; j++) {
-                    gate += *reinterpret_cast<const v4f *>(&part[j][i][row]);
-                    up += *reinterpret_cast<const v4f *>(&part[j][i][32 + row]);
+                for (int j = 1; j < kKWaves; j++) {
+                    gate += *reinterpret_cast<const v4f *>(&mine[j][i][row % 16]);
+                    up += *reinterpret_cast<const v4f *>(&mine[j][i][16 + row % 16]);
                 }
-                const float weight = g.plan->weight[pair];
+                const float weight = plan->weight[pair];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     if (row0 + row + k >= g.hidden)
@@ -425,48 +524,65 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_gate_up_kernel(const A
     }
 }
 
-// 16 output values of all tokens: the chunks of all chosen experts, one expert's behind the other's, are dealt out among the waves.  A wave adds
-// what an expert gives to its own sums of the tokens, and the waves' sums meet in order.
+// 16 output values of all tokens: the chunks of all chosen experts, one expert's behind the other's, are dealt out among the waves of `splits`
+// workgroups.  A wave adds what an expert gives to its own sums of the tokens, and the waves' sums meet in order.
+constexpr int kAhead = 4;    // chunks whose weights a wave has on their way
+
+__device__ __forceinline__ float down_bias(const Args &g, int t, int row)
+{
+    float b = 0.0f;
+    for (int a = 0; a < g.plan->count; a++) {
+        const Entry entry = g.plan->entry[a];
+        for (int p = entry.offset; p < entry.offset + entry.pairs; p++)
+            if (g.plan->token[p] == t)
+                b += g.plan->weight[p] * g.down_bias[(size_t)entry.expert * g.dim + row];
+    }
+    return b;
+}
+
 template <int TILES>
 __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args g)
 {
     extern __shared__ __attribute__((aligned(16))) float sums[];   // [waves, tokens, 16]
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
-    const int row0 = (int)blockIdx.x * 16;
+    const int split = (int)blockIdx.x % g.splits, row0 = (int)blockIdx.x / g.splits * 16;
+    const int count = g.plan->count, all = count * g.hidden_chunks;
     for (int i = (int)threadIdx.x; i < kProductWaves * g.tokens * 16; i += 64 * kProductWaves)
         sums[i] = 0.0f;
     __syncthreads();
     const size_t pitch = (size_t)g.hidden_chunks * kChunkCodes, spitch = (size_t)g.hidden_chunks * kChunkScales;
-    const int count = g.plan->count, all = count * g.hidden_chunks;
-    const int end = (int)((int64_t)all * (w + 1) / kProductWaves);
+    const int share = split * kProductWaves + w, shares = g.splits * kProductWaves;
+    const int end = (int)((int64_t)all * (share + 1) / shares);
     float *const mine = sums + (size_t)w * g.tokens * 16;
-    for (int u = (int)((int64_t)all * w / kProductWaves); u < end;) {
-        const int a = u / g.hidden_chunks, c0 = u - a * g.hidden_chunks, c1 = min(end - a * g.hidden_chunks, g.hidden_chunks);
-        const int e = g.plan->expert[a], offset = g.plan->offset[a], n = g.plan->offset[a + 1] - offset;
-        const size_t row = (size_t)e * g.dim + (size_t)min(row0 + r, g.dim - 1);
+    for (int u = (int)((int64_t)all * share / shares); u < end;) {
+        const int a = u / g.hidden_chunks, c0 = u - a * g.hidden_chunks, c1 = min(min(end - a * g.hidden_chunks, g.hidden_chunks), c0 + kAhead);
+        const Entry entry = g.plan->entry[a];
+        const size_t row = (size_t)entry.expert * g.dim + (size_t)min(row0 + r, g.dim - 1);
         const uint8_t *const wc = g.down.codes + row * pitch + q * 16, *const ws = g.down.scales + row * spitch;
-        for (int first = 0; first < n; first += TILES * kTokensATile) {
-            const int now = min(n - first, TILES * kTokensATile);
+        Weights weights[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+            if (c0 + j < c1)
+                weights[j].load(wc, ws, c0 + j);
+        for (int first = 0; first < entry.pairs; first += TILES * kTokensATile) {
+            const int now = min(entry.pairs - first, TILES * kTokensATile);
             Columns<TILES> h;
-            h.at(g.h_digits, g.h_scales, g.hidden_chunks * kChunk, nullptr, offset + first, now);
+            h.at(g.h_digits, g.h_scales, g.hidden_chunks * kChunk, nullptr, entry.offset + first, now);
             v4f acc[TILES];
 #pragma unroll
             for (int i = 0; i < TILES; i++)
                 acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            for (int c = c0; c < c1; c++) {
-                v4i codes[2];
-                codes[0] = *reinterpret_cast<const v4i *>(wc + (size_t)c * kChunkCodes);
-                codes[1] = *reinterpret_cast<const v4i *>(wc + (size_t)c * kChunkCodes + 64);
-                const v2u scales = *reinterpret_cast<const v2u *>(ws + (size_t)c * kChunkScales);
 #pragma unroll
-                for (int i = 0; i < TILES; i++)
-                    if (i * kTokensATile < now) {
-                        const v2u hs = h.load_scales(i, c);
+            for (int j = 0; j < kAhead; j++)
+                if (c0 + j < c1)
 #pragma unroll
-                        for (int s = 0; s < 2; s++)
-                            acc[i] = mfma_digits(codes[s], h.load(i, c, s), acc[i], (int)(scales[s] >> (8 * q)), h.scale(hs, s));
-                    }
-            }
+                    for (int i = 0; i < TILES; i++)
+                        if (i * kTokensATile < now) {
+                            const v2u hs = h.load_scales(i, c0 + j);
+#pragma unroll
+                            for (int s = 0; s < 2; s++)
+                                acc[i] = mfma_digits(weights[j].codes[s], h.load(i, c0 + j, s), acc[i], weights[j].scale(s), h.scale(hs, s));
+                        }
 #pragma unroll
             for (int i = 0; i < TILES; i++) {
                 v4f v;
@@ -475,7 +591,7 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
                     v[k] = sum_digits(acc[i][k]);
                 const int pair = i * kTokensATile + r / kDigits;
                 if (r % kDigits == 0 && r < 15 && pair < now) {
-                    v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)g.plan->token[offset + first + pair] * 16 + 4 * q);
+                    v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)g.plan->token[entry.offset + first + pair] * 16 + 4 * q);
                     *to = *to + v;
                 }
             }
@@ -491,16 +607,28 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
 #pragma unroll
         for (int j = 1; j < kProductWaves; j++)
             v += sums[(size_t)j * g.tokens * 16 + i];
-        if (g.down_bias) {
-            float b = 0.0f;
-            for (int p = 0, a = 0; a < count; a++)
-                for (; p < g.plan->offset[a + 1]; p++)
-                    if (g.plan->token[p] == t)
-                        b += g.plan->weight[p] * g.down_bias[(size_t)g.plan->expert[a] * g.dim + row];
-            v += b;
+        if (g.splits > 1) {
+            g.parts[((size_t)split * g.tokens + t) * g.dim + row] = v;
+            continue;
         }
+        if (g.down_bias)
+            v += down_bias(g, t, row);
         g.y[(size_t)t * g.dim + row] = v;
     }
+}
+
+// The parts of an output that several workgroups have made, in order.
+__global__ __launch_bounds__(256) void moe_join_kernel(const Args g)
+{
+    const int all = g.tokens * g.dim, i = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (i >= all)
+        return;
+    float v = g.parts[i];
+    for (int s = 1; s < g.splits; s++)
+        v += g.parts[(size_t)s * all + i];
+    if (g.down_bias)
+        v += down_bias(g, i / g.dim, i % g.dim);
+    g.y[i] = v;
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -532,6 +660,7 @@ size_t lay_out(Args &g, char *at)
     g.x_scales = reinterpret_cast<uint8_t *>(take(g.tokens * d / kBlock));
     g.h_digits = reinterpret_cast<uint8_t *>(take(pairs * kDigits * h));
     g.h_scales = reinterpret_cast<uint8_t *>(take(pairs * h / kBlock));
+    g.parts = reinterpret_cast<float *>(take(g.splits > 1 ? (size_t)g.splits * g.tokens * g.dim * sizeof(float) : 0));
     return used;
 }
 
@@ -552,6 +681,9 @@ Args args_of(const vtl_hip_moe *m, int tokens)
     g.renormalize = m->renormalize != 0;
     g.dim_chunks = chunks_of(m->dim);
     g.hidden_chunks = chunks_of(m->hidden);
+    // 512 workgroups for the down product, as long as a wave has four chunks
+    const int rows = (m->dim + 15) / 16, chunks = std::min(m->experts, tokens * m->top_k) * g.hidden_chunks;
+    g.splits = std::max(1, std::min(512 / rows, chunks / (4 * kProductWaves)));
     return g;
 }
 
@@ -591,21 +723,34 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     }
     lay_out(g, ws);
     const hipStream_t st = current_stream();
-    const unsigned scores = (unsigned)(g.experts * ((tokens + kScoreTokens - 1) / kScoreTokens) + (tokens * g.dim_chunks + 3) / 4);
-    hipLaunchKernelGGL(moe_scores_kernel, dim3(scores), dim3(256), 0, st, g);
+    // no more tokens a workgroup than there are: their loads would be made all the same
+    const int at_once = tokens == 1 ? 1 : tokens <= 4 ? 4 : 8;
+    const bool vec = g.dim % 4 == 0 && !((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(g.router)) & 15);
+    const unsigned scores = (unsigned)(g.experts * ((tokens + at_once - 1) / at_once) + (tokens * g.dim_chunks + 3) / 4);
+    const auto scores_vec = at_once == 1 ? moe_scores_kernel<1, true> : at_once == 4 ? moe_scores_kernel<4, true> : moe_scores_kernel<8, true>;
+    const auto scores_any = at_once == 1 ? moe_scores_kernel<1, false> : at_once == 4 ? moe_scores_kernel<4, false> : moe_scores_kernel<8, false>;
+    hipLaunchKernelGGL(vec ? scores_vec : scores_any, dim3(scores), dim3(256), 0, st, g);
     int status = check_launch("moe_scores_kernel");
     if (status != VTL_HIP_OK)
         return status;
-    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, st, g);
-    if ((status = check_launch("moe_plan_kernel")) != VTL_HIP_OK)
-        return status;
+    const bool own_plan = tokens <= kProductWaves, narrow = g.experts <= 2 * kWave;
+    if (!own_plan) {
+        hipLaunchKernelGGL(narrow ? moe_plan_kernel<2> : moe_plan_kernel<kMostExperts / kWave>, dim3(1), dim3(1024), 0, st, g);
+        if ((status = check_launch("moe_plan_kernel")) != VTL_HIP_OK)
+            return status;
+    }
     const unsigned blocks = (unsigned)std::min(g.experts, tokens * g.top) * (unsigned)(g.hidden_chunks * (kChunk / 32));
-    hipLaunchKernelGGL(tokens <= 3 ? moe_gate_up_kernel<1> : moe_gate_up_kernel<2>, dim3(blocks), dim3(64 * kProductWaves), 0, st, g);
+    const auto planned = tokens <= kTokensATile ? (narrow ? moe_gate_up_kernel<1, 2> : moe_gate_up_kernel<1, kMostExperts / kWave>)
+                                                : (narrow ? moe_gate_up_kernel<2, 2> : moe_gate_up_kernel<2, kMostExperts / kWave>);
+    hipLaunchKernelGGL((own_plan ? planned : moe_gate_up_kernel<2, 0>), dim3(blocks), dim3(64 * kProductWaves), 0, st, g);
     if ((status = check_launch("moe_gate_up_kernel")) != VTL_HIP_OK)
         return status;
-    const unsigned lds = (unsigned)(kProductWaves * tokens * 16 * sizeof(float));
-    hipLaunchKernelGGL(tokens <= 3 ? moe_down_kernel<1> : moe_down_kernel<2>, dim3((unsigned)(g.dim + 15) / 16), dim3(64 * kProductWaves), lds, st, g);
-    return check_launch("moe_down_kernel");
+    const unsigned lds = (unsigned)(kProductWaves * tokens * 16 * sizeof(float)), rows = (unsigned)(g.dim + 15) / 16;
+    hipLaunchKernelGGL(tokens <= kTokensATile ? moe_down_kernel<1> : moe_down_kernel<2>, dim3(rows * (unsigned)g.splits), dim3(64 * kProductWaves), lds, st, g);
+    if ((status = check_launch("moe_down_kernel")) != VTL_HIP_OK || g.splits == 1)
+        return status;
+    hipLaunchKernelGGL(moe_join_kernel, dim3((unsigned)(tokens * g.dim + 255) / 256), dim3(256), 0, st, g);
+    return check_launch("moe_join_kernel");
 }
 
 }  // extern "C"
