@@ -169,9 +169,13 @@ class Layer:
 
 
 def check_layer(l, x, workspace=None):
+    """Each value within what a sum of so many terms may be off by at worst; and since roundings do not all go one way, a token's values together
+    within 64 half steps of f32 (2^12 independent ones, as many as the largest layer here has behind each other)."""
     got = moe_mxfp4_hip(l.layer, dev(x), workspace).cpu()
     want, far = l.want(x)
     off = np.abs(got - want)
+    together = np.linalg.norm(off, axis=1) / np.maximum(np.linalg.norm(want, axis=1), 1e-30)
+    assert (together <= 64 * mx.U).all(), (together.max() / mx.U, int(together.argmax()))
     assert (off <= far).all(), (float(np.nanmax(off / far)), np.argwhere(~(off <= far))[:5])
     return got
 

@@ -18,28 +18,32 @@ namespace {
 
 constexpr int kMostTokens = VTL_HIP_MOE_MOST_TOKENS, kMostExperts = VTL_HIP_MOE_MOST_EXPERTS, kMostTop = VTL_HIP_MOE_MOST_TOP;
 constexpr int kDigits = 5, kTokensATile = 3;   // 15 of a tile's 16 columns
+constexpr int kOwnPlan = 8;                    // tokens up to which every workgroup makes the plan for itself
 
 // Which experts have tokens, in order, and which tokens: pairs of an expert and a token.
 struct Entry {
     int expert, offset, pairs, unused;      // the expert's first pair, and how many it has
 };
-struct Plan {
+template <int ENTRIES, int PAIRS>
+struct PlanOf {
     int count, unused[3];                   // experts that somebody chose
-    Entry entry[kMostExperts];
-    int token[kMostTokens * kMostTop];      // of a pair
-    float weight[kMostTokens * kMostTop];
+    Entry entry[ENTRIES];
+    int token[PAIRS];                       // of a pair
+    float weight[PAIRS];
 };
+using Plan = PlanOf<kMostExperts, kMostTokens * kMostTop>;
 
 struct Args {
     const float *x, *router, *router_bias, *gate_up_bias, *down_bias;
     Rows gate_up, down;
     float *y;
     int tokens, experts, top, dim, hidden, renormalize;
-    int dim_chunks, hidden_chunks;
+    int dim_chunks, hidden_chunks;          // of a row of weights
+    int dim_units, hidden_units;            // of a row of digits, which is padded to whole units
     // workspace
     float *scores;                          // [tokens, experts]
     Plan *plan;
-    uint8_t *x_digits, *x_scales;           // [tokens, 5, dim padded], [tokens, dim padded / 32]
+    uint8_t *x_digits, *x_scales;           // [tokens, 5 dim padded], [tokens, dim padded / 32]
     uint8_t *h_digits, *h_scales;           // the same of each pair's hidden values
     float *parts;                           // [splits, tokens, dim] where several workgroups share rows of the output
     int splits;
@@ -83,13 +87,21 @@ __device__ __forceinline__ unsigned digits_of(v4f v, unsigned (&d)[kDigits])
     return bad ? 255u : field - 3u;
 }
 
-__device__ __forceinline__ void store_digits(uint8_t *digits, uint8_t *scales, int cols_padded, int col, v4f v)
+// Where the digits of value k of a row lie, and how far from one digit to the next: the 16 bytes of all five that lanes side by side take lie together, for
+// a lane of the 16x16x128 product has bytes 16 q .. and 64 + 16 q .. of a step of 128 (and the scale of the q-th block).
+constexpr int kDigitStep = 16, kBlockQ = kDigits * kDigitStep, kHalfStep = 4 * kBlockQ, kStep = 2 * kHalfStep;
+__device__ __forceinline__ size_t digit_at(int k)
+{
+    return (size_t)(k / 128) * kStep + (unsigned)(k / 64 % 2 * kHalfStep + k / 16 % 4 * kBlockQ + k % 16);
+}
+
+__device__ __forceinline__ void store_digits(uint8_t *digits, uint8_t *scales, int col, v4f v)
 {
     unsigned d[kDigits];
     const unsigned byte = digits_of(v, d);
 #pragma unroll
     for (int j = 0; j < kDigits; j++)
-        *reinterpret_cast<unsigned *>(digits + (size_t)j * cols_padded + col) = d[j];
+        *reinterpret_cast<unsigned *>(digits + digit_at(col) + j * kDigitStep) = d[j];
     if (col % kBlock == 0)
         scales[col / kBlock] = (uint8_t)byte;
 }
@@ -138,11 +150,12 @@ __global__ __launch_bounds__(256) void moe_scores_kernel(const Args g)
     };
     if (b >= g.experts * groups) {
         const int c = 4 * (b - g.experts * groups) + w;
-        if (c >= g.tokens * g.dim_chunks)
+        const int chunks = 2 * g.dim_units, padded = g.dim_units * kUnit;
+        if (c >= g.tokens * chunks)
             return;
-        const int t = c / g.dim_chunks, col = c % g.dim_chunks * kChunk + 4 * lane, padded = g.dim_chunks * kChunk;
+        const int t = c / chunks, col = c % chunks * kChunk + 4 * lane;
         const v4f v = four(g.x + (size_t)t * g.dim, col);
-        store_digits(g.x_digits + (size_t)t * kDigits * padded, g.x_scales + (size_t)t * (padded / kBlock), padded, col, v);
+        store_digits(g.x_digits + (size_t)t * kDigits * padded, g.x_scales + (size_t)t * (padded / kBlock), col, v);
         return;
     }
     const int e = b % g.experts, t0 = b / g.experts * NT;
@@ -222,16 +235,18 @@ __device__ __forceinline__ unsigned order_of(float v)
     return max(b & 0x80000000u ? ~b : b | 0x80000000u, 2u);
 }
 
+template <int TOKENS, int EACH>
 struct Choice {
-    Plan plan;
-    unsigned long long by[kMostExperts];    // the tokens that chose an expert, a bit each
-    float most[kMostTokens], total[kMostTokens];
+    static constexpr int kPairs = TOKENS * kMostTop;
+    PlanOf<(kPairs < EACH * kWave ? kPairs : EACH * kWave), kPairs> plan;
+    unsigned long long by[EACH * kWave];    // the tokens that chose an expert, a bit each
+    float most[TOKENS], total[TOKENS];
 };
 
 // The plan, made in shared memory by the NW waves of a workgroup: a wave has a token's scores, EACH a lane, finds its `top` largest (the lower
 // index of two that are equal) and notes the token with these experts; then the experts that were noted are put in order.
-template <int EACH, int NW>
-__device__ __forceinline__ void make_plan(const Args &g, Choice &c)
+template <int NW, int TOKENS, int EACH>
+__device__ __forceinline__ void make_plan(const Args &g, Choice<TOKENS, EACH> &c)
 {
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
     for (int e = (int)threadIdx.x; e < EACH * kWave; e += NW * kWave)
@@ -324,8 +339,8 @@ __device__ __forceinline__ void make_plan(const Args &g, Choice &c)
 }
 
 // For the launches behind.
-template <int NW>
-__device__ __forceinline__ void publish(const Args &g, const Choice &c)
+template <int NW, typename C>
+__device__ __forceinline__ void publish(const Args &g, const C &c)
 {
     const int pairs = g.tokens * g.top;
     for (int i = (int)threadIdx.x; i < max(c.plan.count, pairs); i += NW * kWave) {
@@ -343,44 +358,54 @@ __device__ __forceinline__ void publish(const Args &g, const Choice &c)
 template <int EACH>
 __global__ __launch_bounds__(1024) void moe_plan_kernel(const Args g)
 {
-    __shared__ Choice c;
-    make_plan<EACH, 16>(g, c);
+    __shared__ Choice<kMostTokens, EACH> c;
+    make_plan<16>(g, c);
     publish<16>(g, c);
 }
 
 // ---- products -------------------------------------------------------------------------------
 
-// The digits of up to 3 TILES pairs of one expert as the matrix unit takes them: column 5 i + j of tile `tile` is digit j of pair 3 tile + i.  A lane of
-// the 16x16x128 product has bytes 16 q .. and 64 + 16 q .. of a step of 128, and the scale of block q.
+// The digits of up to 3 TILES pairs of one expert as the matrix unit takes them: column 5 i + j of tile `tile` is digit j of pair 3 tile + i.
+// Columns of no pair hold anything, which stays in their column.
 template <int TILES>
 struct Columns {
     const uint8_t *digits[TILES], *scales[TILES];
+    bool present[TILES];
     int down;                       // what this digit's scale byte is less by
-    __device__ __forceinline__ void at(const uint8_t *d, const uint8_t *s, int padded, const int *rows, int first, int count)
+    v8i d[TILES][kUnitSteps];       // a unit
+    v4i s[TILES];
+    __device__ __forceinline__ void at(const uint8_t *first_digits, const uint8_t *first_scales, int units, const int *rows, int first, int count)
     {
-        const int r = min((int)(threadIdx.x % 16), 14), q = (int)(threadIdx.x % kWave) / 16;
+        const int r = (int)(threadIdx.x % 16), q = (int)(threadIdx.x % kWave) / 16;
         down = r % kDigits * 5;
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
-            const int pair = first + min(i * kTokensATile + r / kDigits, count - 1);
-            const size_t row = rows ? (size_t)rows[pair] : (size_t)pair;
-            digits[i] = d + (row * kDigits + r % kDigits) * (size_t)padded + 16 * q;
-            scales[i] = s + row * (size_t)(padded / kBlock);
+            const int pair = i * kTokensATile + r / kDigits;
+            present[i] = r < kTokensATile * kDigits && pair < count;
+            const int at = first + min(pair, count - 1);
+            const size_t row = rows ? (size_t)rows[at] : (size_t)at;
+            digits[i] = first_digits + row * (size_t)(kDigits * kUnit) * units + (q * kBlockQ + r % kDigits * kDigitStep);
+            scales[i] = first_scales + row * (size_t)(kUnit / kBlock) * units;
         }
     }
-    __device__ __forceinline__ v8i load(int tile, int chunk, int step) const
+    // They are asked for in front of the weights of the units behind: loads arrive in order, so that waiting for them would be waiting for those.
+    __device__ __forceinline__ void load(int unit)
     {
-        const uint8_t *const p = digits[tile] + (size_t)chunk * kChunk + 128 * step;
-        const v4i lo = *reinterpret_cast<const v4i *>(p), hi = *reinterpret_cast<const v4i *>(p + 64);
-        return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+        for (int i = 0; i < TILES; i++)
+            if (present[i]) {
+                s[i] = *reinterpret_cast<const v4i *>(scales[i] + (size_t)unit * (kUnit / kBlock));
+                const uint8_t *const p = digits[i] + (size_t)unit * (kUnitSteps * kStep);
+#pragma unroll
+                for (int k = 0; k < kUnitSteps; k++) {
+                    const v4i lo = *reinterpret_cast<const v4i *>(p + k * kStep), hi = *reinterpret_cast<const v4i *>(p + k * kStep + kHalfStep);
+                    d[i][k] = v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                }
+            }
     }
-    __device__ __forceinline__ v2u load_scales(int tile, int chunk) const
+    __device__ __forceinline__ int scale(int tile, int step) const
     {
-        return *reinterpret_cast<const v2u *>(scales[tile] + (size_t)chunk * kChunkScales);
-    }
-    __device__ __forceinline__ int scale(v2u both, int step) const
-    {
-        const int byte = (int)(both[step] >> ((int)(threadIdx.x % kWave) / 16 * 8)) & 255;
+        const int byte = (int)((unsigned)s[tile][step] >> ((int)(threadIdx.x % kWave) / 16 * 8)) & 255;
         return byte == 255 ? 255 : byte - down;
     }
 };
@@ -398,92 +423,87 @@ __device__ __forceinline__ float sum_digits(float v)
     return s + v;
 }
 
-constexpr int kProductWaves = 8, kKWaves = 4;
-
-// Two 16-byte pieces of a row's chunk, and its scales.
-struct Weights {
-    v4i codes[2];
-    v2u scales;
-    __device__ __forceinline__ void load(const uint8_t *c, const uint8_t *s, int chunk)
-    {
-        codes[0] = *reinterpret_cast<const v4i *>(c + (size_t)chunk * kChunkCodes);
-        codes[1] = *reinterpret_cast<const v4i *>(c + (size_t)chunk * kChunkCodes + 64);
-        scales = *reinterpret_cast<const v2u *>(s + (size_t)chunk * kChunkScales);
-    }
-    __device__ __forceinline__ int scale(int step) const { return (int)(scales[step] >> ((int)(threadIdx.x % kWave) / 16 * 8)); }
-};
-
-// 32 hidden values of an expert's tokens: two times 16 rows of its gate and as many of its up, four waves each, which deal K out among them.
-// They go out as digits, already times their weights, so that the next product adds experts up as it adds up K.
+// 16 RW hidden values of an expert's tokens: RW times 16 rows of its gate and as many of its up, KW waves each, which deal K out among them.
+// The values go out as digits, already times their weights, so that the next product adds experts up as it adds up K.
 // EACH: every workgroup makes the plan for itself (a few tokens: less than a launch takes); 0: it is there.
-template <int TILES, int EACH>
-__global__ __launch_bounds__(64 * kProductWaves) void moe_gate_up_kernel(const Args g)
+template <int TILES, int RW, int KW, int EACH>
+__global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 {
-    __shared__ __attribute__((aligned(16))) float part[kProductWaves][TILES * kTokensATile][36];
-    const int tiles = g.hidden_chunks * (kChunk / 32), a = (int)blockIdx.x / tiles, row0 = (int)blockIdx.x % tiles * 32;
-    const Plan *plan = g.plan;
+    constexpr int NW = RW * KW, kRows = 16 * RW, kPairs = TILES * kTokensATile;
+    using S = Stream<2>;
+    static_assert(RW % 2 == 0, "whole blocks of hidden values");
+    extern __shared__ __attribute__((aligned(16))) char smem[];   // two slots a wave
+    __shared__ __attribute__((aligned(16))) float part[NW][kPairs][36];
+    const int tiles = g.hidden_units * (kUnit / kRows), a = (int)blockIdx.x / tiles, row0 = (int)blockIdx.x % tiles * kRows;
+    const Entry *entries = g.plan->entry;
+    const int *tokens = g.plan->token, *count = &g.plan->count;
+    const float *weights = g.plan->weight;
     if constexpr (EACH != 0) {
-        __shared__ Choice c;
-        make_plan<EACH, kProductWaves>(g, c);
+        __shared__ Choice<kOwnPlan, EACH> c;
+        make_plan<NW>(g, c);
         if (blockIdx.x == 0)
-            publish<kProductWaves>(g, c);
-        plan = &c.plan;
+            publish<NW>(g, c);
+        entries = c.plan.entry;
+        tokens = c.plan.token;
+        count = &c.plan.count;
+        weights = c.plan.weight;
     }
-    if (a >= plan->count)
+    if (a >= *count)
         return;
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
-    const int e = __builtin_amdgcn_readfirstlane(plan->entry[a].expert), offset = __builtin_amdgcn_readfirstlane(plan->entry[a].offset),
-              n = __builtin_amdgcn_readfirstlane(plan->entry[a].pairs);
-    const size_t pitch = (size_t)g.dim_chunks * kChunkCodes, spitch = (size_t)g.dim_chunks * kChunkScales;
-    const uint8_t *wc[2], *ws[2];
+    const int e = __builtin_amdgcn_readfirstlane(entries[a].expert), offset = __builtin_amdgcn_readfirstlane(entries[a].offset),
+              n = __builtin_amdgcn_readfirstlane(entries[a].pairs);
+    char *const ring = smem + w * (2 * S::kSlot);
+    const int begin = g.dim_units * (w % KW) / KW, end = g.dim_units * (w % KW + 1) / KW;
+    const int my_row = row0 + w / KW * 16;
+    S stream;
+    if (my_row < g.hidden) {
 #pragma unroll
-    for (int f = 0; f < 2; f++) {
-        const size_t row = ((size_t)e * 2 + f) * g.hidden + (size_t)min(row0 + w / kKWaves * 16 + r, g.hidden - 1);
-        wc[f] = g.gate_up.codes + row * pitch + q * 16;
-        ws[f] = g.gate_up.scales + row * spitch;
+        for (int f = 0; f < 2; f++)
+            stream.rows(f, g.gate_up, ((size_t)e * 2 + f) * g.hidden + my_row, min(16, g.hidden - my_row), g.dim_chunks);
     }
-    const int begin = g.dim_chunks * (w % kKWaves) / kKWaves, end = g.dim_chunks * (w % kKWaves + 1) / kKWaves;
-    for (int first = 0; first < n; first += TILES * kTokensATile) {
-        const int now = min(n - first, TILES * kTokensATile);
-        if (row0 < g.hidden) {
+    for (int first = 0; first < n; first += kPairs) {
+        const int now = min(n - first, kPairs);
+        if (my_row < g.hidden) {
+            if (begin < end)
+                stream.issue(begin, ring);
             Columns<TILES> x;
-            x.at(g.x_digits, g.x_scales, g.dim_chunks * kChunk, plan->token, offset + first, now);
+            x.at(g.x_digits, g.x_scales, g.dim_units, tokens, offset + first, now);
             v4f acc[2][TILES];
 #pragma unroll
             for (int f = 0; f < 2; f++)
 #pragma unroll
                 for (int i = 0; i < TILES; i++)
                     acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            for (int c = begin; c < end; c += 2) {
-                const bool two = c + 1 < end;
-                Weights weights[2][2];
+            for (int u = begin; u < end; u++) {
+                const char *const slot = ring + (u - begin) % 2 * S::kSlot;
+                x.load(u);
+                if (u + 1 < end) {
+                    stream.issue(u + 1, ring + (u + 1 - begin) % 2 * S::kSlot);
+                    wait_vmcnt<S::kLoads>();
+                } else {
+                    wait_vmcnt<0>();
+                }
+                const v4i scales[2] = {S::all_scales(slot, 0), S::all_scales(slot, 1)};
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (h == 0 || two)
+                for (int k = 0; k < kUnitSteps; k++) {
+                    const v4i codes[2] = {S::operand(slot, 0, k), S::operand(slot, 1, k)};
 #pragma unroll
-                        for (int f = 0; f < 2; f++)
-                            weights[h][f].load(wc[f], ws[f], c + h);
+                    for (int i = 0; i < TILES; i++)
+                        if (i * kTokensATile < now) {
+                            const int xb = x.scale(i, k);
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (h == 0 || two)
-#pragma unroll
-                        for (int i = 0; i < TILES; i++)
-                            if (i * kTokensATile < now) {
-                                const v2u xs = x.load_scales(i, c + h);
-#pragma unroll
-                                for (int s = 0; s < 2; s++) {
-                                    const v8i d = x.load(i, c + h, s);
-                                    const int xb = x.scale(xs, s);
-#pragma unroll
-                                    for (int f = 0; f < 2; f++)
-                                        acc[f][i] = mfma_digits(weights[h][f].codes[s], d, acc[f][i], weights[h][f].scale(s), xb);
-                                }
-                            }
+                            for (int f = 0; f < 2; f++)
+                                acc[f][i] = mfma_digits(codes[f], x.d[i][k], acc[f][i], scales[f][k], xb);
+                        }
+                }
+                S::done_reading();
             }
 #pragma unroll
             for (int i = 0; i < TILES; i++)
 #pragma unroll
                 for (int f = 0; f < 2; f++) {
+                    settle(acc[f][i]);
                     v4f v;
 #pragma unroll
                     for (int k = 0; k < 4; k++)
@@ -493,18 +513,18 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_gate_up_kernel(const A
                 }
         }
         __syncthreads();
-        for (int item = (int)threadIdx.x; item < now * 8; item += 64 * kProductWaves) {   // eight lanes: a pair's block of 32
-            const int i = item / 8, row = item % 8 * 4, pair = offset + first + i;
+        for (int item = (int)threadIdx.x; item < now * (kRows / 4); item += 64 * NW) {   // eight lanes: a pair's block of 32
+            const int i = item / (kRows / 4), row = item % (kRows / 4) * 4, pair = offset + first + i;
             v4f h = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (row0 < g.hidden) {
-                const float(*const mine)[TILES * kTokensATile][36] = &part[row / 16 * kKWaves];
+            if (row0 + row < g.hidden) {
+                const float(*const mine)[kPairs][36] = &part[row / 16 * KW];
                 v4f gate = *reinterpret_cast<const v4f *>(&mine[0][i][row % 16]), up = *reinterpret_cast<const v4f *>(&mine[0][i][16 + row % 16]);
 #pragma unroll
-                for (int j = 1; j < kKWaves; j++) {
+                for (int j = 1; j < KW; j++) {
                     gate += *reinterpret_cast<const v4f *>(&mine[j][i][row % 16]);
                     up += *reinterpret_cast<const v4f *>(&mine[j][i][16 + row % 16]);
                 }
-                const float weight = plan->weight[pair];
+                const float weight = weights[pair];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     if (row0 + row + k >= g.hidden)
@@ -517,16 +537,16 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_gate_up_kernel(const A
                     h[k] = gate[k] / (1.0f + expf(-gate[k])) * up[k] * weight;
                 }
             }
-            const int padded = g.hidden_chunks * kChunk;
-            store_digits(g.h_digits + (size_t)pair * kDigits * padded, g.h_scales + (size_t)pair * (padded / kBlock), padded, row0 + row, h);
+            const int padded = g.hidden_units * kUnit;
+            store_digits(g.h_digits + (size_t)pair * kDigits * padded, g.h_scales + (size_t)pair * (padded / kBlock), row0 + row, h);
         }
         __syncthreads();
     }
 }
 
-// 16 output values of all tokens: the chunks of all chosen experts, one expert's behind the other's, are dealt out among the waves of `splits`
+// 16 output values of all tokens: the units of all chosen experts, one expert's behind the other's, are dealt out among the waves of `splits`
 // workgroups.  A wave adds what an expert gives to its own sums of the tokens, and the waves' sums meet in order.
-constexpr int kAhead = 4;    // chunks whose weights a wave has on their way
+constexpr int kProductWaves = 8;
 
 __device__ __forceinline__ float down_bias(const Args &g, int t, int row)
 {
@@ -543,60 +563,88 @@ __device__ __forceinline__ float down_bias(const Args &g, int t, int row)
 template <int TILES>
 __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args g)
 {
-    extern __shared__ __attribute__((aligned(16))) float sums[];   // [waves, tokens, 16]
+    using S = Stream<1>;
+    constexpr int kSlots = 3, kPairs = TILES * kTokensATile;
+    extern __shared__ __attribute__((aligned(16))) char smem[];    // three slots a wave
+    float *const sums = reinterpret_cast<float *>(smem + kProductWaves * kSlots * S::kSlot);   // [waves, tokens, 16]
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
     const int split = (int)blockIdx.x % g.splits, row0 = (int)blockIdx.x / g.splits * 16;
-    const int count = g.plan->count, all = count * g.hidden_chunks;
+    const int units = g.hidden_units, all = g.plan->count * units;
+    const int share = split * kProductWaves + w, shares = g.splits * kProductWaves;
+    const int begin = (int)((int64_t)all * share / shares), end = (int)((int64_t)all * (share + 1) / shares);
+    char *const ring = smem + w * (kSlots * S::kSlot);
+    float *const mine = sums + (size_t)w * g.tokens * 16;
+    const auto expert_of = [&](int u) { return __builtin_amdgcn_readfirstlane(g.plan->entry[u / units].expert); };
+    const auto issue = [&](int u, int e) {
+        S stream;
+        stream.rows(0, g.down, (size_t)e * g.dim + row0, min(16, g.dim - row0), g.hidden_chunks);
+        stream.issue(u % units, ring + (u - begin) % kSlots * S::kSlot);
+    };
+    // two units on their way, and the expert of the third
+    int ahead = 0;
+    if (begin < end)
+        issue(begin, expert_of(begin));
+    if (begin + 1 < end)
+        issue(begin + 1, expert_of(begin + 1));
+    if (begin + 2 < end)
+        ahead = expert_of(begin + 2);
     for (int i = (int)threadIdx.x; i < kProductWaves * g.tokens * 16; i += 64 * kProductWaves)
         sums[i] = 0.0f;
     __syncthreads();
-    const size_t pitch = (size_t)g.hidden_chunks * kChunkCodes, spitch = (size_t)g.hidden_chunks * kChunkScales;
-    const int share = split * kProductWaves + w, shares = g.splits * kProductWaves;
-    const int end = (int)((int64_t)all * (share + 1) / shares);
-    float *const mine = sums + (size_t)w * g.tokens * 16;
-    for (int u = (int)((int64_t)all * share / shares); u < end;) {
-        const int a = u / g.hidden_chunks, c0 = u - a * g.hidden_chunks, c1 = min(min(end - a * g.hidden_chunks, g.hidden_chunks), c0 + kAhead);
+    for (int u = begin; u < end;) {
+        const int a = u / units, stop = min(end, (a + 1) * units);
         const Entry entry = g.plan->entry[a];
-        const size_t row = (size_t)entry.expert * g.dim + (size_t)min(row0 + r, g.dim - 1);
-        const uint8_t *const wc = g.down.codes + row * pitch + q * 16, *const ws = g.down.scales + row * spitch;
-        Weights weights[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; j++)
-            if (c0 + j < c1)
-                weights[j].load(wc, ws, c0 + j);
-        for (int first = 0; first < entry.pairs; first += TILES * kTokensATile) {
-            const int now = min(entry.pairs - first, TILES * kTokensATile);
+        for (; u < stop; u++) {
+            const char *const slot = ring + (u - begin) % kSlots * S::kSlot;
+            const int in_row = u % units;
             Columns<TILES> h;
-            h.at(g.h_digits, g.h_scales, g.hidden_chunks * kChunk, nullptr, entry.offset + first, now);
-            v4f acc[TILES];
+            h.at(g.h_digits, g.h_scales, units, nullptr, entry.offset, min(entry.pairs, kPairs));
+            h.load(in_row);
+            if (u + 2 < end) {
+                issue(u + 2, ahead);
+                if (u + 3 < end)
+                    ahead = expert_of(u + 3);
+                wait_vmcnt<2 * S::kLoads>();
+            } else if (u + 1 < end) {
+                wait_vmcnt<S::kLoads>();
+            } else {
+                wait_vmcnt<0>();
+            }
+            const v4i scales = S::all_scales(slot, 0);
+            for (int first = 0; first < entry.pairs; first += kPairs) {
+                const int now = min(entry.pairs - first, kPairs);
+                if (first) {
+                    h.at(g.h_digits, g.h_scales, units, nullptr, entry.offset + first, now);
+                    h.load(in_row);
+                }
+                v4f acc[TILES];
 #pragma unroll
-            for (int i = 0; i < TILES; i++)
-                acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int i = 0; i < TILES; i++)
+                    acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < kAhead; j++)
-                if (c0 + j < c1)
+                for (int k = 0; k < kUnitSteps; k++) {
+                    const v4i codes = S::operand(slot, 0, k);
 #pragma unroll
                     for (int i = 0; i < TILES; i++)
-                        if (i * kTokensATile < now) {
-                            const v2u hs = h.load_scales(i, c0 + j);
+                        if (i * kTokensATile < now)
+                            acc[i] = mfma_digits(codes, h.d[i][k], acc[i], scales[k], h.scale(i, k));
+                }
 #pragma unroll
-                            for (int s = 0; s < 2; s++)
-                                acc[i] = mfma_digits(weights[j].codes[s], h.load(i, c0 + j, s), acc[i], weights[j].scale(s), h.scale(hs, s));
-                        }
+                for (int i = 0; i < TILES; i++) {
+                    settle(acc[i]);
+                    v4f v;
 #pragma unroll
-            for (int i = 0; i < TILES; i++) {
-                v4f v;
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    v[k] = sum_digits(acc[i][k]);
-                const int pair = i * kTokensATile + r / kDigits;
-                if (r % kDigits == 0 && r < 15 && pair < now) {
-                    v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)g.plan->token[entry.offset + first + pair] * 16 + 4 * q);
-                    *to = *to + v;
+                    for (int k = 0; k < 4; k++)
+                        v[k] = sum_digits(acc[i][k]);
+                    const int pair = i * kTokensATile + r / kDigits;
+                    if (r % kDigits == 0 && r < 15 && pair < now) {
+                        v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)g.plan->token[entry.offset + first + pair] * 16 + 4 * q);
+                        *to = *to + v;
+                    }
                 }
             }
+            S::done_reading();
         }
-        u = a * g.hidden_chunks + c1;
     }
     __syncthreads();
     for (int i = (int)threadIdx.x; i < g.tokens * 16; i += 64 * kProductWaves) {
@@ -633,6 +681,26 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const Args g)
 
 // ---- host -----------------------------------------------------------------------------------
 
+// The kernels with more shared memory than a launch has unasked.
+template <void (*KERNEL)(const Args)>
+int launch_with_lds(unsigned blocks, int threads, int lds, hipStream_t st, const Args &g)
+{
+    static PerDevice<DoneFlag> flags;
+    DoneFlag &done = flags.get();
+    if (!done.load(std::memory_order_acquire)) {
+        VTL_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 136 << 10));
+        done.store(true, std::memory_order_release);
+    }
+    hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3((unsigned)threads), (unsigned)lds, st, g);
+    return check_launch("moe_mxfp4 product");
+}
+
+template <int TILES, int EACH>
+int launch_few(const Args &g, unsigned most, hipStream_t st)
+{
+    return launch_with_lds<moe_gate_up_kernel<TILES, 2, 4, EACH>>(most * (unsigned)(g.hidden_units * (kUnit / 32)), 512, 8 * 2 * Stream<2>::kSlot, st, g);
+}
+
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 int check(const vtl_hip_moe *m, int tokens)
@@ -647,7 +715,7 @@ int check(const vtl_hip_moe *m, int tokens)
 // Lays the workspace out from `at` on; the bytes it takes.
 size_t lay_out(Args &g, char *at)
 {
-    const size_t pairs = (size_t)g.tokens * g.top, d = (size_t)g.dim_chunks * kChunk, h = (size_t)g.hidden_chunks * kChunk;
+    const size_t pairs = (size_t)g.tokens * g.top, d = (size_t)g.dim_units * kUnit, h = (size_t)g.hidden_units * kUnit;
     size_t used = 0;
     auto take = [&](size_t bytes) {
         char *const p = at + used;
@@ -681,9 +749,11 @@ Args args_of(const vtl_hip_moe *m, int tokens)
     g.renormalize = m->renormalize != 0;
     g.dim_chunks = chunks_of(m->dim);
     g.hidden_chunks = chunks_of(m->hidden);
-    // 512 workgroups for the down product, as long as a wave has four chunks
-    const int rows = (m->dim + 15) / 16, chunks = std::min(m->experts, tokens * m->top_k) * g.hidden_chunks;
-    g.splits = std::max(1, std::min(512 / rows, chunks / (4 * kProductWaves)));
+    g.dim_units = (g.dim_chunks + 1) / 2;
+    g.hidden_units = (g.hidden_chunks + 1) / 2;
+    // a workgroup for each compute unit for the down product, as long as a wave has two units
+    const int rows = (m->dim + 15) / 16, units = std::min(m->experts, tokens * m->top_k) * g.hidden_units;
+    g.splits = std::max(1, std::min(256 / rows, units / (2 * kProductWaves)));
     return g;
 }
 
@@ -726,28 +796,33 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     // no more tokens a workgroup than there are: their loads would be made all the same
     const int at_once = tokens == 1 ? 1 : tokens <= 4 ? 4 : 8;
     const bool vec = g.dim % 4 == 0 && !((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(g.router)) & 15);
-    const unsigned scores = (unsigned)(g.experts * ((tokens + at_once - 1) / at_once) + (tokens * g.dim_chunks + 3) / 4);
+    const unsigned scores = (unsigned)(g.experts * ((tokens + at_once - 1) / at_once) + (tokens * 2 * g.dim_units + 3) / 4);
     const auto scores_vec = at_once == 1 ? moe_scores_kernel<1, true> : at_once == 4 ? moe_scores_kernel<4, true> : moe_scores_kernel<8, true>;
     const auto scores_any = at_once == 1 ? moe_scores_kernel<1, false> : at_once == 4 ? moe_scores_kernel<4, false> : moe_scores_kernel<8, false>;
     hipLaunchKernelGGL(vec ? scores_vec : scores_any, dim3(scores), dim3(256), 0, st, g);
     int status = check_launch("moe_scores_kernel");
     if (status != VTL_HIP_OK)
         return status;
-    const bool own_plan = tokens <= kProductWaves, narrow = g.experts <= 2 * kWave;
+    const bool own_plan = tokens <= kOwnPlan, narrow = g.experts <= 2 * kWave;
     if (!own_plan) {
         hipLaunchKernelGGL(narrow ? moe_plan_kernel<2> : moe_plan_kernel<kMostExperts / kWave>, dim3(1), dim3(1024), 0, st, g);
         if ((status = check_launch("moe_plan_kernel")) != VTL_HIP_OK)
             return status;
     }
-    const unsigned blocks = (unsigned)std::min(g.experts, tokens * g.top) * (unsigned)(g.hidden_chunks * (kChunk / 32));
-    const auto planned = tokens <= kTokensATile ? (narrow ? moe_gate_up_kernel<1, 2> : moe_gate_up_kernel<1, kMostExperts / kWave>)
-                                                : (narrow ? moe_gate_up_kernel<2, 2> : moe_gate_up_kernel<2, kMostExperts / kWave>);
-    hipLaunchKernelGGL((own_plan ? planned : moe_gate_up_kernel<2, 0>), dim3(blocks), dim3(64 * kProductWaves), 0, st, g);
-    if ((status = check_launch("moe_gate_up_kernel")) != VTL_HIP_OK)
+    const unsigned most = (unsigned)std::min(g.experts, tokens * g.top);
+    if (!own_plan)
+        status = launch_with_lds<moe_gate_up_kernel<2, 4, 1, 0>>(most * (unsigned)(g.hidden_units * (kUnit / 64)), 256, 4 * 2 * Stream<2>::kSlot, st, g);
+    else if (tokens <= kTokensATile)
+        status = narrow ? launch_few<1, 2>(g, most, st) : launch_few<1, kMostExperts / kWave>(g, most, st);
+    else
+        status = narrow ? launch_few<2, 2>(g, most, st) : launch_few<2, kMostExperts / kWave>(g, most, st);
+    if (status != VTL_HIP_OK)
         return status;
-    const unsigned lds = (unsigned)(kProductWaves * tokens * 16 * sizeof(float)), rows = (unsigned)(g.dim + 15) / 16;
-    hipLaunchKernelGGL(tokens <= kTokensATile ? moe_down_kernel<1> : moe_down_kernel<2>, dim3(rows * (unsigned)g.splits), dim3(64 * kProductWaves), lds, st, g);
-    if ((status = check_launch("moe_down_kernel")) != VTL_HIP_OK || g.splits == 1)
+    const unsigned blocks = (unsigned)(g.dim + 15) / 16 * (unsigned)g.splits;
+    const int lds = kProductWaves * (3 * Stream<1>::kSlot + tokens * 16 * (int)sizeof(float));
+    status = tokens <= kTokensATile ? launch_with_lds<moe_down_kernel<1>>(blocks, 64 * kProductWaves, lds, st, g)
+                                    : launch_with_lds<moe_down_kernel<2>>(blocks, 64 * kProductWaves, lds, st, g);
+    if (status != VTL_HIP_OK || g.splits == 1)
         return status;
     hipLaunchKernelGGL(moe_join_kernel, dim3((unsigned)(tokens * g.dim + 255) / 256), dim3(256), 0, st, g);
     return check_launch("moe_join_kernel");

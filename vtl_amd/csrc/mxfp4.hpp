@@ -55,6 +55,81 @@ __device__ __forceinline__ v4f mfma_16(v4i a, v4i b, v4f c, int sa, int sb)
     const v8i a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, sa, 0, sb);
 }
+
+// In front of anything but a product that reads a 16x16x128 product's registers, which takes 11 wait states after it.  The compiler puts them in
+// where it sees a way from one to the other, but of two ways around conditional code between them it may look at the longer only: a lane's
+// first register was read too early there.
+__device__ __forceinline__ void settle(v4f &v) { asm volatile("s_nop 15" : "+v"(v)); }
+
+#define VTL_GPTR(p) ((const __attribute__((address_space(1))) void *)(p))
+#define VTL_LPTR(p) ((__attribute__((address_space(3))) void *)(p))
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Weights that a wave reads once, for the products of few rows: FRAGS times 16 rows, a unit of 512 values at a time, straight into shared memory
+// of its own, from where they are read as the 16x16x128 product takes them.  By way of shared memory because of how memory is read: a load that gives
+// the matrix unit its operand directly has 64 bytes of each of 16 rows, this one 256 bytes of each of 4.
+constexpr int kUnit = 2 * kChunk, kUnitSteps = kUnit / 128;
+template <int FRAGS>
+struct Stream {
+    static constexpr int kCodes = 16 * kUnit / 2, kFrag = kCodes + 16 * (kUnit / kBlock), kSlot = FRAGS * kFrag;
+    static constexpr int kLoads = 5 * FRAGS;        // of a unit
+
+    // Row `row` of a fragment lies at rows of 256 bytes; 16-byte piece i of it at place i ^ row, so that a read of 16 rows meets all banks.
+    const uint8_t *codes[FRAGS], *scales[FRAGS];    // the fragment's first row
+    unsigned code_at[FRAGS][4], scale_at[FRAGS];    // the lane's rows
+    unsigned pitch, spitch;
+
+    // Fragment f has rows first[f] .. first[f] + 15 of w; rows from `most` of them on are not read (the last one is, instead).
+    __device__ __forceinline__ void rows(int f, const Rows &w, size_t first, int most, int chunks)
+    {
+        const int lane = threadIdx.x % kWave;
+        pitch = (unsigned)chunks * kChunkCodes;
+        spitch = (unsigned)chunks * kChunkScales;
+        codes[f] = w.codes + first * pitch;
+        scales[f] = w.scales + first * spitch;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            code_at[f][j] = (unsigned)min(4 * j + lane / 16, most - 1) * pitch;
+        scale_at[f] = (unsigned)min(lane / 4, most - 1) * spitch;
+    }
+    // The loads of a unit.  Where a row has only the first half of it, the rest is the row's end once more.
+    __device__ __forceinline__ void issue(int unit, char *slot) const
+    {
+        const int lane = threadIdx.x % kWave;
+#pragma unroll
+        for (int f = 0; f < FRAGS; f++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned in_row = min((unsigned)unit * (kUnit / 2) + (unsigned)((lane % 16) ^ (4 * j + lane / 16)) * 16u, pitch - 16u);
+                __builtin_amdgcn_global_load_lds(VTL_GPTR(codes[f] + (code_at[f][j] + in_row)), VTL_LPTR(slot + f * kFrag + j * 1024), 16, 0, 0);
+            }
+            const unsigned in_row = min((unsigned)unit * (kUnit / kBlock) + (unsigned)(lane % 4) * 4u, spitch - 4u);
+            __builtin_amdgcn_global_load_lds(VTL_GPTR(scales[f] + (scale_at[f] + in_row)), VTL_LPTR(slot + f * kFrag + kCodes), 4, 0, 0);
+        }
+    }
+    __device__ __forceinline__ static v4i operand(const char *slot, int f, int step)
+    {
+        const int lane = threadIdx.x % kWave, r = lane % 16, q = lane / 16;
+        return *reinterpret_cast<const v4i *>(slot + f * kFrag + r * (kUnit / 2) + (((4 * step + q) ^ r) << 4));
+    }
+    // The scale bytes of all steps: byte 0 of each.
+    __device__ __forceinline__ static v4i all_scales(const char *slot, int f)
+    {
+        const int lane = threadIdx.x % kWave, r = lane % 16, q = lane / 16;
+        v4i v = *reinterpret_cast<const v4i *>(slot + f * kFrag + kCodes + r * 16);
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+            v[s] = (int)((unsigned)v[s] >> (8 * q));
+        return v;
+    }
+    // What is read of a slot is in registers before the slot is filled again.
+    __device__ __forceinline__ static void done_reading() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+};
 #endif
 
 }  // namespace mx

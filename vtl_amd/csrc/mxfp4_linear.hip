@@ -9,9 +9,6 @@ using namespace vtlhip::mx;
 
 namespace {
 
-#define VTL_GPTR(p) ((const __attribute__((address_space(1))) void *)(p))
-#define VTL_LPTR(p) ((__attribute__((address_space(3))) void *)(p))
-
 struct Args {
     Rows a, w;            // [M, K], [N, K]
     const float *bias;
@@ -99,8 +96,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_mxfp4_kernel(const 
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int j = 0; j < MT; j++)
+        for (int j = 0; j < MT; j++) {
+            settle(acc[i][j]);
             *reinterpret_cast<v4f *>(&part[w][16 * j + r][16 * i + 4 * q]) = acc[i][j];
+        }
     __syncthreads();
     for (int item = threadIdx.x; item < 16 * MT * kFewRows; item += 64 * kFewWaves) {
         const int m = item / kFewRows, nl = item % kFewRows, n = n0 + nl;
@@ -115,12 +114,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_mxfp4_kernel(const 
 }
 
 // ---- many rows -----------------------------------------------------------------------------
-
-template <int N>
-__device__ __forceinline__ void wait_vmcnt()
-{
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
 // Workgroups are dealt round robin to the 8 XCDs; renumber them so that each XCD, which has an L2 of its own, works on a compact patch
 // of the tile grid, and walk the grid in groups of 8 tile rows.
