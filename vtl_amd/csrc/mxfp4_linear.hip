@@ -1,6 +1,7 @@
 // Linear layers on microscaled 4-bit rows (gfx950): y = x . W^T + bias with W as stored, [out_features, in_features], and x either codes
 // too or f32 rows that become codes on the way.
 #include <type_traits>
+#include <utility>
 
 #include "mxfp4.hpp"
 
@@ -20,12 +21,13 @@ struct Args {
     int relu;
 };
 
-__device__ __forceinline__ float finish(float v, float bias, bool has_bias, bool relu)
+// Bias (0: none) and ReLU: what is below `floor` becomes 0 (NaN is not).
+__device__ __forceinline__ float finish(float v, float bias, float floor)
 {
-    if (has_bias)
-        v = v + bias;
-    return relu && v < 0.0f ? 0.0f : v;
+    v = v + bias;
+    return v < floor ? 0.0f : v;
 }
+__device__ __forceinline__ float floor_of(int relu) { return relu ? 0.0f : -__builtin_inff(); }
 
 // ---- few rows ------------------------------------------------------------------------------
 
@@ -109,8 +111,36 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_mxfp4_kernel(const 
 #pragma unroll
         for (int i = 1; i < kFewWaves; i++)
             v += part[i][m][nl];
-        g.y[(int64_t)m * g.N + n] = finish(v, g.bias ? g.bias[n] : 0.0f, g.bias != nullptr, g.relu);
+        g.y[(int64_t)m * g.N + n] = finish(v, g.bias ? g.bias[n] : 0.0f, floor_of(g.relu));
     }
+}
+
+// Value c of lane i of four becomes value i of lane c.
+__device__ __forceinline__ void exchange(v4f &v)
+{
+    const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+    auto from = [](float x, auto control) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(control)::value, 0xF, 0xF, false)); };
+    float x[4];
+#pragma unroll
+    for (int c = 0; c < 4; c += 2) {       // with the neighbour
+        const float got = from(odd ? v[c] : v[c + 1], std::integral_constant<int, 0xB1>{});
+        x[c] = odd ? got : v[c];
+        x[c + 1] = odd ? v[c + 1] : got;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; c++) {          // and with the one behind it
+        const float got = from(upper ? x[c] : x[c + 2], std::integral_constant<int, 0x4E>{});
+        v[c] = upper ? got : x[c];
+        v[c + 2] = upper ? x[c + 2] : got;
+    }
+}
+
+// f(0), f(1) and so on with the numbers as constants: what the compiler leaves as a loop where it finds the body too large would keep the
+// accumulators in memory.
+template <typename F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>)
+{
+    (f(std::integral_constant<int, I>{}), ...);
 }
 
 // ---- many rows -----------------------------------------------------------------------------
@@ -135,25 +165,35 @@ __device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 
 // A workgroup has a tile of BM x BN outputs, WR x WC waves a part of it each.  A chunk of K of both operands, 128 bytes of codes and 8 of
 // scales a row, goes from memory straight into shared memory, STAGES chunks on their way; a lane of the 32x32x64 product takes a block
-// of 16 bytes and its scale byte.
-template <int BM, int BN, int WR, int WC, int STAGES>
+// of 16 bytes and its scale byte.  Operands are read one of the chunk's four steps ahead.  The barrier between two chunks comes in front of a chunk's last step, so that
+// its latency, the first reads of the next chunk and the loads into the stage that became free hide behind that step's products: a read and its
+// share of the loads behind each of them, in this order, because loads in one burst wait for each other in front of the unit that makes their addresses.
+template <int BM, int BN, int WR, int WC, int STAGES, int SPREAD, bool EDGE>
 struct Tile {
     static constexpr int kWaves = WR * WC, kThreads = 64 * kWaves;
     static constexpr int WM = BM / WR, WN = BN / WC, TM = WM / 32, TN = WN / 32;
     static constexpr int kALoads = BM / 8 / kWaves, kBLoads = BN / 8 / kWaves;        // a wave's load: 8 rows of codes
-    static constexpr int kSLoads = (BM + BN) / 32 / kWaves;                           // or the scales of 32 rows
+    // or the scales of 32 rows (8 where rows of scales may end in the middle of a load)
+    static constexpr bool kWide = !EDGE && (BM + BN) / 4 % (32 * kWaves) == 0;
+    static constexpr int kSRows = kWide ? 32 : 8, kSLoads = (BM + BN) / 4 / kSRows / kWaves;
     static constexpr int kLoads = kALoads + kBLoads + kSLoads;
-    static constexpr int kCodes = (BM + BN) * kChunkCodes, kStage = kCodes + (BM + BN) * kChunkScales;
-    static constexpr int kLds = STAGES * kStage;
+    static constexpr int kStage = (BM + BN) * kChunkCodes;
+    // Scales come for kGroup chunks at once, 32 bytes of a row (of each 8 bytes a request would be one for a line of its own, as many as
+    // for the codes: 8192 x 8192 x 8192 KKK), a quarter of the rows with the codes of each chunk; the last quarter of a group with those of its first chunk.
+    static constexpr int kGroup = 4, kGroupRow = kGroup * kChunkScales, kScales = (BM + BN) * kGroupRow;
+    static constexpr int kBuffers = STAGES >= 3 ? 3 : 2;   // of scales: the next group is being loaded up to STAGES + 3 chunks ahead
+    static constexpr int kLds = STAGES * kStage + kBuffers * kScales;
+    static constexpr int kSteps = kChunk / 64;
     static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && (BM + BN) % (32 * kWaves) == 0, "loads are dealt out evenly");
-    static_assert(STAGES >= 2 && STAGES * kLoads <= 63, "the counter of loads has 6 bits");
+    static_assert(STAGES >= 2 && STAGES <= 5 && (STAGES - 1) * kLoads <= 63, "the counter of loads has 6 bits");
 };
 
-template <int BM, int BN, int WR, int WC, int STAGES, bool EDGE>
+template <int BM, int BN, int WR, int WC, int STAGES, int SPREAD, bool EDGE>
 __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const Args g)
 {
-    using T = Tile<BM, BN, WR, WC, STAGES>;
-    constexpr int TM = T::TM, TN = T::TN, NW = T::kWaves;
+    using T = Tile<BM, BN, WR, WC, STAGES, SPREAD, EDGE>;
+    constexpr int TM = T::TM, TN = T::TN, NW = T::kWaves, kSteps = T::kSteps, kLoads = T::kLoads;
+    constexpr bool kWide = T::kWide;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int split = (int)(blockIdx.x % (unsigned)g.splits);
     int tile_m, tile_n;
@@ -163,33 +203,61 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
     const int wr = w / WC, wc = w % WC;
     const int begin = (int)((int64_t)g.chunks * split / g.splits), end = (int)((int64_t)g.chunks * (split + 1) / g.splits);
     const int count = end - begin;
-    const size_t pitch = (size_t)g.chunks * kChunkCodes, spitch = (size_t)g.chunks * kChunkScales;
+    const unsigned pitch = (unsigned)g.chunks * kChunkCodes, spitch = (unsigned)g.chunks * kChunkScales;
 
-    const int lrow = lane / 8;                            // of the 8 rows of a load
-    auto issue = [&](int chunk, int stage) {
+    // A load's address: a uniform base (operand, the tile's first row, the chunk and, without EDGE, the load's rows) and the lane's offset from it,
+    // at most 255 rows.  With EDGE rows past the last are that one, and offsets differ from load to load.
+    const int lrow = 8 * w + lane / 8;                    // of the first load's rows: + 8 NW from one to the next, which keeps the swizzle
+    const unsigned lpiece = (unsigned)((lane % 8) ^ swizzle(lrow)) * 16u;
+    static_assert(8 * NW % 16 == 0, "rows 16 apart share the swizzle");
+    const uint8_t *const a0 = g.a.codes + (size_t)m0 * pitch + (size_t)begin * kChunkCodes;
+    const uint8_t *const b0 = g.w.codes + (size_t)n0 * pitch + (size_t)begin * kChunkCodes;
+    unsigned oa[EDGE ? T::kALoads : 1], ob[EDGE ? T::kBLoads : 1];
+    if constexpr (EDGE) {
+#pragma unroll
+        for (int j = 0; j < T::kALoads; j++)
+            oa[j] = (unsigned)min(lrow + 8 * NW * j, g.M - 1 - m0) * pitch + lpiece;
+#pragma unroll
+        for (int j = 0; j < T::kBLoads; j++)
+            ob[j] = (unsigned)min(lrow + 8 * NW * j, g.N - 1 - n0) * pitch + lpiece;
+    } else {
+        oa[0] = ob[0] = (unsigned)lrow * pitch + lpiece;
+    }
+    char *const scales_at = smem + STAGES * T::kStage;
+    // Of 8 rows of the tile (32 where kWide) from `row` on (first those of x, then those of the weights), the scales of a group.
+    auto load_scales = [&](int group, int row) {
+        const bool of_a = row < BM;
+        const int first = of_a ? m0 + row : n0 + row - BM;
+        // (the group behind the last one is asked for too: it is the last one once more)
+        const int at = kWide ? min(group, g.chunks / T::kGroup - 1) * T::kGroup : begin + group * T::kGroup;
+        const uint8_t *const base = (of_a ? g.a.scales : g.w.scales) + (int64_t)first * spitch + at * kChunkScales;
+        char *const to = scales_at + group % T::kBuffers * T::kScales + row * T::kGroupRow;
+        if constexpr (kWide) {
+            __builtin_amdgcn_global_load_lds(VTL_GPTR(base + ((unsigned)(lane / 2) * spitch + (unsigned)(lane % 2 * 16))), VTL_LPTR(to), 16, 0, 0);
+        } else {
+            const int up = min(lane / 8, (of_a ? g.M : g.N) - 1 - first);       // (below 0 where all of them are past the last)
+            const int in_row = min(lane % 8 * 4, (int)spitch - 4 - at * kChunkScales);
+            __builtin_amdgcn_global_load_lds(VTL_GPTR(base + ((int64_t)up * spitch + in_row)), VTL_LPTR(to), 4, 0, 0);
+        }
+    };
+    auto load = [&](int d, int chunk, int stage) {
         char *const base = smem + stage * T::kStage;
-#pragma unroll
-        for (int j = 0; j < T::kALoads; j++) {
-            const int at = 8 * (w + NW * j), row = at + lrow;
-            const size_t from = (size_t)(EDGE ? min(m0 + row, g.M - 1) : m0 + row) * pitch + (size_t)(begin + chunk) * kChunkCodes +
-                                (unsigned)(((lane % 8) ^ swizzle(row)) * 16);
-            __builtin_amdgcn_global_load_lds(VTL_GPTR(g.a.codes + from), VTL_LPTR(base + at * kChunkCodes), 16, 0, 0);
+        if (d < T::kALoads) {
+            const uint8_t *const p = a0 + (size_t)chunk * kChunkCodes + (EDGE ? 0 : (size_t)(8 * NW * d) * pitch) + oa[EDGE ? d : 0];
+            __builtin_amdgcn_global_load_lds(VTL_GPTR(p), VTL_LPTR(base + 8 * (w + NW * d) * kChunkCodes), 16, 0, 0);
+        } else if (d < T::kALoads + T::kBLoads) {
+            const int j = d - T::kALoads;
+            const uint8_t *const p = b0 + (size_t)chunk * kChunkCodes + (EDGE ? 0 : (size_t)(8 * NW * j) * pitch) + ob[EDGE ? j : 0];
+            __builtin_amdgcn_global_load_lds(VTL_GPTR(p), VTL_LPTR(base + (BM + 8 * (w + NW * j)) * kChunkCodes), 16, 0, 0);
+        } else {
+            const int from = chunk + T::kGroup - 1, group = from / T::kGroup;
+            load_scales(group, from % T::kGroup * ((BM + BN) / T::kGroup) + T::kSRows * (w + NW * (d - T::kALoads - T::kBLoads)));
         }
+    };
+    auto issue = [&](int chunk, int stage) {
 #pragma unroll
-        for (int j = 0; j < T::kBLoads; j++) {
-            const int at = 8 * (w + NW * j), row = at + lrow;
-            const size_t from = (size_t)(EDGE ? min(n0 + row, g.N - 1) : n0 + row) * pitch + (size_t)(begin + chunk) * kChunkCodes +
-                                (unsigned)(((lane % 8) ^ swizzle(row)) * 16);
-            __builtin_amdgcn_global_load_lds(VTL_GPTR(g.w.codes + from), VTL_LPTR(base + (BM + at) * kChunkCodes), 16, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < T::kSLoads; j++) {
-            const int at = 32 * (w + NW * j), row = at + lane / 2;
-            const bool of_a = at < BM;
-            const int in = of_a ? (EDGE ? min(m0 + row, g.M - 1) : m0 + row) : (EDGE ? min(n0 + row - BM, g.N - 1) : n0 + row - BM);
-            const size_t from = (size_t)in * spitch + (size_t)(begin + chunk) * kChunkScales + (unsigned)(lane % 2 * 4);
-            __builtin_amdgcn_global_load_lds(VTL_GPTR((of_a ? g.a.scales : g.w.scales) + from), VTL_LPTR(base + T::kCodes + at * kChunkScales), 4, 0, 0);
-        }
+        for (int d = 0; d < kLoads; d++)
+            load(d, chunk, stage);
     };
 
     v16f acc[TM][TN];
@@ -203,77 +271,173 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
 
     const int r = lane % 32, half = lane / 32;
     const unsigned pick = half ? 0x07050301 : 0x06040200;   // of a row's 8 scale bytes, the four of this half's blocks
+    unsigned at[kSteps];
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; s++)
+    for (int s = 0; s < kSteps; s++)
+        at[s] = (unsigned)(r * kChunkCodes + (((2 * s + half) ^ swizzle(r)) << 4));
+    v4i fa[2][TM], fb[2][TN];
+    v2u raw[TM + TN];               // a chunk's scales as they lie in shared memory, and as the products take them: byte s for step s
+    unsigned scale[TM + TN];
+    // Read i of a step: the columns' operands first, then the rows', which the products below take in this order; then, for a chunk's first step,
+    // the scales.
+    constexpr int kReads = TM + TN;
+    auto read = [&](int i, int chunk, int stage, int s, int buffer) {
+        const char *const base = smem + stage * T::kStage;
+        const char *const scales = scales_at + chunk / T::kGroup % T::kBuffers * T::kScales + chunk % T::kGroup * kChunkScales;
+        if (i < TN)
+            fb[buffer][i] = *reinterpret_cast<const v4i *>(base + (BM + wc * T::WN + 32 * i) * kChunkCodes + at[s]);
+        else if (i < kReads)
+            fa[buffer][i - TN] = *reinterpret_cast<const v4i *>(base + (wr * T::WM + 32 * (i - TN)) * kChunkCodes + at[s]);
+        else if (i < kReads + TN)
+            raw[TM + i - kReads] = *reinterpret_cast<const v2u *>(scales + (BM + wc * T::WN + 32 * (i - kReads) + r) * T::kGroupRow);
+        else
+            raw[i - kReads - TN] = *reinterpret_cast<const v2u *>(scales + (wr * T::WM + 32 * (i - kReads - TN) + r) * T::kGroupRow);
+    };
+    // Step s of a chunk, with the reads of the step behind it and loads d0 .. d1 - 1 of chunk `chunk` between its products.
+    auto step = [&](auto s_t, auto d0_t, auto d1_t, auto last_t, int read_chunk, int read_stage, int chunk, int stage) {
+        constexpr bool kLast = decltype(last_t)::value;    // no step behind it
+        constexpr int s = decltype(s_t)::value, next = (s + 1) % kSteps, buffer = s & 1, d0 = decltype(d0_t)::value, d1 = decltype(d1_t)::value;
+        constexpr int kProducts = TM * TN, kAll = next == 0 ? 2 * kReads : kReads, kEach = (kAll + kProducts - 1) / kProducts;
+        constexpr int kShare = (d1 - d0 + kProducts - 1) / kProducts;
+        if constexpr (s == 0) {
+#pragma unroll
+            for (int i = 0; i < TM + TN; i++)
+                scale[i] = __builtin_amdgcn_perm(raw[i][1], raw[i][0], pick);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        each([&](auto p_t) {
+            constexpr int p = decltype(p_t)::value;
+            const v4i a = fa[buffer][p / TN], b = fb[buffer][p % TN];
+            acc[p / TN][p % TN] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i{a[0], a[1], a[2], a[3], 0, 0, 0, 0}, v8i{b[0], b[1], b[2], b[3], 0, 0, 0, 0},
+                                                                                 acc[p / TN][p % TN], 4, 4, s, (int)scale[p / TN], s, (int)scale[TM + p % TN]);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!kLast) {
+#pragma unroll
+                for (int i = 0; i < kEach; i++)
+                    if (p * kEach + i < kAll)
+                        read(p * kEach + i, read_chunk, read_stage, next, buffer ^ 1);
+            }
+#pragma unroll
+            for (int i = 0; i < kShare; i++)
+                if (d0 + p * kShare + i < d1)
+                    load(d0 + p * kShare + i, chunk, stage);
+            __builtin_amdgcn_sched_barrier(0);
+        }, std::make_integer_sequence<int, kProducts>{});
+    };
+
+    if (count > 0) {
+#pragma unroll
+        for (int i = 0; i < (T::kGroup - 1) * T::kSLoads; i++)     // the other quarters of the first group
+            load_scales(0, i / T::kSLoads * ((BM + BN) / T::kGroup) + T::kSRows * (w + NW * (i % T::kSLoads)));
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES; s++)
         if (s < count)
             issue(s, s);
+    if (count >= STAGES)
+        wait_vmcnt<(STAGES - 1) * kLoads>();
+    else
+        wait_vmcnt<0>();
+    __builtin_amdgcn_s_barrier();
+    if (count > 0) {
+#pragma unroll
+        for (int i = 0; i < 2 * kReads; i++)
+            read(i, 0, 0, 0, 0);
+    }
     int stage = 0;
-    for (int c = 0; c < count; c++) {
-        if (c + STAGES - 1 < count) {
-            issue(c + STAGES - 1, (c + STAGES - 1) % STAGES);
-            wait_vmcnt<(STAGES - 1) * T::kLoads>();
-        } else {
+    using Yes = std::true_type;
+    using No = std::false_type;
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+    // A chunk but the last.  The stage that it leaves takes chunk c + STAGES: the first share of its loads in this chunk's last step (MORE), the
+    // others in the first steps of the next chunk (REST).
+    auto chunk_steps = [&](auto rest_t, auto more_t, int c) {
+        constexpr bool kRest = decltype(rest_t)::value && SPREAD > 1, kMore = decltype(more_t)::value;
+        const int before = stage == 0 ? STAGES - 1 : stage - 1;
+        using First = std::integral_constant<int, kLoads / SPREAD>;
+        using Second = std::integral_constant<int, kRest ? 2 * kLoads / SPREAD : kLoads / SPREAD>;
+        using All = std::integral_constant<int, kRest ? kLoads : kLoads / SPREAD>;
+        step(I0{}, First{}, Second{}, No{}, c, stage, c - 1 + STAGES, before);
+        step(I1{}, Second{}, All{}, No{}, c, stage, c - 1 + STAGES, before);
+        step(I2{}, I0{}, I0{}, No{}, c, stage, 0, 0);
+        // every read of this chunk has been asked for: wait for them, see that the next one has arrived, and hand this one's stage over
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int next = stage + 1 == STAGES ? 0 : stage + 1;
+        if (kMore || c + STAGES - 1 < count)
+            wait_vmcnt<(STAGES - 2) * kLoads>();
+        else
             wait_vmcnt<0>();
-        }
-        __syncthreads();
-        const char *const base = smem + stage * T::kStage;
-        unsigned sa[TM], sb[TN];
-#pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const v2u v = *reinterpret_cast<const v2u *>(base + T::kCodes + (wr * T::WM + 32 * i + r) * kChunkScales);
-            sa[i] = __builtin_amdgcn_perm(v[1], v[0], pick);
-        }
-#pragma unroll
-        for (int j = 0; j < TN; j++) {
-            const v2u v = *reinterpret_cast<const v2u *>(base + T::kCodes + (BM + wc * T::WN + 32 * j + r) * kChunkScales);
-            sb[j] = __builtin_amdgcn_perm(v[1], v[0], pick);
-        }
-        auto step = [&](auto s_t) {
-            constexpr int s = decltype(s_t)::value;
-            v8i fa[TM], fb[TN];
-            const unsigned off = (unsigned)(r * kChunkCodes + (((2 * s + half) ^ swizzle(r)) << 4));
-#pragma unroll
-            for (int i = 0; i < TM; i++) {
-                const v4i v = *reinterpret_cast<const v4i *>(base + (wr * T::WM + 32 * i) * kChunkCodes + off);
-                fa[i] = v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int j = 0; j < TN; j++) {
-                const v4i v = *reinterpret_cast<const v4i *>(base + (BM + wc * T::WN + 32 * j) * kChunkCodes + off);
-                fb[j] = v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int i = 0; i < TM; i++)
-#pragma unroll
-                for (int j = 0; j < TN; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[i], fb[j], acc[i][j], 4, 4, s, (int)sa[i], s, (int)sb[j]);
-        };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
-        step(std::integral_constant<int, 2>{});
-        step(std::integral_constant<int, 3>{});
-        __syncthreads();
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        __builtin_amdgcn_s_barrier();
+        step(I3{}, I0{}, std::integral_constant<int, kMore ? kLoads / SPREAD : 0>{}, No{}, c + 1, next, c + STAGES, stage);
+        stage = next;
+    };
+    int c = 0;
+    if (STAGES < count) {
+        chunk_steps(No{}, Yes{}, 0);
+        for (c = 1; c + STAGES < count; c++)
+            chunk_steps(Yes{}, Yes{}, c);
+        chunk_steps(Yes{}, No{}, c);
+        c++;
+    }
+    for (; c < count - 1; c++)
+        chunk_steps(No{}, No{}, c);
+    if (count > 0) {
+        step(I0{}, I0{}, I0{}, No{}, c, stage, 0, 0);
+        step(I1{}, I0{}, I0{}, No{}, c, stage, 0, 0);
+        step(I2{}, I0{}, I0{}, No{}, c, stage, 0, 0);
+        step(I3{}, I0{}, I0{}, Yes{}, 0, 0, 0, 0);
     }
 
-    // register k of a lane is row 8 (k / 4) + 4 half + k % 4 of a 32 x 32 tile, column r
-    float *const out = g.splits > 1 ? g.partials + (size_t)split * g.M * g.N : g.y;
-    const bool last = g.splits == 1, has_bias = g.bias != nullptr;
+    // Register k of a lane is row 8 (k / 4) + 4 half + k % 4 of a 32 x 32 tile, column r.  Four lanes exchange theirs (lane i gets row i of four
+    // columns), so that a store is 16 bytes a lane and 8 whole lines; single values took a store unit four times as long.  An address is a uniform row
+    // and the lane's offset from it.  Results are not read again here: past the caches.
+    const bool whole = g.splits == 1;
+    float *const out = (whole ? g.y : g.partials + (size_t)split * g.M * g.N) + (size_t)(m0 + wr * T::WM) * g.N + (n0 + wc * T::WN);
+    const float floor = floor_of(whole && g.relu);
+    const int n = n0 + wc * T::WN + r;
+    float bias[TN];
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-        const int n = n0 + wc * T::WN + 32 * j + r;
-        if (EDGE && n >= g.N)
-            continue;
-        const float bias = last && has_bias ? g.bias[n] : 0.0f;
+    for (int j = 0; j < TN; j++)
+        bias[j] = whole && g.bias && (!EDGE || n + 32 * j < g.N) ? g.bias[n + 32 * j] : 0.0f;
+    const bool vectors = !EDGE || (g.N % 4 == 0 && !(reinterpret_cast<uintptr_t>(out) & 15));
+    if (vectors) {
+        const unsigned mine = (unsigned)(4 * half + r % 4) * (unsigned)g.N + (unsigned)(r & ~3);
+        const int n4 = n0 + wc * T::WN + (r & ~3);
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int row = 32 * i + 8 * k;
+                float *const to = out + (size_t)row * g.N + mine;
+                const bool in = !EDGE || m0 + wr * T::WM + row + 4 * half + r % 4 < g.M;
+#pragma unroll
+                for (int j = 0; j < TN; j++) {
+                    v4f v;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        v[c] = finish(acc[i][j][4 * k + c], bias[j], floor);
+                    exchange(v);
+                    if (in && (!EDGE || n4 + 32 * j < g.N))
+                        __builtin_nontemporal_store(v, reinterpret_cast<v4f *>(to + 32 * j));
+                }
+                asm volatile("" ::: "memory");   // all results at once would be more registers than there are
+            }
+    } else {
+        const unsigned mine = (unsigned)(4 * half) * (unsigned)g.N + (unsigned)r;
 #pragma unroll
         for (int i = 0; i < TM; i++)
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                const int m = m0 + wr * T::WM + 32 * i + 8 * (k / 4) + 4 * half + k % 4;
-                if (EDGE && m >= g.M)
-                    continue;
-                const float v = acc[i][j][k];
-                __builtin_nontemporal_store(last ? finish(v, bias, has_bias, g.relu) : v, out + (size_t)m * g.N + n);
+                const int row = 32 * i + 8 * (k / 4) + k % 4;
+                float *const to = out + (size_t)row * g.N + mine;
+                if (m0 + wr * T::WM + row + 4 * half < g.M)
+#pragma unroll
+                    for (int j = 0; j < TN; j++)
+                        if (n + 32 * j < g.N)
+                            to[32 * j] = finish(acc[i][j][k], bias[j], floor);
+                asm volatile("" ::: "memory");
             }
     }
 }
@@ -286,24 +450,28 @@ __global__ __launch_bounds__(256) void linear_join_mxfp4_kernel(const Args g)
         float v = g.partials[i];
         for (int s = 1; s < g.splits; s++)
             v += g.partials[s * all + i];
-        g.y[i] = finish(v, g.bias ? g.bias[i % (size_t)g.N] : 0.0f, g.bias != nullptr, g.relu);
+        g.y[i] = finish(v, g.bias ? g.bias[i % (size_t)g.N] : 0.0f, floor_of(g.relu));
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------
 
-template <int BM, int BN, int WR, int WC, int STAGES>
+template <int BM, int BN, int WR, int WC, int STAGES, int SPREAD>
 int launch_tile(const Args &g, hipStream_t st)
 {
-    using T = Tile<BM, BN, WR, WC, STAGES>;
+    using T = Tile<BM, BN, WR, WC, STAGES, SPREAD, true>;
+    static_assert(T::kLds <= 160 << 10, "shared memory of a compute unit");
     static PerDevice<DoneFlag> done_flags[2];
-    const bool edge = g.M % BM || g.N % BN;
-    const auto kernel = edge ? linear_tile_mxfp4_kernel<BM, BN, WR, WC, STAGES, true> : linear_tile_mxfp4_kernel<BM, BN, WR, WC, STAGES, false>;
+    const bool edge = g.M % BM || g.N % BN || g.chunks % T::kGroup || g.splits > 1 || (reinterpret_cast<uintptr_t>(g.y) & 15) ||
+                      ((reinterpret_cast<uintptr_t>(g.a.scales) | reinterpret_cast<uintptr_t>(g.w.scales)) & 15);
+    const auto kernel = edge ? linear_tile_mxfp4_kernel<BM, BN, WR, WC, STAGES, SPREAD, true> : linear_tile_mxfp4_kernel<BM, BN, WR, WC, STAGES, SPREAD, false>;
     DoneFlag &done = done_flags[edge].get();
     if (!done.load(std::memory_order_acquire)) {
         VTL_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds));
         done.store(true, std::memory_order_release);
     }
+    if (g.N > 1 << 27)      // a lane's offset from a row of results
+        return VTL_HIP_ERR_UNSUPPORTED;
     const int64_t blocks = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.splits;
     if (blocks > 0xffffff)
         return VTL_HIP_ERR_UNSUPPORTED;
@@ -334,8 +502,8 @@ int product(Args g, const Plan &p, hipStream_t st)
     }
     g.splits = p.splits;
     if (g.M > 128 && g.N > 128 && (int64_t)g.M * g.N >= (int64_t)256 * 256 * 128)
-        return launch_tile<256, 256, 2, 2, 2>(g, st);
-    return launch_tile<128, 128, 2, 2, 2>(g, st);
+        return launch_tile<256, 256, 2, 2, 2, 2>(g, st);
+    return launch_tile<128, 128, 2, 2, 2, 1>(g, st);
 }
 
 int check(const Args &g)
