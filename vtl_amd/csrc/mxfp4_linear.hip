@@ -19,6 +19,7 @@ struct Args {
     int chunks;           // of a row
     int splits;
     int relu;
+    int cached;           // results by way of the caches
 };
 
 // Bias (0: none) and ReLU: what is below `floor` becomes 0 (NaN is not).
@@ -391,8 +392,10 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
     }
 
     // Register k of a lane is row 8 (k / 4) + 4 half + k % 4 of a 32 x 32 tile, column r.  Four lanes exchange theirs (lane i gets row i of four
-    // columns), so that a store is 16 bytes a lane and 8 whole lines; single values took a store unit four times as long.  An address is a uniform row
-    // and the lane's offset from it.  Results are not read again here: past the caches.
+    // columns), so that a store is 16 bytes a lane and 8 whole lines.  An address is a uniform row and the lane's offset from it.  Results are not
+    // read again here: past the caches, but where all tiles are at work at once and store at the end (4096 x 4096 x 4096: 41.3 us, else 43.6; 8192 x 8192 x 8192
+    // 291 and 284).
+    const bool cached = g.cached;
     const bool whole = g.splits == 1;
     float *const out = (whole ? g.y : g.partials + (size_t)split * g.M * g.N) + (size_t)(m0 + wr * T::WM) * g.N + (n0 + wc * T::WN);
     const float floor = floor_of(whole && g.relu);
@@ -419,8 +422,12 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
                     for (int c = 0; c < 4; c++)
                         v[c] = finish(acc[i][j][4 * k + c], bias[j], floor);
                     exchange(v);
-                    if (in && (!EDGE || n4 + 32 * j < g.N))
-                        __builtin_nontemporal_store(v, reinterpret_cast<v4f *>(to + 32 * j));
+                    if (in && (!EDGE || n4 + 32 * j < g.N)) {
+                        if (cached)
+                            *reinterpret_cast<v4f *>(to + 32 * j) = v;
+                        else
+                            __builtin_nontemporal_store(v, reinterpret_cast<v4f *>(to + 32 * j));
+                    }
                 }
                 asm volatile("" ::: "memory");   // all results at once would be more registers than there are
             }
@@ -457,7 +464,7 @@ __global__ __launch_bounds__(256) void linear_join_mxfp4_kernel(const Args g)
 // ---- host ----------------------------------------------------------------------------------
 
 template <int BM, int BN, int WR, int WC, int STAGES, int SPREAD>
-int launch_tile(const Args &g, hipStream_t st)
+int launch_tile(Args g, hipStream_t st)
 {
     using T = Tile<BM, BN, WR, WC, STAGES, SPREAD, true>;
     static_assert(T::kLds <= 160 << 10, "shared memory of a compute unit");
@@ -475,6 +482,7 @@ int launch_tile(const Args &g, hipStream_t st)
     const int64_t blocks = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.splits;
     if (blocks > 0xffffff)
         return VTL_HIP_ERR_UNSUPPORTED;
+    g.cached = blocks <= 256;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(T::kThreads), T::kLds, st, g);
     return check_launch("linear_tile_mxfp4_kernel");
 }
