@@ -12,6 +12,7 @@ namespace {
 
 struct Args {
     Rows a, w;            // [M, K], [N, K]
+    const float *x;       // instead of a: f32 rows
     const float *bias;
     float *y;
     float *partials;      // [splits, M, N] sums of ranges of K, where there is more than one
@@ -20,6 +21,7 @@ struct Args {
     int splits;
     int relu;
     int cached;           // results by way of the caches
+    int slots;            // of a wave's shared memory
 };
 
 // Bias (0: none) and ReLU: what is below `floor` becomes 0 (NaN is not).
@@ -32,87 +34,159 @@ __device__ __forceinline__ float floor_of(int relu) { return relu ? 0.0f : -__bu
 
 // ---- few rows ------------------------------------------------------------------------------
 
-// A workgroup has 32 rows of weights and all of x; its waves deal the chunks of K out among them.  Weights go from memory straight into the
-// registers that the matrix unit takes them from (a lane has a block of 16 bytes of one row, four lanes 64 bytes side by side, two loads a chunk).
-constexpr int kFewRows = 32, kFewWaves = 8;
+// A workgroup has 16 FR rows of weights and all of x, up to 4 MX rows; its waves deal the units of K out among them, each with two slots of shared memory
+// that its own loads fill, and their sums meet in order.  The product's first operand is the weights, so a lane has four results of one row of x side by side.
+// XF32: x is f32, and each wave makes the codes of its units itself.
+constexpr int kFewWaves = 8, kFewMost = 16;
 
-template <int MT>
+template <int FR, int MX, bool XF32>
+struct Few {
+    using W = Stream<FR>;
+    static constexpr int kXBytes = 4 * MX * (kUnit / 2) + 256;                      // rows of codes, then the scales of 16
+    static constexpr int kSlot = W::kSlot + kXBytes, kLoads = W::kLoads + (XF32 ? 0 : MX + 1);
+    static constexpr int kPart = 16 * FR + 4;                                       // floats of a row of sums
+    static_assert(MX <= 4, "one product's columns");
+};
+
+// Row m of x in a slot: codes like a row of weights (piece i at place i ^ m), scales behind all of them.
+template <int MX>
+struct XRows {
+    static constexpr int kScalesAt = 4 * MX * (kUnit / 2);
+    v4f v[4 * MX][2];       // a lane's eight values of f32 rows; four lanes are a block
+
+    __device__ __forceinline__ static void issue(const Args &g, int unit, char *x, unsigned pitch, unsigned spitch)
+    {
+        const int lane = threadIdx.x % kWave;
+#pragma unroll
+        for (int j = 0; j < MX; j++) {
+            const int row = 4 * j + lane / 16;
+            const unsigned in_row = min((unsigned)unit * (kUnit / 2) + (unsigned)((lane % 16) ^ row) * 16u, pitch - 16u);
+            __builtin_amdgcn_global_load_lds(VTL_GPTR(g.a.codes + ((size_t)min(row, g.M - 1) * pitch + in_row)), VTL_LPTR(x + j * 1024), 16, 0, 0);
+        }
+        const unsigned in_row = min((unsigned)unit * (kUnit / kBlock) + (unsigned)(lane % 4) * 4u, spitch - 4u);
+        __builtin_amdgcn_global_load_lds(VTL_GPTR(g.a.scales + ((size_t)min(lane / 4, g.M - 1) * spitch + in_row)), VTL_LPTR(x + kScalesAt), 4, 0, 0);
+    }
+    template <bool VEC>
+    __device__ __forceinline__ void load(const Args &g, int unit)
+    {
+        const int col = unit * kUnit + 8 * (int)(threadIdx.x % kWave);
+#pragma unroll
+        for (int m = 0; m < 4 * MX; m++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                v[m][h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                const float *const row = g.x + (size_t)min(m, g.M - 1) * g.K;
+                if constexpr (VEC) {
+                    if (col + 4 * h < g.K)
+                        v[m][h] = *reinterpret_cast<const v4f *>(row + col + 4 * h);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (col + 4 * h + i < g.K)
+                            v[m][h][i] = row[col + 4 * h + i];
+                }
+            }
+    }
+    __device__ __forceinline__ void make_codes(char *x) const
+    {
+        const int lane = threadIdx.x % kWave;
+#pragma unroll
+        for (int m = 0; m < 4 * MX; m++) {
+            unsigned top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                top = max(top, __float_as_uint(v[m][i / 4][i % 4]) & 0x7fffffffu);
+            top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));
+            top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));
+            const unsigned byte = scale_byte(top);
+            const float s = byte == 255 ? 1.0f : scale_of(byte);
+            unsigned q = 0;
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[m][0][0], v[m][0][1], s, 0);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[m][0][2], v[m][0][3], s, 1);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[m][1][0], v[m][1][1], s, 2);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[m][1][2], v[m][1][3], s, 3);
+            *reinterpret_cast<unsigned *>(x + m * (kUnit / 2) + (((lane / 4) ^ m) << 4) + lane % 4 * 4) = byte == 255 ? 0u : q;
+            if (lane % 4 == 0)
+                x[kScalesAt + m * 16 + lane / 4] = (char)byte;
+        }
+    }
+};
+
+template <int FR, int MX, bool XF32, bool VEC>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_few_mxfp4_kernel(const Args g)
 {
-    __shared__ __attribute__((aligned(16))) float part[kFewWaves][16 * MT][kFewRows + 4];
-    const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int r = lane % 16, q = lane / 16;
-    const int n0 = blockIdx.x * kFewRows;
-    const size_t pitch = (size_t)g.chunks * kChunkCodes, spitch = (size_t)g.chunks * kChunkScales;
-    const uint8_t *wc[2], *ws[2], *xc[MT], *xs[MT];
+    using F = Few<FR, MX, XF32>;
+    using W = typename F::W;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
+    const int n0 = (int)blockIdx.x * 16 * FR;
+    const int units = (g.chunks + 1) / 2, begin = (int)((int64_t)units * w / kFewWaves), end = (int)((int64_t)units * (w + 1) / kFewWaves);
+    char *const ring = smem + w * g.slots * F::kSlot;
+    W weights;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const size_t row = (size_t)min(n0 + 16 * i + r, g.N - 1);
-        wc[i] = g.w.codes + row * pitch + q * 16;
-        ws[i] = g.w.scales + row * spitch;
-    }
+    for (int f = 0; f < FR; f++)
+        weights.rows(f, g.w, (size_t)min(n0 + 16 * f, g.N - 1), min(16, max(1, g.N - n0 - 16 * f)), g.chunks);
+    XRows<MX> rows;
+    // (f32 rows in front of the weights: what arrives first is worked on first)
+    auto issue = [&](int u) {
+        char *const slot = ring + (u - begin) % 2 * F::kSlot;
+        if constexpr (XF32)
+            rows.template load<VEC>(g, u);
+        weights.issue(u, slot);
+        if constexpr (!XF32)
+            rows.issue(g, u, slot + W::kSlot, weights.pitch, weights.spitch);
+    };
+    v4f acc[FR];
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        const size_t row = (size_t)min(16 * i + r, g.M - 1);
-        xc[i] = g.a.codes + row * pitch + q * 16;
-        xs[i] = g.a.scales + row * spitch;
-    }
-    v4f acc[2][MT];
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < MT; j++)
-            acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const int begin = (int)((int64_t)g.chunks * w / kFewWaves), end = (int)((int64_t)g.chunks * (w + 1) / kFewWaves);
-    for (int c = begin; c < end; c++) {
-        v4i wf[2][2], xq[MT][2];
-        int wb[2][2], xb[MT][2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-                wf[i][s] = *reinterpret_cast<const v4i *>(wc[i] + (size_t)c * kChunkCodes + 64 * s);
-            const v2u scales = *reinterpret_cast<const v2u *>(ws[i] + (size_t)c * kChunkScales);
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-                wb[i][s] = (int)(scales[s] >> (8 * q));
+    for (int i = 0; i < FR; i++)
+        acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (begin < end)
+        issue(begin);
+    const int m = r % (4 * MX);      // (columns of no row repeat others)
+    for (int u = begin; u < end; u++) {
+        char *const slot = ring + (u - begin) % 2 * F::kSlot, *const x = slot + W::kSlot;
+        if constexpr (XF32)
+            rows.make_codes(x);
+        if (u + 1 < end) {
+            issue(u + 1);
+            wait_vmcnt<F::kLoads>();
+        } else {
+            wait_vmcnt<0>();
         }
+        const bool two = 2 * u + 1 < g.chunks;  // the second half of the last unit may be missing
+        v4i sw[FR];
 #pragma unroll
-        for (int j = 0; j < MT; j++) {
+        for (int i = 0; i < FR; i++)
+            sw[i] = W::all_scales(slot, i);
+        const v4i sx = *reinterpret_cast<const v4i *>(x + XRows<MX>::kScalesAt + m * 16);
 #pragma unroll
-            for (int s = 0; s < 2; s++)
-                xq[j][s] = *reinterpret_cast<const v4i *>(xc[j] + (size_t)c * kChunkCodes + 64 * s);
-            const v2u scales = *reinterpret_cast<const v2u *>(xs[j] + (size_t)c * kChunkScales);
+        for (int s = 0; s < kUnitSteps; s++)
+            if (s < 2 || two) {
+                const v4i cx = *reinterpret_cast<const v4i *>(x + m * (kUnit / 2) + (((4 * s + q) ^ m) << 4));
 #pragma unroll
-            for (int s = 0; s < 2; s++)
-                xb[j][s] = (int)(scales[s] >> (8 * q));
-        }
-#pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < MT; j++)
-                    acc[i][j] = mfma_16(wf[i][s], xq[j][s], acc[i][j], wb[i][s], xb[j][s]);
+                for (int i = 0; i < FR; i++)
+                    acc[i] = mfma_16(W::operand(slot, i, s), cx, acc[i], sw[i][s], (int)((unsigned)sx[s] >> (8 * q)));
+            }
+        W::done_reading();
     }
-    // a lane has rows 4 q .. 4 q + 3 of the weights and column r
+    __syncthreads();        // every wave is done with its slots
+    float *const part = reinterpret_cast<float *>(smem);     // [waves][4 MX][kPart]
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < MT; j++) {
-            settle(acc[i][j]);
-            *reinterpret_cast<v4f *>(&part[w][16 * j + r][16 * i + 4 * q]) = acc[i][j];
-        }
+    for (int i = 0; i < FR; i++) {
+        settle(acc[i]);
+        if (r < 4 * MX)
+            *reinterpret_cast<v4f *>(part + (w * 4 * MX + r) * F::kPart + 16 * i + 4 * q) = acc[i];
+    }
     __syncthreads();
-    for (int item = threadIdx.x; item < 16 * MT * kFewRows; item += 64 * kFewWaves) {
-        const int m = item / kFewRows, nl = item % kFewRows, n = n0 + nl;
-        if (m >= g.M || n >= g.N)
+    for (int item = (int)threadIdx.x; item < 4 * MX * 16 * FR; item += 64 * kFewWaves) {
+        const int row = item / (16 * FR), nl = item % (16 * FR), n = n0 + nl;
+        if (row >= g.M || n >= g.N)
             continue;
-        float v = part[0][m][nl];
+        float v = part[row * F::kPart + nl];
 #pragma unroll
         for (int i = 1; i < kFewWaves; i++)
-            v += part[i][m][nl];
-        g.y[(int64_t)m * g.N + n] = finish(v, g.bias ? g.bias[n] : 0.0f, floor_of(g.relu));
+            v += part[(i * 4 * MX + row) * F::kPart + nl];
+        g.y[(int64_t)row * g.N + n] = finish(v, g.bias ? g.bias[n] : 0.0f, floor_of(g.relu));
     }
 }
 
@@ -487,26 +561,59 @@ int launch_tile(Args g, hipStream_t st)
     return check_launch("linear_tile_mxfp4_kernel");
 }
 
-// How a product is made: by the kernel for few rows, or by tiles, with K in so many ranges.
+template <int FR, int MX, bool XF32, bool VEC>
+int launch_few(Args g, hipStream_t st)
+{
+    using F = Few<FR, MX, XF32>;
+    constexpr int kMostLds = kFewWaves * 2 * F::kSlot;
+    static_assert(kMostLds <= 160 << 10 && kFewWaves * 4 * MX * F::kPart * 4 <= kMostLds / 2, "shared memory of a compute unit, and sums fit where operands were");
+    const auto kernel = linear_few_mxfp4_kernel<FR, MX, XF32, VEC>;
+    static PerDevice<DoneFlag> flags;
+    DoneFlag &done = flags.get();
+    if (!done.load(std::memory_order_acquire)) {
+        VTL_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds));
+        done.store(true, std::memory_order_release);
+    }
+    const int units = (g.chunks + 1) / 2;
+    g.slots = units <= kFewWaves ? 1 : 2;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((g.N + 16 * FR - 1) / (16 * FR))), dim3(64 * kFewWaves), kFewWaves * g.slots * F::kSlot, st, g);
+    return check_launch("linear_few_mxfp4_kernel");
+}
+
+template <int MX, bool XF32, bool VEC>
+int launch_few(const Args &g, hipStream_t st)
+{
+    if constexpr (MX == 1)
+        if (g.N > 16 * 256)
+            return launch_few<2, MX, XF32, VEC>(g, st);
+    return launch_few<1, MX, XF32, VEC>(g, st);
+}
+
+// How a product is made: by the kernel for few rows, which may make their codes itself, or by tiles, with K in so many ranges.
 struct Plan {
-    bool few;
+    bool few, codes;
     int splits;
     size_t partials;   // bytes
 };
 
 Plan plan_of(int M, int N, int K)
 {
-    Plan p{M <= 32, 1, 0};
+    Plan p{M <= kFewMost, M > 8, 1, 0};
     return p;
 }
 
 int product(Args g, const Plan &p, hipStream_t st)
 {
     if (p.few) {
-        const unsigned blocks = (unsigned)((g.N + kFewRows - 1) / kFewRows);
-        const auto kernel = g.M <= 16 ? linear_few_mxfp4_kernel<1> : linear_few_mxfp4_kernel<2>;
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kFewWaves), 0, st, g);
-        return check_launch("linear_few_mxfp4_kernel");
+        if (g.x) {
+            const bool vec = g.K % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.x) & 15);
+            if (g.M <= 4)
+                return vec ? launch_few<1, true, true>(g, st) : launch_few<1, true, false>(g, st);
+            return vec ? launch_few<2, true, true>(g, st) : launch_few<2, true, false>(g, st);
+        }
+        return g.M <= 4 ? launch_few<1, false, true>(g, st)
+               : g.M <= 8 ? launch_few<2, false, true>(g, st)
+                           : launch_few<4, false, true>(g, st);
     }
     g.splits = p.splits;
     if (g.M > 128 && g.N > 128 && (int64_t)g.M * g.N >= (int64_t)256 * 256 * 128)
@@ -543,13 +650,13 @@ size_t vtl_hip_linear_f32_mxfp4_workspace(int M, int N, int K)
     if (M <= 0 || N <= 0 || K <= 0 || K > kMostCols)
         return 0;
     const Plan p = plan_of(M, N, K);
-    return codes_workspace(M, K) + up256(p.partials);
+    return p.codes ? codes_workspace(M, K) + up256(p.partials) : 0;
 }
 
 int vtl_hip_linear_mxfp4_f32(const uint8_t *x, const uint8_t *x_scales, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M,
                              int N, int K, int relu, void *workspace, size_t workspace_bytes)
 {
-    Args g{{x, x_scales}, {w, w_scales}, bias, Y, nullptr, M, N, K, 0, 1, relu};
+    Args g{{x, x_scales}, {w, w_scales}, nullptr, bias, Y, nullptr, M, N, K, 0, 1, relu};
     const int rc = check(g);
     if (rc != VTL_HIP_OK || M == 0 || N == 0)
         return rc;
@@ -562,7 +669,7 @@ int vtl_hip_linear_mxfp4_f32(const uint8_t *x, const uint8_t *x_scales, const ui
 int vtl_hip_linear_f32_mxfp4(const float *X, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M, int N, int K, int relu,
                              void *workspace, size_t workspace_bytes)
 {
-    Args g{{nullptr, nullptr}, {w, w_scales}, bias, Y, nullptr, M, N, K, 0, 1, relu};
+    Args g{{nullptr, nullptr}, {w, w_scales}, X, bias, Y, nullptr, M, N, K, 0, 1, relu};
     const int rc = check(g);
     if (rc != VTL_HIP_OK || M == 0 || N == 0)
         return rc;
@@ -571,22 +678,25 @@ int vtl_hip_linear_f32_mxfp4(const float *X, const uint8_t *w, const uint8_t *w_
     g.chunks = chunks_of(K);
     const Plan p = plan_of(M, N, K);
     const hipStream_t st = current_stream();
-    const size_t need = vtl_hip_linear_f32_mxfp4_workspace(M, N, K);
-    char *ws = static_cast<char *>(workspace);
-    if (!ws) {
-        if (workspace_bytes)
+    if (p.codes) {
+        const size_t need = vtl_hip_linear_f32_mxfp4_workspace(M, N, K);
+        char *ws = static_cast<char *>(workspace);
+        if (!ws) {
+            if (workspace_bytes)
+                return VTL_HIP_ERR_INVALID_ARG;
+            ws = static_cast<char *>(library_workspace(need, 1));
+            if (!ws && need)
+                return workspace_status();
+        } else if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)) {
             return VTL_HIP_ERR_INVALID_ARG;
-        ws = static_cast<char *>(library_workspace(need, 1));
-        if (!ws && need)
-            return workspace_status();
-    } else if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)) {
-        return VTL_HIP_ERR_INVALID_ARG;
+        }
+        uint8_t *const codes = reinterpret_cast<uint8_t *>(ws), *const scales = codes + up256((size_t)M * g.chunks * kChunkCodes);
+        const int q = launch_quantize(X, K, M, K, codes, scales, st);
+        if (q != VTL_HIP_OK)
+            return q;
+        g.a = {codes, scales};
+        g.x = nullptr;
     }
-    uint8_t *const codes = reinterpret_cast<uint8_t *>(ws), *const scales = codes + up256((size_t)M * g.chunks * kChunkCodes);
-    const int q = launch_quantize(X, K, M, K, codes, scales, st);
-    if (q != VTL_HIP_OK)
-        return q;
-    g.a = {codes, scales};
     return product(g, p, st);
 }
 
