@@ -250,7 +250,7 @@ struct Tile {
     static constexpr int kALoads = BM / 8 / kWaves, kBLoads = BN / 8 / kWaves;        // a wave's load: 8 rows of codes
     // or the scales of 32 rows (8 where rows of scales may end in the middle of a load)
     static constexpr bool kWide = !EDGE && (BM + BN) / 4 % (32 * kWaves) == 0;
-    static constexpr int kSRows = kWide ? 32 : 8, kSLoads = (BM + BN) / 4 / kSRows / kWaves;
+    static constexpr int kSRows = kWide ? 32 : 8, kSAll = (BM + BN) / 4 / kSRows, kSLoads = (kSAll + kWaves - 1) / kWaves;
     static constexpr int kLoads = kALoads + kBLoads + kSLoads;
     static constexpr int kStage = (BM + BN) * kChunkCodes;
     // Scales come for kGroup chunks at once, 32 bytes of a row (of each 8 bytes a request would be one for a line of its own, as many as
@@ -259,7 +259,7 @@ struct Tile {
     static constexpr int kBuffers = STAGES >= 3 ? 3 : 2;   // of scales: the next group is being loaded up to STAGES + 3 chunks ahead
     static constexpr int kLds = STAGES * kStage + kBuffers * kScales;
     static constexpr int kSteps = kChunk / 64;
-    static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && (BM + BN) % (32 * kWaves) == 0, "loads are dealt out evenly");
+    static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && (BM + BN) % (4 * kSRows) == 0, "loads are dealt out evenly");
     static_assert(STAGES >= 2 && STAGES <= 5 && (STAGES - 1) * kLoads <= 63, "the counter of loads has 6 bits");
 };
 
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
             __builtin_amdgcn_global_load_lds(VTL_GPTR(p), VTL_LPTR(base + (BM + 8 * (w + NW * j)) * kChunkCodes), 16, 0, 0);
         } else {
             const int from = chunk + T::kGroup - 1, group = from / T::kGroup;
-            load_scales(group, from % T::kGroup * ((BM + BN) / T::kGroup) + T::kSRows * (w + NW * (d - T::kALoads - T::kBLoads)));
+            load_scales(group, from % T::kGroup * ((BM + BN) / T::kGroup) + T::kSRows * min(w + NW * (d - T::kALoads - T::kBLoads), T::kSAll - 1));
         }
     };
     auto issue = [&](int chunk, int stage) {
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
     if (count > 0) {
 #pragma unroll
         for (int i = 0; i < (T::kGroup - 1) * T::kSLoads; i++)     // the other quarters of the first group
-            load_scales(0, i / T::kSLoads * ((BM + BN) / T::kGroup) + T::kSRows * (w + NW * (i % T::kSLoads)));
+            load_scales(0, i / T::kSLoads * ((BM + BN) / T::kGroup) + T::kSRows * min(w + NW * (i % T::kSLoads), T::kSAll - 1));
     }
 #pragma unroll
     for (int s = 0; s < STAGES; s++)
@@ -592,13 +592,49 @@ int launch_few(const Args &g, hipStream_t st)
 // How a product is made: by the kernel for few rows, which may make their codes itself, or by tiles, with K in so many ranges.
 struct Plan {
     bool few, codes;
-    int splits;
+    int tile, splits;
     size_t partials;   // bytes
 };
 
+// Tiles and what they cost, by which one is chosen: microseconds for a chunk of K where a compute unit has one workgroup (and two, where it takes two), and
+// for a workgroup's beginning and end.  Measured on 17 to 1024 rows, 1024 to 14336 columns, K of 4096 and 14336; the choice was the fastest
+// or within 8 % of it there (us: 201 x 4096 x 11008 128 x 128 17.3, 64 x 64 19.0, 256 x 128 21.5; 256 x 4096 x 4096 64 x 64 9.5, 128 x 128 15;
+// 512 x 4096 x 11008 256 x 128 24.3, 128 x 128 26.2; 1024 x 4096 x 11008 256 x 256 34.8, 128 x 128 40.9; 64 x 14336 x 4096 64 x 64 with K in four
+// 12.7, in one 17).
+struct TileCost {
+    int rows, cols;
+    float one, two, ends;
+};
+constexpr TileCost kTiles[] = {{32, 64, 0.30f, 0.40f, 2.0f}, {64, 64, 0.34f, 0.50f, 2.0f}, {128, 128, 0.73f, 1.20f, 2.5f}, {256, 128, 1.2f, 0.0f, 4.0f}, {256, 256, 1.7f, 0.0f, 8.0f}};
+constexpr float kJoin = 3.0f, kJoinBytes = 2.5e-7f;     // for the launch that adds ranges up, and for a byte of their sums
+constexpr int kUnits = 256;
+
 Plan plan_of(int M, int N, int K)
 {
-    Plan p{M <= kFewMost, M > 8, 1, 0};
+    Plan p{M <= kFewMost, M > 8, 0, 1, 0};
+    if (p.few)
+        return p;
+    const int chunks = chunks_of(K);
+    float best = 0.0f;
+    for (int t = 0; t < (int)(sizeof(kTiles) / sizeof(kTiles[0])); t++) {
+        const TileCost &c = kTiles[t];
+        const int64_t tiles = (((int64_t)M + c.rows - 1) / c.rows) * (((int64_t)N + c.cols - 1) / c.cols);
+        for (int splits = 1; splits <= 8; splits += splits < 4 ? 1 : 2) {
+            if (splits > 1 && (chunks < 2 * splits || tiles * splits > 2 * kUnits))
+                break;
+            const int64_t all = tiles * splits, at_once = c.two > 0.0f && all > kUnits ? 2 * kUnits : kUnits;
+            const float chunk = at_once > kUnits ? c.two : c.one;
+            const size_t bytes = splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0;
+            const float cost = (float)((all + at_once - 1) / at_once) * ((float)((chunks + splits - 1) / splits) * chunk + c.ends) +
+                               (splits > 1 ? kJoin + kJoinBytes * (float)bytes : 0.0f);
+            if (best == 0.0f || cost < best) {
+                best = cost;
+                p.tile = t;
+                p.splits = splits;
+                p.partials = bytes;
+            }
+        }
+    }
     return p;
 }
 
@@ -611,28 +647,82 @@ int product(Args g, const Plan &p, hipStream_t st)
                 return vec ? launch_few<1, true, true>(g, st) : launch_few<1, true, false>(g, st);
             return vec ? launch_few<2, true, true>(g, st) : launch_few<2, true, false>(g, st);
         }
-        return g.M <= 4 ? launch_few<1, false, true>(g, st)
-               : g.M <= 8 ? launch_few<2, false, true>(g, st)
-                           : launch_few<4, false, true>(g, st);
+        return g.M <= 4 ? launch_few<1, false, true>(g, st) : g.M <= 8 ? launch_few<2, false, true>(g, st) : launch_few<4, false, true>(g, st);
     }
     g.splits = p.splits;
-    if (g.M > 128 && g.N > 128 && (int64_t)g.M * g.N >= (int64_t)256 * 256 * 128)
-        return launch_tile<256, 256, 2, 2, 2, 2>(g, st);
-    return launch_tile<128, 128, 2, 2, 2, 1>(g, st);
-}
-
-int check(const Args &g)
-{
-    if (g.M < 0 || g.N < 0 || g.K < 0)
-        return VTL_HIP_ERR_INVALID_ARG;
-    if (g.K > kMostCols || (int64_t)g.M * g.N > ((int64_t)1 << 40))
-        return VTL_HIP_ERR_UNSUPPORTED;
-    return VTL_HIP_OK;
+    const int rc = p.tile == 0   ? launch_tile<32, 64, 1, 2, 4, 3>(g, st)
+                   : p.tile == 1 ? launch_tile<64, 64, 2, 2, 4, 3>(g, st)
+                   : p.tile == 2 ? launch_tile<128, 128, 2, 2, 2, 1>(g, st)
+                   : p.tile == 3 ? launch_tile<256, 128, 2, 2, 2, 2>(g, st)
+                                 : launch_tile<256, 256, 2, 2, 2, 2>(g, st);
+    if (rc != VTL_HIP_OK || p.splits == 1)
+        return rc;
+    const size_t blocks = ((size_t)g.M * g.N + 255) / 256;
+    hipLaunchKernelGGL(linear_join_mxfp4_kernel, dim3((unsigned)std::min<size_t>(blocks, 8192)), dim3(256), 0, st, g);
+    return check_launch("linear_join_mxfp4_kernel");
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t codes_workspace(int M, int K) { return up256((size_t)M * chunks_of(K) * kChunkCodes) + up256((size_t)M * chunks_of(K) * kChunkScales); }
+
+// What a product needs beside its operands: codes of f32 rows, and sums of ranges of K.
+size_t workspace_of(const Plan &p, int M, int K, bool f32) { return (f32 && p.codes ? codes_workspace(M, K) : 0) + up256(p.partials); }
+
+// The caller's, or the library's own where there is none.
+int workspace_at(void *given, size_t bytes, size_t need, char *&at)
+{
+    at = static_cast<char *>(given);
+    if (!at && bytes)
+        return VTL_HIP_ERR_INVALID_ARG;
+    if (at)
+        return bytes < need || (reinterpret_cast<uintptr_t>(at) & 15) ? VTL_HIP_ERR_INVALID_ARG : VTL_HIP_OK;
+    if (need && !(at = static_cast<char *>(library_workspace(need))))
+        return workspace_status();
+    return VTL_HIP_OK;
+}
+
+int linear(Args g, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M, int N, int K, int relu, void *workspace,
+           size_t workspace_bytes, bool f32 = false)
+{
+    if (M < 0 || N < 0 || K < 0)
+        return VTL_HIP_ERR_INVALID_ARG;
+    if (K > kMostCols || (int64_t)M * chunks_of(K) > INT32_MAX || (int64_t)N * chunks_of(K) > INT32_MAX)
+        return VTL_HIP_ERR_UNSUPPORTED;
+    if (M == 0 || N == 0)
+        return VTL_HIP_OK;
+    if (!Y || (K > 0 && ((f32 ? !g.x : !g.a.codes || !g.a.scales) || !w || !w_scales)) || !rows_aligned(g.a.codes, g.a.scales) || !rows_aligned(w, w_scales))
+        return VTL_HIP_ERR_INVALID_ARG;
+    g.chunks = chunks_of(K);
+    const size_t pitch = (size_t)g.chunks * kChunkCodes, spitch = (size_t)g.chunks * kChunkScales, results = (size_t)M * N * sizeof(float);
+    if (meet(Y, results, g.x, (size_t)M * K * sizeof(float)) || meet(Y, results, g.a.codes, M * pitch) || meet(Y, results, g.a.scales, M * spitch) ||
+        meet(Y, results, w, N * pitch) || meet(Y, results, w_scales, N * spitch) || meet(Y, results, bias, (size_t)N * sizeof(float)))
+        return VTL_HIP_ERR_INVALID_ARG;
+    g.w = {w, w_scales};
+    g.bias = bias;
+    g.y = Y;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.relu = relu;
+    const Plan p = plan_of(M, N, K);
+    char *at = nullptr;
+    const int rc = workspace_at(workspace, workspace_bytes, workspace_of(p, M, K, f32), at);
+    if (rc != VTL_HIP_OK)
+        return rc;
+    const hipStream_t st = current_stream();
+    if (f32 && p.codes) {
+        uint8_t *const codes = reinterpret_cast<uint8_t *>(at), *const scales = codes + up256(M * pitch);
+        at += codes_workspace(M, K);
+        const int quantized = launch_quantize(g.x, K, M, K, codes, scales, st);
+        if (quantized != VTL_HIP_OK)
+            return quantized;
+        g.a = {codes, scales};
+        g.x = nullptr;
+    }
+    g.partials = reinterpret_cast<float *>(at);
+    return product(g, p, st);
+}
 
 }  // namespace
 
@@ -640,64 +730,28 @@ extern "C" {
 
 size_t vtl_hip_linear_mxfp4_workspace(int M, int N, int K)
 {
-    if (M <= 0 || N <= 0 || K <= 0 || K > kMostCols)
-        return 0;
-    return up256(plan_of(M, N, K).partials);
+    return M <= 0 || N <= 0 || K <= 0 || K > kMostCols ? 0 : workspace_of(plan_of(M, N, K), M, K, false);
 }
 
 size_t vtl_hip_linear_f32_mxfp4_workspace(int M, int N, int K)
 {
-    if (M <= 0 || N <= 0 || K <= 0 || K > kMostCols)
-        return 0;
-    const Plan p = plan_of(M, N, K);
-    return p.codes ? codes_workspace(M, K) + up256(p.partials) : 0;
+    return M <= 0 || N <= 0 || K <= 0 || K > kMostCols ? 0 : workspace_of(plan_of(M, N, K), M, K, true);
 }
 
 int vtl_hip_linear_mxfp4_f32(const uint8_t *x, const uint8_t *x_scales, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M,
                              int N, int K, int relu, void *workspace, size_t workspace_bytes)
 {
-    Args g{{x, x_scales}, {w, w_scales}, nullptr, bias, Y, nullptr, M, N, K, 0, 1, relu};
-    const int rc = check(g);
-    if (rc != VTL_HIP_OK || M == 0 || N == 0)
-        return rc;
-    if (!Y || (K > 0 && (!x || !x_scales || !w || !w_scales)) || !rows_aligned(x, x_scales) || !rows_aligned(w, w_scales))
-        return VTL_HIP_ERR_INVALID_ARG;
-    g.chunks = chunks_of(K);
-    return product(g, plan_of(M, N, K), current_stream());
+    Args g{};
+    g.a = {x, x_scales};
+    return linear(g, w, w_scales, bias, Y, M, N, K, relu, workspace, workspace_bytes);
 }
 
 int vtl_hip_linear_f32_mxfp4(const float *X, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M, int N, int K, int relu,
                              void *workspace, size_t workspace_bytes)
 {
-    Args g{{nullptr, nullptr}, {w, w_scales}, X, bias, Y, nullptr, M, N, K, 0, 1, relu};
-    const int rc = check(g);
-    if (rc != VTL_HIP_OK || M == 0 || N == 0)
-        return rc;
-    if (!Y || (K > 0 && (!X || !w || !w_scales)) || !rows_aligned(w, w_scales))
-        return VTL_HIP_ERR_INVALID_ARG;
-    g.chunks = chunks_of(K);
-    const Plan p = plan_of(M, N, K);
-    const hipStream_t st = current_stream();
-    if (p.codes) {
-        const size_t need = vtl_hip_linear_f32_mxfp4_workspace(M, N, K);
-        char *ws = static_cast<char *>(workspace);
-        if (!ws) {
-            if (workspace_bytes)
-                return VTL_HIP_ERR_INVALID_ARG;
-            ws = static_cast<char *>(library_workspace(need, 1));
-            if (!ws && need)
-                return workspace_status();
-        } else if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)) {
-            return VTL_HIP_ERR_INVALID_ARG;
-        }
-        uint8_t *const codes = reinterpret_cast<uint8_t *>(ws), *const scales = codes + up256((size_t)M * g.chunks * kChunkCodes);
-        const int q = launch_quantize(X, K, M, K, codes, scales, st);
-        if (q != VTL_HIP_OK)
-            return q;
-        g.a = {codes, scales};
-        g.x = nullptr;
-    }
-    return product(g, p, st);
+    Args g{};
+    g.x = X;
+    return linear(g, w, w_scales, bias, Y, M, N, K, relu, workspace, workspace_bytes, true);
 }
 
 }  // extern "C"
