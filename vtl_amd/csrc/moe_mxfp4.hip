@@ -7,6 +7,7 @@
 // 8, each an integer from -16 to 16 and therefore an e4m3 number: 25 bits, to 2^-24 of that binade.  The digits are columns of the product (three
 // tokens of five columns), each with a scale of its own, and their sums are added at the end.  A block's products are multiples of a
 // half up to 96, so its sum is exact in the unit; only sums of blocks are rounded, to f32.
+#include <cmath>
 #include <type_traits>
 
 #include "mxfp4.hpp"
@@ -55,23 +56,25 @@ __device__ __forceinline__ v4f mfma_digits(v4i w, v8i d, v4f c, int sw, int sd)
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, d, c, 4, 0, 0, sw, 0, sd);
 }
 
-// Digits of four values a lane, eight lanes a block; the byte is that of the first digit (the next ones' are 5 less each).  Blocks below
-// 2^-103 are cut off at 2^-128.
-__device__ __forceinline__ unsigned digits_of(v4f v, unsigned (&d)[kDigits])
+__device__ __forceinline__ unsigned max_bits(v4f v)
 {
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));
-    m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));
-    m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));
-    const unsigned field = max(m >> 23, 23u);
-    const bool bad = field == 255;
-    const float to_unit = __uint_as_float((bad ? 127u : 257u - field) << 23);
+    return m;
+}
+
+// Of a block whose largest magnitude has the bits `top`: the scale byte of the first digits (the next ones' are 5 less each; 255: no number), and the
+// digits of four of its values.  Blocks below 2^-103 are cut off at 2^-128.
+__device__ __forceinline__ unsigned digit_byte(unsigned top) { return top >= 0x7f800000u ? 255u : max(top >> 23, 23u) - 3u; }
+__device__ __forceinline__ void digits_of(v4f v, unsigned top, unsigned (&d)[kDigits])
+{
+    const unsigned byte = digit_byte(top);
+    const float to_unit = byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23);
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        v[i] = bad ? 0.0f : v[i] * to_unit;
+        v[i] = byte == 255u ? 0.0f : v[i] * to_unit;
 #pragma unroll
     for (int j = 0; j < kDigits; j++) {
         float n[4];
@@ -84,7 +87,6 @@ __device__ __forceinline__ unsigned digits_of(v4f v, unsigned (&d)[kDigits])
         q = __builtin_amdgcn_cvt_pk_fp8_f32(n[2], n[3], q, true);
         d[j] = (unsigned)q;
     }
-    return bad ? 255u : field - 3u;
 }
 
 // Where the digits of value k of a row lie, and how far from one digit to the next: the 16 bytes of all five that lanes side by side take lie together, for
@@ -95,15 +97,19 @@ __device__ __forceinline__ size_t digit_at(int k)
     return (size_t)(k / 128) * kStep + (unsigned)(k / 64 % 2 * kHalfStep + k / 16 % 4 * kBlockQ + k % 16);
 }
 
+// Those of four values a lane, eight lanes a block.
 __device__ __forceinline__ void store_digits(uint8_t *digits, uint8_t *scales, int col, v4f v)
 {
-    unsigned d[kDigits];
-    const unsigned byte = digits_of(v, d);
+    unsigned top = max_bits(v), d[kDigits];
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, false));
+    digits_of(v, top, d);
 #pragma unroll
     for (int j = 0; j < kDigits; j++)
         *reinterpret_cast<unsigned *>(digits + digit_at(col) + j * kDigitStep) = d[j];
     if (col % kBlock == 0)
-        scales[col / kBlock] = (uint8_t)byte;
+        scales[col / kBlock] = (uint8_t)digit_byte(top);
 }
 
 // ---- scores ---------------------------------------------------------------------------------
@@ -235,12 +241,31 @@ __device__ __forceinline__ unsigned order_of(float v)
     return max(b & 0x80000000u ? ~b : b | 0x80000000u, 2u);
 }
 
+// Added up over a wave's lanes up to each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned plus_from(unsigned v)
+{
+    return v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ unsigned wave_scan_u32(unsigned v)
+{
+    v = plus_from<0x111, 0xF>(v);   // row_shr
+    v = plus_from<0x112, 0xF>(v);
+    v = plus_from<0x114, 0xF>(v);
+    v = plus_from<0x118, 0xF>(v);
+    v = plus_from<0x142, 0xA>(v);   // lane 15 of a row into the next row
+    return plus_from<0x143, 0xC>(v);  // lane 31 into the upper half
+}
+
 template <int TOKENS, int EACH>
 struct Choice {
     static constexpr int kPairs = TOKENS * kMostTop;
     PlanOf<(kPairs < EACH * kWave ? kPairs : EACH * kWave), kPairs> plan;
     unsigned long long by[EACH * kWave];    // the tokens that chose an expert, a bit each
-    float most[TOKENS], total[TOKENS];
+    int offset[EACH * kWave];               // its first pair
+    int expert[kPairs];                     // a token's choices, and what the exponentials of their scores are
+    float part[kPairs];
+    float total[TOKENS];
 };
 
 // The plan, made in shared memory by the NW waves of a workgroup: a wave has a token's scores, EACH a lane, finds its `top` largest (the lower
@@ -254,21 +279,20 @@ __device__ __forceinline__ void make_plan(const Args &g, Choice<TOKENS, EACH> &c
     __syncthreads();
     for (int t = w; t < g.tokens; t += NW) {
         float v[EACH];
-        unsigned key[EACH], top = 0;
+        unsigned key[EACH], first = 0;
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             const int e = lane + i * kWave;
             v[i] = e < g.experts ? g.scores[(size_t)t * g.experts + e] : -__builtin_inff();
         }
-        float high = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             key[i] = lane + i * kWave < g.experts ? order_of(v[i]) : 0u;
-            top = max(top, key[i]);
+            first = max(first, key[i]);
         }
-        top = wave_max_u32(top);
+        first = wave_max_u32(first);
         // the largest score: NaN where there is nothing else, and then so is all that follows
-        high = top == 1u ? __builtin_nanf("") : __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
+        const float high = first == 1u ? __builtin_nanf("") : __uint_as_float(first & 0x80000000u ? first & 0x7fffffffu : ~first);
         float sum = 0.0f, taken = 0.0f;
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
@@ -293,47 +317,36 @@ __device__ __forceinline__ void make_plan(const Args &g, Choice<TOKENS, EACH> &c
                     if (lane == at) {
                         key[i] = 0;
                         atomicOr(&c.by[lane + i * kWave], 1ull << t);
+                        c.expert[t * kMostTop + k] = lane + i * kWave;
+                        c.part[t * kMostTop + k] = v[i];
                     }
                 }
             }
         }
-        if (lane == 0) {
-            c.most[t] = high;
+        if (lane == 0)
             c.total[t] = g.renormalize && sum == sum ? taken : sum;
-        }
     }
     __syncthreads();
     if (w == 0) {
-        int count = 0, at = 0;
+        unsigned before = 0;     // experts with tokens, and 65536 times their pairs
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-            const int e = i * kWave + lane;
-            const unsigned long long who = c.by[e], some = __ballot(who != 0);
-            const int n = __popcll(who);
-            int first = n;
-#pragma unroll
-            for (int step = 1; step < kWave; step <<= 1) {
-                const int from = __shfl_up(first, step);
-                if (lane >= step)
-                    first += from;
-            }
-            if (who)
-                c.plan.entry[count + __popcll(some & ((1ull << lane) - 1))] = Entry{e, at + first - n, n, 0};
-            count += __popcll(some);
-            at += __shfl(first, kWave - 1);
+            const int e = i * kWave + lane, n = __popcll(c.by[e]);
+            const unsigned mine = (unsigned)n << 16 | (n ? 1u : 0u), up_to = before + wave_scan_u32(mine), at = up_to - mine;
+            c.offset[e] = (int)(at >> 16);
+            if (n)
+                c.plan.entry[at & 0xffff] = Entry{e, (int)(at >> 16), n, 0};
+            before = (unsigned)__builtin_amdgcn_readlane((int)up_to, kWave - 1);
         }
         if (lane == 0)
-            c.plan.count = count;
+            c.plan.count = (int)(before & 0xffff);
     }
     __syncthreads();
-    for (int a = (int)threadIdx.x; a < c.plan.count; a += NW * kWave) {
-        const Entry entry = c.plan.entry[a];
-        unsigned long long who = c.by[entry.expert];
-        for (int i = entry.offset; who; who &= who - 1, i++) {
-            const int t = __ffsll(who) - 1;
-            c.plan.token[i] = t;
-            c.plan.weight[i] = expf(g.scores[(size_t)t * g.experts + entry.expert] - c.most[t]) / c.total[t];
-        }
+    for (int i = (int)threadIdx.x; i < g.tokens * g.top; i += NW * kWave) {
+        const int t = i / g.top, from = t * kMostTop + i % g.top, e = c.expert[from];
+        const int pair = c.offset[e] + __popcll(c.by[e] & ((1ull << t) - 1));
+        c.plan.token[pair] = t;
+        c.plan.weight[pair] = c.part[from] / c.total[t];
     }
     __syncthreads();
 }
@@ -423,6 +436,211 @@ __device__ __forceinline__ float sum_digits(float v)
     return s + v;
 }
 
+// SiLU(gate) * up * weight.  The exponential is the vector unit's of a rounded exponent, off by |gate| half steps and one, which is |gate| steps of a value that is
+// as much smaller; the reciprocal is its own, corrected once.  (By the library's functions, a wave's 32 values of a token took longer than their weights.)
+__device__ __forceinline__ float hidden_value(float gate, float up, float weight)
+{
+    const float e = __builtin_amdgcn_exp2f(fminf(gate * -1.44269504f, 125.5f));    // (whose sum with 1 has a reciprocal)
+    const float d = 1.0f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(r, fmaf(-d, r, 1.0f), r);
+    return gate * r * up * weight;
+}
+
+// Up to this many experts' pairs have tokens in a workgroup's copy of the plan: all of them.
+struct Held {
+    Plan plan;
+    __device__ __forceinline__ void copy(const Args &g)
+    {
+        const int count = g.plan->count, pairs = g.tokens * g.top, threads = (int)blockDim.x;
+        if (threadIdx.x == 0)
+            plan.count = count;
+        for (int i = (int)threadIdx.x; i < count; i += threads)
+            plan.entry[i] = g.plan->entry[i];
+        for (int i = (int)threadIdx.x; i < pairs; i += threads) {
+            plan.token[i] = g.plan->token[i];
+            plan.weight[i] = g.plan->weight[i];
+        }
+        __syncthreads();
+    }
+};
+
+// Hidden values of all chosen experts, where there are enough of them for all compute units.  A job is 32 of an expert's, the rows of its gate and of its up in two
+// halves of 16, and a wave's own from the first load to the digits that go out: eight waves a compute unit have jobs behind each other, the next unit's weights on their
+// way while one is worked on, and meet nowhere.  (Workgroups with rounds of their own, one for 64 values of an expert, took 52 us for 24 tokens
+// of 128 experts of 2048 x 1024, 32 of them without a weight read; four waves with 32 rows at once 63, a compute unit's waves then wait one by one.)
+constexpr int kJobWaves = 8;
+
+template <int TILES>
+__global__ __launch_bounds__(64 * kJobWaves) void moe_gate_up_jobs_kernel(const Args g)
+{
+    using S = Stream<2>;
+    constexpr int kPairs = TILES * kTokensATile;
+    extern __shared__ __attribute__((aligned(16))) char smem[];   // two slots a wave
+    __shared__ Held held;
+    held.copy(g);
+    const Plan &plan = held.plan;
+    const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
+    const int tiles = (g.hidden + 31) / 32, all = __builtin_amdgcn_readfirstlane(plan.count) * tiles, units = g.dim_units;
+    const int share = (int)blockIdx.x * kJobWaves + w, shares = (int)gridDim.x * kJobWaves;
+    const int begin = (int)((int64_t)all * share / shares), end = (int)((int64_t)all * (share + 1) / shares);
+    if (begin == end)
+        return;
+    char *const ring = smem + w * (2 * S::kSlot);
+    struct At {
+        int job, expert, offset, pairs, first, half, unit;
+    };
+    const auto start = [&](At &at, int job) {
+        const Entry entry = plan.entry[min(job, all - 1) / tiles];
+        at.job = job;
+        at.expert = __builtin_amdgcn_readfirstlane(entry.expert);
+        at.offset = __builtin_amdgcn_readfirstlane(entry.offset);
+        at.pairs = __builtin_amdgcn_readfirstlane(entry.pairs);
+        at.first = at.half = at.unit = 0;
+    };
+    S stream;
+    const auto rows = [&](const At &at) {
+        const int row = min(at.job % tiles * 32 + at.half * 16, g.hidden - 1);
+#pragma unroll
+        for (int f = 0; f < 2; f++)
+            stream.rows(f, g.gate_up, ((size_t)at.expert * 2 + f) * g.hidden + row, min(16, g.hidden - row), g.dim_chunks);
+    };
+    // the position behind one; false: there is none
+    const auto advance = [&](At &at) __attribute__((always_inline)) {
+        if (++at.unit < units)
+            return true;
+        at.unit = 0;
+        at.half ^= 1;
+        if (at.half == 0) {
+            at.first += kPairs;
+            if (at.first >= at.pairs) {
+                if (at.job + 1 >= end)
+                    return false;
+                start(at, at.job + 1);
+            }
+        }
+        return true;
+    };
+    Columns<TILES> x[2];
+    v4f acc[2][TILES], first_half[TILES];
+    int streamed = -1;          // whose rows `stream` has
+    // A unit's digits, and behind them its weights: loads arrive in order, and the digits are waited for together with the unit's weights in front of them.
+    const auto ask = [&](const At &at, Columns<TILES> &to, char *slot) __attribute__((always_inline)) {
+        to.at(g.x_digits, g.x_scales, units, plan.token, at.offset + at.first, min(at.pairs - at.first, kPairs));
+        to.load(at.unit);
+        if (streamed != at.job * 2 + at.half) {
+            rows(at);
+            streamed = at.job * 2 + at.half;
+        }
+        stream.issue(at.unit, slot);
+    };
+    const auto work = [&](const At &now, const Columns<TILES> &x, const char *slot) __attribute__((always_inline)) {
+        if (now.unit == 0)
+#pragma unroll
+            for (int f = 0; f < 2; f++)
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+                    acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        const int here = min(now.pairs - now.first, kPairs);
+        const v4i scales[2] = {S::all_scales(slot, 0), S::all_scales(slot, 1)};
+#pragma unroll
+        for (int k = 0; k < kUnitSteps; k++) {
+            const v4i codes[2] = {S::operand(slot, 0, k), S::operand(slot, 1, k)};
+#pragma unroll
+            for (int i = 0; i < TILES; i++)
+                if (i * kTokensATile < here) {
+                    const int xb = x.scale(i, k);
+#pragma unroll
+                    for (int f = 0; f < 2; f++)
+                        acc[f][i] = mfma_digits(codes[f], x.d[i][k], acc[f][i], scales[f][k], xb);
+                }
+        }
+        S::done_reading();
+        if (now.unit != units - 1)
+            return;
+        const int row0 = now.job % tiles * 32, padded = g.hidden_units * kUnit;
+#pragma unroll
+        for (int i = 0; i < TILES; i++)
+            if (i * kTokensATile < here) {
+                settle(acc[0][i]);
+                settle(acc[1][i]);
+                const int pair = min(i * kTokensATile + r / kDigits, here - 1), at = now.offset + now.first + pair;
+                const float weight = plan.weight[at];
+                v4f h;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    float gate = sum_digits(acc[0][i][k]), up = sum_digits(acc[1][i][k]);
+                    const int row = row0 + 16 * now.half + 4 * q + k;
+                    h[k] = 0.0f;
+                    if (row < g.hidden) {
+                        if (g.gate_up_bias) {
+                            const float *const bias = g.gate_up_bias + (size_t)now.expert * 2 * g.hidden + row;
+                            gate += bias[0];
+                            up += bias[g.hidden];
+                        }
+                        h[k] = hidden_value(gate, up, weight);
+                    }
+                }
+                if (now.half == 0) {
+                    first_half[i] = h;
+                    continue;
+                }
+                // the four lanes q of a column have its block of 32
+                unsigned top = max(max_bits(first_half[i]), max_bits(h));
+                top = max(top, (unsigned)__shfl_xor((int)top, 16));
+                top = max(top, (unsigned)__shfl_xor((int)top, 32));
+                if (r % kDigits == 0 && x.present[i]) {
+                    uint8_t *const digits = g.h_digits + (size_t)at * kDigits * padded, *const bytes = g.h_scales + (size_t)at * (padded / kBlock);
+#pragma unroll
+                    for (int f = 0; f < 2; f++) {
+                        unsigned d[kDigits];
+                        digits_of(f ? h : first_half[i], top, d);
+#pragma unroll
+                        for (int j = 0; j < kDigits; j++)
+                            *reinterpret_cast<unsigned *>(digits + digit_at(row0 + 16 * f + 4 * q) + j * kDigitStep) = d[j];
+                    }
+                    if (q == 0)
+                        bytes[row0 / kBlock] = (uint8_t)digit_byte(top);
+                    if (row0 + 32 >= g.hidden)      // behind the last value
+                        for (int col = row0 + 32 + 4 * q; col < padded; col += 16) {
+#pragma unroll
+                            for (int j = 0; j < kDigits; j++)
+                                *reinterpret_cast<unsigned *>(digits + digit_at(col) + j * kDigitStep) = 0u;
+                            if (col % kBlock == 0)
+                                bytes[col / kBlock] = (uint8_t)digit_byte(0);
+                        }
+                }
+            }
+    };
+    char *const slots[2] = {ring, ring + S::kSlot};
+    At at[2];
+    start(at[0], begin);
+    ask(at[0], x[0], slots[0]);
+    at[1] = at[0];
+    if (!advance(at[1])) {
+        wait_vmcnt<0>();
+        work(at[0], x[0], slots[0]);
+        return;
+    }
+    ask(at[1], x[1], slots[1]);
+    // Two units on their way at the top of a round, on every way there: the compiler waits for digits as for the way with the fewest loads behind them.
+    const auto round = [&](auto i_t) __attribute__((always_inline)) {
+        constexpr int i = decltype(i_t)::value, o = i ^ 1;
+        wait_vmcnt<S::kLoads>();
+        work(at[i], x[i], slots[i]);
+        at[i] = at[o];
+        if (!advance(at[i])) {
+            wait_vmcnt<0>();
+            work(at[o], x[o], slots[o]);
+            return false;
+        }
+        ask(at[i], x[i], slots[i]);
+        return true;
+    };
+    while (round(std::integral_constant<int, 0>{}) && round(std::integral_constant<int, 1>{}))
+        ;
+}
+
 // 16 RW hidden values of an expert's tokens: RW times 16 rows of its gate and as many of its up, KW waves each, which deal K out among them.
 // The values go out as digits, already times their weights, so that the next product adds experts up as it adds up K.
 // EACH: every workgroup makes the plan for itself (a few tokens: less than a launch takes); 0: it is there.
@@ -475,15 +693,7 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 #pragma unroll
                 for (int i = 0; i < TILES; i++)
                     acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            for (int u = begin; u < end; u++) {
-                const char *const slot = ring + (u - begin) % 2 * S::kSlot;
-                x.load(u);
-                if (u + 1 < end) {
-                    stream.issue(u + 1, ring + (u + 1 - begin) % 2 * S::kSlot);
-                    wait_vmcnt<S::kLoads>();
-                } else {
-                    wait_vmcnt<0>();
-                }
+            const auto work = [&](const char *slot) {
                 const v4i scales[2] = {S::all_scales(slot, 0), S::all_scales(slot, 1)};
 #pragma unroll
                 for (int k = 0; k < kUnitSteps; k++) {
@@ -498,6 +708,18 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
                         }
                 }
                 S::done_reading();
+            };
+            // (the last unit by itself: the compiler waits for digits as for the way with the fewest loads behind them)
+            for (int u = begin; u < end - 1; u++) {
+                x.load(u);
+                stream.issue(u + 1, ring + (u + 1 - begin) % 2 * S::kSlot);
+                wait_vmcnt<S::kLoads>();
+                work(ring + (u - begin) % 2 * S::kSlot);
+            }
+            if (begin < end) {
+                x.load(end - 1);
+                wait_vmcnt<0>();
+                work(ring + (end - 1 - begin) % 2 * S::kSlot);
             }
 #pragma unroll
             for (int i = 0; i < TILES; i++)
@@ -534,7 +756,7 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
                         gate[k] += bias[0];
                         up[k] += bias[g.hidden];
                     }
-                    h[k] = gate[k] / (1.0f + expf(-gate[k])) * up[k] * weight;
+                    h[k] = hidden_value(gate[k], up[k], weight);
                 }
             }
             const int padded = g.hidden_units * kUnit;
@@ -548,14 +770,14 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 // workgroups.  A wave adds what an expert gives to its own sums of the tokens, and the waves' sums meet in order.
 constexpr int kProductWaves = 8;
 
-__device__ __forceinline__ float down_bias(const Args &g, int t, int row)
+__device__ __forceinline__ float down_bias(const Args &g, const Plan &plan, int t, int row)
 {
     float b = 0.0f;
-    for (int a = 0; a < g.plan->count; a++) {
-        const Entry entry = g.plan->entry[a];
+    for (int a = 0; a < plan.count; a++) {
+        const Entry entry = plan.entry[a];
         for (int p = entry.offset; p < entry.offset + entry.pairs; p++)
-            if (g.plan->token[p] == t)
-                b += g.plan->weight[p] * g.down_bias[(size_t)entry.expert * g.dim + row];
+            if (plan.token[p] == t)
+                b += plan.weight[p] * g.down_bias[(size_t)entry.expert * g.dim + row];
     }
     return b;
 }
@@ -568,83 +790,97 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
     extern __shared__ __attribute__((aligned(16))) char smem[];    // three slots a wave
     float *const sums = reinterpret_cast<float *>(smem + kProductWaves * kSlots * S::kSlot);   // [waves, tokens, 16]
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
+    __shared__ Held held;
+    held.copy(g);
+    const Plan &plan = held.plan;
     const int split = (int)blockIdx.x % g.splits, row0 = (int)blockIdx.x / g.splits * 16;
-    const int units = g.hidden_units, all = g.plan->count * units;
+    const int units = g.hidden_units, all = __builtin_amdgcn_readfirstlane(plan.count) * units;
     const int share = split * kProductWaves + w, shares = g.splits * kProductWaves;
     const int begin = (int)((int64_t)all * share / shares), end = (int)((int64_t)all * (share + 1) / shares);
     char *const ring = smem + w * (kSlots * S::kSlot);
     float *const mine = sums + (size_t)w * g.tokens * 16;
-    const auto expert_of = [&](int u) { return __builtin_amdgcn_readfirstlane(g.plan->entry[u / units].expert); };
-    const auto issue = [&](int u, int e) {
-        S stream;
-        stream.rows(0, g.down, (size_t)e * g.dim + row0, min(16, g.dim - row0), g.hidden_chunks);
-        stream.issue(u % units, ring + (u - begin) % kSlots * S::kSlot);
+    S stream;
+    int streamed = -1;      // whose rows it has
+    const auto issue = [&](int u) {
+        const int a = u / units;
+        if (a != streamed) {
+            stream.rows(0, g.down, (size_t)__builtin_amdgcn_readfirstlane(plan.entry[a].expert) * g.dim + row0, min(16, g.dim - row0), g.hidden_chunks);
+            streamed = a;
+        }
+        stream.issue(u - a * units, ring + (u - begin) % kSlots * S::kSlot);
     };
-    // two units on their way, and the expert of the third
-    int ahead = 0;
+    // two units on their way
     if (begin < end)
-        issue(begin, expert_of(begin));
+        issue(begin);
     if (begin + 1 < end)
-        issue(begin + 1, expert_of(begin + 1));
-    if (begin + 2 < end)
-        ahead = expert_of(begin + 2);
-    for (int i = (int)threadIdx.x; i < kProductWaves * g.tokens * 16; i += 64 * kProductWaves)
-        sums[i] = 0.0f;
-    __syncthreads();
+        issue(begin + 1);
+    for (int i = lane; i < g.tokens * 16; i += kWave)
+        mine[i] = 0.0f;
     for (int u = begin; u < end;) {
         const int a = u / units, stop = min(end, (a + 1) * units);
-        const Entry entry = g.plan->entry[a];
-        for (; u < stop; u++) {
-            const char *const slot = ring + (u - begin) % kSlots * S::kSlot;
-            const int in_row = u % units;
-            Columns<TILES> h;
-            h.at(g.h_digits, g.h_scales, units, nullptr, entry.offset, min(entry.pairs, kPairs));
-            h.load(in_row);
-            if (u + 2 < end) {
-                issue(u + 2, ahead);
-                if (u + 3 < end)
-                    ahead = expert_of(u + 3);
-                wait_vmcnt<2 * S::kLoads>();
-            } else if (u + 1 < end) {
-                wait_vmcnt<S::kLoads>();
-            } else {
-                wait_vmcnt<0>();
-            }
-            const v4i scales = S::all_scales(slot, 0);
-            for (int first = 0; first < entry.pairs; first += kPairs) {
-                const int now = min(entry.pairs - first, kPairs);
-                if (first) {
-                    h.at(g.h_digits, g.h_scales, units, nullptr, entry.offset + first, now);
-                    h.load(in_row);
-                }
-                v4f acc[TILES];
+        const Entry entry = plan.entry[a];
+        const int offset = __builtin_amdgcn_readfirstlane(entry.offset), pairs = __builtin_amdgcn_readfirstlane(entry.pairs);
+        Columns<TILES> h;
+        v4f acc[TILES];
+        const auto multiply = [&](const char *slot, const v4i scales, int now) {
+#pragma unroll
+            for (int k = 0; k < kUnitSteps; k++) {
+                const v4i codes = S::operand(slot, 0, k);
 #pragma unroll
                 for (int i = 0; i < TILES; i++)
-                    acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (i * kTokensATile < now)
+                        acc[i] = mfma_digits(codes, h.d[i][k], acc[i], scales[k], h.scale(i, k));
+            }
+        };
+        const auto add = [&](int first, int now) {
 #pragma unroll
-                for (int k = 0; k < kUnitSteps; k++) {
-                    const v4i codes = S::operand(slot, 0, k);
+            for (int i = 0; i < TILES; i++) {
+                settle(acc[i]);
+                v4f v;
 #pragma unroll
-                    for (int i = 0; i < TILES; i++)
-                        if (i * kTokensATile < now)
-                            acc[i] = mfma_digits(codes, h.d[i][k], acc[i], scales[k], h.scale(i, k));
+                for (int k = 0; k < 4; k++)
+                    v[k] = sum_digits(acc[i][k]);
+                const int pair = i * kTokensATile + r / kDigits;
+                if (r % kDigits == 0 && r < 15 && pair < now) {
+                    v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)plan.token[offset + first + pair] * 16 + 4 * q);
+                    *to = *to + v;
                 }
+                acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        };
 #pragma unroll
-                for (int i = 0; i < TILES; i++) {
-                    settle(acc[i]);
-                    v4f v;
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        v[k] = sum_digits(acc[i][k]);
-                    const int pair = i * kTokensATile + r / kDigits;
-                    if (r % kDigits == 0 && r < 15 && pair < now) {
-                        v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)g.plan->token[entry.offset + first + pair] * 16 + 4 * q);
-                        *to = *to + v;
-                    }
+        for (int i = 0; i < TILES; i++)
+            acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        h.at(g.h_digits, g.h_scales, units, nullptr, offset, min(pairs, kPairs));
+        const auto work = [&](const char *slot, int in_row) {
+            const v4i scales = S::all_scales(slot, 0);
+            multiply(slot, scales, min(pairs, kPairs));
+            if (pairs > kPairs) {       // more than fit: unit by unit
+                add(0, kPairs);
+                for (int first = kPairs; first < pairs; first += kPairs) {
+                    h.at(g.h_digits, g.h_scales, units, nullptr, offset + first, min(pairs - first, kPairs));
+                    h.load(in_row);
+                    multiply(slot, scales, min(pairs - first, kPairs));
+                    add(first, min(pairs - first, kPairs));
                 }
+                h.at(g.h_digits, g.h_scales, units, nullptr, offset, kPairs);
             }
             S::done_reading();
+        };
+        // (the last two units by themselves: the compiler waits for digits as for the way with the fewest loads behind them)
+        for (; u < min(stop, end - 2); u++) {
+            h.load(u - a * units);
+            issue(u + 2);
+            wait_vmcnt<2 * S::kLoads>();
+            work(ring + (u - begin) % kSlots * S::kSlot, u - a * units);
         }
+        for (; u < stop; u++) {
+            h.load(u - a * units);
+            wait_vmcnt<0>();
+            work(ring + (u - begin) % kSlots * S::kSlot, u - a * units);
+        }
+        if (pairs <= kPairs)
+            add(0, pairs);
     }
     __syncthreads();
     for (int i = (int)threadIdx.x; i < g.tokens * 16; i += 64 * kProductWaves) {
@@ -660,7 +896,7 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
             continue;
         }
         if (g.down_bias)
-            v += down_bias(g, t, row);
+            v += down_bias(g, plan, t, row);
         g.y[(size_t)t * g.dim + row] = v;
     }
 }
@@ -675,7 +911,7 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const Args g)
     for (int s = 1; s < g.splits; s++)
         v += g.parts[(size_t)s * all + i];
     if (g.down_bias)
-        v += down_bias(g, i / g.dim, i % g.dim);
+        v += down_bias(g, *g.plan, i / g.dim, i % g.dim);
     g.y[i] = v;
 }
 
@@ -803,7 +1039,10 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     int status = check_launch("moe_scores_kernel");
     if (status != VTL_HIP_OK)
         return status;
-    const bool own_plan = tokens <= kOwnPlan, narrow = g.experts <= 2 * kWave;
+    // 32 hidden values for each wave, if the tokens choose experts as they would by chance
+    const double chosen = g.experts * (1.0 - std::pow(1.0 - (double)g.top / g.experts, tokens));
+    const bool many = chosen * ((g.hidden + 31) / 32) >= 1024;
+    const bool own_plan = tokens <= kOwnPlan && !many, narrow = g.experts <= 2 * kWave;
     if (!own_plan) {
         hipLaunchKernelGGL(narrow ? moe_plan_kernel<2> : moe_plan_kernel<kMostExperts / kWave>, dim3(1), dim3(1024), 0, st, g);
         if ((status = check_launch("moe_plan_kernel")) != VTL_HIP_OK)
@@ -811,7 +1050,7 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     }
     const unsigned most = (unsigned)std::min(g.experts, tokens * g.top);
     if (!own_plan)
-        status = launch_with_lds<moe_gate_up_kernel<2, 4, 1, 0>>(most * (unsigned)(g.hidden_units * (kUnit / 64)), 256, 4 * 2 * Stream<2>::kSlot, st, g);
+        status = many ? launch_with_lds<moe_gate_up_jobs_kernel<2>>(256, 64 * kJobWaves, kJobWaves * 2 * Stream<2>::kSlot, st, g) : launch_few<2, 0>(g, most, st);
     else if (tokens <= kTokensATile)
         status = narrow ? launch_few<1, 2>(g, most, st) : launch_few<1, kMostExperts / kWave>(g, most, st);
     else

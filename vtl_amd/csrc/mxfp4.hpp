@@ -97,19 +97,22 @@ struct Stream {
             code_at[f][j] = (unsigned)min(4 * j + lane / 16, most - 1) * pitch;
         scale_at[f] = (unsigned)min(lane / 4, most - 1) * spitch;
     }
-    // The loads of a unit.  Where a row has only the first half of it, the rest is the row's end once more.
+    // The loads of a unit.  Where a row has only the first half of it, the rest is the row's end once more.  (Buffer loads: behind global ones into
+    // shared memory the compiler takes loads into registers to arrive in any order, and waits for all that there are.)
     __device__ __forceinline__ void issue(int unit, char *slot) const
     {
         const int lane = threadIdx.x % kWave;
 #pragma unroll
         for (int f = 0; f < FRAGS; f++) {
+            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(codes[f]), 0, (int)(16u * pitch), 0x00027000);
+            const __amdgpu_buffer_rsrc_t scales_from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(scales[f]), 0, (int)(16u * spitch), 0x00027000);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const unsigned in_row = min((unsigned)unit * (kUnit / 2) + (unsigned)((lane % 16) ^ (4 * j + lane / 16)) * 16u, pitch - 16u);
-                __builtin_amdgcn_global_load_lds(VTL_GPTR(codes[f] + (code_at[f][j] + in_row)), VTL_LPTR(slot + f * kFrag + j * 1024), 16, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(from, VTL_LPTR(slot + f * kFrag + j * 1024), 16, (int)(code_at[f][j] + in_row), 0, 0, 0);
             }
             const unsigned in_row = min((unsigned)unit * (kUnit / kBlock) + (unsigned)(lane % 4) * 4u, spitch - 4u);
-            __builtin_amdgcn_global_load_lds(VTL_GPTR(scales[f] + (scale_at[f] + in_row)), VTL_LPTR(slot + f * kFrag + kCodes), 4, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(scales_from, VTL_LPTR(slot + f * kFrag + kCodes), 4, (int)(scale_at[f] + in_row), 0, 0, 0);
         }
     }
     __device__ __forceinline__ static v4i operand(const char *slot, int f, int step)
