@@ -32,8 +32,9 @@
  *     K-split partial sums of the matmuls, with f32 and f64 operands from
  *     K = 2048 on (for the gradients the dimension that is summed over, for
  *     column sums 128 rows), vtl_hip_linear_i8_requant,
- *     vtl_hip_linear_f32_dynquant and vtl_hip_attention_i8_f32 with workspace ==
- *     NULL, int8 operands that need repacking).  There is one such buffer per purpose and device,
+ *     vtl_hip_linear_f32_dynquant, vtl_hip_attention_i8_f32, the MXFP4 products
+ *     and vtl_hip_moe_mxfp4_f32 with workspace == NULL, int8 operands that need
+ *     repacking).  There is one such buffer per purpose and device,
  *     shared by every stream: calls that use it must not overlap on a device,
  *     i.e. issue them on one stream (or order the streams yourself).  Calls
  *     on whole host tensors have blocks of their own instead while no stream
@@ -420,7 +421,7 @@ typedef struct {
 /* Y[tokens, dim] of X[tokens, dim], for a few tokens: up to VTL_HIP_MOE_MOST_TOKENS, and experts, top_k, dim and hidden within the limits
  * above (VTL_HIP_ERR_UNSUPPORTED beyond).  x, and p times the hidden values, enter the products with 24 bits of the largest among 32 (to 2^-128 where that is below
  * 2^-103), sums are f32; the same call gives the same bits.  A token with an infinity or NaN, or without a finite score, gives NaN, and so does a
- * chosen expert's block of weights without a number.  X and Y may not share memory.
+ * chosen expert's block of weights without a number.  Y may not share memory with X or the layer.
  * workspace: as above, of vtl_hip_moe_mxfp4_workspace() bytes (0: no such layer). */
 size_t vtl_hip_moe_mxfp4_workspace(const vtl_hip_moe *layer, int tokens);
 int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, int tokens, void *workspace, size_t workspace_bytes);

@@ -197,6 +197,34 @@ def test_experts(guard_bands, experts, dim, hidden, top, tokens, renormalize, bi
     assert np.array_equal(moe_mxfp4_hip(l.layer, dev(x), ws).cpu(), got)
 
 
+class LargeLayer(Layer):
+    """Of codes and scales drawn as such."""
+
+    def __init__(self, experts, dim, hidden, top, bias, seed=0):
+        rng = np.random.default_rng(seed)
+
+        def rows(n, cols):
+            codes = rng.integers(0, 256, (n, mx.padded(cols) // 2), np.uint8)
+            scales = (127 - int(np.log2(3 * cols ** 0.5)) + rng.integers(-1, 2, (n, mx.padded(cols) // 32))).astype(np.uint8)
+            return HipMxfp4.from_packed(codes[:, :-(-cols // 2)], scales[:, :-(-cols // 32)], cols), mx.decode(codes, scales, cols)
+
+        self.top, self.renormalize = top, True
+        self.router = normal(seed, experts, dim, std=dim ** -0.5)
+        self.gate_up, gu = rows(experts * 2 * hidden, dim)
+        self.down, dn = rows(experts * dim, hidden)
+        self.gu, self.dn = gu.reshape(experts, 2 * hidden, dim), dn.reshape(experts, dim, hidden)
+        self.biases = (normal(seed + 3, experts, std=0.3), normal(seed + 4, experts, 2 * hidden, std=0.3), normal(seed + 5, experts, dim, std=0.3)) if bias else (None,) * 3
+        self.hip()
+
+
+@pytest.mark.parametrize("experts,dim,hidden,top,tokens,bias", [
+    (64, 96, 1000, 6, 40, False), (16, 550, 2100, 8, 12, True), (8, 40, 4112, 4, 9, False), (64, 64, 1030, 16, 8, True), (20, 64, 2080, 16, 1, False)])
+def test_hidden_values_for_every_compute_unit(guard_bands, experts, dim, hidden, top, tokens, bias):
+    l = LargeLayer(experts, dim, hidden, top, bias)
+    x = normal(98, tokens, dim)
+    assert np.array_equal(check_layer(l, x), check_layer(l, x))
+
+
 def test_equal_scores_go_to_the_lowest_experts():
     l = Layer(12, 64, 32, 3, True, False)
     l.router[:] = l.router[0]

@@ -8,7 +8,6 @@
 // tokens of five columns), each with a scale of its own, and their sums are added at the end.  A block's products are multiples of a
 // half up to 96, so its sum is exact in the unit; only sums of blocks are rounded, to f32.
 #include <cmath>
-#include <type_traits>
 
 #include "mxfp4.hpp"
 
@@ -423,17 +422,16 @@ struct Columns {
     }
 };
 
-// The sum of a pair's five columns, in the lanes of the first; the smallest digits first.
+// The sum of a pair's five columns, in the lanes of the first.
+template <int N>
+__device__ __forceinline__ float plus_right(float v, float of)
+{
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(of), 0x100 + N, 0xF, 0xF, true));   // row_shl
+}
 __device__ __forceinline__ float sum_digits(float v)
 {
-    auto right = [&](auto n) {
-        constexpr int kControl = 0x100 + decltype(n)::value;   // row_shl
-        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kControl, 0xF, 0xF, true));
-    };
-    float s = right(std::integral_constant<int, 4>{}) + right(std::integral_constant<int, 3>{});
-    s += right(std::integral_constant<int, 2>{});
-    s += right(std::integral_constant<int, 1>{});
-    return s + v;
+    const float two = plus_right<1>(v, v), four = plus_right<2>(two, two);
+    return plus_right<4>(four, v);
 }
 
 // SiLU(gate) * up * weight.  The exponential is the vector unit's of a rounded exponent, off by |gate| half steps and one, which is |gate| steps of a value that is
@@ -465,184 +463,14 @@ struct Held {
     }
 };
 
-// Hidden values of all chosen experts, where there are enough of them for all compute units.  A job is 32 of an expert's, the rows of its gate and of its up in two
-// halves of 16, and a wave's own from the first load to the digits that go out: eight waves a compute unit have jobs behind each other, the next unit's weights on their
-// way while one is worked on, and meet nowhere.  (Workgroups with rounds of their own, one for 64 values of an expert, took 52 us for 24 tokens
-// of 128 experts of 2048 x 1024, 32 of them without a weight read; four waves with 32 rows at once 63, a compute unit's waves then wait one by one.)
-constexpr int kJobWaves = 8;
-
-template <int TILES>
-__global__ __launch_bounds__(64 * kJobWaves) void moe_gate_up_jobs_kernel(const Args g)
-{
-    using S = Stream<2>;
-    constexpr int kPairs = TILES * kTokensATile;
-    extern __shared__ __attribute__((aligned(16))) char smem[];   // two slots a wave
-    __shared__ Held held;
-    held.copy(g);
-    const Plan &plan = held.plan;
-    const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
-    const int tiles = (g.hidden + 31) / 32, all = __builtin_amdgcn_readfirstlane(plan.count) * tiles, units = g.dim_units;
-    const int share = (int)blockIdx.x * kJobWaves + w, shares = (int)gridDim.x * kJobWaves;
-    const int begin = (int)((int64_t)all * share / shares), end = (int)((int64_t)all * (share + 1) / shares);
-    if (begin == end)
-        return;
-    char *const ring = smem + w * (2 * S::kSlot);
-    struct At {
-        int job, expert, offset, pairs, first, half, unit;
-    };
-    const auto start = [&](At &at, int job) {
-        const Entry entry = plan.entry[min(job, all - 1) / tiles];
-        at.job = job;
-        at.expert = __builtin_amdgcn_readfirstlane(entry.expert);
-        at.offset = __builtin_amdgcn_readfirstlane(entry.offset);
-        at.pairs = __builtin_amdgcn_readfirstlane(entry.pairs);
-        at.first = at.half = at.unit = 0;
-    };
-    S stream;
-    const auto rows = [&](const At &at) {
-        const int row = min(at.job % tiles * 32 + at.half * 16, g.hidden - 1);
-#pragma unroll
-        for (int f = 0; f < 2; f++)
-            stream.rows(f, g.gate_up, ((size_t)at.expert * 2 + f) * g.hidden + row, min(16, g.hidden - row), g.dim_chunks);
-    };
-    // the position behind one; false: there is none
-    const auto advance = [&](At &at) __attribute__((always_inline)) {
-        if (++at.unit < units)
-            return true;
-        at.unit = 0;
-        at.half ^= 1;
-        if (at.half == 0) {
-            at.first += kPairs;
-            if (at.first >= at.pairs) {
-                if (at.job + 1 >= end)
-                    return false;
-                start(at, at.job + 1);
-            }
-        }
-        return true;
-    };
-    Columns<TILES> x[2];
-    v4f acc[2][TILES], first_half[TILES];
-    int streamed = -1;          // whose rows `stream` has
-    // A unit's digits, and behind them its weights: loads arrive in order, and the digits are waited for together with the unit's weights in front of them.
-    const auto ask = [&](const At &at, Columns<TILES> &to, char *slot) __attribute__((always_inline)) {
-        to.at(g.x_digits, g.x_scales, units, plan.token, at.offset + at.first, min(at.pairs - at.first, kPairs));
-        to.load(at.unit);
-        if (streamed != at.job * 2 + at.half) {
-            rows(at);
-            streamed = at.job * 2 + at.half;
-        }
-        stream.issue(at.unit, slot);
-    };
-    const auto work = [&](const At &now, const Columns<TILES> &x, const char *slot) __attribute__((always_inline)) {
-        if (now.unit == 0)
-#pragma unroll
-            for (int f = 0; f < 2; f++)
-#pragma unroll
-                for (int i = 0; i < TILES; i++)
-                    acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        const int here = min(now.pairs - now.first, kPairs);
-        const v4i scales[2] = {S::all_scales(slot, 0), S::all_scales(slot, 1)};
-#pragma unroll
-        for (int k = 0; k < kUnitSteps; k++) {
-            const v4i codes[2] = {S::operand(slot, 0, k), S::operand(slot, 1, k)};
-#pragma unroll
-            for (int i = 0; i < TILES; i++)
-                if (i * kTokensATile < here) {
-                    const int xb = x.scale(i, k);
-#pragma unroll
-                    for (int f = 0; f < 2; f++)
-                        acc[f][i] = mfma_digits(codes[f], x.d[i][k], acc[f][i], scales[f][k], xb);
-                }
-        }
-        S::done_reading();
-        if (now.unit != units - 1)
-            return;
-        const int row0 = now.job % tiles * 32, padded = g.hidden_units * kUnit;
-#pragma unroll
-        for (int i = 0; i < TILES; i++)
-            if (i * kTokensATile < here) {
-                settle(acc[0][i]);
-                settle(acc[1][i]);
-                const int pair = min(i * kTokensATile + r / kDigits, here - 1), at = now.offset + now.first + pair;
-                const float weight = plan.weight[at];
-                v4f h;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    float gate = sum_digits(acc[0][i][k]), up = sum_digits(acc[1][i][k]);
-                    const int row = row0 + 16 * now.half + 4 * q + k;
-                    h[k] = 0.0f;
-                    if (row < g.hidden) {
-                        if (g.gate_up_bias) {
-                            const float *const bias = g.gate_up_bias + (size_t)now.expert * 2 * g.hidden + row;
-                            gate += bias[0];
-                            up += bias[g.hidden];
-                        }
-                        h[k] = hidden_value(gate, up, weight);
-                    }
-                }
-                if (now.half == 0) {
-                    first_half[i] = h;
-                    continue;
-                }
-                // the four lanes q of a column have its block of 32
-                unsigned top = max(max_bits(first_half[i]), max_bits(h));
-                top = max(top, (unsigned)__shfl_xor((int)top, 16));
-                top = max(top, (unsigned)__shfl_xor((int)top, 32));
-                if (r % kDigits == 0 && x.present[i]) {
-                    uint8_t *const digits = g.h_digits + (size_t)at * kDigits * padded, *const bytes = g.h_scales + (size_t)at * (padded / kBlock);
-#pragma unroll
-                    for (int f = 0; f < 2; f++) {
-                        unsigned d[kDigits];
-                        digits_of(f ? h : first_half[i], top, d);
-#pragma unroll
-                        for (int j = 0; j < kDigits; j++)
-                            *reinterpret_cast<unsigned *>(digits + digit_at(row0 + 16 * f + 4 * q) + j * kDigitStep) = d[j];
-                    }
-                    if (q == 0)
-                        bytes[row0 / kBlock] = (uint8_t)digit_byte(top);
-                    if (row0 + 32 >= g.hidden)      // behind the last value
-                        for (int col = row0 + 32 + 4 * q; col < padded; col += 16) {
-#pragma unroll
-                            for (int j = 0; j < kDigits; j++)
-                                *reinterpret_cast<unsigned *>(digits + digit_at(col) + j * kDigitStep) = 0u;
-                            if (col % kBlock == 0)
-                                bytes[col / kBlock] = (uint8_t)digit_byte(0);
-                        }
-                }
-            }
-    };
-    char *const slots[2] = {ring, ring + S::kSlot};
-    At at[2];
-    start(at[0], begin);
-    ask(at[0], x[0], slots[0]);
-    at[1] = at[0];
-    if (!advance(at[1])) {
-        wait_vmcnt<0>();
-        work(at[0], x[0], slots[0]);
-        return;
-    }
-    ask(at[1], x[1], slots[1]);
-    // Two units on their way at the top of a round, on every way there: the compiler waits for digits as for the way with the fewest loads behind them.
-    const auto round = [&](auto i_t) __attribute__((always_inline)) {
-        constexpr int i = decltype(i_t)::value, o = i ^ 1;
-        wait_vmcnt<S::kLoads>();
-        work(at[i], x[i], slots[i]);
-        at[i] = at[o];
-        if (!advance(at[i])) {
-            wait_vmcnt<0>();
-            work(at[o], x[o], slots[o]);
-            return false;
-        }
-        ask(at[i], x[i], slots[i]);
-        return true;
-    };
-    while (round(std::integral_constant<int, 0>{}) && round(std::integral_constant<int, 1>{}))
-        ;
-}
-
 // 16 RW hidden values of an expert's tokens: RW times 16 rows of its gate and as many of its up, KW waves each, which deal K out among them.
 // The values go out as digits, already times their weights, so that the next product adds experts up as it adds up K.
+// One wave along K where that gives every compute unit eight, else four.  For 24 tokens of 128 experts of 2048 x 1024, us (their weights alone take 41):
+//   waves along K (32 values a workgroup)       1: 45.4     2: 51.4     4: 72.8
+//   64 values, 128                              46.1, 54.4; two waves along K and 64 values 58.1
+//   one tile (three tokens a pass)              48.0 with one wave along K, 51.9 with two
+// Also measured: a workgroup for each compute unit that goes through a run of (expert, 32 values) with the next one's weights on their way 51.8, waves that
+// do so by themselves 60.
 // EACH: every workgroup makes the plan for itself (a few tokens: less than a launch takes); 0: it is there.
 template <int TILES, int RW, int KW, int EACH>
 __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
@@ -931,10 +759,10 @@ int launch_with_lds(unsigned blocks, int threads, int lds, hipStream_t st, const
     return check_launch("moe_mxfp4 product");
 }
 
-template <int TILES, int EACH>
-int launch_few(const Args &g, unsigned most, hipStream_t st)
+template <int TILES, int KW, int EACH>
+int launch_gate_up(const Args &g, unsigned most, hipStream_t st)
 {
-    return launch_with_lds<moe_gate_up_kernel<TILES, 2, 4, EACH>>(most * (unsigned)(g.hidden_units * (kUnit / 32)), 512, 8 * 2 * Stream<2>::kSlot, st, g);
+    return launch_with_lds<moe_gate_up_kernel<TILES, 2, KW, EACH>>(most * (unsigned)(g.hidden_units * (kUnit / 32)), 2 * KW * kWave, 2 * KW * 2 * Stream<2>::kSlot, st, g);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -1014,6 +842,13 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
         !rows_aligned(layer->gate_up, layer->gate_up_scales) || !rows_aligned(layer->down, layer->down_scales))
         return VTL_HIP_ERR_INVALID_ARG;
     Args g = args_of(layer, tokens);
+    const size_t results = (size_t)tokens * g.dim * sizeof(float), experts = (size_t)g.experts, into = experts * 2 * g.hidden, out = experts * g.dim;
+    const auto shared = [&](const void *p, size_t bytes) { return meet(Y, results, p, bytes); };
+    if (shared(X, results) || shared(layer->router, experts * g.dim * sizeof(float)) || shared(layer->router_bias, experts * sizeof(float)) ||
+        shared(layer->gate_up, into * g.dim_chunks * kChunkCodes) || shared(layer->gate_up_scales, into * g.dim_chunks * kChunkScales) ||
+        shared(layer->gate_up_bias, into * sizeof(float)) || shared(layer->down, out * g.hidden_chunks * kChunkCodes) ||
+        shared(layer->down_scales, out * g.hidden_chunks * kChunkScales) || shared(layer->down_bias, out * sizeof(float)))
+        return VTL_HIP_ERR_INVALID_ARG;
     g.x = X;
     g.y = Y;
     const size_t need = vtl_hip_moe_mxfp4_workspace(layer, tokens);
@@ -1039,7 +874,7 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     int status = check_launch("moe_scores_kernel");
     if (status != VTL_HIP_OK)
         return status;
-    // 32 hidden values for each wave, if the tokens choose experts as they would by chance
+    // workgroups of 32 hidden values, if the tokens choose experts as they would by chance
     const double chosen = g.experts * (1.0 - std::pow(1.0 - (double)g.top / g.experts, tokens));
     const bool many = chosen * ((g.hidden + 31) / 32) >= 1024;
     const bool own_plan = tokens <= kOwnPlan && !many, narrow = g.experts <= 2 * kWave;
@@ -1050,11 +885,11 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     }
     const unsigned most = (unsigned)std::min(g.experts, tokens * g.top);
     if (!own_plan)
-        status = many ? launch_with_lds<moe_gate_up_jobs_kernel<2>>(256, 64 * kJobWaves, kJobWaves * 2 * Stream<2>::kSlot, st, g) : launch_few<2, 0>(g, most, st);
+        status = many ? launch_gate_up<2, 1, 0>(g, most, st) : launch_gate_up<2, 4, 0>(g, most, st);
     else if (tokens <= kTokensATile)
-        status = narrow ? launch_few<1, 2>(g, most, st) : launch_few<1, kMostExperts / kWave>(g, most, st);
+        status = narrow ? launch_gate_up<1, 4, 2>(g, most, st) : launch_gate_up<1, 4, kMostExperts / kWave>(g, most, st);
     else
-        status = narrow ? launch_few<2, 2>(g, most, st) : launch_few<2, kMostExperts / kWave>(g, most, st);
+        status = narrow ? launch_gate_up<2, 4, 2>(g, most, st) : launch_gate_up<2, 4, kMostExperts / kWave>(g, most, st);
     if (status != VTL_HIP_OK)
         return status;
     const unsigned blocks = (unsigned)(g.dim + 15) / 16 * (unsigned)g.splits;
