@@ -381,7 +381,7 @@ int vtl_hip_attention_i8_f32(const vtl_hip_kv_cache *cache, const vtl_hip_kv_bat
 int vtl_hip_mxfp4_padded_row(int cols);
 
 /* Rows of f32, x_stride elements from one to the next: b = max(0, e - 2) with e the exponent field of the block's largest magnitude, each code the
- * nearest to x / 2^(b - 127), the even one of two, at most 6 in magnitude.  A block with an infinity or NaN gets b = 255 and zero codes. */
+ * nearest to x / 2^(b - 127), the even one of two, at most 6 in magnitude.  A block with an infinity or NaN gets b = 255 and zero codes.  Codes and scales may not share memory with x. */
 int vtl_hip_quantize_f32_mxfp4(const float *x, int64_t x_stride, int64_t rows, int64_t cols, uint8_t *codes, uint8_t *scales);
 /* x = code * 2^(b - 127) in f32. */
 int vtl_hip_dequantize_mxfp4_f32(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, float *x, int64_t x_stride);

@@ -254,7 +254,7 @@ struct Tile {
     static constexpr int kLoads = kALoads + kBLoads + kSLoads;
     static constexpr int kStage = (BM + BN) * kChunkCodes;
     // Scales come for kGroup chunks at once, 32 bytes of a row (of each 8 bytes a request would be one for a line of its own, as many as
-    // for the codes: 8192 x 8192 x 8192 KKK), a quarter of the rows with the codes of each chunk; the last quarter of a group with those of its first chunk.
+    // for the codes: 37.8 million requests to the L2 caches for 8192 x 8192 x 8192, so 25.7), a quarter of the rows with the codes of each chunk; the last quarter of a group with those of its first chunk.
     static constexpr int kGroup = 4, kGroupRow = kGroup * kChunkScales, kScales = (BM + BN) * kGroupRow;
     static constexpr int kBuffers = STAGES >= 3 ? 3 : 2;   // of scales: the next group is being loaded up to STAGES + 3 chunks ahead
     static constexpr int kLds = STAGES * kStage + kBuffers * kScales;
@@ -551,8 +551,6 @@ int launch_tile(Args g, hipStream_t st)
         VTL_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds));
         done.store(true, std::memory_order_release);
     }
-    if (g.N > 1 << 27)      // a lane's offset from a row of results
-        return VTL_HIP_ERR_UNSUPPORTED;
     const int64_t blocks = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.splits;
     if (blocks > 0xffffff)
         return VTL_HIP_ERR_UNSUPPORTED;
@@ -597,16 +595,18 @@ struct Plan {
 };
 
 // Tiles and what they cost, by which one is chosen: microseconds for a chunk of K where a compute unit has one workgroup (and two, where it takes two), and
-// for a workgroup's beginning and end.  Measured on 17 to 1024 rows, 1024 to 14336 columns, K of 4096 and 14336; the choice was the fastest
-// or within 8 % of it there (us: 201 x 4096 x 11008 128 x 128 17.3, 64 x 64 19.0, 256 x 128 21.5; 256 x 4096 x 4096 64 x 64 9.5, 128 x 128 15;
-// 512 x 4096 x 11008 256 x 128 24.3, 128 x 128 26.2; 1024 x 4096 x 11008 256 x 256 34.8, 128 x 128 40.9; 64 x 14336 x 4096 64 x 64 with K in four
-// 12.7, in one 17).
+// for a workgroup's beginning and end.  Fitted to all tiles and ranges of K for 48 to 1024 rows, 1024 to 14336 columns, K of 4096 and 14336, where the choice is the
+// fastest or within 6 % of it, 0.2 % on average.  Some of them, us (rows x columns x K):
+//    256 x  4096 x  4096   64 x 64  9.5, 128 x 128 15.4           512 x 11008 x 4096   256 x 128 24.3, 128 x 128 26.2, 64 x 64 33.5
+//    201 x 11008 x  4096   128 x 128 17.3, 64 x 64 19.0          1024 x 11008 x 4096   256 x 256 34.8, 128 x 128 40.9
+//     64 x  4096 x 14336   64 x 64 with K in four 12.7, in two 14.7, in eight 14.3
+// (A tile of 32 x 64 for 17 to 32 rows gains nothing for K of 4096, and has 12.4 us for 13.4 where K is 14336: not worth a kernel.)
 struct TileCost {
     int rows, cols;
     float one, two, ends;
 };
-constexpr TileCost kTiles[] = {{32, 64, 0.30f, 0.40f, 2.0f}, {64, 64, 0.34f, 0.50f, 2.0f}, {128, 128, 0.73f, 1.20f, 2.5f}, {256, 128, 1.2f, 0.0f, 4.0f}, {256, 256, 1.7f, 0.0f, 8.0f}};
-constexpr float kJoin = 3.0f, kJoinBytes = 2.5e-7f;     // for the launch that adds ranges up, and for a byte of their sums
+constexpr TileCost kTiles[] = {{64, 64, 0.34f, 0.50f, 3.0f}, {128, 128, 0.78f, 1.40f, 3.0f}, {256, 128, 1.2f, 0.0f, 5.0f}, {256, 256, 1.7f, 0.0f, 8.0f}};
+constexpr float kJoin = 3.0f, kJoinBytes = 6e-7f;     // for the launch that adds ranges up, and for a byte of their sums
 constexpr int kUnits = 256;
 
 Plan plan_of(int M, int N, int K)
@@ -620,7 +620,7 @@ Plan plan_of(int M, int N, int K)
         const TileCost &c = kTiles[t];
         const int64_t tiles = (((int64_t)M + c.rows - 1) / c.rows) * (((int64_t)N + c.cols - 1) / c.cols);
         for (int splits = 1; splits <= 8; splits += splits < 4 ? 1 : 2) {
-            if (splits > 1 && (chunks < 2 * splits || tiles * splits > 2 * kUnits))
+            if (splits > 1 && (chunks < 4 * splits || tiles * splits > 2 * kUnits))
                 break;
             const int64_t all = tiles * splits, at_once = c.two > 0.0f && all > kUnits ? 2 * kUnits : kUnits;
             const float chunk = at_once > kUnits ? c.two : c.one;
@@ -650,10 +650,9 @@ int product(Args g, const Plan &p, hipStream_t st)
         return g.M <= 4 ? launch_few<1, false, true>(g, st) : g.M <= 8 ? launch_few<2, false, true>(g, st) : launch_few<4, false, true>(g, st);
     }
     g.splits = p.splits;
-    const int rc = p.tile == 0   ? launch_tile<32, 64, 1, 2, 4, 3>(g, st)
-                   : p.tile == 1 ? launch_tile<64, 64, 2, 2, 4, 3>(g, st)
-                   : p.tile == 2 ? launch_tile<128, 128, 2, 2, 2, 1>(g, st)
-                   : p.tile == 3 ? launch_tile<256, 128, 2, 2, 2, 2>(g, st)
+    const int rc = p.tile == 0   ? launch_tile<64, 64, 2, 2, 4, 3>(g, st)
+                   : p.tile == 1 ? launch_tile<128, 128, 2, 2, 2, 1>(g, st)
+                   : p.tile == 2 ? launch_tile<256, 128, 2, 2, 2, 2>(g, st)
                                  : launch_tile<256, 256, 2, 2, 2, 2>(g, st);
     if (rc != VTL_HIP_OK || p.splits == 1)
         return rc;
@@ -687,7 +686,8 @@ int linear(Args g, const uint8_t *w, const uint8_t *w_scales, const float *bias,
 {
     if (M < 0 || N < 0 || K < 0)
         return VTL_HIP_ERR_INVALID_ARG;
-    if (K > kMostCols || (int64_t)M * chunks_of(K) > INT32_MAX || (int64_t)N * chunks_of(K) > INT32_MAX)
+    // (a lane's offset from a row of results and a grid's threads are counted in 32 bits)
+    if (K > kMostCols || M >= 1 << 30 || N > (1 << 27) - 16 || (int64_t)M * chunks_of(K) > INT32_MAX || (int64_t)N * chunks_of(K) > INT32_MAX)
         return VTL_HIP_ERR_UNSUPPORTED;
     if (M == 0 || N == 0)
         return VTL_HIP_OK;

@@ -142,6 +142,13 @@ int sizes(int64_t rows, int64_t cols, int64_t stride, Args &a)
     return VTL_HIP_OK;
 }
 
+// Whether one side's memory is the other's: waves read and write chunks in no order.
+bool shared(const Args &a, const float *x, const uint8_t *codes, const uint8_t *scales)
+{
+    const size_t rows = a.chunks / a.per_row, bytes = ((rows - 1) * (size_t)a.stride + (size_t)a.cols) * sizeof(float);
+    return meet(x, bytes, codes, (size_t)a.chunks * kChunkCodes) || meet(x, bytes, scales, (size_t)a.chunks * kChunkScales);
+}
+
 // Chunks of a wave at once, one where there are not enough of them for all compute units' waves.  (14336 x 4096 f32 into codes with 1 / 2 / 4 / 8
 // at once: 51.7 / 45.6 / 43.7 / 43.0 us, 6.1 TB/s; back 37.3 / 37.7 / 38.8 / 41.8; 16384 x 16384 213 / 196 / 195 / 195 and 223 / 200 / 203 / 217.)
 constexpr int kQuantizeAtOnce = 4, kDequantizeAtOnce = 2;
@@ -199,6 +206,8 @@ int vtl_hip_quantize_f32_mxfp4(const float *x, int64_t x_stride, int64_t rows, i
         return rc;
     if (!x || !codes || !scales || !rows_aligned(codes, scales))
         return VTL_HIP_ERR_INVALID_ARG;
+    if (shared(a, x, codes, scales))
+        return VTL_HIP_ERR_INVALID_ARG;
     a.x = x;
     a.codes = codes;
     a.scales = scales;
@@ -212,6 +221,8 @@ int vtl_hip_dequantize_mxfp4_f32(const uint8_t *codes, const uint8_t *scales, in
     if (rc != VTL_HIP_OK || a.chunks == 0)
         return rc;
     if (!x || !codes || !scales || !rows_aligned(codes, scales))
+        return VTL_HIP_ERR_INVALID_ARG;
+    if (shared(a, x, codes, scales))
         return VTL_HIP_ERR_INVALID_ARG;
     a.out = x;
     a.codes = const_cast<uint8_t *>(codes);
