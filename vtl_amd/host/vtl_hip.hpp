@@ -451,6 +451,141 @@ inline HipTensor<float> attention_i8_hip(const HipKVCache &cache, const HipKVBat
     return out;
 }
 
+// `HipMxfp4{codes; scales; rows; cols}`: a matrix of microscaled 4-bit values, in rows padded to vtl_hip_mxfp4_padded_row(cols).
+class HipMxfp4 {
+public:
+    HipStorage<uint8_t> codes, scales;
+    int rows = 0, cols = 0;
+
+    HipMxfp4() = default;
+    HipMxfp4(int rows_, int cols_, HipParams p = {}) : rows(rows_), cols(cols_)
+    {
+        const int padded = vtl_hip_mxfp4_padded_row(cols);
+        if (!padded || rows < 0)
+            throw std::invalid_argument("HipMxfp4: no rows of this size");
+        codes = HipStorage<uint8_t>((size_t)rows * (padded / 2), p);
+        scales = HipStorage<uint8_t>((size_t)rows * (padded / 32), p);
+    }
+    // Codes [rows, padded / 2], the even value in the low four bits, and scales [rows, padded / 32] of a checkpoint.
+    static HipMxfp4 from_packed(const std::vector<uint8_t> &codes, const std::vector<uint8_t> &scales, int rows, int cols, HipParams p = {})
+    {
+        const size_t padded = (size_t)vtl_hip_mxfp4_padded_row(cols);
+        if (!padded || rows < 0 || codes.size() != (size_t)rows * (padded / 2) || scales.size() != (size_t)rows * (padded / 32))
+            throw std::invalid_argument("HipMxfp4: codes and scales of padded rows expected");
+        HipMxfp4 q;
+        q.rows = rows;
+        q.cols = cols;
+        q.codes = HipStorage<uint8_t>::from_cpu(codes, p);
+        q.scales = HipStorage<uint8_t>::from_cpu(scales, p);
+        return q;
+    }
+    // `(q &HipMxfp4) dequantize() !&HipTensor[f32]`
+    HipTensor<float> dequantize() const
+    {
+        HipTensor<float> x({rows, cols}, HipParams{codes.device_id});
+        hip_check(vtl_hip_dequantize_mxfp4_f32((const uint8_t *)codes.ptr, (const uint8_t *)scales.ptr, rows, cols, (float *)x.data.ptr, cols),
+                  "vtl_hip_dequantize_mxfp4_f32");
+        return x;
+    }
+    const uint8_t *code_rows() const { return (const uint8_t *)codes.ptr; }
+    const uint8_t *scale_rows() const { return (const uint8_t *)scales.ptr; }
+    void release()
+    {
+        codes.release();
+        scales.release();
+    }
+};
+
+// `quantize_mxfp4_hip(x) !&HipMxfp4`
+inline HipMxfp4 quantize_mxfp4_hip(const HipTensor<float> &x)
+{
+    if (!x.is_matrix())
+        throw std::invalid_argument("Matrix expected");
+    HipMxfp4 q(x.shape[0], x.shape[1], HipParams{x.data.device_id});
+    hip_check(vtl_hip_quantize_f32_mxfp4((const float *)x.data.ptr, q.cols, q.rows, q.cols, (uint8_t *)q.codes.ptr, (uint8_t *)q.scales.ptr),
+              "vtl_hip_quantize_f32_mxfp4");
+    return q;
+}
+
+inline const float *mxfp4_bias(const HipTensor<float> *bias, size_t n)
+{
+    if (bias && bias->size != n)
+        throw std::invalid_argument("bias: one entry per output feature expected");
+    return bias ? (const float *)bias->data.ptr : nullptr;
+}
+
+// `linear_mxfp4_workspace(m, n, k, codes) usize`: bytes of the workspace that linear_f32_mxfp4_hip takes, or linear_mxfp4_hip where
+// codes is set; 0: none is needed.
+inline size_t linear_mxfp4_workspace(int m, int n, int k, bool codes = false)
+{
+    return codes ? vtl_hip_linear_mxfp4_workspace(m, n, k) : vtl_hip_linear_f32_mxfp4_workspace(m, n, k);
+}
+
+// `linear_mxfp4_hip(x, w, bias, relu, workspace) !&HipTensor[f32]`: x . w^T + bias of codes; bias and workspace may be null.
+inline HipTensor<float> linear_mxfp4_hip(const HipMxfp4 &x, const HipMxfp4 &w, const HipTensor<float> *bias = nullptr, bool relu = false,
+                                         const HipStorage<uint8_t> *workspace = nullptr)
+{
+    if (x.cols != w.cols)
+        throw std::invalid_argument("Invalid shapes for matrix multiplication");
+    const float *const b = mxfp4_bias(bias, (size_t)w.rows);
+    HipTensor<float> y({x.rows, w.rows}, HipParams{x.codes.device_id});
+    hip_check(vtl_hip_linear_mxfp4_f32(x.code_rows(), x.scale_rows(), w.code_rows(), w.scale_rows(), b, (float *)y.data.ptr, x.rows, w.rows, w.cols, relu,
+                                       workspace ? workspace->ptr : nullptr, workspace ? workspace->size : 0),
+              "vtl_hip_linear_mxfp4_f32");
+    return y;
+}
+
+// `linear_f32_mxfp4_hip(x, w, bias, relu, workspace) !&HipTensor[f32]`: the same of f32 rows, which become codes on the way.
+inline HipTensor<float> linear_f32_mxfp4_hip(const HipTensor<float> &x, const HipMxfp4 &w, const HipTensor<float> *bias = nullptr, bool relu = false,
+                                             const HipStorage<uint8_t> *workspace = nullptr)
+{
+    if (!x.is_matrix() || x.shape[1] != w.cols)
+        throw std::invalid_argument("Invalid shapes for matrix multiplication");
+    const float *const b = mxfp4_bias(bias, (size_t)w.rows);
+    HipTensor<float> y({x.shape[0], w.rows}, HipParams{x.data.device_id});
+    hip_check(vtl_hip_linear_f32_mxfp4((const float *)x.data.ptr, w.code_rows(), w.scale_rows(), b, (float *)y.data.ptr, x.shape[0], w.rows, w.cols, relu,
+                                       workspace ? workspace->ptr : nullptr, workspace ? workspace->size : 0),
+              "vtl_hip_linear_f32_mxfp4");
+    return y;
+}
+
+// `HipMoE{router; gate_up; down; top_k; renormalize; biases}`: a layer of experts over tensors that live as long as it does.  router [experts, dim],
+// gate_up [experts * 2 * hidden, dim] (for each expert the rows of its gate and then those of its up), down [experts * dim, hidden].
+class HipMoE {
+public:
+    vtl_hip_moe handle{};
+
+    HipMoE(const HipTensor<float> &router, const HipMxfp4 &gate_up, const HipMxfp4 &down, int top_k, bool renormalize = true,
+           const HipTensor<float> *router_bias = nullptr, const HipTensor<float> *gate_up_bias = nullptr, const HipTensor<float> *down_bias = nullptr)
+    {
+        if (!router.is_matrix())
+            throw std::invalid_argument("HipMoE: a router [experts, dim] expected");
+        const int experts = router.shape[0], dim = router.shape[1], hidden = down.cols;
+        const int64_t into = (int64_t)experts * 2 * hidden, out = (int64_t)experts * dim;
+        if (gate_up.cols != dim || gate_up.rows != into || down.rows != out)
+            throw std::invalid_argument("HipMoE: shapes of router, gate_up and down disagree");
+        if (top_k < 1 || top_k > experts)
+            throw std::invalid_argument("HipMoE: top_k");
+        handle = {experts, top_k, dim, hidden, renormalize ? 1 : 0, (const float *)router.data.ptr, mxfp4_bias(router_bias, (size_t)experts),
+                  gate_up.code_rows(), gate_up.scale_rows(), mxfp4_bias(gate_up_bias, (size_t)into),
+                  down.code_rows(), down.scale_rows(), mxfp4_bias(down_bias, (size_t)out)};
+    }
+    // `moe_mxfp4_workspace(layer, tokens) !usize`
+    size_t workspace(int tokens) const { return vtl_hip_moe_mxfp4_workspace(&handle, tokens); }
+};
+
+// `moe_mxfp4_hip(layer, x, workspace) !&HipTensor[f32]`: the layer's output for a few tokens [tokens, dim]; workspace may be null.
+inline HipTensor<float> moe_mxfp4_hip(const HipMoE &layer, const HipTensor<float> &x, const HipStorage<uint8_t> *workspace = nullptr)
+{
+    if (!x.is_matrix() || x.shape[1] != layer.handle.dim)
+        throw std::invalid_argument("moe_mxfp4_hip: tokens [tokens, dim] expected");
+    HipTensor<float> y(x.shape, HipParams{x.data.device_id});
+    hip_check(vtl_hip_moe_mxfp4_f32(&layer.handle, (const float *)x.data.ptr, (float *)y.data.ptr, x.shape[0], workspace ? workspace->ptr : nullptr,
+                                    workspace ? workspace->size : 0),
+              "vtl_hip_moe_mxfp4_f32");
+    return y;
+}
+
 // `linear_backward_hip_f32(grad, input, weight, bias_needs_grad) ![]&vtl.Tensor[f32]`
 // (cf. linear_backward_vulkan_f32, nn/internal/linear_vulkan_backward_d_vulkan.v:9-38):
 // host tensors in, {d_input[M,K], d_weight[N,K], d_bias[1,N]} out; d_bias is zeros
