@@ -445,19 +445,19 @@ __device__ __forceinline__ float hidden_value(float gate, float up, float weight
     return gate * r * up * weight;
 }
 
-// Up to this many experts' pairs have tokens in a workgroup's copy of the plan: all of them.
+// A workgroup's copy of the plan.  All entries that there may be, so that nothing waits for their number.
 struct Held {
     Plan plan;
     __device__ __forceinline__ void copy(const Args &g)
     {
-        const int count = g.plan->count, pairs = g.tokens * g.top, threads = (int)blockDim.x;
+        const int pairs = g.tokens * g.top, most = min(g.experts, pairs), threads = (int)blockDim.x;
         if (threadIdx.x == 0)
-            plan.count = count;
-        for (int i = (int)threadIdx.x; i < count; i += threads)
-            plan.entry[i] = g.plan->entry[i];
+            plan.count = g.plan->count;
         for (int i = (int)threadIdx.x; i < pairs; i += threads) {
             plan.token[i] = g.plan->token[i];
             plan.weight[i] = g.plan->weight[i];
+            if (i < most)
+                plan.entry[i] = g.plan->entry[i];
         }
         __syncthreads();
     }
@@ -478,6 +478,7 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
     constexpr int NW = RW * KW, kRows = 16 * RW, kPairs = TILES * kTokensATile;
     using S = Stream<2>;
     static_assert(RW % 2 == 0, "whole blocks of hidden values");
+    static_assert(64 * NW % (kRows / 4) == 0, "a thread's values are the same of every pair");
     extern __shared__ __attribute__((aligned(16))) char smem[];   // two slots a wave
     __shared__ __attribute__((aligned(16))) float part[NW][kPairs][36];
     const int tiles = g.hidden_units * (kUnit / kRows), a = (int)blockIdx.x / tiles, row0 = (int)blockIdx.x % tiles * kRows;
@@ -494,11 +495,12 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
         count = &c.plan.count;
         weights = c.plan.weight;
     }
+    // (an entry behind the last holds anything; it is read beside the number, not behind it)
+    const Entry entry = entries[a];
     if (a >= *count)
         return;
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
-    const int e = __builtin_amdgcn_readfirstlane(entries[a].expert), offset = __builtin_amdgcn_readfirstlane(entries[a].offset),
-              n = __builtin_amdgcn_readfirstlane(entries[a].pairs);
+    const int e = __builtin_amdgcn_readfirstlane(entry.expert), offset = __builtin_amdgcn_readfirstlane(entry.offset), n = __builtin_amdgcn_readfirstlane(entry.pairs);
     char *const ring = smem + w * (2 * S::kSlot);
     const int begin = g.dim_units * (w % KW) / KW, end = g.dim_units * (w % KW + 1) / KW;
     const int my_row = row0 + w / KW * 16;
@@ -507,6 +509,18 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 #pragma unroll
         for (int f = 0; f < 2; f++)
             stream.rows(f, g.gate_up, ((size_t)e * 2 + f) * g.hidden + my_row, min(16, g.hidden - my_row), g.dim_chunks);
+    }
+    // A thread's four of the hidden values below, whatever the pair: their biases are asked for in front of the weights.
+    const int row = (int)threadIdx.x % (kRows / 4) * 4;
+    v4f gate_bias = {0.0f, 0.0f, 0.0f, 0.0f}, up_bias = gate_bias;
+    if (g.gate_up_bias) {
+        const float *const bias = g.gate_up_bias + (size_t)e * 2 * g.hidden + row0 + row;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (row0 + row + k < g.hidden) {
+                gate_bias[k] = bias[k];
+                up_bias[k] = bias[g.hidden + k];
+            }
     }
     for (int first = 0; first < n; first += kPairs) {
         const int now = min(n - first, kPairs);
@@ -564,7 +578,7 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
         }
         __syncthreads();
         for (int item = (int)threadIdx.x; item < now * (kRows / 4); item += 64 * NW) {   // eight lanes: a pair's block of 32
-            const int i = item / (kRows / 4), row = item % (kRows / 4) * 4, pair = offset + first + i;
+            const int i = item / (kRows / 4), pair = offset + first + i;
             v4f h = {0.0f, 0.0f, 0.0f, 0.0f};
             if (row0 + row < g.hidden) {
                 const float(*const mine)[kPairs][36] = &part[row / 16 * KW];
@@ -577,14 +591,8 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
                 const float weight = weights[pair];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    if (row0 + row + k >= g.hidden)
-                        continue;
-                    if (g.gate_up_bias) {
-                        const float *const bias = g.gate_up_bias + (size_t)e * 2 * g.hidden + row0 + row + k;
-                        gate[k] += bias[0];
-                        up[k] += bias[g.hidden];
-                    }
-                    h[k] = hidden_value(gate[k], up[k], weight);
+                    if (row0 + row + k < g.hidden)
+                        h[k] = hidden_value(gate[k] + gate_bias[k], up[k] + up_bias[k], weight);
                 }
             }
             const int padded = g.hidden_units * kUnit;
@@ -597,18 +605,6 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 // 16 output values of all tokens: the units of all chosen experts, one expert's behind the other's, are dealt out among the waves of `splits`
 // workgroups.  A wave adds what an expert gives to its own sums of the tokens, and the waves' sums meet in order.
 constexpr int kProductWaves = 8;
-
-__device__ __forceinline__ float down_bias(const Args &g, const Plan &plan, int t, int row)
-{
-    float b = 0.0f;
-    for (int a = 0; a < plan.count; a++) {
-        const Entry entry = plan.entry[a];
-        for (int p = entry.offset; p < entry.offset + entry.pairs; p++)
-            if (plan.token[p] == t)
-                b += plan.weight[p] * g.down_bias[(size_t)entry.expert * g.dim + row];
-    }
-    return b;
-}
 
 template <int TILES>
 __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args g)
@@ -648,6 +644,13 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
         const int a = u / units, stop = min(end, (a + 1) * units);
         const Entry entry = plan.entry[a];
         const int offset = __builtin_amdgcn_readfirstlane(entry.offset), pairs = __builtin_amdgcn_readfirstlane(entry.pairs);
+        // The wave that has an expert's first unit adds its bias, in the lanes that have a pair's sums.
+        v4f bias = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (g.down_bias && u == a * units)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (row0 + 4 * q + k < g.dim)
+                    bias[k] = g.down_bias[(size_t)entry.expert * g.dim + row0 + 4 * q + k];
         Columns<TILES> h;
         v4f acc[TILES];
         const auto multiply = [&](const char *slot, const v4i scales, int now) {
@@ -670,8 +673,11 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
                     v[k] = sum_digits(acc[i][k]);
                 const int pair = i * kTokensATile + r / kDigits;
                 if (r % kDigits == 0 && r < 15 && pair < now) {
-                    v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)plan.token[offset + first + pair] * 16 + 4 * q);
-                    *to = *to + v;
+                    const float weight = plan.weight[offset + first + pair];
+                    v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)plan.token[offset + first + pair] * 16 + 4 * q), sum = *to;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        (*to)[k] = sum[k] + fmaf(weight, bias[k], v[k]);
                 }
                 acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             }
@@ -692,6 +698,7 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
                     add(first, min(pairs - first, kPairs));
                 }
                 h.at(g.h_digits, g.h_scales, units, nullptr, offset, kPairs);
+                bias = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             }
             S::done_reading();
         };
@@ -723,8 +730,6 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
             g.parts[((size_t)split * g.tokens + t) * g.dim + row] = v;
             continue;
         }
-        if (g.down_bias)
-            v += down_bias(g, plan, t, row);
         g.y[(size_t)t * g.dim + row] = v;
     }
 }
@@ -738,8 +743,6 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const Args g)
     float v = g.parts[i];
     for (int s = 1; s < g.splits; s++)
         v += g.parts[(size_t)s * all + i];
-    if (g.down_bias)
-        v += down_bias(g, *g.plan, i / g.dim, i % g.dim);
     g.y[i] = v;
 }
 
