@@ -164,7 +164,7 @@ for M in (17, 40, 100, 201, 256, 512, 1024, 4096):
             assert [l[0] for l in log[1:]] == ["linear_join_mxfp4_kernel"] * (splits > 1), (M, N, K, log)
             need = capi.lib().vtl_hip_linear_mxfp4_workspace(M, N, K)
             assert need >= (4 * splits * M * N if splits > 1 else 0) and splits * 4 <= max(4, -(-K // 256)), (M, N, K, splits)
-assert tiles == {(64, 64), (128, 128), (256, 128), (256, 256)}, tiles
+assert tiles == {(64, 64), (128, 96), (128, 128), (256, 128), (256, 256)}, tiles
 print("done")
 """)
 

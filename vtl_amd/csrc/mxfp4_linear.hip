@@ -597,15 +597,16 @@ struct Plan {
 // Tiles and what they cost, by which one is chosen: microseconds for a chunk of K where a compute unit has one workgroup (and two, where it takes two), and
 // for a workgroup's beginning and end.  Fitted to all tiles and ranges of K for 48 to 1024 rows, 1024 to 14336 columns, K of 4096 and 14336, where the choice is the
 // fastest or within 6 % of it, 0.2 % on average.  Some of them, us (rows x columns x K):
-//    256 x  4096 x  4096   64 x 64  9.5, 128 x 128 15.4           512 x 11008 x 4096   256 x 128 24.3, 128 x 128 26.2, 64 x 64 33.5
-//    201 x 11008 x  4096   128 x 128 17.3, 64 x 64 19.0          1024 x 11008 x 4096   256 x 256 34.8, 128 x 128 40.9
+//    256 x  4096 x  4096   64 x 64  9.5, 128 x 128 15.4           512 x 11008 x 4096   128 x 96 23.5, 256 x 128 25.5, 128 x 128 26.2
+//    201 x 11008 x  4096   128 x 96 15.6, 128 x 128 17.0, 64 x 64 19.0    1024 x 11008 x 4096   256 x 256 34.8, 128 x 128 40.9
 //     64 x  4096 x 14336   64 x 64 with K in four 12.7, in two 14.7, in eight 14.3
-// (A tile of 32 x 64 for 17 to 32 rows gains nothing for K of 4096, and has 12.4 us for 13.4 where K is 14336: not worth a kernel.)
+// 128 x 96 is for what would be 129 to 192 or 257 to 384 tiles of 128 x 128; with three or four chunks on their way it takes 16.2 us in the place of 15.6.
+// A tile of 32 x 64 for 17 to 32 rows gains nothing for K of 4096, and has 12.4 us for 13.4 where K is 14336: not worth a kernel.
 struct TileCost {
     int rows, cols;
     float one, two, ends;
 };
-constexpr TileCost kTiles[] = {{64, 64, 0.34f, 0.50f, 3.0f}, {128, 128, 0.78f, 1.40f, 3.0f}, {256, 128, 1.2f, 0.0f, 5.0f}, {256, 256, 1.7f, 0.0f, 8.0f}};
+constexpr TileCost kTiles[] = {{64, 64, 0.34f, 0.50f, 3.0f}, {128, 96, 0.70f, 1.14f, 3.0f}, {128, 128, 0.78f, 1.40f, 3.0f}, {256, 128, 1.2f, 0.0f, 5.0f}, {256, 256, 1.7f, 0.0f, 8.0f}};
 constexpr float kJoin = 3.0f, kJoinBytes = 6e-7f;     // for the launch that adds ranges up, and for a byte of their sums
 constexpr int kUnits = 256;
 
@@ -651,8 +652,9 @@ int product(Args g, const Plan &p, hipStream_t st)
     }
     g.splits = p.splits;
     const int rc = p.tile == 0   ? launch_tile<64, 64, 2, 2, 4, 3>(g, st)
-                   : p.tile == 1 ? launch_tile<128, 128, 2, 2, 2, 1>(g, st)
-                   : p.tile == 2 ? launch_tile<256, 128, 2, 2, 2, 2>(g, st)
+                   : p.tile == 1 ? launch_tile<128, 96, 4, 1, 2, 1>(g, st)
+                   : p.tile == 2 ? launch_tile<128, 128, 2, 2, 2, 1>(g, st)
+                   : p.tile == 3 ? launch_tile<256, 128, 2, 2, 2, 2>(g, st)
                                  : launch_tile<256, 256, 2, 2, 2, 2>(g, st);
     if (rc != VTL_HIP_OK || p.splits == 1)
         return rc;
