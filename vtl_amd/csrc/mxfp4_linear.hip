@@ -467,8 +467,9 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
 
     // Register k of a lane is row 8 (k / 4) + 4 half + k % 4 of a 32 x 32 tile, column r.  Four lanes exchange theirs (lane i gets row i of four
     // columns), so that a store is 16 bytes a lane and 8 whole lines.  An address is a uniform row and the lane's offset from it.  Results are not
-    // read again here: past the caches, but where all tiles are at work at once and store at the end (4096 x 4096 x 4096: 41.3 us, else 43.6; 8192 x 8192 x 8192
-    // 291 and 284).
+    // read again here.  Where all tiles are at work at once and store at the end, by way of the caches (4096 x 4096 x 4096: 41.3 us, else 43.6).  Else past them, and rows of 1024
+    // bytes at a time where a tile has them: what memory takes of a matrix that no cache holds depends on that (8192 x 8192 f32 in tiles of 256 x 256, nothing
+    // but stores: 8 rows of 128 bytes 76 us, 2 of 512 70, one of 1024 50; 4096 x 4096 11 each).  So 8192 x 8192 x 8192 takes 286 us for 295, 8192 x 28672 x 2048 368 for 396.
     const bool cached = g.cached;
     const bool whole = g.splits == 1;
     float *const out = (whole ? g.y : g.partials + (size_t)split * g.M * g.N) + (size_t)(m0 + wr * T::WM) * g.N + (n0 + wc * T::WN);
@@ -479,6 +480,44 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
     for (int j = 0; j < TN; j++)
         bias[j] = whole && g.bias && (!EDGE || n + 32 * j < g.N) ? g.bias[n + 32 * j] : 0.0f;
     const bool vectors = !EDGE || (g.N % 4 == 0 && !(reinterpret_cast<uintptr_t>(out) & 15));
+    if constexpr (BN == 256 && !EDGE) {
+        if (!cached) {
+            // Rows of the tile by way of shared memory, 32 of each wave at a time: 16-byte piece i of row m lies at place i ^ 4 (m % 4), so that neither writes
+            // of four rows nor reads of a whole one meet a bank twice.
+            constexpr int kRows = 32 * WR, kEach = kRows / NW;
+            static_assert(2 * kRows * BN * 4 <= T::kLds && kRows % NW == 0, "two turns' rows");
+            float *const rows = reinterpret_cast<float *>(smem);
+            const int turn = (r % 4) << 2;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                float *const at_i = rows + i % 2 * kRows * BN;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    float *const to = at_i + (32 * wr + 8 * k + 4 * half + r % 4) * BN;
+#pragma unroll
+                    for (int j = 0; j < TN; j++) {
+                        v4f v;
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            v[c] = finish(acc[i][j][4 * k + c], bias[j], floor);
+                        exchange(v);
+                        *reinterpret_cast<v4f *>(to + (((wc * T::WN + 32 * j) / 4 + r / 4) ^ turn) * 4) = v;
+                    }
+                    asm volatile("" ::: "memory");   // all results at once would be more registers than there are
+                }
+                __syncthreads();
+                const int n4 = n0 + 4 * lane;
+#pragma unroll 4
+                for (int k = 0; k < kEach; k++) {
+                    const int row = w * kEach + k, m = m0 + row / 32 * T::WM + 32 * i + row % 32;
+                    const v4f v = *reinterpret_cast<const v4f *>(at_i + row * BN + (lane ^ ((row % 4) << 2)) * 4);
+                    __builtin_nontemporal_store(v, reinterpret_cast<v4f *>(g.y + (size_t)m * g.N + n4));
+                }
+            }
+            return;
+        }
+    }
     if (vectors) {
         const unsigned mine = (unsigned)(4 * half + r % 4) * (unsigned)g.N + (unsigned)(r & ~3);
         const int n4 = n0 + wc * T::WN + (r & ~3);
