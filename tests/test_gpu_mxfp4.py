@@ -98,7 +98,10 @@ LINEARS = [(1, 1, 1), (1, 33, 31), (2, 64, 256), (3, 100, 1000), (5, 31, 4096), 
            (33, 64, 256), (64, 130, 520), (65, 65, 65), (100, 1024, 96), (128, 128, 2048), (129, 257, 777), (200, 640, 1300), (256, 256, 256),
            (300, 300, 8000), (513, 770, 256), (1000, 1100, 520), (40, 5000, 512), (2048, 70, 300), (1500, 1536, 512),
            (512, 512, 1024), (256, 768, 3584), (256, 256, 2048), (2560, 4096, 1024),
-           (256, 10752, 1024), (201, 9000, 2100), (66, 2886, 13742), (4096, 8192, 1024)]
+           (256, 10752, 1024), (201, 9000, 2100), (66, 2886, 13742), (4096, 8192, 1024),
+           (20, 6000, 1300), (64, 4100, 1100), (2, 9000, 2500), (3, 17000, 2500), (6, 6200, 4200), (7, 700, 3000), (90, 1000, 6000),
+           (1280, 256, 1024), (33, 4666, 64), (33, 4200, 4591), (65, 6064, 10917), (768, 4096, 1024), (263, 8702, 64), (66, 8581, 8726), (566, 10095, 2594),
+           (768, 11008, 1024), (1172, 10044, 261), (768, 8192, 4096)]
 
 
 def check_linear(got, want, far):

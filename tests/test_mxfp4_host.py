@@ -141,13 +141,18 @@ def _run(fake, program):
 
 
 def test_launches_of_products(fake_runtime):
-    """Few rows are one launch, f32 rows are made codes in it up to 8; tiles with K in ranges are joined by a launch of their own."""
+    """Up to 16 rows are one launch, f32 rows are made codes in it up to 8 (4 beside large weights); more are a launch of the same kernel or of tiles, and K in ranges is joined by a launch
+    of its own."""
     _run(fake_runtime, r"""
 for M in range(1, 17):
     for index, name in ((0, "vtl_hip_linear_mxfp4_f32"), (1, "vtl_hip_linear_f32_mxfp4")):
         args = (t.X,) if index else (t.CODES, t.SCALES)
         log = of(capi.status(name, *args, t.W, t.WS, None, t.Y, M, 4096, 4096, 0, BIG["ws"], BIG["ws_bytes"]))
         assert [l[0] for l in log] == ["quantize_mxfp4_kernel"] * (index and M > 8) + ["linear_few_mxfp4_kernel"], (M, log)
+        if index:
+            log = of(capi.status(name, t.X, t.W, t.WS, None, t.Y, M, 8192, 4096, 0, BIG["ws"], BIG["ws_bytes"]))
+            assert [l[0] for l in log] == ["quantize_mxfp4_kernel"] * (M > 4) + ["linear_few_mxfp4_kernel"], (M, log)
+            assert (capi.lib().vtl_hip_linear_f32_mxfp4_workspace(M, 8192, 4096) > 0) == (M > 4)
 def tile(M, N, K):
     st = capi.status("vtl_hip_linear_mxfp4_f32", t.CODES, t.SCALES, t.W, t.WS, None, t.Y, M, N, K, 0, BIG["ws"], BIG["ws_bytes"])
     return of(st)
@@ -157,6 +162,10 @@ for M in (17, 40, 100, 201, 256, 512, 1024, 4096):
         for K in (0, 1, 256, 4096, 11008, 14336):
             log = tile(M, N, K)
             bm, bn = log[0][2][:2]
+            if log[0][0] == "linear_few_mxfp4_kernel":
+                assert bn == 8 and len(log) == 1 and log[0][1] == -(-N // (16 * bm)) * -(-M // 32), (M, N, K, log)
+                tiles.add((32, 16 * bm))
+                continue
             tiles.add((bm, bn))
             whole = -(-M // bm) * -(-N // bn)
             assert log[0][0] == "linear_tile_mxfp4_kernel" and log[0][1] % whole == 0, (M, N, K, log)
@@ -164,7 +173,7 @@ for M in (17, 40, 100, 201, 256, 512, 1024, 4096):
             assert [l[0] for l in log[1:]] == ["linear_join_mxfp4_kernel"] * (splits > 1), (M, N, K, log)
             need = capi.lib().vtl_hip_linear_mxfp4_workspace(M, N, K)
             assert need >= (4 * splits * M * N if splits > 1 else 0) and splits * 4 <= max(4, -(-K // 256)), (M, N, K, splits)
-assert tiles == {(64, 64), (128, 96), (128, 128), (256, 128), (256, 256)}, tiles
+assert tiles == {(32, 16), (32, 32), (64, 64), (128, 96), (128, 128), (256, 128), (256, 256)}, tiles
 print("done")
 """)
 
@@ -181,7 +190,7 @@ for M, N in ((1, most_n), (8, most_n), (16, most_n), (17, most_n), (33, most_n),
     else:
         assert st == capi.OK, (M, N, st)
     for name, blocks, sizes in log:
-        assert blocks * (512 if "few" in name else 256) < 1 << 32, (M, N, log)
+        assert blocks * 256 < 1 << 32, (M, N, log)
 print("done")
 """)
 

@@ -34,24 +34,28 @@ __device__ __forceinline__ float floor_of(int relu) { return relu ? 0.0f : -__bu
 
 // ---- few rows ------------------------------------------------------------------------------
 
-// A workgroup has 16 FR rows of weights and all of x, up to 4 MX rows; its waves deal the units of K out among them, each with two slots of shared memory
+// A workgroup has 16 FR rows of weights and 4 MX rows of x; its waves deal the units of K out among them, each with two slots of shared memory
 // that its own loads fill, and their sums meet in order.  The product's first operand is the weights, so a lane has four results of one row of x side by side.
 // XF32: x is f32, and each wave makes the codes of its units itself.
-constexpr int kFewWaves = 8, kFewMost = 16;
+// Bound by the weights' way from memory: one row and 28672 x 8192 weights 19.0 us, 6.6 TB/s (eight waves a workgroup, and with them one workgroup a compute unit, 24.3);
+// 14336 x 4096 7.0, 4.5 TB/s: it begins and ends.  From 17 rows on bound by x's way into shared memory too, four or eight times that of the weights: 32 rows and
+// 4096 x 4096 4.2 us (one row 3.1), 4096 x 14336 9.4 (7.1).
+constexpr int kFewMost = 16;     // rows up to which there is no other way
 
 template <int FR, int MX, bool XF32>
 struct Few {
     using W = Stream<FR>;
-    static constexpr int kXBytes = 4 * MX * (kUnit / 2) + 256;                      // rows of codes, then the scales of 16
-    static constexpr int kSlot = W::kSlot + kXBytes, kLoads = W::kLoads + (XF32 ? 0 : MX + 1);
+    static constexpr int kTiles = (MX + 3) / 4;                                     // of 16 columns
+    static constexpr int kXBytes = 4 * MX * (kUnit / 2) + 256 * kTiles;             // rows of codes, then scales of whole tiles
+    static constexpr int kSlot = W::kSlot + kXBytes, kLoads = W::kLoads + (XF32 ? 0 : MX + kTiles);
     static constexpr int kPart = 16 * FR + 4;                                       // floats of a row of sums
-    static_assert(MX <= 4, "one product's columns");
+    static_assert(MX <= 4 || MX % 4 == 0, "whole tiles");
 };
 
-// Row m of x in a slot: codes like a row of weights (piece i at place i ^ m), scales behind all of them.
+// Row m of x in a slot: codes like a row of weights (piece i at place i ^ m % 16), scales behind all of them.
 template <int MX>
 struct XRows {
-    static constexpr int kScalesAt = 4 * MX * (kUnit / 2);
+    static constexpr int kScalesAt = 4 * MX * (kUnit / 2), kTiles = (MX + 3) / 4;
     v4f v[4 * MX][2];       // a lane's eight values of f32 rows; four lanes are a block
 
     __device__ __forceinline__ static void issue(const Args &g, int unit, char *x, unsigned pitch, unsigned spitch)
@@ -60,11 +64,13 @@ struct XRows {
 #pragma unroll
         for (int j = 0; j < MX; j++) {
             const int row = 4 * j + lane / 16;
-            const unsigned in_row = min((unsigned)unit * (kUnit / 2) + (unsigned)((lane % 16) ^ row) * 16u, pitch - 16u);
+            const unsigned in_row = min((unsigned)unit * (kUnit / 2) + (unsigned)((lane % 16) ^ (row % 16)) * 16u, pitch - 16u);
             __builtin_amdgcn_global_load_lds(VTL_GPTR(g.a.codes + ((size_t)min(row, g.M - 1) * pitch + in_row)), VTL_LPTR(x + j * 1024), 16, 0, 0);
         }
         const unsigned in_row = min((unsigned)unit * (kUnit / kBlock) + (unsigned)(lane % 4) * 4u, spitch - 4u);
-        __builtin_amdgcn_global_load_lds(VTL_GPTR(g.a.scales + ((size_t)min(lane / 4, g.M - 1) * spitch + in_row)), VTL_LPTR(x + kScalesAt), 4, 0, 0);
+#pragma unroll
+        for (int j = 0; j < kTiles; j++)
+            __builtin_amdgcn_global_load_lds(VTL_GPTR(g.a.scales + ((size_t)min(16 * j + lane / 4, g.M - 1) * spitch + in_row)), VTL_LPTR(x + kScalesAt + 256 * j), 4, 0, 0);
     }
     template <bool VEC>
     __device__ __forceinline__ void load(const Args &g, int unit)
@@ -112,15 +118,22 @@ struct XRows {
     }
 };
 
-template <int FR, int MX, bool XF32, bool VEC>
-__global__ __launch_bounds__(64 * kFewWaves) void linear_few_mxfp4_kernel(const Args g)
+template <int FR, int MX, bool XF32, bool VEC, int NW>
+__global__ __launch_bounds__(64 * NW) void linear_few_mxfp4_kernel(Args g)
 {
     using F = Few<FR, MX, XF32>;
     using W = typename F::W;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
-    const int n0 = (int)blockIdx.x * 16 * FR;
-    const int units = (g.chunks + 1) / 2, begin = (int)((int64_t)units * w / kFewWaves), end = (int)((int64_t)units * (w + 1) / kFewWaves);
+    const int blocks = (g.N + 16 * FR - 1) / (16 * FR), n0 = (int)blockIdx.x % blocks * 16 * FR;
+    if constexpr (MX == 8) {        // more rows than these: blocks of them
+        const int m0 = (int)blockIdx.x / blocks * 4 * MX;
+        g.a.codes += (size_t)m0 * g.chunks * kChunkCodes;
+        g.a.scales += (size_t)m0 * g.chunks * kChunkScales;
+        g.y += (size_t)m0 * g.N;
+        g.M = min(g.M - m0, 4 * MX);
+    }
+    const int units = (g.chunks + 1) / 2, begin = (int)((int64_t)units * w / NW), end = (int)((int64_t)units * (w + 1) / NW);
     char *const ring = smem + w * g.slots * F::kSlot;
     W weights;
 #pragma unroll
@@ -136,10 +149,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_mxfp4_kernel(const 
         if constexpr (!XF32)
             rows.issue(g, u, slot + W::kSlot, weights.pitch, weights.spitch);
     };
-    v4f acc[FR];
+    v4f acc[FR][F::kTiles];
 #pragma unroll
     for (int i = 0; i < FR; i++)
-        acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < F::kTiles; j++)
+            acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (begin < end)
         issue(begin);
     const int m = r % (4 * MX);      // (columns of no row repeat others)
@@ -158,33 +173,45 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_mxfp4_kernel(const 
 #pragma unroll
         for (int i = 0; i < FR; i++)
             sw[i] = W::all_scales(slot, i);
-        const v4i sx = *reinterpret_cast<const v4i *>(x + XRows<MX>::kScalesAt + m * 16);
+        v4i sx[F::kTiles];
+#pragma unroll
+        for (int j = 0; j < F::kTiles; j++)
+            sx[j] = *reinterpret_cast<const v4i *>(x + XRows<MX>::kScalesAt + (16 * j + m) * 16);
 #pragma unroll
         for (int s = 0; s < kUnitSteps; s++)
             if (s < 2 || two) {
-                const v4i cx = *reinterpret_cast<const v4i *>(x + m * (kUnit / 2) + (((4 * s + q) ^ m) << 4));
+                v4i cw[FR];
 #pragma unroll
                 for (int i = 0; i < FR; i++)
-                    acc[i] = mfma_16(W::operand(slot, i, s), cx, acc[i], sw[i][s], (int)((unsigned)sx[s] >> (8 * q)));
+                    cw[i] = W::operand(slot, i, s);
+#pragma unroll
+                for (int j = 0; j < F::kTiles; j++) {
+                    const v4i cx = *reinterpret_cast<const v4i *>(x + (16 * j + m) * (kUnit / 2) + (((4 * s + q) ^ m) << 4));
+#pragma unroll
+                    for (int i = 0; i < FR; i++)
+                        acc[i][j] = mfma_16(cw[i], cx, acc[i][j], sw[i][s], (int)((unsigned)sx[j][s] >> (8 * q)));
+                }
             }
         W::done_reading();
     }
     __syncthreads();        // every wave is done with its slots
     float *const part = reinterpret_cast<float *>(smem);     // [waves][4 MX][kPart]
 #pragma unroll
-    for (int i = 0; i < FR; i++) {
-        settle(acc[i]);
-        if (r < 4 * MX)
-            *reinterpret_cast<v4f *>(part + (w * 4 * MX + r) * F::kPart + 16 * i + 4 * q) = acc[i];
-    }
+    for (int i = 0; i < FR; i++)
+#pragma unroll
+        for (int j = 0; j < F::kTiles; j++) {
+            settle(acc[i][j]);
+            if (r < 4 * MX)
+                *reinterpret_cast<v4f *>(part + (w * 4 * MX + 16 * j + r) * F::kPart + 16 * i + 4 * q) = acc[i][j];
+        }
     __syncthreads();
-    for (int item = (int)threadIdx.x; item < 4 * MX * 16 * FR; item += 64 * kFewWaves) {
+    for (int item = (int)threadIdx.x; item < 4 * MX * 16 * FR; item += 64 * NW) {
         const int row = item / (16 * FR), nl = item % (16 * FR), n = n0 + nl;
         if (row >= g.M || n >= g.N)
             continue;
         float v = part[row * F::kPart + nl];
 #pragma unroll
-        for (int i = 1; i < kFewWaves; i++)
+        for (int i = 1; i < NW; i++)
             v += part[(i * 4 * MX + row) * F::kPart + nl];
         g.y[(int64_t)row * g.N + n] = finish(v, g.bias ? g.bias[n] : 0.0f, floor_of(g.relu));
     }
@@ -598,13 +625,13 @@ int launch_tile(Args g, hipStream_t st)
     return check_launch("linear_tile_mxfp4_kernel");
 }
 
-template <int FR, int MX, bool XF32, bool VEC>
+template <int FR, int MX, bool XF32, bool VEC, int NW>
 int launch_few(Args g, hipStream_t st)
 {
     using F = Few<FR, MX, XF32>;
-    constexpr int kMostLds = kFewWaves * 2 * F::kSlot;
-    static_assert(kMostLds <= 160 << 10 && kFewWaves * 4 * MX * F::kPart * 4 <= kMostLds / 2, "shared memory of a compute unit, and sums fit where operands were");
-    const auto kernel = linear_few_mxfp4_kernel<FR, MX, XF32, VEC>;
+    constexpr int kMostLds = NW * 2 * F::kSlot;
+    static_assert(kMostLds <= 160 << 10 && NW * 4 * MX * F::kPart * 4 <= kMostLds / 2, "shared memory of a compute unit, and sums fit where operands were");
+    const auto kernel = linear_few_mxfp4_kernel<FR, MX, XF32, VEC, NW>;
     static PerDevice<DoneFlag> flags;
     DoneFlag &done = flags.get();
     if (!done.load(std::memory_order_acquire)) {
@@ -612,9 +639,20 @@ int launch_few(Args g, hipStream_t st)
         done.store(true, std::memory_order_release);
     }
     const int units = (g.chunks + 1) / 2;
-    g.slots = units <= kFewWaves ? 1 : 2;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((g.N + 16 * FR - 1) / (16 * FR))), dim3(64 * kFewWaves), kFewWaves * g.slots * F::kSlot, st, g);
+    g.slots = units <= NW ? 1 : 2;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((g.N + 16 * FR - 1) / (16 * FR) * ((g.M + 4 * MX - 1) / (4 * MX)))), dim3(64 * NW), NW * g.slots * F::kSlot, st, g);
     return check_launch("linear_few_mxfp4_kernel");
+}
+
+// Four waves; eight where they make codes of f32 rows, have a unit each and are not begun again and again: one row and 14336 x 4096 weights 7.0 us, with four 7.7;
+// 4096 x 14336 9.1 and 10.5; but 28672 x 8192 26.4 and 22.0, 8192 x 2048 4.1 and 3.7.
+template <int FR, int MX, bool XF32, bool VEC>
+int launch_few(const Args &g, hipStream_t st)
+{
+    if constexpr (XF32)
+        if (g.chunks > 8 && g.N <= 16 * FR * 512)
+            return launch_few<FR, MX, XF32, VEC, 8>(g, st);
+    return launch_few<FR, MX, XF32, VEC, 4>(g, st);
 }
 
 template <int MX, bool XF32, bool VEC>
@@ -629,6 +667,7 @@ int launch_few(const Args &g, hipStream_t st)
 // How a product is made: by the kernel for few rows, which may make their codes itself, or by tiles, with K in so many ranges.
 struct Plan {
     bool few, codes;
+    int fragments;     // of weights in a workgroup, for more rows than kFewMost
     int tile, splits;
     size_t partials;   // bytes
 };
@@ -648,14 +687,32 @@ struct TileCost {
 constexpr TileCost kTiles[] = {{64, 64, 0.34f, 0.50f, 3.0f}, {128, 96, 0.70f, 1.14f, 3.0f}, {128, 128, 0.78f, 1.40f, 3.0f}, {256, 128, 1.2f, 0.0f, 5.0f}, {256, 256, 1.7f, 0.0f, 8.0f}};
 constexpr float kJoin = 3.0f, kJoinBytes = 6e-7f;     // for the launch that adds ranges up, and for a byte of their sums
 constexpr int kUnits = 256;
+// The same of the kernel for few rows, 32 of them and 16 or 32 columns in a workgroup, one of which fills a compute unit; and what the launch takes.  It has all of a
+// K within a workgroup, and wins where there is little else to deal out, us: 17 to 32 rows x 4096 x 4096 4.2 (64 x 64 8.5), x 14336 9.4 (13.4), 28672 columns of 8192 26 (21.7);
+// 64 rows x 4096 x 4096 5.5 (8.9), x 8192 columns of 4096 9.6 (9.4); 128 rows x 1024 x 4096 4.1 (8.7), x 4096 x 4096 9.5 (9.3).
+constexpr TileCost kFewTiles[] = {{32, 16, 0.11f, 0.0f, 0.84f}, {32, 32, 0.18f, 0.0f, 1.0f}};
+constexpr float kFewLaunch = 1.6f;
 
 Plan plan_of(int M, int N, int K)
 {
-    Plan p{M <= kFewMost, M > 8, 0, 1, 0};
+    // Every workgroup makes the codes of all rows: 8 rows and 4096 x 4096 weights 4.9 us, with a launch for the codes 6.0; 11008 x 4096 9.6 and 8.9, 28672 x 8192
+    // 35 and 22; four rows are level at worst.
+    const bool codes = M > 8 || (M > 4 && (int64_t)N * K > 6144 * 4096);
+    Plan p{M <= kFewMost, codes, 0, 0, 1, 0};
     if (p.few)
         return p;
     const int chunks = chunks_of(K);
     float best = 0.0f;
+    for (int f = 0; f < 2; f++) {
+        const TileCost &c = kFewTiles[f];
+        const int64_t tiles = (((int64_t)M + c.rows - 1) / c.rows) * (((int64_t)N + c.cols - 1) / c.cols);
+        const float cost = kFewLaunch + (float)((tiles + kUnits - 1) / kUnits) * ((float)chunks * c.one + c.ends);
+        if (f == 0 || cost < best) {
+            best = cost;
+            p.few = true;
+            p.fragments = f + 1;
+        }
+    }
     for (int t = 0; t < (int)(sizeof(kTiles) / sizeof(kTiles[0])); t++) {
         const TileCost &c = kTiles[t];
         const int64_t tiles = (((int64_t)M + c.rows - 1) / c.rows) * (((int64_t)N + c.cols - 1) / c.cols);
@@ -667,8 +724,9 @@ Plan plan_of(int M, int N, int K)
             const size_t bytes = splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0;
             const float cost = (float)((all + at_once - 1) / at_once) * ((float)((chunks + splits - 1) / splits) * chunk + c.ends) +
                                (splits > 1 ? kJoin + kJoinBytes * (float)bytes : 0.0f);
-            if (best == 0.0f || cost < best) {
+            if (cost < best) {
                 best = cost;
+                p.few = false;
                 p.tile = t;
                 p.splits = splits;
                 p.partials = bytes;
@@ -687,7 +745,10 @@ int product(Args g, const Plan &p, hipStream_t st)
                 return vec ? launch_few<1, true, true>(g, st) : launch_few<1, true, false>(g, st);
             return vec ? launch_few<2, true, true>(g, st) : launch_few<2, true, false>(g, st);
         }
-        return g.M <= 4 ? launch_few<1, false, true>(g, st) : g.M <= 8 ? launch_few<2, false, true>(g, st) : launch_few<4, false, true>(g, st);
+        return g.M <= 4    ? launch_few<1, false, true>(g, st)
+               : g.M <= 8  ? launch_few<2, false, true>(g, st)
+               : g.M <= kFewMost ? launch_few<4, false, true>(g, st)
+               : p.fragments == 1 ? launch_few<1, 8, false, true>(g, st) : launch_few<2, 8, false, true>(g, st);
     }
     g.splits = p.splits;
     const int rc = p.tile == 0   ? launch_tile<64, 64, 2, 2, 4, 3>(g, st)
