@@ -47,6 +47,7 @@ struct Args {
     uint8_t *h_digits, *h_scales;           // the same of each pair's hidden values
     float *parts;                           // [splits, tokens, dim] where several workgroups share rows of the output
     int splits;
+    int many, dense;                        // how the products are launched
 };
 
 __device__ __forceinline__ v4f mfma_digits(v4i w, v8i d, v4f c, int sw, int sd)
@@ -465,24 +466,30 @@ struct Held {
     }
 };
 
-// 16 RW hidden values of an expert's tokens: RW times 16 rows of its gate and as many of its up, KW waves each, which deal K out among them.
+// 16 RW FH hidden values of an expert's tokens: RW times 16 FH rows of its gate and as many of its up, KW waves each, which deal K out among them.
 // The values go out as digits, already times their weights, so that the next product adds experts up as it adds up K.
-// One wave along K where that gives every compute unit eight, else four.  For 24 tokens of 128 experts of 2048 x 1024, us (their weights alone take 41):
+// Bound by the weights; from some pairs of an expert on by the digits, which every wave asks for by itself: five bytes of a pair for half a byte of each row.
+// One wave along K where that gives 640 workgroups or more, else two (whole calls, us, with one / two / four waves: 1 token, 6 of 64 experts of 4096 x 1024 20.3 / 19.4 / 19.5;
+// 1 token, 2 of 8 of 4096 x 7168 25.7 / 25.7 / 29.4; 8 tokens, 2 of 8 of 2048 x 3584, 806 workgroups, 32.9 / 34.5 / 39.7; 4 tokens, 8 of 256 of 4096 x 1024 56 / 57 / 62, and
+// 67 to 74 with the plan made in every workgroup).  For 24 tokens of 128 experts of 2048 x 1024, us (their weights alone take 41):
 //   waves along K (32 values a workgroup)       1: 45.4     2: 51.4     4: 72.8
 //   64 values, 128                              46.1, 54.4; two waves along K and 64 values 58.1
 //   one tile (three tokens a pass)              48.0 with one wave along K, 51.9 with two
 // Also measured: a workgroup for each compute unit that goes through a run of (expert, 32 values) with the next one's weights on their way 51.8, waves that
 // do so by themselves 60.
+// FH 2 and four tiles where an expert has four pairs or more by chance (whole calls of 8 experts of 4096 x 7168, 2 a token, us: 16 tokens 105 for 114, 32 125 for 160,
+// 64 221 for 254; 64 tokens and 6 of 64 of 2048 x 1408 110 for 125; but 24 tokens and 8 of 128 95 for 86).  Digits by way of shared memory for four
+// waves with all pairs' sums in registers were no faster but for 36 pairs of an expert: one wave a SIMD, which waits for its own reads.
 // EACH: every workgroup makes the plan for itself (a few tokens: less than a launch takes); 0: it is there.
-template <int TILES, int RW, int KW, int EACH>
+template <int TILES, int RW, int KW, int EACH, int FH = 1>
 __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 {
-    constexpr int NW = RW * KW, kRows = 16 * RW, kPairs = TILES * kTokensATile;
-    using S = Stream<2>;
-    static_assert(RW % 2 == 0, "whole blocks of hidden values");
+    constexpr int NW = RW * KW, kRows = 16 * RW * FH, kPairs = TILES * kTokensATile;
+    using S = Stream<2 * FH>;
+    static_assert(RW * FH % 2 == 0, "whole blocks of hidden values");
     static_assert(64 * NW % (kRows / 4) == 0, "a thread's values are the same of every pair");
     extern __shared__ __attribute__((aligned(16))) char smem[];   // two slots a wave
-    __shared__ __attribute__((aligned(16))) float part[NW][kPairs][36];
+    __shared__ __attribute__((aligned(16))) float part[NW * FH][kPairs][36];
     const int tiles = g.hidden_units * (kUnit / kRows), a = (int)blockIdx.x / tiles, row0 = (int)blockIdx.x % tiles * kRows;
     const Entry *entries = g.plan->entry;
     const int *tokens = g.plan->token, *count = &g.plan->count;
@@ -505,12 +512,14 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
     const int e = __builtin_amdgcn_readfirstlane(entry.expert), offset = __builtin_amdgcn_readfirstlane(entry.offset), n = __builtin_amdgcn_readfirstlane(entry.pairs);
     char *const ring = smem + w * (2 * S::kSlot);
     const int begin = g.dim_units * (w % KW) / KW, end = g.dim_units * (w % KW + 1) / KW;
-    const int my_row = row0 + w / KW * 16;
+    const int my_row = row0 + w / KW * 16 * FH;
     S stream;
     if (my_row < g.hidden) {
 #pragma unroll
-        for (int f = 0; f < 2; f++)
-            stream.rows(f, g.gate_up, ((size_t)e * 2 + f) * g.hidden + my_row, min(16, g.hidden - my_row), g.dim_chunks);
+        for (int f = 0; f < 2 * FH; f++) {
+            const int row_f = min(my_row + f / 2 * 16, g.hidden - 1);
+            stream.rows(f, g.gate_up, ((size_t)e * 2 + f % 2) * g.hidden + row_f, min(16, g.hidden - row_f), g.dim_chunks);
+        }
     }
     // A thread's four of the hidden values below, whatever the pair: their biases are asked for in front of the weights.
     const int row = (int)threadIdx.x % (kRows / 4) * 4;
@@ -531,23 +540,29 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
                 stream.issue(begin, ring);
             Columns<TILES> x;
             x.at(g.x_digits, g.x_scales, g.dim_units, tokens, offset + first, now);
-            v4f acc[2][TILES];
+            v4f acc[2 * FH][TILES];
 #pragma unroll
-            for (int f = 0; f < 2; f++)
+            for (int f = 0; f < 2 * FH; f++)
 #pragma unroll
                 for (int i = 0; i < TILES; i++)
                     acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             const auto work = [&](const char *slot) {
-                const v4i scales[2] = {S::all_scales(slot, 0), S::all_scales(slot, 1)};
+                v4i scales[2 * FH];
+#pragma unroll
+                for (int f = 0; f < 2 * FH; f++)
+                    scales[f] = S::all_scales(slot, f);
 #pragma unroll
                 for (int k = 0; k < kUnitSteps; k++) {
-                    const v4i codes[2] = {S::operand(slot, 0, k), S::operand(slot, 1, k)};
+                    v4i codes[2 * FH];
+#pragma unroll
+                    for (int f = 0; f < 2 * FH; f++)
+                        codes[f] = S::operand(slot, f, k);
 #pragma unroll
                     for (int i = 0; i < TILES; i++)
                         if (i * kTokensATile < now) {
                             const int xb = x.scale(i, k);
 #pragma unroll
-                            for (int f = 0; f < 2; f++)
+                            for (int f = 0; f < 2 * FH; f++)
                                 acc[f][i] = mfma_digits(codes[f], x.d[i][k], acc[f][i], scales[f][k], xb);
                         }
                 }
@@ -568,14 +583,14 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 #pragma unroll
             for (int i = 0; i < TILES; i++)
 #pragma unroll
-                for (int f = 0; f < 2; f++) {
+                for (int f = 0; f < 2 * FH; f++) {
                     settle(acc[f][i]);
                     v4f v;
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                         v[k] = sum_digits(acc[f][i][k]);
                     if (r % kDigits == 0 && r < 15)
-                        *reinterpret_cast<v4f *>(&part[w][i * kTokensATile + r / kDigits][16 * f + 4 * q]) = v;
+                        *reinterpret_cast<v4f *>(&part[w + f / 2 * NW][i * kTokensATile + r / kDigits][16 * (f % 2) + 4 * q]) = v;
                 }
         }
         __syncthreads();
@@ -583,7 +598,7 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
             const int i = item / (kRows / 4), pair = offset + first + i;
             v4f h = {0.0f, 0.0f, 0.0f, 0.0f};
             if (row0 + row < g.hidden) {
-                const float(*const mine)[kPairs][36] = &part[row / 16 * KW];
+                const float(*const mine)[kPairs][36] = &part[row / (16 * FH) * KW + row / 16 % FH * NW];
                 v4f gate = *reinterpret_cast<const v4f *>(&mine[0][i][row % 16]), up = *reinterpret_cast<const v4f *>(&mine[0][i][16 + row % 16]);
 #pragma unroll
                 for (int j = 1; j < KW; j++) {
@@ -604,35 +619,38 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
     }
 }
 
-// 16 output values of all tokens: the units of all chosen experts, one expert's behind the other's, are dealt out among the waves of `splits`
+// 16 F output values of all tokens: the units of all chosen experts, one expert's behind the other's, are dealt out among the waves of `splits`
 // workgroups.  A wave adds what an expert gives to its own sums of the tokens, and the waves' sums meet in order.
-// Bound by the weights, and by the hidden values' digits, five bytes of each pair for half a byte of weights: 24 tokens of 128 experts of 2048 x 1024 27.5 us, 4.1 TB/s
+// Bound by the weights, and by the hidden values' digits as above: 24 tokens of 128 experts of 2048 x 1024 27.5 us, 4.1 TB/s
 // (24.8 without the digits; four waves a workgroup and twice as many workgroups 27.9, sixteen waves a compute unit 32.6); one token, 6 of 4096 x 1024 6.4.
-constexpr int kProductWaves = 8;
-
-template <int TILES>
-__global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args g)
+template <int TILES, int F, int NW>
+__global__ __launch_bounds__(64 * NW) void moe_down_kernel(const Args g)
 {
-    using S = Stream<1>;
-    constexpr int kSlots = 3, kPairs = TILES * kTokensATile;
+    using S = Stream<F>;
+    constexpr int kSlots = 3, kPairs = TILES * kTokensATile, kRows = 16 * F;
     extern __shared__ __attribute__((aligned(16))) char smem[];    // three slots a wave
-    float *const sums = reinterpret_cast<float *>(smem + kProductWaves * kSlots * S::kSlot);   // [waves, tokens, 16]
+    float *const sums = reinterpret_cast<float *>(smem + NW * kSlots * S::kSlot);   // [waves, tokens, kRows]
     const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r = lane % 16, q = lane / 16;
     __shared__ Held held;
     held.copy(g);
     const Plan &plan = held.plan;
-    const int split = (int)blockIdx.x % g.splits, row0 = (int)blockIdx.x / g.splits * 16;
+    const int split = (int)blockIdx.x % g.splits, row0 = (int)blockIdx.x / g.splits * kRows;
     const int units = g.hidden_units, all = __builtin_amdgcn_readfirstlane(plan.count) * units;
-    const int share = split * kProductWaves + w, shares = g.splits * kProductWaves;
+    const int share = split * NW + w, shares = g.splits * NW;
     const int begin = (int)((int64_t)all * share / shares), end = (int)((int64_t)all * (share + 1) / shares);
     char *const ring = smem + w * (kSlots * S::kSlot);
-    float *const mine = sums + (size_t)w * g.tokens * 16;
+    float *const mine = sums + (size_t)w * g.tokens * kRows;
     S stream;
     int streamed = -1;      // whose rows it has
     const auto issue = [&](int u) {
         const int a = u / units;
         if (a != streamed) {
-            stream.rows(0, g.down, (size_t)__builtin_amdgcn_readfirstlane(plan.entry[a].expert) * g.dim + row0, min(16, g.dim - row0), g.hidden_chunks);
+            const size_t expert = (size_t)__builtin_amdgcn_readfirstlane(plan.entry[a].expert) * g.dim;
+#pragma unroll
+            for (int f = 0; f < F; f++) {
+                const int row = min(row0 + 16 * f, g.dim - 1);
+                stream.rows(f, g.down, expert + row, min(16, g.dim - row), g.hidden_chunks);
+            }
             streamed = a;
         }
         stream.issue(u - a * units, ring + (u - begin) % kSlots * S::kSlot);
@@ -642,56 +660,77 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
         issue(begin);
     if (begin + 1 < end)
         issue(begin + 1);
-    for (int i = lane; i < g.tokens * 16; i += kWave)
+    for (int i = lane; i < g.tokens * kRows; i += kWave)
         mine[i] = 0.0f;
     for (int u = begin; u < end;) {
         const int a = u / units, stop = min(end, (a + 1) * units);
         const Entry entry = plan.entry[a];
         const int offset = __builtin_amdgcn_readfirstlane(entry.offset), pairs = __builtin_amdgcn_readfirstlane(entry.pairs);
         // The wave that has an expert's first unit adds its bias, in the lanes that have a pair's sums.
-        v4f bias = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (g.down_bias && u == a * units)
+        v4f bias[F];
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (row0 + 4 * q + k < g.dim)
-                    bias[k] = g.down_bias[(size_t)entry.expert * g.dim + row0 + 4 * q + k];
-        Columns<TILES> h;
-        v4f acc[TILES];
-        const auto multiply = [&](const char *slot, const v4i scales, int now) {
-#pragma unroll
-            for (int k = 0; k < kUnitSteps; k++) {
-                const v4i codes = S::operand(slot, 0, k);
-#pragma unroll
-                for (int i = 0; i < TILES; i++)
-                    if (i * kTokensATile < now)
-                        acc[i] = mfma_digits(codes, h.d[i][k], acc[i], scales[k], h.scale(i, k));
-            }
-        };
-        const auto add = [&](int first, int now) {
-#pragma unroll
-            for (int i = 0; i < TILES; i++) {
-                settle(acc[i]);
-                v4f v;
+        for (int f = 0; f < F; f++) {
+            bias[f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            if (g.down_bias && u == a * units)
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    v[k] = sum_digits(acc[i][k]);
-                const int pair = i * kTokensATile + r / kDigits;
-                if (r % kDigits == 0 && r < 15 && pair < now) {
-                    const float weight = plan.weight[offset + first + pair];
-                    v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)plan.token[offset + first + pair] * 16 + 4 * q), sum = *to;
+                    if (row0 + 16 * f + 4 * q + k < g.dim)
+                        bias[f][k] = g.down_bias[(size_t)entry.expert * g.dim + row0 + 16 * f + 4 * q + k];
+        }
+        Columns<TILES> h;
+        v4f acc[F][TILES];
+        const auto multiply = [&](const char *slot, const v4i (&scales)[F], int now) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        (*to)[k] = sum[k] + fmaf(weight, bias[k], v[k]);
-                }
-                acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k = 0; k < kUnitSteps; k++) {
+                v4i codes[F];
+#pragma unroll
+                for (int f = 0; f < F; f++)
+                    codes[f] = S::operand(slot, f, k);
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+                    if (i * kTokensATile < now) {
+                        const int hb = h.scale(i, k);
+#pragma unroll
+                        for (int f = 0; f < F; f++)
+                            acc[f][i] = mfma_digits(codes[f], h.d[i][k], acc[f][i], scales[f][k], hb);
+                    }
             }
         };
+        const auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < TILES; i++)
-            acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int f = 0; f < F; f++)
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+                    acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        };
+        const auto add = [&](int first, int now) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < TILES; i++)
+#pragma unroll
+                for (int f = 0; f < F; f++) {
+                    settle(acc[f][i]);
+                    v4f v;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        v[k] = sum_digits(acc[f][i][k]);
+                    const int pair = i * kTokensATile + r / kDigits;
+                    if (r % kDigits == 0 && r < 15 && pair < now) {
+                        const float weight = plan.weight[offset + first + pair];
+                        v4f *const to = reinterpret_cast<v4f *>(mine + (size_t)plan.token[offset + first + pair] * kRows + 16 * f + 4 * q), sum = *to;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            (*to)[k] = sum[k] + fmaf(weight, bias[f][k], v[k]);
+                    }
+                }
+            clear();
+        };
+        clear();
         h.at(g.h_digits, g.h_scales, units, nullptr, offset, min(pairs, kPairs));
         const auto work = [&](const char *slot, int in_row) {
-            const v4i scales = S::all_scales(slot, 0);
+            v4i scales[F];
+#pragma unroll
+            for (int f = 0; f < F; f++)
+                scales[f] = S::all_scales(slot, f);
             multiply(slot, scales, min(pairs, kPairs));
             if (pairs > kPairs) {       // more than fit: unit by unit
                 add(0, kPairs);
@@ -702,7 +741,9 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
                     add(first, min(pairs - first, kPairs));
                 }
                 h.at(g.h_digits, g.h_scales, units, nullptr, offset, kPairs);
-                bias = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int f = 0; f < F; f++)
+                    bias[f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             }
             S::done_reading();
         };
@@ -722,14 +763,14 @@ __global__ __launch_bounds__(64 * kProductWaves) void moe_down_kernel(const Args
             add(0, pairs);
     }
     __syncthreads();
-    for (int i = (int)threadIdx.x; i < g.tokens * 16; i += 64 * kProductWaves) {
-        const int t = i / 16, row = row0 + i % 16;
+    for (int i = (int)threadIdx.x; i < g.tokens * kRows; i += 64 * NW) {
+        const int t = i / kRows, row = row0 + i % kRows;
         if (row >= g.dim)
             continue;
         float v = sums[i];
 #pragma unroll
-        for (int j = 1; j < kProductWaves; j++)
-            v += sums[(size_t)j * g.tokens * 16 + i];
+        for (int j = 1; j < NW; j++)
+            v += sums[(size_t)j * g.tokens * kRows + i];
         if (g.splits > 1) {
             g.parts[((size_t)split * g.tokens + t) * g.dim + row] = v;
             continue;
@@ -752,24 +793,38 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const Args g)
 
 // ---- host -----------------------------------------------------------------------------------
 
+// Pairs of an expert, if tokens choose by chance, from which on waves have twice the weights, so that digits are asked for half as often.
+constexpr double kDenseFrom = 4.0;
+
 // The kernels with more shared memory than a launch has unasked.
-template <void (*KERNEL)(const Args)>
+template <void (*KERNEL)(const Args), int MOST>
 int launch_with_lds(unsigned blocks, int threads, int lds, hipStream_t st, const Args &g)
 {
     static PerDevice<DoneFlag> flags;
     DoneFlag &done = flags.get();
     if (!done.load(std::memory_order_acquire)) {
-        VTL_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 136 << 10));
+        VTL_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, MOST));
         done.store(true, std::memory_order_release);
     }
     hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3((unsigned)threads), (unsigned)lds, st, g);
     return check_launch("moe_mxfp4 product");
 }
 
-template <int TILES, int KW, int EACH>
+template <int TILES, int KW, int EACH, int RW = 2, int FH = 1>
 int launch_gate_up(const Args &g, unsigned most, hipStream_t st)
 {
-    return launch_with_lds<moe_gate_up_kernel<TILES, 2, KW, EACH>>(most * (unsigned)(g.hidden_units * (kUnit / 32)), 2 * KW * kWave, 2 * KW * 2 * Stream<2>::kSlot, st, g);
+    constexpr int kLds = RW * KW * 2 * Stream<2 * FH>::kSlot;
+    return launch_with_lds<moe_gate_up_kernel<TILES, RW, KW, EACH, FH>, kLds>(most * (unsigned)(g.hidden_units * (kUnit / (16 * RW * FH))), RW * KW * kWave, kLds, st, g);
+}
+
+// Fragments and waves of a workgroup of down's.
+constexpr int kDownWaves = 8, kDenseWaves = 4;
+template <int TILES, int F, int NW>
+int launch_down(const Args &g, hipStream_t st)
+{
+    constexpr int kLds = NW * 3 * Stream<F>::kSlot, kToken = NW * 16 * F * (int)sizeof(float);
+    const unsigned blocks = (unsigned)(g.dim + 16 * F - 1) / (16 * F) * (unsigned)g.splits;
+    return launch_with_lds<moe_down_kernel<TILES, F, NW>, kLds + kMostTokens * kToken>(blocks, 64 * NW, kLds + g.tokens * kToken, st, g);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -822,9 +877,13 @@ Args args_of(const vtl_hip_moe *m, int tokens)
     g.hidden_chunks = chunks_of(m->hidden);
     g.dim_units = (g.dim_chunks + 1) / 2;
     g.hidden_units = (g.hidden_chunks + 1) / 2;
+    // if the tokens choose experts as they would by chance: workgroups of 32 hidden values, and pairs of an expert
+    const double chosen = g.experts * (1.0 - std::pow(1.0 - (double)g.top / g.experts, tokens));
+    g.many = chosen * ((g.hidden + 31) / 32) >= 640;
+    g.dense = tokens * g.top >= kDenseFrom * chosen;
     // a workgroup for each compute unit for the down product, as long as a wave has two units
-    const int rows = (m->dim + 15) / 16, units = std::min(m->experts, tokens * m->top_k) * g.hidden_units;
-    g.splits = std::max(1, std::min(256 / rows, units / (2 * kProductWaves)));
+    const int rows = g.dense ? (m->dim + 31) / 32 : (m->dim + 15) / 16, units = std::min(m->experts, tokens * m->top_k) * g.hidden_units;
+    g.splits = std::max(1, std::min(256 / rows, units / (2 * (g.dense ? kDenseWaves : kDownWaves))));
     return g;
 }
 
@@ -881,28 +940,26 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     int status = check_launch("moe_scores_kernel");
     if (status != VTL_HIP_OK)
         return status;
-    // workgroups of 32 hidden values, if the tokens choose experts as they would by chance
-    const double chosen = g.experts * (1.0 - std::pow(1.0 - (double)g.top / g.experts, tokens));
-    const bool many = chosen * ((g.hidden + 31) / 32) >= 1024;
-    const bool own_plan = tokens <= kOwnPlan && !many, narrow = g.experts <= 2 * kWave;
+    const bool own_plan = tokens <= kOwnPlan && !g.many && !g.dense, narrow = g.experts <= 2 * kWave;
     if (!own_plan) {
         hipLaunchKernelGGL(narrow ? moe_plan_kernel<2> : moe_plan_kernel<kMostExperts / kWave>, dim3(1), dim3(1024), 0, st, g);
         if ((status = check_launch("moe_plan_kernel")) != VTL_HIP_OK)
             return status;
     }
     const unsigned most = (unsigned)std::min(g.experts, tokens * g.top);
-    if (!own_plan)
-        status = many ? launch_gate_up<2, 1, 0>(g, most, st) : launch_gate_up<2, 4, 0>(g, most, st);
+    if (g.dense)
+        status = launch_gate_up<4, 1, 0, 1, 2>(g, most, st);
+    else if (!own_plan)
+        status = g.many ? launch_gate_up<2, 1, 0>(g, most, st) : launch_gate_up<2, 2, 0>(g, most, st);
     else if (tokens <= kTokensATile)
-        status = narrow ? launch_gate_up<1, 4, 2>(g, most, st) : launch_gate_up<1, 4, kMostExperts / kWave>(g, most, st);
+        status = narrow ? launch_gate_up<1, 2, 2>(g, most, st) : launch_gate_up<1, 2, kMostExperts / kWave>(g, most, st);
     else
-        status = narrow ? launch_gate_up<2, 4, 2>(g, most, st) : launch_gate_up<2, 4, kMostExperts / kWave>(g, most, st);
+        status = narrow ? launch_gate_up<2, 2, 2>(g, most, st) : launch_gate_up<2, 2, kMostExperts / kWave>(g, most, st);
     if (status != VTL_HIP_OK)
         return status;
-    const unsigned blocks = (unsigned)(g.dim + 15) / 16 * (unsigned)g.splits;
-    const int lds = kProductWaves * (3 * Stream<1>::kSlot + tokens * 16 * (int)sizeof(float));
-    status = tokens <= kTokensATile ? launch_with_lds<moe_down_kernel<1>>(blocks, 64 * kProductWaves, lds, st, g)
-                                    : launch_with_lds<moe_down_kernel<2>>(blocks, 64 * kProductWaves, lds, st, g);
+    status = g.dense                    ? launch_down<4, 2, kDenseWaves>(g, st)
+             : tokens <= kTokensATile ? launch_down<1, 1, kDownWaves>(g, st)
+                                      : launch_down<2, 1, kDownWaves>(g, st);
     if (status != VTL_HIP_OK || g.splits == 1)
         return status;
     hipLaunchKernelGGL(moe_join_kernel, dim3((unsigned)(tokens * g.dim + 255) / 256), dim3(256), 0, st, g);

@@ -640,7 +640,10 @@ int launch_few(Args g, hipStream_t st)
     }
     const int units = (g.chunks + 1) / 2;
     g.slots = units <= NW ? 1 : 2;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((g.N + 16 * FR - 1) / (16 * FR) * ((g.M + 4 * MX - 1) / (4 * MX)))), dim3(64 * NW), NW * g.slots * F::kSlot, st, g);
+    const int64_t blocks = (int64_t)((g.N + 16 * FR - 1) / (16 * FR)) * ((g.M + 4 * MX - 1) / (4 * MX));
+    if (blocks * 64 * NW > 0xffffffffll)
+        return VTL_HIP_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), NW * g.slots * F::kSlot, st, g);
     return check_launch("linear_few_mxfp4_kernel");
 }
 
