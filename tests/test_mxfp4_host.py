@@ -202,23 +202,24 @@ def names(tokens, **changes):
     return of(t.experts(t.layer(**changes), tokens, **BIG))
 few = names(1, experts=64, top_k=6, dim=2048, hidden=512)
 # (six experts of one unit each are less than two for each of 16 waves)
-assert [l[0] for l in few] == ["moe_scores_kernel", "moe_gate_up_kernel", "moe_down_kernel"] and few[1][2] == [1, 2, 2, 2, 1], few
+assert [l[0] for l in few] == ["moe_scores_kernel", "moe_gate_up_kernel", "moe_down_kernel"] and few[1][2] == [1, 2, 2, 2, 1, 0], few
 assert [l[0] for l in names(1, experts=64, top_k=6, dim=2048, hidden=4096)] == [
     "moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel", "moe_join_kernel"]      # 768 workgroups of 32 hidden values
 assert [l[0] for l in names(1, experts=64, top_k=6, dim=4096, hidden=512)] == ["moe_scores_kernel", "moe_gate_up_kernel", "moe_down_kernel"]
-assert names(1, experts=129, top_k=6, dim=4096, hidden=512)[1][2] == [1, 2, 2, 8, 1]
-assert names(4, experts=64, top_k=6, dim=4096, hidden=512)[1][2] == [2, 2, 2, 2, 1]
-assert names(8, experts=300, top_k=2, dim=4096, hidden=512)[1][2] == [2, 2, 2, 8, 1]
+assert names(1, experts=129, top_k=6, dim=4096, hidden=512)[1][2] == [1, 2, 2, 8, 1, 0]
+assert names(4, experts=64, top_k=6, dim=4096, hidden=512)[1][2] == [2, 2, 2, 2, 1, 0]
+assert names(8, experts=300, top_k=2, dim=4096, hidden=512)[1][2] == [2, 2, 2, 8, 1, 0]
 nine = names(9, experts=64, top_k=2, dim=4096, hidden=512)
-assert [l[0] for l in nine] == ["moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel"] and nine[2][2] == [2, 2, 2, 0, 1], nine
+assert [l[0] for l in nine] == ["moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel"] and nine[2][2] == [2, 2, 2, 0, 1, 0], nine
 many = names(24, experts=128, top_k=8, dim=2048, hidden=1024)
-assert [l[0] for l in many] == ["moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel", "moe_join_kernel"] and many[2][2] == [2, 2, 1, 0, 1], many
-assert names(2, experts=128, top_k=16, dim=2048, hidden=2048)[2][2] == [2, 2, 1, 0, 1]
+assert [l[0] for l in many] == ["moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel", "moe_join_kernel"] and many[2][2] == [2, 2, 1, 0, 1, 1] and many[3][2] == [2, 1, 8, 1], many
+assert names(24, experts=128, top_k=8, dim=512, hidden=1024)[2][2] == [2, 2, 1, 0, 1, 0]
+assert names(2, experts=128, top_k=16, dim=2048, hidden=2048)[2][2] == [2, 2, 1, 0, 1, 1]
 # four pairs of an expert and more: waves with twice the weights
 dense = names(16, experts=8, top_k=2, dim=4096, hidden=2048)
 assert [l[0] for l in dense] == ["moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel", "moe_join_kernel"], dense
-assert dense[2][2] == [4, 1, 1, 0, 2] and dense[3][2] == [4, 2, 4] and dense[3][1] == 2 * 128, dense
-assert names(8, experts=8, top_k=4, dim=4096, hidden=64)[2][2] == [4, 1, 1, 0, 2]
+assert dense[2][2] == [4, 1, 1, 0, 2, 0] and dense[3][2] == [4, 2, 4, 0] and dense[3][1] == 2 * 128, dense
+assert names(8, experts=8, top_k=4, dim=4096, hidden=64)[2][2] == [4, 1, 1, 0, 2, 0]
 most = names(64, experts=512, top_k=16, dim=65536, hidden=65536)
 assert all(blocks * 512 < 1 << 32 for _, blocks, _ in most), most
 print("done")

@@ -47,7 +47,7 @@ struct Args {
     uint8_t *h_digits, *h_scales;           // the same of each pair's hidden values
     float *parts;                           // [splits, tokens, dim] where several workgroups share rows of the output
     int splits;
-    int many, dense;                        // how the products are launched
+    int many, dense, large;                 // how the products are launched
 };
 
 __device__ __forceinline__ v4f mfma_digits(v4i w, v8i d, v4f c, int sw, int sd)
@@ -481,11 +481,11 @@ struct Held {
 // 64 221 for 254; 64 tokens and 6 of 64 of 2048 x 1408 110 for 125; but 24 tokens and 8 of 128 95 for 86).  Digits by way of shared memory for four
 // waves with all pairs' sums in registers were no faster but for 36 pairs of an expert: one wave a SIMD, which waits for its own reads.
 // EACH: every workgroup makes the plan for itself (a few tokens: less than a launch takes); 0: it is there.
-template <int TILES, int RW, int KW, int EACH, int FH = 1>
+template <int TILES, int RW, int KW, int EACH, int FH = 1, bool PAST = false>
 __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 {
     constexpr int NW = RW * KW, kRows = 16 * RW * FH, kPairs = TILES * kTokensATile;
-    using S = Stream<2 * FH>;
+    using S = Stream<2 * FH, PAST>;
     static_assert(RW * FH % 2 == 0, "whole blocks of hidden values");
     static_assert(64 * NW % (kRows / 4) == 0, "a thread's values are the same of every pair");
     extern __shared__ __attribute__((aligned(16))) char smem[];   // two slots a wave
@@ -623,10 +623,10 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
 // workgroups.  A wave adds what an expert gives to its own sums of the tokens, and the waves' sums meet in order.
 // Bound by the weights, and by the hidden values' digits as above: 24 tokens of 128 experts of 2048 x 1024 27.5 us, 4.1 TB/s
 // (24.8 without the digits; four waves a workgroup and twice as many workgroups 27.9, sixteen waves a compute unit 32.6); one token, 6 of 4096 x 1024 6.4.
-template <int TILES, int F, int NW>
+template <int TILES, int F, int NW, bool PAST = false>
 __global__ __launch_bounds__(64 * NW) void moe_down_kernel(const Args g)
 {
-    using S = Stream<F>;
+    using S = Stream<F, PAST>;
     constexpr int kSlots = 3, kPairs = TILES * kTokensATile, kRows = 16 * F;
     extern __shared__ __attribute__((aligned(16))) char smem[];    // three slots a wave
     float *const sums = reinterpret_cast<float *>(smem + NW * kSlots * S::kSlot);   // [waves, tokens, kRows]
@@ -796,6 +796,11 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const Args g)
 // Pairs of an expert, if tokens choose by chance, from which on waves have twice the weights, so that digits are asked for half as often.
 constexpr double kDenseFrom = 4.0;
 
+// Bytes of the chosen experts' weights from which on they are read past the caches: half the last-level one.  (24 tokens, 8 of 128 experts of 2048 x 1024, 337 MB, gate and up
+// 43.4 us for 45.1; whole calls of 4 tokens, 8 of 256 of 4096 x 1024, 204 MB, 53.8 for 57.0; 8 tokens, 2 of 8 of 4096 x 7168, 336 MB, 87.8 for 92.7; but one token, 2 of 8, 94 MB, 27.7
+// for 25.8, and 64 tokens, whose pairs take two passes, 226 for 220.)
+constexpr double kLargeFrom = 128e6;
+
 // The kernels with more shared memory than a launch has unasked.
 template <void (*KERNEL)(const Args), int MOST>
 int launch_with_lds(unsigned blocks, int threads, int lds, hipStream_t st, const Args &g)
@@ -810,21 +815,21 @@ int launch_with_lds(unsigned blocks, int threads, int lds, hipStream_t st, const
     return check_launch("moe_mxfp4 product");
 }
 
-template <int TILES, int KW, int EACH, int RW = 2, int FH = 1>
+template <int TILES, int KW, int EACH, int RW = 2, int FH = 1, bool PAST = false>
 int launch_gate_up(const Args &g, unsigned most, hipStream_t st)
 {
     constexpr int kLds = RW * KW * 2 * Stream<2 * FH>::kSlot;
-    return launch_with_lds<moe_gate_up_kernel<TILES, RW, KW, EACH, FH>, kLds>(most * (unsigned)(g.hidden_units * (kUnit / (16 * RW * FH))), RW * KW * kWave, kLds, st, g);
+    return launch_with_lds<moe_gate_up_kernel<TILES, RW, KW, EACH, FH, PAST>, kLds>(most * (unsigned)(g.hidden_units * (kUnit / (16 * RW * FH))), RW * KW * kWave, kLds, st, g);
 }
 
 // Fragments and waves of a workgroup of down's.
 constexpr int kDownWaves = 8, kDenseWaves = 4;
-template <int TILES, int F, int NW>
+template <int TILES, int F, int NW, bool PAST = false>
 int launch_down(const Args &g, hipStream_t st)
 {
     constexpr int kLds = NW * 3 * Stream<F>::kSlot, kToken = NW * 16 * F * (int)sizeof(float);
     const unsigned blocks = (unsigned)(g.dim + 16 * F - 1) / (16 * F) * (unsigned)g.splits;
-    return launch_with_lds<moe_down_kernel<TILES, F, NW>, kLds + kMostTokens * kToken>(blocks, 64 * NW, kLds + g.tokens * kToken, st, g);
+    return launch_with_lds<moe_down_kernel<TILES, F, NW, PAST>, kLds + kMostTokens * kToken>(blocks, 64 * NW, kLds + g.tokens * kToken, st, g);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -881,6 +886,7 @@ Args args_of(const vtl_hip_moe *m, int tokens)
     const double chosen = g.experts * (1.0 - std::pow(1.0 - (double)g.top / g.experts, tokens));
     g.many = chosen * ((g.hidden + 31) / 32) >= 640;
     g.dense = tokens * g.top >= kDenseFrom * chosen;
+    g.large = g.many && !g.dense && chosen * g.hidden * g.dim * (3 * 17.0 / 32.0) >= kLargeFrom;
     // a workgroup for each compute unit for the down product, as long as a wave has two units
     const int rows = g.dense ? (m->dim + 31) / 32 : (m->dim + 15) / 16, units = std::min(m->experts, tokens * m->top_k) * g.hidden_units;
     g.splits = std::max(1, std::min(256 / rows, units / (2 * (g.dense ? kDenseWaves : kDownWaves))));
@@ -950,14 +956,17 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     if (g.dense)
         status = launch_gate_up<4, 1, 0, 1, 2>(g, most, st);
     else if (!own_plan)
-        status = g.many ? launch_gate_up<2, 1, 0>(g, most, st) : launch_gate_up<2, 2, 0>(g, most, st);
+        status = g.large  ? launch_gate_up<2, 1, 0, 2, 1, true>(g, most, st)
+                 : g.many ? launch_gate_up<2, 1, 0>(g, most, st)
+                          : launch_gate_up<2, 2, 0>(g, most, st);
     else if (tokens <= kTokensATile)
         status = narrow ? launch_gate_up<1, 2, 2>(g, most, st) : launch_gate_up<1, 2, kMostExperts / kWave>(g, most, st);
     else
         status = narrow ? launch_gate_up<2, 2, 2>(g, most, st) : launch_gate_up<2, 2, kMostExperts / kWave>(g, most, st);
     if (status != VTL_HIP_OK)
         return status;
-    status = g.dense                    ? launch_down<4, 2, kDenseWaves>(g, st)
+    status = g.dense                  ? launch_down<4, 2, kDenseWaves>(g, st)
+             : g.large                ? launch_down<2, 1, kDownWaves, true>(g, st)
              : tokens <= kTokensATile ? launch_down<1, 1, kDownWaves>(g, st)
                                       : launch_down<2, 1, kDownWaves>(g, st);
     if (status != VTL_HIP_OK || g.splits == 1)

@@ -74,7 +74,9 @@ __device__ __forceinline__ void wait_vmcnt()
 // of its own, from where they are read as the 16x16x128 product takes them.  By way of shared memory because of how memory is read: a load that gives
 // the matrix unit its operand directly has 64 bytes of each of 16 rows, this one 256 bytes of each of 4.
 constexpr int kUnit = 2 * kChunk, kUnitSteps = kUnit / 128;
-template <int FRAGS>
+// PAST: past the caches, for weights that none of them holds until the next call (reading 218 MB that way 33.2 us, 6.6 TB/s, else 37.2; but 31 MB that are read over and
+// over 8.5 for 7.9).
+template <int FRAGS, bool PAST = false>
 struct Stream {
     static constexpr int kCodes = 16 * kUnit / 2, kFrag = kCodes + 16 * (kUnit / kBlock), kSlot = FRAGS * kFrag;
     static constexpr int kLoads = 5 * FRAGS;        // of a unit
@@ -109,7 +111,7 @@ struct Stream {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const unsigned in_row = min((unsigned)unit * (kUnit / 2) + (unsigned)((lane % 16) ^ (4 * j + lane / 16)) * 16u, pitch - 16u);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(from, VTL_LPTR(slot + f * kFrag + j * 1024), 16, (int)(code_at[f][j] + in_row), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(from, VTL_LPTR(slot + f * kFrag + j * 1024), 16, (int)(code_at[f][j] + in_row), 0, 0, PAST ? 2 : 0);
             }
             const unsigned in_row = min((unsigned)unit * (kUnit / kBlock) + (unsigned)(lane % 4) * 4u, spitch - 4u);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(scales_from, VTL_LPTR(slot + f * kFrag + kCodes), 4, (int)(scale_at[f] + in_row), 0, 0, 0);
