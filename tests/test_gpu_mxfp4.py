@@ -224,7 +224,8 @@ class LargeLayer(Layer):
 
 @pytest.mark.parametrize("experts,dim,hidden,top,tokens,bias", [
     (64, 96, 1000, 6, 40, False), (16, 550, 2100, 8, 12, True), (8, 40, 4112, 4, 9, False), (64, 64, 1030, 16, 8, True), (20, 64, 2080, 16, 1, False),
-    (96, 1028, 1450, 5, 17, True)])      # 128 MB of weights
+    (96, 1028, 1450, 5, 17, True),      # 128 MB of weights
+    (8, 100, 2600, 4, 40, True)])       # 20 pairs of an expert
 def test_hidden_values_for_every_compute_unit(guard_bands, experts, dim, hidden, top, tokens, bias):
     l = LargeLayer(experts, dim, hidden, top, bias)
     x = normal(98, tokens, dim)

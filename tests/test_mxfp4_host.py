@@ -216,10 +216,13 @@ assert [l[0] for l in many] == ["moe_scores_kernel", "moe_plan_kernel", "moe_gat
 assert names(24, experts=128, top_k=8, dim=512, hidden=1024)[2][2] == [2, 2, 1, 0, 1, 0]
 assert names(2, experts=128, top_k=16, dim=2048, hidden=2048)[2][2] == [2, 2, 1, 0, 1, 1]
 # four pairs of an expert and more: waves with twice the weights
-dense = names(16, experts=8, top_k=2, dim=4096, hidden=2048)
+dense = names(16, experts=8, top_k=2, dim=4096, hidden=2816)
 assert [l[0] for l in dense] == ["moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel", "moe_join_kernel"], dense
 assert dense[2][2] == [4, 1, 1, 0, 2, 0] and dense[3][2] == [4, 2, 4, 0] and dense[3][1] == 2 * 128, dense
-assert names(8, experts=8, top_k=4, dim=4096, hidden=64)[2][2] == [4, 1, 1, 0, 2, 0]
+assert names(8, experts=8, top_k=4, dim=4096, hidden=64)[1][2] == [2, 2, 2, 2, 1, 0]
+# few workgroups: up to eleven passes over 64 pairs beside each other
+small = names(64, experts=4, top_k=2, dim=4096, hidden=64)
+assert small[2][1:] == (4 * 16 * 11, [2, 2, 2, 0, 1, 0]), small
 most = names(64, experts=512, top_k=16, dim=65536, hidden=65536)
 assert all(blocks * 512 < 1 << 32 for _, blocks, _ in most), most
 print("done")

@@ -48,6 +48,7 @@ struct Args {
     float *parts;                           // [splits, tokens, dim] where several workgroups share rows of the output
     int splits;
     int many, dense, large;                 // how the products are launched
+    int passes;                             // workgroups of gate and up among which an expert's pairs are dealt out
 };
 
 __device__ __forceinline__ v4f mfma_digits(v4i w, v8i d, v4f c, int sw, int sd)
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
     static_assert(64 * NW % (kRows / 4) == 0, "a thread's values are the same of every pair");
     extern __shared__ __attribute__((aligned(16))) char smem[];   // two slots a wave
     __shared__ __attribute__((aligned(16))) float part[NW * FH][kPairs][36];
-    const int tiles = g.hidden_units * (kUnit / kRows), a = (int)blockIdx.x / tiles, row0 = (int)blockIdx.x % tiles * kRows;
+    const int tiles = g.hidden_units * (kUnit / kRows), a = (int)blockIdx.x / tiles / g.passes, pass = (int)blockIdx.x / tiles % g.passes, row0 = (int)blockIdx.x % tiles * kRows;
     const Entry *entries = g.plan->entry;
     const int *tokens = g.plan->token, *count = &g.plan->count;
     const float *weights = g.plan->weight;
@@ -533,7 +534,7 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
                 up_bias[k] = bias[g.hidden + k];
             }
     }
-    for (int first = 0; first < n; first += kPairs) {
+    for (int first = pass * kPairs; first < n; first += g.passes * kPairs) {
         const int now = min(n - first, kPairs);
         if (my_row < g.hidden) {
             if (begin < end)
@@ -793,7 +794,13 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const Args g)
 
 // ---- host -----------------------------------------------------------------------------------
 
-// Pairs of an expert, if tokens choose by chance, from which on waves have twice the weights, so that digits are asked for half as often.
+// Workgroups of 32 hidden values from which on they are enough with one wave along K each.  Fewer of them deal out an expert's passes over its pairs too, up to twice as many
+// workgroups as that (whole calls, us: 32 tokens, 2 of 4 experts of 4096 x 256 29.6, else 43.9; 64 tokens, 2 of 8 of 256 x 128 25.7 and 30.0; 16 tokens, 2 of 8 of 1024 x 512
+// 18.6 and 20.5).
+constexpr double kManyFrom = 640;
+
+// Pairs of an expert, if tokens choose by chance, from which on waves have twice the weights, so that digits are asked for half as often, where workgroups are enough
+// (with fewer: 32 tokens, 2 of 8 of 1024 x 1024 34.5 for 28.1).
 constexpr double kDenseFrom = 4.0;
 
 // Bytes of the chosen experts' weights from which on they are read past the caches: half the last-level one.  (24 tokens, 8 of 128 experts of 2048 x 1024, 337 MB, gate and up
@@ -819,7 +826,7 @@ template <int TILES, int KW, int EACH, int RW = 2, int FH = 1, bool PAST = false
 int launch_gate_up(const Args &g, unsigned most, hipStream_t st)
 {
     constexpr int kLds = RW * KW * 2 * Stream<2 * FH>::kSlot;
-    return launch_with_lds<moe_gate_up_kernel<TILES, RW, KW, EACH, FH, PAST>, kLds>(most * (unsigned)(g.hidden_units * (kUnit / (16 * RW * FH))), RW * KW * kWave, kLds, st, g);
+    return launch_with_lds<moe_gate_up_kernel<TILES, RW, KW, EACH, FH, PAST>, kLds>(most * (unsigned)(g.passes * g.hidden_units * (kUnit / (16 * RW * FH))), RW * KW * kWave, kLds, st, g);
 }
 
 // Fragments and waves of a workgroup of down's.
@@ -883,10 +890,12 @@ Args args_of(const vtl_hip_moe *m, int tokens)
     g.dim_units = (g.dim_chunks + 1) / 2;
     g.hidden_units = (g.hidden_chunks + 1) / 2;
     // if the tokens choose experts as they would by chance: workgroups of 32 hidden values, and pairs of an expert
-    const double chosen = g.experts * (1.0 - std::pow(1.0 - (double)g.top / g.experts, tokens));
-    g.many = chosen * ((g.hidden + 31) / 32) >= 640;
-    g.dense = tokens * g.top >= kDenseFrom * chosen;
+    const double chosen = g.experts * (1.0 - std::pow(1.0 - (double)g.top / g.experts, tokens)), workgroups = chosen * ((g.hidden + 31) / 32);
+    g.many = workgroups >= kManyFrom;
+    g.dense = g.many && tokens * g.top >= kDenseFrom * chosen;
     g.large = g.many && !g.dense && chosen * g.hidden * g.dim * (3 * 17.0 / 32.0) >= kLargeFrom;
+    // where they are few, an expert's passes over its pairs in workgroups of their own
+    g.passes = g.many || tokens <= kOwnPlan ? 1 : std::min((tokens + 2 * kTokensATile - 1) / (2 * kTokensATile), (int)std::ceil(2 * kManyFrom / workgroups));
     // a workgroup for each compute unit for the down product, as long as a wave has two units
     const int rows = g.dense ? (m->dim + 31) / 32 : (m->dim + 15) / 16, units = std::min(m->experts, tokens * m->top_k) * g.hidden_units;
     g.splits = std::max(1, std::min(256 / rows, units / (2 * (g.dense ? kDenseWaves : kDownWaves))));
