@@ -188,7 +188,7 @@ def check_layer(l, x, workspace=None):
 MOES = [  # experts, dim, hidden, top, tokens
     (1, 1, 1, 1, 1), (2, 32, 32, 1, 3), (4, 256, 256, 2, 1), (8, 300, 100, 2, 5), (8, 256, 512, 8, 4), (20, 1000, 72, 3, 5), (64, 512, 256, 6, 1),
     (64, 520, 160, 6, 24), (128, 256, 64, 8, 64), (60, 96, 33, 4, 17), (512, 64, 32, 16, 9), (3, 2048, 40, 1, 64), (5, 64, 2000, 5, 33), (130, 40, 16, 2, 2),
-    (6, 300, 100, 6, 7), (4, 1000, 530, 2, 20), (16, 264, 72, 16, 64), (200, 96, 64, 2, 6), (9, 2100, 48, 1, 50)]
+    (6, 300, 100, 6, 7), (4, 1000, 530, 2, 20), (16, 264, 72, 16, 64), (200, 96, 64, 2, 6), (9, 2100, 48, 1, 50), (256, 64, 32, 8, 40), (257, 40, 32, 3, 7), (255, 40, 32, 16, 2)]
 
 
 @pytest.mark.parametrize("experts,dim,hidden,top,tokens", MOES)

@@ -206,7 +206,9 @@ assert [l[0] for l in few] == ["moe_scores_kernel", "moe_gate_up_kernel", "moe_d
 assert [l[0] for l in names(1, experts=64, top_k=6, dim=2048, hidden=4096)] == [
     "moe_scores_kernel", "moe_plan_kernel", "moe_gate_up_kernel", "moe_down_kernel", "moe_join_kernel"]      # 768 workgroups of 32 hidden values
 assert [l[0] for l in names(1, experts=64, top_k=6, dim=4096, hidden=512)] == ["moe_scores_kernel", "moe_gate_up_kernel", "moe_down_kernel"]
-assert names(1, experts=129, top_k=6, dim=4096, hidden=512)[1][2] == [1, 2, 2, 8, 1, 0]
+for experts, each in ((128, 2), (129, 4), (256, 4), (257, 8), (512, 8)):
+    assert names(1, experts=experts, top_k=6, dim=4096, hidden=512)[1][2] == [1, 2, 2, each, 1, 0], experts
+    assert names(64, experts=experts, top_k=1, dim=4096, hidden=32)[1] == ("moe_plan_kernel", 1, [each]), experts
 assert names(4, experts=64, top_k=6, dim=4096, hidden=512)[1][2] == [2, 2, 2, 2, 1, 0]
 assert names(8, experts=300, top_k=2, dim=4096, hidden=512)[1][2] == [2, 2, 2, 8, 1, 0]
 nine = names(9, experts=64, top_k=2, dim=4096, hidden=512)

@@ -271,8 +271,9 @@ struct Choice {
 
 // The plan, made in shared memory by the NW waves of a workgroup: a wave has a token's scores, EACH a lane, finds its `top` largest (the lower
 // index of two that are equal) and notes the token with these experts; then the experts that were noted are put in order.
-// Bound by latencies: the scores' way through memory, then `top` maxima over a wave behind each other.  As a launch 6.0 us for 24 tokens of 128 experts; in
-// the workgroups of the next launch 3.8 for one token of 64 (with launch and end), 5.5 for five of 20.
+// Bound by latencies: the scores' way through memory, then `top` maxima over a wave behind each other.  As a launch 6.0 us for 24 tokens of 128 experts, for 64 tokens 11.4, of 256
+// experts 14.4 (with EACH 8 21), of 512 21.5; in the workgroups of the next launch 3.8 for one token of 64 (with launch and end), 5.5 for five of 20.  Two tokens of a
+// wave beside each other: 1 us less for 64 tokens, 1 us more for one.
 template <int NW, int TOKENS, int EACH>
 __device__ __forceinline__ void make_plan(const Args &g, Choice<TOKENS, EACH> &c)
 {
@@ -829,7 +830,16 @@ int launch_gate_up(const Args &g, unsigned most, hipStream_t st)
     return launch_with_lds<moe_gate_up_kernel<TILES, RW, KW, EACH, FH, PAST>, kLds>(most * (unsigned)(g.passes * g.hidden_units * (kUnit / (16 * RW * FH))), RW * KW * kWave, kLds, st, g);
 }
 
-// Fragments and waves of a workgroup of down's.
+// With the plan made in every workgroup, of so many scores a lane.
+template <int TILES>
+int launch_few(const Args &g, int each, unsigned most, hipStream_t st)
+{
+    return each == 2   ? launch_gate_up<TILES, 2, 2>(g, most, st)
+           : each == 4 ? launch_gate_up<TILES, 2, 4>(g, most, st)
+                       : launch_gate_up<TILES, 2, kMostExperts / kWave>(g, most, st);
+}
+
+// Waves of a workgroup of down's.
 constexpr int kDownWaves = 8, kDenseWaves = 4;
 template <int TILES, int F, int NW, bool PAST = false>
 int launch_down(const Args &g, hipStream_t st)
@@ -955,9 +965,10 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     int status = check_launch("moe_scores_kernel");
     if (status != VTL_HIP_OK)
         return status;
-    const bool own_plan = tokens <= kOwnPlan && !g.many && !g.dense, narrow = g.experts <= 2 * kWave;
+    const bool own_plan = tokens <= kOwnPlan && !g.many && !g.dense;
+    const int each = g.experts <= 2 * kWave ? 2 : g.experts <= 4 * kWave ? 4 : kMostExperts / kWave;     // scores of a token a lane
     if (!own_plan) {
-        hipLaunchKernelGGL(narrow ? moe_plan_kernel<2> : moe_plan_kernel<kMostExperts / kWave>, dim3(1), dim3(1024), 0, st, g);
+        hipLaunchKernelGGL(each == 2 ? moe_plan_kernel<2> : each == 4 ? moe_plan_kernel<4> : moe_plan_kernel<kMostExperts / kWave>, dim3(1), dim3(1024), 0, st, g);
         if ((status = check_launch("moe_plan_kernel")) != VTL_HIP_OK)
             return status;
     }
@@ -969,9 +980,9 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
                  : g.many ? launch_gate_up<2, 1, 0>(g, most, st)
                           : launch_gate_up<2, 2, 0>(g, most, st);
     else if (tokens <= kTokensATile)
-        status = narrow ? launch_gate_up<1, 2, 2>(g, most, st) : launch_gate_up<1, 2, kMostExperts / kWave>(g, most, st);
+        status = launch_few<1>(g, each, most, st);
     else
-        status = narrow ? launch_gate_up<2, 2, 2>(g, most, st) : launch_gate_up<2, 2, kMostExperts / kWave>(g, most, st);
+        status = launch_few<2>(g, each, most, st);
     if (status != VTL_HIP_OK)
         return status;
     status = g.dense                  ? launch_down<4, 2, kDenseWaves>(g, st)
