@@ -37,7 +37,7 @@ __device__ __forceinline__ float floor_of(int relu) { return relu ? 0.0f : -__bu
 // A workgroup has 16 FR rows of weights and 4 MX rows of x; its waves deal the units of K out among them, each with two slots of shared memory
 // that its own loads fill, and their sums meet in order.  The product's first operand is the weights, so a lane has four results of one row of x side by side.
 // XF32: x is f32, and each wave makes the codes of its units itself.
-// Bound by the weights' way from memory: one row and 28672 x 8192 weights 19.0 us, 6.6 TB/s (eight waves a workgroup, and with them one workgroup a compute unit, 24.3);
+// Bound by the weights' way from memory: one row and 28672 x 8192 weights 19.0 us, 6.6 TB/s with the last-level cache's part in it (eight waves a workgroup, and with them one workgroup a compute unit, 24.3);
 // 14336 x 4096 7.0, 4.5 TB/s: it begins and ends.  From 17 rows on bound by x's way into shared memory too, four or eight times that of the weights: 32 rows and
 // 4096 x 4096 4.2 us (one row 3.1), 4096 x 14336 9.4 (7.1).
 constexpr int kFewMost = 16;     // rows up to which there is no other way
@@ -270,6 +270,8 @@ __device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 // of 16 bytes and its scale byte.  Operands are read one of the chunk's four steps ahead.  The barrier between two chunks comes in front of a chunk's last step, so that
 // its latency, the first reads of the next chunk and the loads into the stage that became free hide behind that step's products: a read and its
 // share of the loads behind each of them, in this order, because loads in one burst wait for each other in front of the unit that makes their addresses.
+// Tiles of 256 x 256 are bound by power: 8192 x 8192 x 8192 265 to 286 us from card to card, 3.8 to 4.15 PFLOP/s; 1.68 us a chunk, of which the products alone take 1.34 on random codes (reads left out
+// 1.49, loads left out 1.43).  Smaller ones by the way from the L2 into shared memory, some 22 bytes a cycle of a compute unit whatever the tile: 201 x 11008 x 4096 15.6 us.
 template <int BM, int BN, int WR, int WC, int STAGES, int SPREAD, bool EDGE>
 struct Tile {
     static constexpr int kWaves = WR * WC, kThreads = 64 * kWaves;
