@@ -2,6 +2,7 @@
 import numpy as np
 
 GRID = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+BORDERS = (GRID[1:] + GRID[:-1]) / 2
 U = 2.0 ** -24      # half a step of f32
 
 
@@ -21,9 +22,9 @@ def encode(x):
     e = np.frexp(np.where(top > 0, top, 1))[1] - 1                  # 2^e <= top < 2^(e + 1)
     byte = np.where(top > 0, np.maximum(e + 127 - 2, 0), 0)
     q = np.abs(clean) / np.exp2(byte - 127.0)[..., None]
-    away = np.abs(q[..., None] - GRID)
-    # the nearest, the even one of two
-    code = np.argmin(np.where(away == away.min(-1, keepdims=True), np.arange(8) % 2, 9), -1)
+    # the nearest, the even one of two: how many borders between neighbours lie below, and one more on a border above an odd code
+    code = np.searchsorted(BORDERS, q)
+    code = code + ((code % 2 == 1) & (q == BORDERS[np.minimum(code, 6)]))
     code = np.where(np.signbit(blocks) & good[..., None], code + 8, code)
     code = code.reshape(rows, -1).astype(np.uint8)
     return code[:, 0::2] | (code[:, 1::2] << 4), np.where(good, byte, 255).astype(np.uint8)
