@@ -233,10 +233,10 @@ __device__ __forceinline__ float wave_sum_f32(float v)
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kWave - 1));
 }
 
-// Numbers in their order, from 2 on; 1: NaN, behind all of them.
+// Numbers in their order, from 2 on, the two zeros as one (a sum too small for f32 is -0 where it is negative); 1: NaN, behind all of them.
 __device__ __forceinline__ unsigned order_of(float v)
 {
-    const unsigned b = __float_as_uint(v);
+    const unsigned b = __float_as_uint(v + 0.0f);
     if (v != v)
         return 1u;
     return max(b & 0x80000000u ? ~b : b | 0x80000000u, 2u);
