@@ -439,15 +439,17 @@ __device__ __forceinline__ float sum_digits(float v)
     return plus_right<4>(four, v);
 }
 
-// SiLU(gate) * up * weight.  The exponential is the vector unit's of a rounded exponent, off by |gate| half steps and one, which is |gate| steps of a value that is
-// as much smaller; the reciprocal is its own, corrected once.  (By the library's functions, a wave's 32 values of a token took longer than their weights.)
+// SiLU(gate) * up * weight, as gate * up / (1 + e) where gate is positive and gate * up * e / (1 + e) where it is not, e = exp(-|gate|): e and its sum with 1 are
+// numbers for any gate.  Of e the fourth root is made, and goes into factor after factor: e itself is below f32's least number from 104 on, where gate * up * e
+// need not be (up to 185, where the root is 2^-67).  The exponential is the vector unit's of a rounded exponent, off by |gate| half steps and some; the reciprocal is its own,
+// corrected once.  (By the library's functions, a wave's 32 values of a token took longer than their weights.)
 __device__ __forceinline__ float hidden_value(float gate, float up, float weight)
 {
-    const float e = __builtin_amdgcn_exp2f(fminf(gate * -1.44269504f, 125.5f));    // (whose sum with 1 has a reciprocal)
-    const float d = 1.0f + e;
+    const float root = __builtin_amdgcn_exp2f(fabsf(gate) * -0.36067376f), part = gate < 0.0f ? root : 1.0f, half = root * root;
+    const float d = fmaf(half, half, 1.0f);
     float r = __builtin_amdgcn_rcpf(d);
     r = fmaf(r, fmaf(-d, r, 1.0f), r);
-    return gate * r * up * weight;
+    return (gate * part) * (up * part) * part * part * r * weight;
 }
 
 // A workgroup's copy of the plan.  All entries that there may be, so that nothing waits for their number.
