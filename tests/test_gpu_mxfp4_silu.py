@@ -44,3 +44,15 @@ def test_every_gate(tokens, up):
     far = np.abs(want) * mx.U * (1.25 * np.minimum(np.abs(gate), 400) + 32) + 2.0 ** -127
     off = np.abs(got - want)
     assert (off <= far).all(), [(float(gate[i]), float(got[t, i]), float(want[i])) for t, i in np.argwhere(~(off <= far))[:6]]
+
+
+@pytest.mark.parametrize("low,high", [(-100.0, -80.0), (-80.0, -40.0), (-40.0, -8.0), (-8.0, 8.0)])
+def test_exponentials_are_those_of_the_gate(low, high):
+    """Not of a gate rounded to fewer digits.  The exponential's fourth root is off by a step of the instruction's and a rounding, 3 half steps and so 12 in the
+    value; the reciprocal of its sum with 1 by 9, the products by 7, digits by 1, sums by 5."""
+    gate = np.linspace(low, high, 1500).astype(np.float32).astype(np.float64)
+    up = np.float64(np.float32(1.7))
+    want = silu_up(gate, up)
+    got = hidden_values(gate, np.full_like(gate, up), 1)[0]
+    off = np.abs(got - want) / (np.abs(want) * mx.U + 2.0 ** -127)
+    assert (off <= 40).all(), (float(off.max()), float(gate[off.argmax()]))

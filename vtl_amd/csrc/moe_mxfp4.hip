@@ -441,11 +441,14 @@ __device__ __forceinline__ float sum_digits(float v)
 
 // SiLU(gate) * up * weight, as gate * up / (1 + e) where gate is positive and gate * up * e / (1 + e) where it is not, e = exp(-|gate|): e and its sum with 1 are
 // numbers for any gate.  Of e the fourth root is made, and goes into factor after factor: e itself is below f32's least number from 104 on, where gate * up * e
-// need not be (up to 185, where the root is 2^-67).  The exponential is the vector unit's of a rounded exponent, off by |gate| half steps and some; the reciprocal is its own,
-// corrected once.  (By the library's functions, a wave's 32 values of a token took longer than their weights.)
+// need not be (up to 185, where the root is 2^-67).  The exponential is the vector unit's, corrected by what its argument lost to rounding (|gate| half steps of the value);
+// the reciprocal is its own, corrected once.  (By the library's functions, a wave's 32 values of a token took longer than their weights.)
 __device__ __forceinline__ float hidden_value(float gate, float up, float weight)
 {
-    const float root = __builtin_amdgcn_exp2f(fabsf(gate) * -0.36067376f), part = gate < 0.0f ? root : 1.0f, half = root * root;
+    const float m = fabsf(gate), t = m * -0.36067376f;
+    float root = __builtin_amdgcn_exp2f(t);
+    root = fmaf(root, fmaf(m, -4.81491e-09f, fmaf(m, -0.36067376f, -t)) * 0.6931472f, root);    // (times 2 to what t has lost)
+    const float part = gate < 0.0f ? root : 1.0f, half = root * root;
     const float d = fmaf(half, half, 1.0f);
     float r = __builtin_amdgcn_rcpf(d);
     r = fmaf(r, fmaf(-d, r, 1.0f), r);
