@@ -420,8 +420,8 @@ typedef struct {
 } vtl_hip_moe;
 
 /* Y[tokens, dim] of X[tokens, dim], for a few tokens: up to VTL_HIP_MOE_MOST_TOKENS, and experts, top_k, dim and hidden within the limits
- * above (VTL_HIP_ERR_UNSUPPORTED beyond).  x, and p times the hidden values, enter the products with 24 bits of the largest among 32 (to 2^-128 where that is below
- * 2^-103), sums are f32; the same call gives the same bits.  A token with an infinity or NaN, or without a finite score, gives NaN, and so do a
+ * above (VTL_HIP_ERR_UNSUPPORTED beyond).  x, and p times the hidden values, enter the products with their 24 bits, those below 2^-6 of the largest among 32
+ * with all but 2^-30 of that one (2^-137 where it is below 2^-107); sums are f32; the same call gives the same bits.  A token with an infinity or NaN, or without a finite score, gives NaN, and so do a
  * chosen expert's block of weights without a number and hidden values beyond f32's range.  Y may not share memory with X or the layer.
  * workspace: as above, of vtl_hip_moe_mxfp4_workspace() bytes (0: no such layer). */
 size_t vtl_hip_moe_mxfp4_workspace(const vtl_hip_moe *layer, int tokens);
