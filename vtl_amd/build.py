@@ -33,8 +33,12 @@ HIPCC_FLAGS = [
 # Flags of single sources.  The f64 MFMA accumulators of the matmul kernel fit
 # the architectural VGPRs; asking for the VGPR form of MFMA keeps the compiler
 # from shuttling them to and from the accumulation registers every k-step.
+# So do most of the experts' accumulators, and what waits for a product in front
+# of its result's first reader (settle() in mxfp4.hpp) is in front of that one then
+# and not behind a copy.
 SOURCE_FLAGS = {
     "matmul_f64acc.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "moe_mxfp4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

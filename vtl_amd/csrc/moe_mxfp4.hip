@@ -590,11 +590,11 @@ __global__ __launch_bounds__(64 * RW * KW) void moe_gate_up_kernel(const Args g)
                 wait_vmcnt<0>();
                 work(ring + (end - 1 - begin) % 2 * S::kSlot);
             }
+            settle();
 #pragma unroll
             for (int i = 0; i < TILES; i++)
 #pragma unroll
                 for (int f = 0; f < 2 * FH; f++) {
-                    settle(acc[f][i]);
                     v4f v;
 #pragma unroll
                     for (int k = 0; k < 4; k++)
@@ -714,11 +714,11 @@ __global__ __launch_bounds__(64 * NW) void moe_down_kernel(const Args g)
                     acc[f][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         };
         const auto add = [&](int first, int now) __attribute__((always_inline)) {
+            settle();
 #pragma unroll
             for (int i = 0; i < TILES; i++)
 #pragma unroll
                 for (int f = 0; f < F; f++) {
-                    settle(acc[f][i]);
                     v4f v;
 #pragma unroll
                     for (int k = 0; k < 4; k++)

@@ -56,10 +56,16 @@ __device__ __forceinline__ v4f mfma_16(v4i a, v4i b, v4f c, int sa, int sb)
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, sa, 0, sb);
 }
 
-// In front of anything but a product that reads a 16x16x128 product's registers, which takes 11 wait states after it.  The compiler puts them in
-// where it sees a way from one to the other, but of two ways around conditional code between them it may look at the longer only: a lane's
-// first register was read too early there.
-__device__ __forceinline__ void settle(v4f &v) { asm volatile("s_nop 15" : "+v"(v)); }
+// Between the last product and anything else that reads or writes results: a 16x16x128 product with an 8-bit operand and a 32x32x64 product of 4-bit ones take 12
+// wait states until then, a 16x16x128 product of 4-bit ones 8.  The compiler puts them in where it sees a way from one to the other, but of two ways around conditional code
+// between them it once looked at the longer only: a lane's first register was read too early there.  Without an operand, and with nothing moved
+// past it: of results in accumulation registers the copy into a vector register is the read, and would come in front of a wait that names the copy.
+__device__ __forceinline__ void settle()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 #define VTL_GPTR(p) ((const __attribute__((address_space(1))) void *)(p))
 #define VTL_LPTR(p) ((__attribute__((address_space(3))) void *)(p))

@@ -194,16 +194,15 @@ __global__ __launch_bounds__(64 * NW) void linear_few_mxfp4_kernel(Args g)
             }
         W::done_reading();
     }
+    settle();
     __syncthreads();        // every wave is done with its slots
     float *const part = reinterpret_cast<float *>(smem);     // [waves][4 MX][kPart]
 #pragma unroll
     for (int i = 0; i < FR; i++)
 #pragma unroll
-        for (int j = 0; j < F::kTiles; j++) {
-            settle(acc[i][j]);
+        for (int j = 0; j < F::kTiles; j++)
             if (r < 4 * MX)
                 *reinterpret_cast<v4f *>(part + (w * 4 * MX + 16 * j + r) * F::kPart + 16 * i + 4 * q) = acc[i][j];
-        }
     __syncthreads();
     for (int item = (int)threadIdx.x; item < 4 * MX * 16 * FR; item += 64 * NW) {
         const int row = item / (16 * FR), nl = item % (16 * FR), n = n0 + nl;
@@ -492,6 +491,7 @@ __global__ __launch_bounds__(64 * WR * WC) void linear_tile_mxfp4_kernel(const A
         step(I1{}, I0{}, I0{}, No{}, c, stage, 0, 0);
         step(I2{}, I0{}, I0{}, No{}, c, stage, 0, 0);
         step(I3{}, I0{}, I0{}, Yes{}, 0, 0, 0, 0);
+        settle();
     }
 
     // Register k of a lane is row 8 (k / 4) + 4 half + k % 4 of a 32 x 32 tile, column r.  Four lanes exchange theirs (lane i gets row i of four
