@@ -390,8 +390,8 @@ int vtl_hip_dequantize_mxfp4_f32(const uint8_t *codes, const uint8_t *scales, in
  * Sums of 32 products are exact, and added up in f32; in how many ranges K is cut depends on M, N and K alone, so the same
  * call gives the same bits, a row among other rows need not.  A block without a number makes its row's or column's outputs NaN.
  * workspace: device memory of vtl_hip_linear_mxfp4_workspace() bytes (0: none is needed), 16-byte aligned; NULL (with size 0): the library's own (see
- * above).  Calls that may overlap on a device need one each.  The bytes are those of these sizes: fewer rows may take more.  Y may not share memory with an
- * operand.  K is at most 2^24, N at most 2^27 - 16, M below 2^30, and rows have the limit above (VTL_HIP_ERR_UNSUPPORTED beyond). */
+ * above).  Calls that may overlap on a device need one each.  The bytes are those of these sizes: fewer rows may take more.  Neither Y nor these bytes of
+ * the workspace may share memory with an operand or with each other.  K is at most 2^24, N at most 2^27 - 16, M below 2^30, and rows have the limit above (VTL_HIP_ERR_UNSUPPORTED beyond). */
 size_t vtl_hip_linear_mxfp4_workspace(int M, int N, int K);
 int vtl_hip_linear_mxfp4_f32(const uint8_t *x, const uint8_t *x_scales, const uint8_t *w, const uint8_t *w_scales, const float *bias, float *Y, int M,
                              int N, int K, int relu, void *workspace, size_t workspace_bytes);
@@ -423,7 +423,7 @@ typedef struct {
  * above (VTL_HIP_ERR_UNSUPPORTED beyond).  x, and p times the hidden values, enter the products with their 24 bits, those below 2^-6 of the largest among 32
  * with all but 2^-30 of that one (2^-137 where it is below 2^-107); sums are f32; the same call gives the same bits.  A token with an infinity or NaN, or without a finite score, gives NaN, and so do a
  * chosen expert's block of weights without a number and hidden values beyond f32's range.  Y may not share memory with X or the layer.
- * workspace: as above, of vtl_hip_moe_mxfp4_workspace() bytes (0: no such layer). */
+ * workspace: as above, apart from X, Y and the layer, of vtl_hip_moe_mxfp4_workspace() bytes (0: no such layer). */
 size_t vtl_hip_moe_mxfp4_workspace(const vtl_hip_moe *layer, int tokens);
 int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, int tokens, void *workspace, size_t workspace_bytes);
 

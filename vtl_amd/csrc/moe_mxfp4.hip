@@ -942,15 +942,15 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
         return VTL_HIP_ERR_INVALID_ARG;
     Args g = args_of(layer, tokens);
     const size_t results = (size_t)tokens * g.dim * sizeof(float), experts = (size_t)g.experts, into = experts * 2 * g.hidden, out = experts * g.dim;
-    const auto shared = [&](const void *p, size_t bytes) { return meet(Y, results, p, bytes); };
-    if (shared(X, results) || shared(layer->router, experts * g.dim * sizeof(float)) || shared(layer->router_bias, experts * sizeof(float)) ||
+    const size_t need = vtl_hip_moe_mxfp4_workspace(layer, tokens);
+    const auto shared = [&](const void *p, size_t bytes) { return meet(Y, results, p, bytes) || meet(workspace, need, p, bytes); };
+    if (meet(Y, results, workspace, need) || shared(X, results) || shared(layer->router, experts * g.dim * sizeof(float)) || shared(layer->router_bias, experts * sizeof(float)) ||
         shared(layer->gate_up, into * g.dim_chunks * kChunkCodes) || shared(layer->gate_up_scales, into * g.dim_chunks * kChunkScales) ||
         shared(layer->gate_up_bias, into * sizeof(float)) || shared(layer->down, out * g.hidden_chunks * kChunkCodes) ||
         shared(layer->down_scales, out * g.hidden_chunks * kChunkScales) || shared(layer->down_bias, out * sizeof(float)))
         return VTL_HIP_ERR_INVALID_ARG;
     g.x = X;
     g.y = Y;
-    const size_t need = vtl_hip_moe_mxfp4_workspace(layer, tokens);
     char *ws = static_cast<char *>(workspace);
     if (!ws) {
         if (workspace_bytes)

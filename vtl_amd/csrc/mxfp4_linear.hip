@@ -802,8 +802,11 @@ int linear(Args g, const uint8_t *w, const uint8_t *w_scales, const float *bias,
         return VTL_HIP_ERR_INVALID_ARG;
     g.chunks = chunks_of(K);
     const size_t pitch = (size_t)g.chunks * kChunkCodes, spitch = (size_t)g.chunks * kChunkScales, results = (size_t)M * N * sizeof(float);
-    if (meet(Y, results, g.x, (size_t)M * K * sizeof(float)) || meet(Y, results, g.a.codes, M * pitch) || meet(Y, results, g.a.scales, M * spitch) ||
-        meet(Y, results, w, N * pitch) || meet(Y, results, w_scales, N * spitch) || meet(Y, results, bias, (size_t)N * sizeof(float)))
+    const Plan p = plan_of(M, N, K);
+    const size_t need = workspace_of(p, M, K, f32);
+    const auto written = [&](const void *operand, size_t bytes) { return meet(Y, results, operand, bytes) || meet(workspace, need, operand, bytes); };
+    if (written(g.x, (size_t)M * K * sizeof(float)) || written(g.a.codes, M * pitch) || written(g.a.scales, M * spitch) || written(w, N * pitch) ||
+        written(w_scales, N * spitch) || written(bias, (size_t)N * sizeof(float)) || meet(Y, results, workspace, need))
         return VTL_HIP_ERR_INVALID_ARG;
     g.w = {w, w_scales};
     g.bias = bias;
@@ -812,9 +815,8 @@ int linear(Args g, const uint8_t *w, const uint8_t *w_scales, const float *bias,
     g.N = N;
     g.K = K;
     g.relu = relu;
-    const Plan p = plan_of(M, N, K);
     char *at = nullptr;
-    const int rc = workspace_at(workspace, workspace_bytes, workspace_of(p, M, K, f32), at);
+    const int rc = workspace_at(workspace, workspace_bytes, need, at);
     if (rc != VTL_HIP_OK)
         return rc;
     const hipStream_t st = current_stream();
