@@ -159,6 +159,10 @@ private:
 };
 
 #ifdef __HIPCC__
+// Pointers as loads straight into shared memory take them.
+#define VTL_GPTR(p) ((const __attribute__((address_space(1))) void *)(p))
+#define VTL_LPTR(p) ((__attribute__((address_space(3))) void *)(p))
+
 // A result element: with a signal to raise it goes through the caches to where the host sees it.
 template <typename T>
 __device__ __forceinline__ void store_result(T *p, T v, const DoneSignal &done)
@@ -188,6 +192,21 @@ template <int HOW = kThrough>
 __device__ __forceinline__ void store_through(void *out, unsigned off, Words4 v)
 {
     __builtin_amdgcn_raw_buffer_store_b128(v, result_buffer(out), off, 0, HOW);
+}
+
+// Workgroups are dealt round robin to the 8 XCDs; renumber them so that each XCD, which has an L2 of its own, works on a compact patch
+// of the tile grid, and walk the grid in groups of 8 tile rows.
+__device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int block, int &tile_m, int &tile_n)
+{
+    const int total = tiles_m * tiles_n;
+    const int xcd = block & 7, rest = total & 7;
+    const int pid = xcd * (total >> 3) + min(xcd, rest) + (block >> 3);
+    constexpr int kGroup = 8;
+    const int group_size = kGroup * tiles_n;
+    const int first_m = (pid / group_size) * kGroup;
+    const int gm = min(tiles_m - first_m, kGroup);
+    tile_m = first_m + (pid % group_size) % gm;
+    tile_n = (pid % group_size) / gm;
 }
 
 // Called by every thread of a workgroup after its last store_result.  Those are written through, so their

@@ -30,9 +30,6 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-#define VTL_GPTR(p) ((const __attribute__((address_space(1))) void *)(p))
-#define VTL_LPTR(p) ((__attribute__((address_space(3))) void *)(p))
-
 using vtlhip::HostResult;
 using vtlhip::raise_when_last;
 using vtlhip::store_result;
@@ -110,23 +107,6 @@ template <int N>
 __device__ __forceinline__ void wait_vmcnt()
 {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-// Workgroups are dealt round-robin to the 8 XCDs; renumber them so that each
-// XCD (own L2) works on a compact patch of the tile grid (XCD x holds
-// total/8 tiles, one more when x < total%8), then walk the grid in groups of
-// 8 tile rows.
-__device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int block, int &tile_m, int &tile_n)
-{
-    const int total = tiles_m * tiles_n;
-    const int xcd = block & 7, rest = total & 7;
-    const int pid = xcd * (total >> 3) + min(xcd, rest) + (block >> 3);
-    constexpr int GM = 8;
-    const int group_size = GM * tiles_n;
-    const int first_m = (pid / group_size) * GM;
-    const int gm = min(tiles_m - first_m, GM);
-    tile_m = first_m + (pid % group_size) % gm;
-    tile_n = (pid % group_size) / gm;
 }
 
 // Scales and bias of a block tile, fetched by the threads of the workgroup before the K loop

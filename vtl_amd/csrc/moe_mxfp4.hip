@@ -857,8 +857,6 @@ int launch_down(const Args &g, hipStream_t st)
     return launch_with_lds<moe_down_kernel<TILES, F, NW, PAST>, kLds + kMostTokens * kToken>(blocks, 64 * NW, kLds + g.tokens * kToken, st, g);
 }
 
-size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-
 int check(const vtl_hip_moe *m, int tokens)
 {
     if (!m || tokens < 0 || m->experts < 1 || m->top_k < 1 || m->top_k > m->experts || m->dim < 1 || m->hidden < 1)
@@ -973,7 +971,7 @@ int vtl_hip_moe_mxfp4_f32(const vtl_hip_moe *layer, const float *X, float *Y, in
     int status = check_launch("moe_scores_kernel");
     if (status != VTL_HIP_OK)
         return status;
-    const bool own_plan = tokens <= kOwnPlan && !g.many && !g.dense;
+    const bool own_plan = tokens <= kOwnPlan && !g.many;
     const int each = g.experts <= 2 * kWave ? 2 : g.experts <= 4 * kWave ? 4 : kMostExperts / kWave;     // scores of a token a lane
     if (!own_plan) {
         hipLaunchKernelGGL(each == 2 ? moe_plan_kernel<2> : each == 4 ? moe_plan_kernel<4> : moe_plan_kernel<kMostExperts / kWave>, dim3(1), dim3(1024), 0, st, g);

@@ -16,6 +16,7 @@ constexpr int kBlock = 32, kChunk = 256;
 constexpr int kChunkCodes = kChunk / 2, kChunkScales = kChunk / kBlock;   // bytes
 constexpr int kMostCols = 1 << 24;                                       // a tile's rows stay within 32 bits of bytes
 
+inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 inline int chunks_of(int cols) { return (cols + kChunk - 1) / kChunk; }
 
 // Rows of codes and scales.
@@ -66,9 +67,6 @@ __device__ __forceinline__ void settle()
     asm volatile("s_nop 15" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
-
-#define VTL_GPTR(p) ((const __attribute__((address_space(1))) void *)(p))
-#define VTL_LPTR(p) ((__attribute__((address_space(3))) void *)(p))
 
 template <int N>
 __device__ __forceinline__ void wait_vmcnt()

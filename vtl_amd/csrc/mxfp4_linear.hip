@@ -246,21 +246,6 @@ __device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>)
 
 // ---- many rows -----------------------------------------------------------------------------
 
-// Workgroups are dealt round robin to the 8 XCDs; renumber them so that each XCD, which has an L2 of its own, works on a compact patch
-// of the tile grid, and walk the grid in groups of 8 tile rows.
-__device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int block, int &tile_m, int &tile_n)
-{
-    const int total = tiles_m * tiles_n;
-    const int xcd = block & 7, rest = total & 7;
-    const int pid = xcd * (total >> 3) + min(xcd, rest) + (block >> 3);
-    constexpr int kGroup = 8;
-    const int group_size = kGroup * tiles_n;
-    const int first_m = (pid / group_size) * kGroup;
-    const int gm = min(tiles_m - first_m, kGroup);
-    tile_m = first_m + (pid % group_size) % gm;
-    tile_n = (pid % group_size) / gm;
-}
-
 // 16-byte pieces of a tile's rows of 128 bytes are put where a wave's read of 32 rows meets every bank as often.
 __device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 
@@ -767,8 +752,6 @@ int product(Args g, const Plan &p, hipStream_t st)
     hipLaunchKernelGGL(linear_join_mxfp4_kernel, dim3((unsigned)std::min<size_t>(blocks, 8192)), dim3(256), 0, st, g);
     return check_launch("linear_join_mxfp4_kernel");
 }
-
-size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t codes_workspace(int M, int K) { return up256((size_t)M * chunks_of(K) * kChunkCodes) + up256((size_t)M * chunks_of(K) * kChunkScales); }
 
