@@ -255,7 +255,8 @@ __device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 // its latency, the first reads of the next chunk and the loads into the stage that became free hide behind that step's products: a read and its
 // share of the loads behind each of them, in this order, because loads in one burst wait for each other in front of the unit that makes their addresses.
 // Tiles of 256 x 256 are bound by power: 8192 x 8192 x 8192 265 to 286 us from card to card, 3.8 to 4.15 PFLOP/s; 1.68 us a chunk, of which the products alone take 1.34 on random codes (reads left out
-// 1.49, loads left out 1.43).  Smaller ones by the way from the L2 into shared memory, some 22 bytes a cycle of a compute unit whatever the tile: 201 x 11008 x 4096 15.6 us.
+// 1.49, loads left out 1.43).  Smaller ones by their operands' way from the L2 into shared memory, with these loads some 22 bytes a cycle of a compute unit whatever
+// the tile: 201 x 11008 x 4096 15.6 us.
 template <int BM, int BN, int WR, int WC, int STAGES, int SPREAD, bool EDGE>
 struct Tile {
     static constexpr int kWaves = WR * WC, kThreads = 64 * kWaves;
