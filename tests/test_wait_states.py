@@ -110,7 +110,7 @@ def test_results_of_products_are_waited_for(tmp_path):
             bad += [(name, *b) for b in early]
             # written in the source in front of whatever comes first, copies from accumulation registers among it
             close += [(name, least)] * (least < 1)
-    assert with_products > 40 and not bad, (with_products, bad[:4])
+    assert with_products > 20 and not bad, (with_products, bad[:4])
     assert not close, close
 
 
